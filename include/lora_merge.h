@@ -256,6 +256,49 @@ int lm_routed_residual(const void* x, const void* y, void* out, int64_t T, int64
                        const lm_routed_factor* factors, int32_t count, void* workspace, size_t workspace_bytes,
                        void* stream);
 
+/* ---------------- products with merged weights ------------------------
+ * No reference counterpart.  Linear layers over weights as they are stored
+ * here, and over one weight per group of consecutive rows (experts, one
+ * adapter per request):
+ *   lm_linear             y[t,n]  = sum_k x[t,k] W[n,k] + bias[n]
+ *   lm_linear_input_grad  dx[t,k] = sum_n dy[t,n] W[n,k]
+ *   lm_linear_weight_grad dw[e,n,k] = sum over group e's rows of dy[t,n] x[t,k]
+ * accumulated in fp32 and rounded once to `dtype` (LM_BF16 / LM_F16, the type
+ * of x, dy, y, dx, dw, bias and of a dense weight).
+ *
+ * `w` is a HOST struct.  dtype LM_E2M1: MXFP4, codes [experts, N, K/2]
+ * (16-byte aligned, K % 32 == 0) and e8m0 scales per expert as lm_mx_merge has
+ * them (plain or swizzled, one expert after the other); fp16 rows see each
+ * weight rounded to fp16, bf16 rows see it exactly.  Otherwise a dense weight
+ * [experts, N, K] of `dtype`.
+ * `ends`: device int32[experts]; group e's rows are [ends[e-1], ends[e]).  Rows
+ * past ends[experts-1] get zeros.  NULL with one expert: all T rows.  Ends
+ * that fall or pass T are clamped.
+ * input_dtype: `dtype`, or LM_E2M1 (MXFP4 weights): x is quantised to MXFP4
+ * first, as lm_mx_requant with LM_MX_FLOOR does; a block with an infinity or a
+ * NaN makes its row NaN.  The input gradient passes straight through that
+ * rounding.
+ * Strides are in elements; outputs are contiguous.  Workspace:
+ * lm_linear_workspace_size bytes, 256-byte aligned; NULL when that is 0. */
+#define LM_LINEAR_MAX_EXPERTS 1024
+typedef struct lm_weight {
+  const void* q;
+  const uint8_t* scale; /* NULL for dense weights */
+  int64_t N;
+  int64_t K;
+  int32_t dtype;
+  int32_t swizzled;
+  int32_t experts;
+  int32_t reserved;
+} lm_weight;
+size_t lm_linear_workspace_size(int64_t T, int64_t N, int64_t K, int32_t experts, int32_t input_dtype);
+int lm_linear(const void* x, int64_t ldx, const lm_weight* w, const void* bias, const int32_t* ends, void* y, int64_t T,
+              int32_t dtype, int32_t input_dtype, void* workspace, size_t workspace_bytes, void* stream);
+int lm_linear_input_grad(const void* dy, int64_t lddy, const lm_weight* w, const int32_t* ends, void* dx, int64_t T,
+                         int32_t dtype, void* stream);
+int lm_linear_weight_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int32_t* ends, void* dw,
+                          int64_t T, int64_t N, int64_t K, int32_t experts, int32_t dtype, void* stream);
+
 /* ---------------- stacks: many targets, one grouped launch ------------
  * `items` is a HOST array of `count` descriptors.  Each target gets its own
  * seed (derive_seed(param_path, merge_index)).  An item's outputs may alias

@@ -9,11 +9,14 @@ Host layer over the gfx950 HIP kernels in ``libpiper_lora_merge.so``:
   plain tensors;
 * ``kernels`` -- drop-in replacements for the Triton merge functions;
 * ``stack`` -- grouped multi-target merges;
-* ``routed`` -- routed LoRA: the residual hook (P/lora.py:792-930).
+* ``routed`` -- routed LoRA: the residual hook (P/lora.py:792-930);
+* ``linear`` -- products with MXFP4 weights and with one weight per group of
+  rows, with gradients.
 """
 
 from .adapters import Float8Adapter, GgufAdapter, Int8Adapter, MxAdapter, Nvfp4Adapter, RegularAdapter
 from .formats import Float8Weight, GGUFWeight, Int8Weight, MXWeight, NVFP4Weight
+from .linear import expert_view, grouped_linear, mx_linear
 from .lora import LoRA, LoRAFactor, LoRATransform, ScaledLoRAFactor
 from .merge import merge_lora
 from .registry import param_representation, register_adapter, select_adapter
@@ -39,8 +42,11 @@ __all__ = [
     "RegularAdapter",
     "ScaledLoRAFactor",
     "derive_seed",
+    "expert_view",
+    "grouped_linear",
     "install_routed_residual_hook",
     "merge_lora",
+    "mx_linear",
     "param_representation",
     "register_adapter",
     "routed_residual",

@@ -16,7 +16,7 @@ import torch
 __all__ = [
     "LM_F32", "LM_BF16", "LM_F16", "LM_E4M3", "LM_E5M2", "LM_E2M1", "LM_E8M0",
     "LM_ROUND_NEAREST", "LM_ROUND_STOCHASTIC",
-    "LoraStruct", "RoundingStruct", "RoutedFactor", "StackItem",
+    "LoraStruct", "RoundingStruct", "RoutedFactor", "StackItem", "WeightStruct",
     "check", "lib", "library_path", "torch_dtype_id", "workspace",
 ]
 
@@ -63,7 +63,15 @@ class RoutedFactor(ctypes.Structure):
     _fields_ = [("a", _P), ("b", _P), ("bias", _P), ("strength", ctypes.c_float), ("rank", _I32)]
 
 
+class WeightStruct(ctypes.Structure):
+    """Mirror of ``lm_weight``."""
+
+    _fields_ = [("q", _P), ("scale", _P), ("N", _I64), ("K", _I64), ("dtype", _I32), ("swizzled", _I32),
+                ("experts", _I32), ("reserved", _I32)]
+
+
 _L = ctypes.POINTER(LoraStruct)
+_W = ctypes.POINTER(WeightStruct)
 _R = ctypes.POINTER(RoundingStruct)
 
 _SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -93,6 +101,10 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lm_routed_workspace_size": (_SZ, [_I64, _I64, ctypes.POINTER(RoutedFactor), _I32]),
     "lm_routed_residual": (_I32, [_P, _P, _P, _I64, _I64, _I64, _I32, ctypes.POINTER(RoutedFactor), _I32, _P, _SZ,
                                   _P]),
+    "lm_linear_workspace_size": (_SZ, [_I64, _I64, _I64, _I32, _I32]),
+    "lm_linear": (_I32, [_P, _I64, _W, _P, _P, _P, _I64, _I32, _I32, _P, _SZ, _P]),
+    "lm_linear_input_grad": (_I32, [_P, _I64, _W, _P, _P, _I64, _I32, _P]),
+    "lm_linear_weight_grad": (_I32, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _P]),
     "lm_timer_enable": (_I32, [_I32]),
     "lm_timer_read": (_I32, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int64)]),
 }

@@ -13,6 +13,15 @@ the C ABI:
 * :func:`merge_dense_lora_` <- RegularAdapter.merge_lora_ (P/tensor_adapters.py:686-696)
 * :func:`dequantize_gguf`   <- P/gguf_dequant.py:303-331 (all 15 dispatched types)
 
+Products with weights as they are stored (no reference counterpart; with
+autograd in :mod:`.linear`):
+
+* :func:`mx_matmul`, :func:`mx_matmul_input_grad` -- one MXFP4 weight
+* :func:`grouped_matmul`, :func:`grouped_matmul_input_grad`,
+  :func:`grouped_matmul_weight_grad` -- one dense weight per group of rows
+* :func:`grouped_mx_matmul`, :func:`grouped_mx_matmul_input_grad` -- one MXFP4
+  weight per group of rows
+
 The ``*_into`` variants write into caller-provided (possibly aliasing)
 outputs; the adapters use them to merge in place without a copy.
 """
@@ -33,6 +42,11 @@ __all__ = [
     "dequantize_int8",
     "dequantize_mx",
     "dequantize_nvfp4",
+    "grouped_matmul",
+    "grouped_matmul_input_grad",
+    "grouped_matmul_weight_grad",
+    "grouped_mx_matmul",
+    "grouped_mx_matmul_input_grad",
     "merge_dense_lora_",
     "merge_float8_lora",
     "merge_float8_lora_into",
@@ -42,6 +56,8 @@ __all__ = [
     "merge_nvfp4_lora",
     "merge_nvfp4_lora_into",
     "merge_q8_0_lora",
+    "mx_matmul",
+    "mx_matmul_input_grad",
     "requantize_float8",
     "requantize_int8",
     "requantize_mx",
@@ -615,3 +631,202 @@ def merge_dense_lora_(weight: torch.Tensor, b: torch.Tensor, a: torch.Tensor, st
     lora = L.lora_struct(b, a, strength)
     ws_bytes = L.workspace_size(rows, cols, a.shape[0])
     _run("lm_dense_merge", device, ws_bytes, _ptr(weight), rows, cols, weight.stride(0), ctypes.byref(lora))
+
+
+# ---------------------------------------------------------------------------
+# Products with stored weights
+# ---------------------------------------------------------------------------
+_MAX_EXPERTS = 1024
+
+
+def _rows(label: str, x: torch.Tensor, cols: int) -> torch.Tensor:
+    """``x`` [..., cols] as [rows, cols] whose rows are contiguous (their stride is free)."""
+    if x.ndim < 1 or x.shape[-1] != cols:
+        raise ValueError(f"{label}: expected rows of {cols} elements, got shape {tuple(x.shape)}.")
+    if x.dtype not in _FACTOR_DTYPES:
+        raise ValueError(f"{label} supports bfloat16 and float16 rows, got {x.dtype}.")
+    x = x.reshape(-1, cols)
+    if (cols > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < cols):
+        x = x.contiguous()
+    return x
+
+
+def _stride(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]  # (the stride of a single row may be anything)
+
+
+def _ends(label: str, ends: torch.Tensor, experts: int) -> torch.Tensor:
+    if ends.dtype is not torch.int32 or ends.ndim != 1 or ends.shape[0] != experts:
+        raise ValueError(f"{label}: ends must be int32 [{experts}] (the end of each group's rows), got "
+                         f"{ends.dtype} {tuple(ends.shape)}.")
+    if not 1 <= experts <= _MAX_EXPERTS:
+        raise ValueError(f"{label} takes 1 to {_MAX_EXPERTS} groups, got {experts}.")
+    return ends.contiguous()
+
+
+def _mx_stack(label: str, qdata: torch.Tensor, scale: torch.Tensor, swizzled: bool, experts: int | None) -> tuple[int, int]:
+    """Check MXFP4 storage ([rows, cols/2], or [experts, rows, cols/2]); returns (rows, cols)."""
+    ndim = 2 if experts is None else 3
+    if qdata.ndim != ndim or scale.ndim != ndim:
+        raise ValueError(f"{label} expects rank-{'two' if ndim == 2 else 'three'} MXFP4 codes and scales.")
+    if qdata.dtype is not torch.uint8 and qdata.dtype is not _FP4_DTYPE:
+        raise ValueError(f"{label} expects packed uint8 MXFP4 codes, got {qdata.dtype}.")
+    if scale.dtype is not torch.uint8 and scale.dtype is not _E8M0_DTYPE:
+        raise ValueError(f"{label} expects E8M0 scales, got {scale.dtype}.")
+    if not qdata.is_contiguous() or not scale.is_contiguous():
+        raise ValueError(f"{label} requires contiguous MXFP4 storage.")
+    rows, cols = qdata.shape[-2], qdata.shape[-1] * 2
+    if rows == 0 or cols == 0:
+        raise ValueError(f"{label} requires a non-empty weight.")
+    if cols % 32 != 0:
+        raise ValueError(f"{label} requires columns divisible by 32.")
+    if tuple(scale.shape) != qdata.shape[:-2] + _mx_scale_shape(rows, cols, swizzled):
+        raise ValueError(f"{label}: the scale shape {tuple(scale.shape)} does not match its block layout.")
+    return rows, cols
+
+
+def _linear_forward(label: str, x: torch.Tensor, weight: L.WeightStruct, bias: torch.Tensor | None,
+                    ends: torch.Tensor | None, activation_dtype: torch.dtype | None, device: torch.device) -> torch.Tensor:
+    n, k = weight.N, weight.K
+    x2 = _rows(label, x, k)
+    dtype_id = L.torch_dtype_id(x.dtype)
+    input_id = dtype_id
+    if activation_dtype is not None:
+        if activation_dtype is not _FP4_DTYPE or _FP4_DTYPE is None:
+            raise ValueError(f"{label} quantises its input to float4_e2m1fn_x2 only, got {activation_dtype}.")
+        input_id = L.LM_E2M1
+    if bias is not None:
+        if bias.dtype is not x.dtype or tuple(bias.shape) != (n,):
+            raise ValueError(f"{label}: bias must be {x.dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}.")
+        bias = bias.contiguous()
+    t = x2.shape[0]
+    y = torch.empty((t, n), dtype=x.dtype, device=device)
+    if t:
+        handle = L.lib()
+        ws_bytes = handle.lm_linear_workspace_size(t, n, k, weight.experts, input_id)
+        with L.on_device(device):
+            ws = L.workspace(ws_bytes, device) if ws_bytes else None
+            rc = handle.lm_linear(x2.data_ptr(), _stride(x2), ctypes.byref(weight), _ptr(bias), _ptr(ends), y.data_ptr(), t,
+                                  dtype_id, input_id, None if ws is None else L.aligned_ptr(ws), ws_bytes,
+                                  L.stream_ptr(device))
+        if rc:
+            L.check(rc)
+    return y.view(*x.shape[:-1], n)
+
+
+def _linear_input_grad(label: str, dy: torch.Tensor, weight: L.WeightStruct, ends: torch.Tensor | None,
+                       device: torch.device) -> torch.Tensor:
+    dy2 = _rows(label, dy, weight.N)
+    t = dy2.shape[0]
+    dx = torch.empty((t, weight.K), dtype=dy.dtype, device=device)
+    if t:
+        handle = L.lib()
+        with L.on_device(device):
+            rc = handle.lm_linear_input_grad(dy2.data_ptr(), _stride(dy2), ctypes.byref(weight), _ptr(ends), dx.data_ptr(),
+                                             t, L.torch_dtype_id(dy.dtype), L.stream_ptr(device))
+        if rc:
+            L.check(rc)
+    return dx.view(*dy.shape[:-1], weight.K)
+
+
+def mx_matmul(x: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, *, swizzled: bool = False,
+              bias: torch.Tensor | None = None, activation_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``x @ W.T + bias`` with ``W`` stored in MXFP4 (``qdata`` [out, in/2], ``scale`` as in :class:`MXWeight`).
+
+    ``x`` [..., in] bfloat16 or float16; sums in fp32, rounded once to ``x.dtype``.  With
+    ``activation_dtype=torch.float4_e2m1fn_x2`` ``x`` is quantised first, as :func:`requantize_mx` does it.
+    """
+    label = "MX product"
+    device = _same_device(label, x, qdata, scale, bias)
+    n, k = _mx_stack(label, qdata, scale, swizzled, None)
+    weight = L.WeightStruct(qdata.data_ptr(), scale.data_ptr(), n, k, L.LM_E2M1, int(swizzled), 1, 0)
+    return _linear_forward(label, x, weight, bias, None, activation_dtype, device)
+
+
+def mx_matmul_input_grad(dy: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, *,
+                         swizzled: bool = False) -> torch.Tensor:
+    """``dy @ W``: the input gradient of :func:`mx_matmul` (straight through a quantised input)."""
+    label = "MX product gradient"
+    device = _same_device(label, dy, qdata, scale)
+    n, k = _mx_stack(label, qdata, scale, swizzled, None)
+    weight = L.WeightStruct(qdata.data_ptr(), scale.data_ptr(), n, k, L.LM_E2M1, int(swizzled), 1, 0)
+    return _linear_input_grad(label, dy, weight, None, device)
+
+
+def _dense_stack(label: str, rows: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> L.WeightStruct:
+    if weight.ndim != 3 or 0 in weight.shape:
+        raise ValueError(f"{label} expects a weight [groups, out, in], got {tuple(weight.shape)}.")
+    if weight.dtype is not rows.dtype:
+        raise ValueError(f"{label} requires the weight in the rows' dtype {rows.dtype}, got {weight.dtype}.")
+    if not weight.is_contiguous():
+        raise ValueError(f"{label} requires a contiguous weight.")
+    e, n, k = weight.shape
+    return L.WeightStruct(weight.data_ptr(), None, n, k, L.torch_dtype_id(weight.dtype), 0, e, 0)
+
+
+def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
+    """Rows ``ends[e-1] : ends[e]`` of ``x`` [rows, in] times ``weight[e].T`` (``weight`` [groups, out, in]).
+
+    ``ends`` int32 [groups] stays on the GPU (no synchronization); rows past the last end give zeros.
+    """
+    label = "Grouped product"
+    device = _same_device(label, x, weight, ends)
+    w = _dense_stack(label, x, weight, ends)
+    return _linear_forward(label, x, w, None, _ends(label, ends, w.experts), None, device)
+
+
+def grouped_matmul_input_grad(dy: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
+    """The gradient of :func:`grouped_matmul` to ``x``; zeros for rows of no group."""
+    label = "Grouped product gradient"
+    device = _same_device(label, dy, weight, ends)
+    w = _dense_stack(label, dy, weight, ends)
+    return _linear_input_grad(label, dy, w, _ends(label, ends, w.experts), device)
+
+
+def grouped_matmul_weight_grad(dy: torch.Tensor, x: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
+    """The gradient of :func:`grouped_matmul` to ``weight``: ``dy[group].T @ x[group]``, zeros for empty groups."""
+    label = "Grouped product weight gradient"
+    device = _same_device(label, dy, x, ends)
+    if dy.ndim < 1 or x.ndim < 1 or dy.shape[:-1] != x.shape[:-1]:
+        raise ValueError(f"{label}: dy {tuple(dy.shape)} and x {tuple(x.shape)} differ in their rows.")
+    if dy.dtype is not x.dtype:
+        raise ValueError(f"{label} requires dy and x in one dtype, got {dy.dtype} and {x.dtype}.")
+    n, k = dy.shape[-1], x.shape[-1]
+    if n == 0 or k == 0:
+        raise ValueError(f"{label} requires non-empty rows.")
+    dy2, x2 = _rows(label, dy, n), _rows(label, x, k)
+    ends = _ends(label, ends, ends.shape[0] if ends.ndim == 1 else -1)
+    e = ends.shape[0]
+    dw = torch.empty((e, n, k), dtype=x.dtype, device=device)
+    handle = L.lib()
+    with L.on_device(device):
+        rc = handle.lm_linear_weight_grad(dy2.data_ptr(), _stride(dy2), x2.data_ptr(), _stride(x2), ends.data_ptr(),
+                                          dw.data_ptr(), x2.shape[0], n, k, e, L.torch_dtype_id(x.dtype),
+                                          L.stream_ptr(device))
+    if rc:
+        L.check(rc)
+    return dw
+
+
+def grouped_mx_matmul(x: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, ends: torch.Tensor, *,
+                      swizzled: bool = False, activation_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """:func:`grouped_matmul` with MXFP4 weights: ``qdata`` [groups, out, in/2], scales of each group's weight."""
+    label = "Grouped MX product"
+    device = _same_device(label, x, qdata, scale, ends)
+    experts = qdata.shape[0] if qdata.ndim else 0
+    n, k = _mx_stack(label, qdata, scale, swizzled, experts)
+    ends = _ends(label, ends, experts)
+    weight = L.WeightStruct(qdata.data_ptr(), scale.data_ptr(), n, k, L.LM_E2M1, int(swizzled), experts, 0)
+    return _linear_forward(label, x, weight, None, ends, activation_dtype, device)
+
+
+def grouped_mx_matmul_input_grad(dy: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, ends: torch.Tensor, *,
+                                 swizzled: bool = False) -> torch.Tensor:
+    """The gradient of :func:`grouped_mx_matmul` to ``x``; zeros for rows of no group."""
+    label = "Grouped MX product gradient"
+    device = _same_device(label, dy, qdata, scale, ends)
+    experts = qdata.shape[0] if qdata.ndim else 0
+    n, k = _mx_stack(label, qdata, scale, swizzled, experts)
+    ends = _ends(label, ends, experts)
+    weight = L.WeightStruct(qdata.data_ptr(), scale.data_ptr(), n, k, L.LM_E2M1, int(swizzled), experts, 0)
+    return _linear_input_grad(label, dy, weight, ends, device)
