@@ -26,53 +26,94 @@ static inline int64_t lin_scale_bytes(int64_t N, int64_t K, int swizzled) {
   return swizzled ? (N + 127) / 128 * ((K + 127) / 128) * 512 : N * (K / 32);
 }
 
-// Rows [b, e) of group g.  Ends that fall, are negative or pass T are clamped
-// to what came before and to T, so no index leaves the tensors whatever the
-// caller's memory holds.
+// ---- groups of rows --------------------------------------------------------
+// Ends that fall, are negative or pass T are clamped to what came before and to
+// T, so no index leaves the tensors whatever the caller's memory holds.  A wave
+// scans 64 groups at a time, one per lane (all lanes active; every wave of a
+// workgroup does it for itself).
+
+// lane i: end of group c + i, given the end of group c - 1
+DEV int lin_ends64(const LinArgs& a, int c, int before) {
+  const int i = c + (int)(threadIdx.x & 63);
+  int x = i < a.experts ? a.ends[i] : 0;
+  x = x > (int)a.T ? (int)a.T : x;
+  x = x < before ? before : x;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int y = __shfl_up(x, d);
+    if ((int)(threadIdx.x & 63) >= d) x = y > x ? y : x;
+  }
+  return x;
+}
+// Rows [b, e) of group g.
 DEV void lin_group(const LinArgs& a, int g, int64_t& b, int64_t& e) {
   if (!a.ends) {
     b = 0;
     e = a.T;
     return;
   }
-  b = 0;
-  e = 0;
-  for (int i = 0; i <= g; ++i) {
-    const int64_t x = a.ends[i];
-    b = e;
-    e = x < e ? e : (x > a.T ? a.T : x);
+  int before = 0;
+  for (int c = 0;; c += 64) {
+    const int x = lin_ends64(a, c, before);
+    if (g < c + 64) {
+      e = __shfl(x, g - c);
+      b = g == c ? before : __shfl(x, g - c > 0 ? g - c - 1 : 0);
+      break;
+    }
+    before = __shfl(x, 63);
   }
+  b = __builtin_amdgcn_readfirstlane((int)b);
+  e = __builtin_amdgcn_readfirstlane((int)e);
 }
 
-// Tile t of BM rows: its group and rows [r0, r1).  Groups are tiled one after
-// the other, each from its own first row; group `experts` holds the rows of no
-// group.  False past the last tile.
+// Groups are tiled one after the other, BM rows a tile, each from its own first
+// row; group `experts` holds the rows of no group.  Finds tile t: its group
+// and rows [r0, r1), false past the last tile; t < 0 counts the tiles into g.
 template <int BM>
-DEV bool lin_tile(const LinArgs& a, int64_t t, int& g, int64_t& r0, int64_t& r1) {
-  if (!a.ends) {
-    g = 0;
-    r0 = t * BM;
-    r1 = a.T;
-    return r0 < a.T;
-  }
-  int64_t e = 0;
-  for (g = 0; g <= a.experts; ++g) {
-    const int64_t b = e;
-    if (g < a.experts) {
-      const int64_t x = a.ends[g];
-      e = x < e ? e : (x > a.T ? a.T : x);
-    } else {
-      e = a.T;
+DEV bool lin_find(const LinArgs& a, int t, int& g, int64_t& r0, int64_t& r1) {
+  const int lane = threadIdx.x & 63;
+  int before = 0, tiles = 0;
+  for (int c = 0; c <= a.experts; c += 64) {
+    int x = lin_ends64(a, c, before);
+    if (c + lane >= a.experts) x = (int)a.T;  // the rows of no group, then empty ones
+    int b = __shfl_up(x, 1);
+    if (lane == 0) b = before;
+    int n = (x - b + BM - 1) / BM, sum = n;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int y = __shfl_up(sum, d);
+      if (lane >= d) sum += y;
     }
-    const int64_t n = (e - b + BM - 1) / BM;
-    if (t < n) {
-      r0 = b + t * BM;
-      r1 = e;
+    const uint64_t hit = __ballot(t >= tiles && t < tiles + sum);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      g = c + l;
+      const int first = tiles + __shfl(sum - n, l);
+      r0 = __builtin_amdgcn_readfirstlane(__shfl(b, l) + (t - first) * BM);
+      r1 = __builtin_amdgcn_readfirstlane(__shfl(x, l));
+      g = __builtin_amdgcn_readfirstlane(g);
       return true;
     }
-    t -= n;
+    before = __shfl(x, 63);
+    tiles += __shfl(sum, 63);
   }
+  g = __builtin_amdgcn_readfirstlane(tiles);
   return false;
+}
+template <int BM>
+DEV bool lin_tile(const LinArgs& a, int64_t t, int& g, int64_t& r0, int64_t& r1) {
+  if (a.ends) return lin_find<BM>(a, (int)t, g, r0, r1);
+  g = 0;
+  r0 = t * BM;
+  r1 = a.T;
+  return r0 < a.T;
+}
+template <int BM>
+DEV int lin_count(const LinArgs& a) {
+  int g;
+  int64_t r0, r1;
+  lin_find<BM>(a, -1, g, r0, r1);
+  return g;
 }
 // at most this many tiles: every group may end in a part of one
 template <int BM>

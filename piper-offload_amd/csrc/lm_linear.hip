@@ -9,6 +9,7 @@
 // store.  An MXFP4 value is e2m1 * 2^(scale - 127); in bf16 it is exact.
 #include "lm_impl.h"
 #include "lm_linear.h"
+#include "lm_linear_mm.h"
 
 // ---------------------------------------------------------------------------
 // x quantised to MXFP4: blocks of 32 along K, scale 2^(floor(log2 max) - 2)
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(256) void k_lin_general(LinArgs a) {
 // ---------------------------------------------------------------------------
 static int check_lin(const lm_weight* w, int64_t T, int32_t dtype, const int32_t* ends, int32_t experts) {
   if (dtype != LM_BF16 && dtype != LM_F16) return fail(LM_EUNSUPPORTED, "products take bf16 and fp16 rows");
-  if (T < 0) return fail(LM_EINVAL, "negative number of rows");
+  if (T < 0 || T > 0x7fffffff) return fail(LM_EINVAL, "number of rows must be 0 to 2^31 - 1");
   if (experts < 1 || experts > LM_LINEAR_MAX_EXPERTS)
     return fail(LM_EINVAL, "number of groups must be 1 to %d, got %d", LM_LINEAR_MAX_EXPERTS, experts);
   if (experts > 1 && !ends) return fail(LM_EINVAL, "several groups need their ends");
@@ -176,8 +177,45 @@ static int run_general(const LinArgs& a, hipStream_t st) {
   LAUNCH_CHECK();
   return LM_OK;
 }
+// Whole 16-byte pieces along every row that is read, offsets inside a tile below
+// 2^31, fewer tiles than a grid holds.
+static bool mm_ok(const LinArgs& a, int op, bool mx) {
+  const int64_t len = op == LIN_FORWARD ? a.K : a.N;
+  if (a.lda % 8 || ((uintptr_t)a.a & 15) || a.lda >= (1 << 22) || a.K >= (1 << 22) || a.N >= (1 << 22)) return false;
+  if (op == LIN_WEIGHT_GRAD) return a.ldb % 8 == 0 && ((uintptr_t)a.b & 15) == 0 && a.ldb < (1 << 22);
+  if (len % 8) return false;
+  return mx || (a.K % 8 == 0 && ((uintptr_t)a.w & 15) == 0);
+}
+
+template <int DT, int OP, bool MX, int B, int WM, int WN>
+static int launch_mm(const LinArgs& a, hipStream_t st) {
+  TimedLaunch timed("linear", st);
+  const int64_t J = OP == LIN_FORWARD ? a.N : a.K, gj = (J + B - 1) / B;
+  const int64_t gi = OP == LIN_WEIGHT_GRAD ? (a.N + B - 1) / B : lin_tiles<B>(a.T, a.experts, a.ends != nullptr);
+  if (gi * gj > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+  hipLaunchKernelGGL((k_lin_mm<DT, OP, MX, B, B, WM, WN>), dim3((unsigned)(gi * gj), OP == LIN_WEIGHT_GRAD ? a.experts : 1),
+                     dim3(WM * WN * 64), 0, st, a);
+  LAUNCH_CHECK();
+  return LM_OK;
+}
+template <int OP, bool MX>
+static int run_mm(const LinArgs& a, int dtype, hipStream_t st) {
+  const int64_t J = OP == LIN_FORWARD ? a.N : a.K, I = OP == LIN_WEIGHT_GRAD ? a.N : a.T;
+  const int64_t big = I / 256 * ((J + 255) / 256) * (OP == LIN_WEIGHT_GRAD ? a.experts : 1);
+  const bool wide = big >= 192 && (OP == LIN_WEIGHT_GRAD || a.T / a.experts >= 256);
+  if (dtype == LM_F16)
+    return wide ? launch_mm<F16, OP, MX, 256, 2, 4>(a, st) : launch_mm<F16, OP, MX, 128, 2, 2>(a, st);
+  return wide ? launch_mm<BF16, OP, MX, 256, 2, 4>(a, st) : launch_mm<BF16, OP, MX, 128, 2, 2>(a, st);
+}
+
 template <int OP>
 static int run_product(const LinArgs& a, int dtype, bool mx, bool quant, hipStream_t st) {
+  if (!quant && mm_ok(a, OP, mx)) {
+    if constexpr (OP != LIN_WEIGHT_GRAD) {
+      if (mx) return run_mm<OP, true>(a, dtype, st);
+    }
+    return run_mm<OP, false>(a, dtype, st);
+  }
   if constexpr (OP == LIN_FORWARD) {
     if (quant) return dtype == LM_F16 ? run_general<F16, true, true, OP>(a, st) : run_general<BF16, true, true, OP>(a, st);
   }

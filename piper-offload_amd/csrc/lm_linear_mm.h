@@ -1,0 +1,375 @@
+// lm_linear_mm.h -- products of many rows: LDS-tiled MFMA kernels.
+//
+// An output tile of BM rows x BN columns per workgroup, the contraction in
+// tiles of 64, two LDS buffers: while the waves multiply tile k out of one, the
+// loads of tile k + 1 are on their way into the other (buffer loads straight
+// to LDS, no registers in between).  One barrier a tile.
+//
+// Operands are named by the output index they carry: I (rows) and J
+// (columns).  Their tiles lie in LDS as
+//   KC16  contraction contiguous in memory: a slot of 128 bytes per I/J index,
+//         its eight 16-byte chunks rotated by XOR with slot & 7, so that the
+//         16 lanes that read one chunk of 16 slots hit all banks
+//   KS16  contraction strided (the index contiguous): a row per contraction
+//         step; read transposed (ds_read_b64_tr_b16); chunks XORed with
+//         4 (row & 3) for the same reason
+//   KC4   MXFP4 codes as they are stored, 32 bytes per slot, decoded to 16 bits
+//         after the read (v_cvt_scalef32_pk: exact products in bf16)
+//   KS4   MXFP4 with the contraction strided: every code of a run of 32 shares a
+//         scale but the 8 codes of an MFMA lane do not, so these are decoded on
+//         their way into LDS and then are KS16
+// The MFMA's first operand is J, so a lane's accumulators are consecutive output
+// columns; the columns of a pair of 16-column fragments are interleaved in
+// fours, which makes them 8 in a row: one 16-byte store.
+#pragma once
+#include "lm_linear.h"
+
+enum : int { KC16, KS16, KC4, KS4 };
+
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef __attribute__((address_space(3))) lm_u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) lm_u32x2 lds_u32x2;
+typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
+
+// Where a product's rows are too far apart for 32-bit offsets inside a tile the
+// general kernel runs instead.
+constexpr int64_t LIN_SPAN = 0x7fffffff;
+
+DEV __amdgpu_buffer_rsrc_t lin_rsrc(const void* p, int64_t bytes) {
+  const uint32_t n = bytes < 0 ? 0u : (bytes > LIN_SPAN ? (uint32_t)LIN_SPAN : (uint32_t)bytes);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, n, 0x00027000);
+}
+// 16 bytes per lane to LDS at base + 16 lane; past the resource's end: zeros
+DEV void lin_dma(__amdgpu_buffer_rsrc_t r, lds_u8* base, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)base, 16, (int)off, 0, 0, 0);
+}
+
+// Slot of a J tile -> column: pairs of fragments of 16 interleaved in fours
+DEV int lin_jcol(int slot) { return (slot & ~31) + 8 * ((slot & 15) >> 2) + (slot & 3) + 4 * ((slot >> 4) & 1); }
+
+// The tile of this workgroup: group, first row, end of the group's rows, number of
+// the column tile.  Tiles of up to 8 row tiles x all columns, row tiles
+// first, are neighbours; each XCD takes a contiguous part of them, so its L2
+// holds the weight tiles that several row tiles share.
+struct LinTile {
+  int group;
+  int64_t r0, r1, j0;
+};
+template <int BM, int BN>
+DEV bool lin_pick(const LinArgs& a, int64_t jend, LinTile& t) {
+  const int gn = (int)((jend + BN - 1) / BN);
+  int tiles;
+  if (!a.ends) tiles = (int)((a.T + BM - 1) / BM);
+  else tiles = lin_count<BM>(a);
+  const uint32_t total = (uint32_t)tiles * (uint32_t)gn;
+  if (blockIdx.x >= total) return false;
+  const uint32_t u = xcd_unit(blockIdx.x, total);
+  constexpr uint32_t GM = 8;
+  const uint32_t band = u / (GM * gn), in = u - band * GM * gn;
+  const uint32_t left = (uint32_t)tiles - band * GM, h = left < GM ? left : GM;
+  const uint32_t tm = band * GM + in % h, tn = in / h;
+  t.j0 = (int64_t)tn * BN;
+  if (!a.ends) {
+    t.group = 0;
+    t.r0 = (int64_t)tm * BM;
+    t.r1 = a.T;
+    return true;
+  }
+  return lin_find<BM>(a, (int)tm, t.group, t.r0, t.r1);
+}
+
+template <int DT, int OP, bool MX, int BM, int BN, int WM, int WN>
+struct MmTraits {
+  static constexpr int NW = WM * WN, NT = NW * 64;
+  static constexpr int IK = OP == LIN_WEIGHT_GRAD ? KS16 : KC16;
+  static constexpr int JK = OP == LIN_FORWARD ? (MX ? KC4 : KC16) : (OP == LIN_INPUT_GRAD && MX ? KS4 : KS16);
+  static constexpr int FI = BM / WM / 16, FJ = BN / WN / 16;
+  static constexpr int IB = BM * 128, JB = JK == KC4 ? BN * 32 : BN * 128;  // bytes of a tile
+  static constexpr int IL = IB / 1024 / NW, JL = JB / 1024 / NW;            // loads per wave
+  static_assert(IL * 1024 * NW == IB && JL * 1024 * NW == JB, "tiles are whole loads of all waves");
+  static_assert(JK != KS4 || NT * 32 == 64 * BN, "a run of 32 codes per thread");
+  // chunk c of contraction 8-groups that lane group g takes in MFMA step s: with
+  // KC4 a lane reads the codes of both steps at once, so they are neighbours
+  DEV static int chunk(int s, int g) { return JK == KC4 ? 2 * g + s : 4 * s + g; }
+};
+
+// per-lane byte offsets of the DMA loads of one operand tile
+template <int KIND, int B, int L, int NW, bool PERM>
+DEV void mm_offsets(uint32_t (&off)[L], int wave, int lane, int64_t ld) {
+#pragma unroll
+  for (int n = 0; n < L; ++n) {
+    const int piece = (n * NW + wave) * 64 + lane;  // 16-byte piece of the tile
+    if constexpr (KIND == KC16) {
+      const int slot = piece >> 3, c = (piece & 7) ^ (slot & 7);
+      off[n] = (uint32_t)((PERM ? lin_jcol(slot) : slot) * ld * 2) + c * 16;
+    } else if constexpr (KIND == KC4) {
+      const int slot = piece >> 1;
+      off[n] = (uint32_t)(lin_jcol(slot) * (ld >> 1)) + (piece & 1) * 16;
+    } else {  // KS16
+      const int row = piece / (B / 8), c = (piece % (B / 8)) ^ ((row & 3) << 2);
+      off[n] = (uint32_t)(row * ld * 2) + c * 16;
+    }
+  }
+}
+
+template <int KIND, int B>
+DEV lm_u32x4 mm_frag(const lds_u8* t, int slot0, int f, int lane, int s, int c) {
+  if constexpr (KIND == KC16) {
+    const int slot = slot0 + f * 16 + (lane & 15);
+    return *(const lds_u32x4*)(t + slot * 128 + ((c ^ (slot & 7)) << 4));
+  } else {
+    return lm_u32x4{};
+  }
+}
+// 8 contraction steps x this lane's index, read transposed: two loads of 4 steps
+// each.  Lane p of 16 points at 4 indices of row p >> 2.
+template <int B, bool PERM>
+DEV lm_u32x4 mm_frag_tr(const lds_u8* t, int col0, int f, int lane, int s) {
+  const int p = lane & 15, g = lane >> 4, q = p & 3;
+  const int row = 32 * s + 8 * g + (p >> 2);
+  const int col = col0 + (PERM ? (f >> 1) * 32 + 8 * q + 4 * (f & 1) : f * 16 + 4 * q);
+  const int at = row * (B * 2) + ((((col >> 3) ^ ((row & 3) << 2)) << 4) | ((col & 4) << 1));
+  const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(t + at));
+  const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(t + at + 4 * (B * 2)));  // row + 4: same XOR
+  return lm_u32x4{__builtin_bit_cast(lm_u32x2, lo)[0], __builtin_bit_cast(lm_u32x2, lo)[1],
+                  __builtin_bit_cast(lm_u32x2, hi)[0], __builtin_bit_cast(lm_u32x2, hi)[1]};
+}
+
+// 8 codes -> 8 values of 16 bits
+template <bool HALF>
+DEV lm_u32x4 mm_decode(uint32_t codes, float scale) {
+  lm_u32x4 v;
+  if constexpr (HALF) {
+    v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0));
+    v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1));
+    v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 2));
+    v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3));
+  } else {
+    v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
+    v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1));
+    v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2));
+    v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
+  }
+  return v;
+}
+
+template <int DT, int OP, bool MX, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
+  using P = MmTraits<DT, OP, MX, BM, BN, WM, WN>;
+  constexpr bool HALF = DT == F16;
+  constexpr int FI = P::FI, FJ = P::FJ;
+  __shared__ __attribute__((aligned(1024))) uint8_t si0[P::IB], si1[P::IB], sj0[P::JB], sj1[P::JB];
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wi = wave / WN, wj = wave % WN;
+  const int64_t jend = OP == LIN_FORWARD ? a.N : a.K;
+  LinTile t;
+  int64_t len;  // of the contraction
+  const uint8_t *ip, *jp;
+  int64_t ibytes, jbytes, istep, jstep;  // bytes of the resources, and per tile of 64
+  int64_t lda = a.lda, ldb;
+  if constexpr (OP == LIN_WEIGHT_GRAD) {
+    const int gm = (int)((a.N + BM - 1) / BM);
+    t.group = blockIdx.y;
+    t.r0 = (int64_t)(blockIdx.x % gm) * BM;
+    t.r1 = a.N;
+    t.j0 = (int64_t)(blockIdx.x / gm) * BN;
+    int64_t b, e;
+    lin_group(a, t.group, b, e);
+    len = e - b;
+    ldb = a.ldb;
+    ip = (const uint8_t*)a.a + (b * lda + t.r0) * 2;
+    jp = (const uint8_t*)a.b + (b * ldb + t.j0) * 2;
+    // (whole pieces of 16 bytes: what a piece holds past the row's end goes to columns that are not stored)
+    ibytes = (((len - 1) * lda + a.N - t.r0) * 2 + 15) & ~(int64_t)15;
+    jbytes = (((len - 1) * ldb + a.K - t.j0) * 2 + 15) & ~(int64_t)15;
+    istep = 128 * lda;
+    jstep = 128 * ldb;
+  } else {
+    if (!lin_pick<BM, BN>(a, jend, t)) return;
+    len = t.group == a.experts ? 0 : (OP == LIN_FORWARD ? a.K : a.N);
+    ip = (const uint8_t*)a.a + t.r0 * lda * 2;
+    ibytes = ((t.r1 - t.r0 - 1) * lda + len) * 2;
+    istep = 128;
+    ldb = a.K;
+    const int64_t first = OP == LIN_FORWARD ? (t.group * a.N + t.j0) * a.K : t.group * a.N * a.K + t.j0;
+    const int64_t count = OP == LIN_FORWARD ? (a.N - t.j0) * a.K : a.N * a.K - t.j0;
+    jp = (const uint8_t*)a.w + (MX ? first >> 1 : first * 2);
+    jbytes = MX ? count >> 1 : count * 2;
+    jstep = OP == LIN_FORWARD ? (MX ? 32 : 128) : 64 * (MX ? a.K >> 1 : a.K * 2);
+  }
+  const int nk = (int)((len + 63) >> 6);
+  v4f32 acc[FI][FJ] = {};
+
+  if (nk > 0) {
+    uint32_t io[P::IL], jo[P::JL];
+    mm_offsets<P::IK, BM, P::IL, P::NW, false>(io, wave, lane, lda);
+    if constexpr (P::JK != KS4) mm_offsets<P::JK, BN, P::JL, P::NW, true>(jo, wave, lane, ldb);
+    // scales of KC4: per fragment column, the byte of block 2 kt + (g >> 1)
+    const uint8_t* sp = MX ? a.scale + t.group * a.scale_stride : nullptr;
+    uint32_t so[P::JK == KC4 ? FJ : 1];
+    uint32_t sv[P::JK == KC4 ? FJ : 1];
+    const int64_t nb = a.K >> 5;
+    if constexpr (P::JK == KC4) {
+#pragma unroll
+      for (int f = 0; f < FJ; ++f) {
+        int64_t n = t.j0 + wj * (FJ * 16) + lin_jcol(f * 16 + (lane & 15));
+        if (n >= a.N) n = a.N - 1;
+        so[f] = a.swizzled ? (uint32_t)((n >> 7) * ((nb + 3) >> 2) * 512 + (n & 31) * 16 + ((n & 127) >> 5) * 4) : (uint32_t)(n * nb);
+      }
+    }
+    // KS4: this thread decodes 32 codes of contraction row kr
+    const int kr = tid / (BN / 32), kc = tid % (BN / 32);
+    lm_u32x4 code = {};
+    uint32_t code_s = 0;
+
+    auto load = [&](int kt, lds_u8* ti, lds_u8* tj) {
+      const __amdgpu_buffer_rsrc_t ri = lin_rsrc(ip + kt * istep, ibytes - kt * istep);
+      const bool cut = (kt + 1) * 64 > len;
+#pragma unroll
+      for (int n = 0; n < P::IL; ++n) {
+        uint32_t o = io[n];
+        if (P::IK == KC16 && cut) {  // chunks past the row's end are zeros, not the next row
+          const int piece = (n * P::NW + wave) * 64 + lane;
+          const int c = (piece & 7) ^ ((piece >> 3) & 7);
+          if (kt * 64 + c * 8 >= len) o = 0x80000000u;
+        }
+        lin_dma(ri, ti + (n * P::NW + wave) * 1024, o);
+      }
+      if constexpr (P::JK != KS4) {
+        const __amdgpu_buffer_rsrc_t rj = lin_rsrc(jp + kt * jstep, jbytes - kt * jstep);
+#pragma unroll
+        for (int n = 0; n < P::JL; ++n) {
+          uint32_t o = jo[n];
+          if (P::JK != KS16 && cut) {
+            const int piece = (n * P::NW + wave) * 64 + lane;
+            const int c = P::JK == KC4 ? (piece & 1) * 4 : (piece & 7) ^ ((piece >> 3) & 7);
+            if (kt * 64 + c * 8 >= len) o = 0x80000000u;
+          }
+          lin_dma(rj, tj + (n * P::NW + wave) * 1024, o);
+        }
+      }
+    };
+    auto load_scales = [&](int kt) {
+      if constexpr (P::JK == KC4) {
+        int64_t kb = 2 * kt + (g >> 1);
+        if (kb >= nb) kb = nb - 1;
+        const uint32_t at = a.swizzled ? (uint32_t)((kb >> 2) * 512 + (kb & 3)) : (uint32_t)kb;
+#pragma unroll
+        for (int f = 0; f < FJ; ++f) sv[f] = sp[so[f] + at];
+      } else if constexpr (P::JK == KS4) {
+        const int64_t n = (int64_t)kt * 64 + kr, k = t.j0 + kc * 32;
+        code = lm_u32x4{};
+        code_s = 0;
+        if (n < len && k < a.K) {
+          code = *(const LM_GLOBAL lm_u32x4*)(jp + n * (a.K >> 1) + kc * 16);
+          code_s = sp[blocked_offset(n, k >> 5, nb, a.swizzled)];
+        }
+      }
+    };
+    auto store_codes = [&](lds_u8* tj) {
+      if constexpr (P::JK == KS4) {
+        const float s = e8m0_value(code_s);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          *(lds_u32x4*)(tj + kr * (BN * 2) + (((kc * 4 + c) ^ ((kr & 3) << 2)) << 4)) = mm_decode<HALF>(code[c], s);
+      }
+    };
+    auto compute = [&](const lds_u8* ti, const lds_u8* tj, const float* scales) {
+      lm_u32x2 jc[P::JK == KC4 ? FJ : 1];
+      if constexpr (P::JK == KC4) {
+#pragma unroll
+        for (int f = 0; f < FJ; ++f)
+          jc[f] = *(const lds_u32x2*)(tj + (wj * (FJ * 16) + f * 16 + (lane & 15)) * 32 + g * 8);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        lm_u32x4 fi[FI], fj[FJ];
+#pragma unroll
+        for (int f = 0; f < FJ; ++f) {
+          if constexpr (P::JK == KC4) fj[f] = mm_decode<HALF>(jc[f][s], scales[f]);
+          else if constexpr (P::JK == KC16) fj[f] = mm_frag<KC16, BN>(tj, wj * (FJ * 16), f, lane, s, P::chunk(s, g));
+          else fj[f] = mm_frag_tr<BN, true>(tj, wj * (FJ * 16), f, lane, s);
+        }
+#pragma unroll
+        for (int f = 0; f < FI; ++f) {
+          if constexpr (P::IK == KC16) fi[f] = mm_frag<KC16, BM>(ti, wi * (FI * 16), f, lane, s, P::chunk(s, g));
+          else fi[f] = mm_frag_tr<BM, false>(ti, wi * (FI * 16), f, lane, s);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int x = 0; x < FI; ++x)
+#pragma unroll
+          for (int y = 0; y < FJ; ++y) acc[x][y] = lin_mfma<HALF>(fj[y], fi[x], acc[x][y]);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    lds_u8 *i0 = (lds_u8*)si0, *i1 = (lds_u8*)si1, *j0 = (lds_u8*)sj0, *j1 = (lds_u8*)sj1;
+    auto scales_now = [&](float(&out)[P::JK == KC4 ? FJ : 1]) {
+      if constexpr (P::JK == KC4) {
+#pragma unroll
+        for (int f = 0; f < FJ; ++f) out[f] = e8m0_value(sv[f]);
+      }
+    };
+    load(0, i0, j0);
+    load_scales(0);
+    store_codes(j0);
+    float sc[P::JK == KC4 ? FJ : 1];
+    int kt = 0;
+    for (; kt + 1 < nk; kt += 2) {  // (no way out of the middle: it would keep two copies of the accumulators)
+      __syncthreads();
+      scales_now(sc);
+      load(kt + 1, i1, j1);
+      load_scales(kt + 1);
+      compute(i0, j0, sc);
+      store_codes(j1);
+      __syncthreads();
+      scales_now(sc);
+      if (kt + 2 < nk) {
+        load(kt + 2, i0, j0);
+        load_scales(kt + 2);
+      }
+      compute(i1, j1, sc);
+      if (kt + 2 < nk) store_codes(j0);
+    }
+    if (kt < nk) {
+      __syncthreads();
+      scales_now(sc);
+      compute(i0, j0, sc);
+    }
+  }
+
+  uint16_t* out = (uint16_t*)a.out + (OP == LIN_WEIGHT_GRAD ? t.group * a.N * a.K : 0);
+#pragma unroll
+  for (int y = 0; y < FJ; y += 2) {
+    const int64_t j = t.j0 + wj * (FJ * 16) + y * 16 + 8 * g;
+    float bias[8] = {};
+    if (OP == LIN_FORWARD && a.bias && t.group < a.experts) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        bias[e] = val_dt<DT>(((const LM_GLOBAL uint16_t*)a.bias)[j + e < jend ? j + e : jend - 1]);
+    }
+#pragma unroll
+    for (int x = 0; x < FI; ++x) {
+      const int64_t i = t.r0 + wi * (FI * 16) + x * 16 + (lane & 15);
+      lm_u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float lo = acc[x][y + (e >> 1)][2 * (e & 1)] + bias[2 * e], hi = acc[x][y + (e >> 1)][2 * (e & 1) + 1] + bias[2 * e + 1];
+        w[e] = DT == F16 ? (uint32_t)f16_bits(lo) | (uint32_t)f16_bits(hi) << 16 : pack_bf16x2(lo, hi);
+      }
+      uint16_t* p = out + i * jend + j;
+      if (i < t.r1) {
+        if (j + 8 <= jend) {
+          *(LM_GLOBAL lm_u32x4_any*)p = w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (j + e < jend) ((LM_GLOBAL uint16_t*)p)[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+        }
+      }
+    }
+  }
+}
