@@ -10,8 +10,12 @@ struct LinArgs {
   int64_t lda;
   const void* b;  // x in the weight gradient: [T, ldb]
   int64_t ldb;
-  const uint8_t* xq;  // x quantised: codes [T, K/2], scales [T, K/32]
+  // 4-bit inputs: codes [64 padded, K/2], scales and the weight's scales packed in
+  // pieces of 64 rows x 256 of K (k_lin_prep4); every group starts on a piece
+  const uint8_t* xq;
   const uint8_t* xs;
+  const uint8_t* wsc;
+  int64_t padded;  // 64-row pieces of xq
   const void* w;  // [experts, N, K] dense or [experts, N, K/2] codes
   const uint8_t* scale;
   int64_t scale_stride;  // bytes of one expert's scales
@@ -69,20 +73,25 @@ DEV void lin_group(const LinArgs& a, int g, int64_t& b, int64_t& e) {
 // Groups are tiled one after the other, BM rows a tile, each from its own first
 // row; group `experts` holds the rows of no group.  Finds tile t: its group
 // and rows [r0, r1), false past the last tile; t < 0 counts the tiles into g.
+// pad: r0 if every group's rows were padded to a multiple of 64.
 template <int BM>
-DEV bool lin_find(const LinArgs& a, int t, int& g, int64_t& r0, int64_t& r1) {
+DEV bool lin_find(const LinArgs& a, int t, int& g, int64_t& r0, int64_t& r1, int64_t& pad) {
   const int lane = threadIdx.x & 63;
-  int before = 0, tiles = 0;
+  int before = 0, tiles = 0, pieces = 0;
   for (int c = 0; c <= a.experts; c += 64) {
     int x = lin_ends64(a, c, before);
     if (c + lane >= a.experts) x = (int)a.T;  // the rows of no group, then empty ones
     int b = __shfl_up(x, 1);
     if (lane == 0) b = before;
-    int n = (x - b + BM - 1) / BM, sum = n;
+    const int n = (x - b + BM - 1) / BM, n64 = (x - b + 63) >> 6;
+    int sum = n, sum64 = n64;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-      const int y = __shfl_up(sum, d);
-      if (lane >= d) sum += y;
+      const int y = __shfl_up(sum, d), z = __shfl_up(sum64, d);
+      if (lane >= d) {
+        sum += y;
+        sum64 += z;
+      }
     }
     const uint64_t hit = __ballot(t >= tiles && t < tiles + sum);
     if (hit) {
@@ -91,28 +100,59 @@ DEV bool lin_find(const LinArgs& a, int t, int& g, int64_t& r0, int64_t& r1) {
       const int first = tiles + __shfl(sum - n, l);
       r0 = __builtin_amdgcn_readfirstlane(__shfl(b, l) + (t - first) * BM);
       r1 = __builtin_amdgcn_readfirstlane(__shfl(x, l));
+      pad = __builtin_amdgcn_readfirstlane((pieces + __shfl(sum64 - n64, l)) * 64 + (t - first) * BM);
       g = __builtin_amdgcn_readfirstlane(g);
       return true;
     }
     before = __shfl(x, 63);
     tiles += __shfl(sum, 63);
+    pieces += __shfl(sum64, 63);
   }
   g = __builtin_amdgcn_readfirstlane(tiles);
   return false;
 }
 template <int BM>
 DEV bool lin_tile(const LinArgs& a, int64_t t, int& g, int64_t& r0, int64_t& r1) {
-  if (a.ends) return lin_find<BM>(a, (int)t, g, r0, r1);
+  int64_t pad;
+  if (a.ends) return lin_find<BM>(a, (int)t, g, r0, r1, pad);
   g = 0;
   r0 = t * BM;
   r1 = a.T;
   return r0 < a.T;
 }
+// Row t: its group, and its place if every group's rows were padded to 64.
+DEV bool lin_row(const LinArgs& a, int t, int& g, int64_t& p) {
+  const int lane = threadIdx.x & 63;
+  int before = 0, pieces = 0;
+  for (int c = 0; c <= a.experts; c += 64) {
+    int x = lin_ends64(a, c, before);
+    if (c + lane >= a.experts) x = (int)a.T;
+    int b = __shfl_up(x, 1);
+    if (lane == 0) b = before;
+    const int n64 = (x - b + 63) >> 6;
+    int sum64 = n64;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int z = __shfl_up(sum64, d);
+      if (lane >= d) sum64 += z;
+    }
+    const uint64_t hit = __ballot(t >= b && t < x);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      g = c + l;
+      p = (pieces + __shfl(sum64 - n64, l)) * 64 + t - __shfl(b, l);
+      return true;
+    }
+    before = __shfl(x, 63);
+    pieces += __shfl(sum64, 63);
+  }
+  return false;
+}
 template <int BM>
 DEV int lin_count(const LinArgs& a) {
   int g;
-  int64_t r0, r1;
-  lin_find<BM>(a, -1, g, r0, r1);
+  int64_t r0, r1, pad;
+  lin_find<BM>(a, -1, g, r0, r1, pad);
   return g;
 }
 // at most this many tiles: every group may end in a part of one
@@ -121,30 +161,25 @@ static inline int64_t lin_tiles(int64_t T, int experts, bool grouped) {
   return (T + BM - 1) / BM + (grouped ? experts : 0);
 }
 
-// 32 values -> 16 bytes of e2m1 codes and the e8m0 scale.  A block with an
-// infinity or a NaN gets the NaN scale, so the rows it feeds come out NaN
-// instead of a finite number.
-DEV uint32_t lin_quant32(const float (&v)[32], uint32_t (&w)[4]) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const uint32_t b = f2u(v[j]) & 0x7fffffffu;
-    top = b > top ? b : top;
+// The e8m0 scale of a block whose largest magnitude has these bits, and its
+// inverse.  A block with an infinity or a NaN gets the NaN scale, so the rows it
+// feeds come out NaN instead of a finite number.
+DEV uint32_t lin_scale4(uint32_t top, float& inv) {
+  if (top >= 0x7f800000u) {
+    inv = 0.0f;
+    return 255u;
   }
-  float inv;
-  const uint32_t s = top >= 0x7f800000u ? 255u : mx_scale(u2f(top), MX_FLOOR, 2, 6.0f, 1, inv);
-  if (s == 255u) inv = 0.0f;
+  return mx_scale(u2f(top), MX_FLOOR, 2, 6.0f, 1, inv);
+}
+DEV uint32_t lin_codes8(const float (&v)[8], float inv) {
+  uint32_t w = 0;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    w[k] = 0;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const float lo = __builtin_amdgcn_fmed3f(v[8 * k + 2 * t] * inv, -6.0f, 6.0f);
-      const float hi = __builtin_amdgcn_fmed3f(v[8 * k + 2 * t + 1] * inv, -6.0f, 6.0f);
-      w[k] |= e2m1_pack2(lo, hi) << (8 * t);
-    }
+  for (int t = 0; t < 4; ++t) {
+    const float lo = __builtin_amdgcn_fmed3f(v[2 * t] * inv, -6.0f, 6.0f);
+    const float hi = __builtin_amdgcn_fmed3f(v[2 * t + 1] * inv, -6.0f, 6.0f);
+    w |= e2m1_pack2(lo, hi) << (8 * t);
   }
-  return s;
+  return w;
 }
 
 template <bool HALF>

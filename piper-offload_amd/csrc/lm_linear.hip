@@ -12,39 +12,86 @@
 #include "lm_linear_mm.h"
 
 // ---------------------------------------------------------------------------
-// x quantised to MXFP4: blocks of 32 along K, scale 2^(floor(log2 max) - 2)
+// 4-bit inputs: x quantised to MXFP4 (blocks of 32 along K, scale
+// 2^(floor(log2 max) - 2)), and its scales and the weight's in the order the
+// scaled MFMA takes them.  One launch: the first workgroups take a row of x per
+// wave (8 values a lane: 16 bytes in, 4 out, a block's maximum over 4 lanes
+// by DPP), the others one packed piece of weight scales per wave.
 // ---------------------------------------------------------------------------
+// byte of (slot, block) in the packed scales: pieces of 64 slots x 8 blocks
+DEV int64_t lin_packed(int64_t slot, int64_t block, int64_t nk) {
+  const int f = (int)(slot >> 4) & 3, r = (int)slot & 15, g = (int)(block & 7) >> 1;
+  return ((slot >> 6) * nk + (block >> 3)) * 512 + (16 * g + r) * 8 + 2 * f + (block & 1);
+}
 template <int DT>
-__global__ __launch_bounds__(256) void k_lin_quant(const uint16_t* x, int64_t ldx, int64_t T, int64_t K, uint8_t* q,
-                                                   uint8_t* s) {
-  const int64_t nb = K >> 5, total = T * nb;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t t = i / nb, b = i - t * nb;
-    const uint16_t* p = x + t * ldx + b * 32;
-    float v[32];
+__global__ __launch_bounds__(256) void k_lin_prep4(LinArgs a, int row_blocks, uint8_t* xq, uint8_t* xs, uint8_t* wsc) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t nk = (a.K + 255) >> 8, nb = a.K >> 5;
+  if ((int)blockIdx.x < row_blocks) {
+    const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+    if (t >= a.T) return;
+    int64_t p = t;
+    if (a.ends) {
+      int g;
+      if (!lin_row(a, (int)t, g, p) || g == a.experts) return;  // a row of no group
+    }
+    const uint16_t* x = (const uint16_t*)a.a + t * a.lda;
+    const int64_t units = a.K >> 3, padded = nk * 32;
+    for (int64_t u = lane; u < padded; u += 64) {
+      float v[8] = {};
+      if (u < units) {
+        const lm_u32x4 w = *(const LM_GLOBAL lm_u32x4_any*)(x + u * 8);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = val_dt<DT>(p[j]);
-    uint32_t w[4];
-    s[i] = (uint8_t)lin_quant32(v, w);
+        for (int j = 0; j < 8; ++j) v[j] = val_dt<DT>(j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu);
+      }
+      uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ((uint32_t*)(q + i * 16))[j] = w[j];
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t b = f2u(v[j]) & 0x7fffffffu;
+        top = b > top ? b : top;
+      }
+#pragma unroll
+      for (int d = 1; d <= 2; ++d) {
+        const uint32_t o = (uint32_t)(d == 1 ? __builtin_amdgcn_update_dpp((int)top, (int)top, 0xB1, 0xf, 0xf, false)
+                                             : __builtin_amdgcn_update_dpp((int)top, (int)top, 0x4E, 0xf, 0xf, false));
+        top = o > top ? o : top;
+      }
+      float inv;
+      const uint32_t s = lin_scale4(top, inv);
+      const uint32_t w = lin_codes8(v, inv);
+      if (u < units) *(LM_GLOBAL uint32_t*)(xq + p * (a.K >> 1) + u * 4) = w;
+      // (blocks past K are zeros with the smallest scale)
+      if ((lane & 3) == 0) *(LM_GLOBAL uint8_t*)(xs + lin_packed(p, u >> 2, nk)) = (uint8_t)(u < units ? s : 0);
+    }
+  } else {
+    const int64_t gj = (a.N + 63) >> 6, piece = (int64_t)(blockIdx.x - row_blocks) * 4 + wave;
+    if (piece >= gj * nk * a.experts) return;
+    const int64_t kt = piece % nk, eg = piece / nk, e = eg / gj, n0 = (eg % gj) * 64;
+    const int g = lane >> 4;
+    uint16_t s[4];
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+      const int64_t n = n0 + lin_jcol(16 * f + (lane & 15));
+      s[f] = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t b = kt * 8 + 2 * g + h;
+        if (n < a.N && b < nb) s[f] |= (uint16_t)(a.scale[e * a.scale_stride + blocked_offset(n, b, nb, a.swizzled)] << (8 * h));
+      }
+    }
+    *(LM_GLOBAL lm_u32x2*)(wsc + piece * 512 + lane * 8) = lm_u32x2{s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16};
   }
 }
 
 // ---------------------------------------------------------------------------
 // the general product: any sizes, strides and alignment, 64 x 64 tiles
 // ---------------------------------------------------------------------------
-template <int DT, bool MX, bool QUANT>
+template <int DT, bool MX>
 struct LinOps {
-  static constexpr bool HALF = DT == F16 && !QUANT;  // operands in fp16; quantised ones are exact in bf16
+  static constexpr bool HALF = DT == F16;
   DEV static uint16_t bits(float v) { return HALF ? f16_bits(v) : bf16_bits(v); }
   DEV static uint16_t act(const LinArgs& a, int64_t m, int64_t c) {
-    if constexpr (QUANT) {
-      const uint32_t code = a.xq[m * (a.K >> 1) + (c >> 1)] >> (4 * (c & 1));
-      return bits(e2m1_value(code) * e8m0_value(a.xs[m * (a.K >> 5) + (c >> 5)]));
-    } else {
-      return ((const uint16_t*)a.a)[m * a.lda + c];
-    }
+    return ((const uint16_t*)a.a)[m * a.lda + c];
   }
   DEV static uint16_t weight(const LinArgs& a, int64_t e, int64_t n, int64_t k) {
     if constexpr (MX) {
@@ -57,9 +104,9 @@ struct LinOps {
   }
 };
 
-template <int DT, bool MX, bool QUANT, int OP>
+template <int DT, bool MX, int OP>
 __global__ __launch_bounds__(256) void k_lin_general(LinArgs a) {
-  using O = LinOps<DT, MX, QUANT>;
+  using O = LinOps<DT, MX>;
   __shared__ __attribute__((aligned(16))) uint16_t la[64 * 40], lb[64 * 40];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int64_t e, m0, m1, i0, iend, c0 = 0, cend;
@@ -129,6 +176,7 @@ static int check_lin(const lm_weight* w, int64_t T, int32_t dtype, const int32_t
   if (!w) return LM_OK;
   if (!w->q) return fail(LM_EINVAL, "weight pointer must be non-null");
   if (w->N <= 0 || w->K <= 0) return fail(LM_EINVAL, "empty weight");
+  if (w->N >= (1 << 22) || w->K >= (1 << 22)) return fail(LM_EUNSUPPORTED, "products take rows and columns below 2^22");
   if (w->dtype == LM_E2M1) {
     if (!w->scale) return fail(LM_EINVAL, "MXFP4 weight without scales");
     if (w->K % 32 != 0) return fail(LM_EINVAL, "MXFP4 requires columns divisible by 32, got %lld", (long long)w->K);
@@ -153,26 +201,30 @@ static LinArgs lin_args(const lm_weight* w, const int32_t* ends, int64_t T) {
   return a;
 }
 
+// workspace of 4-bit inputs; padded: 64-row pieces that the rows of T rows in
+// `experts` groups can fill
 struct LinWs {
-  size_t xq, xs, total;
+  int64_t padded;
+  size_t xs, wsc, total;
 };
-static LinWs lin_ws(int64_t T, int64_t K, bool quant) {
-  LinWs w{0, 0, 0};
-  if (quant) {
-    w.xs = align256((size_t)T * (size_t)(K / 2));
-    w.total = w.xs + align256((size_t)T * (size_t)(K / 32));
-  }
+static LinWs lin_ws(int64_t T, int64_t N, int64_t K, int64_t experts, bool grouped) {
+  LinWs w;
+  const int64_t nk = (K + 255) / 256;
+  w.padded = (T + 63) / 64 + (grouped ? experts : 0);
+  w.xs = align256((size_t)(w.padded * 64) * (size_t)(K / 2));
+  w.wsc = w.xs + (size_t)(w.padded * nk) * 512;
+  w.total = w.wsc + (size_t)(experts * ((N + 63) / 64) * nk) * 512;
   return w;
 }
 
-template <int DT, bool MX, bool QUANT, int OP>
+template <int DT, bool MX, int OP>
 static int run_general(const LinArgs& a, hipStream_t st) {
   TimedLaunch timed("linear", st);
   const int64_t J = OP == LIN_FORWARD ? a.N : a.K;
   const int64_t gx = (J + 63) / 64;
   const int64_t gy = OP == LIN_WEIGHT_GRAD ? (a.N + 63) / 64 : lin_tiles<64>(a.T, a.experts, a.ends != nullptr);
   if (gx > 0x7fffffff || gy > 65535) return fail(LM_EUNSUPPORTED, "product too large for one launch");
-  hipLaunchKernelGGL((k_lin_general<DT, MX, QUANT, OP>), dim3((unsigned)gx, (unsigned)gy, OP == LIN_WEIGHT_GRAD ? a.experts : 1),
+  hipLaunchKernelGGL((k_lin_general<DT, MX, OP>), dim3((unsigned)gx, (unsigned)gy, OP == LIN_WEIGHT_GRAD ? a.experts : 1),
                      dim3(256), 0, st, a);
   LAUNCH_CHECK();
   return LM_OK;
@@ -181,13 +233,13 @@ static int run_general(const LinArgs& a, hipStream_t st) {
 // 2^31, fewer tiles than a grid holds.
 static bool mm_ok(const LinArgs& a, int op, bool mx) {
   const int64_t len = op == LIN_FORWARD ? a.K : a.N;
-  if (a.lda % 8 || ((uintptr_t)a.a & 15) || a.lda >= (1 << 22) || a.K >= (1 << 22) || a.N >= (1 << 22)) return false;
+  if (a.lda % 8 || ((uintptr_t)a.a & 15) || a.lda >= (1 << 22)) return false;
   if (op == LIN_WEIGHT_GRAD) return a.ldb % 8 == 0 && ((uintptr_t)a.b & 15) == 0 && a.ldb < (1 << 22);
   if (len % 8) return false;
   return mx || (a.K % 8 == 0 && ((uintptr_t)a.w & 15) == 0);
 }
 
-template <int DT, int OP, bool MX, int B, int WM, int WN>
+template <int DT, int OP, int MX, int B, int WM, int WN>
 static int launch_mm(const LinArgs& a, hipStream_t st) {
   TimedLaunch timed("linear", st);
   const int64_t J = OP == LIN_FORWARD ? a.N : a.K, gj = (J + B - 1) / B;
@@ -198,7 +250,7 @@ static int launch_mm(const LinArgs& a, hipStream_t st) {
   LAUNCH_CHECK();
   return LM_OK;
 }
-template <int OP, bool MX>
+template <int OP, int MX>
 static int run_mm(const LinArgs& a, int dtype, hipStream_t st) {
   const int64_t J = OP == LIN_FORWARD ? a.N : a.K, I = OP == LIN_WEIGHT_GRAD ? a.N : a.T;
   const int64_t big = I / 256 * ((J + 255) / 256) * (OP == LIN_WEIGHT_GRAD ? a.experts : 1);
@@ -209,27 +261,22 @@ static int run_mm(const LinArgs& a, int dtype, hipStream_t st) {
 }
 
 template <int OP>
-static int run_product(const LinArgs& a, int dtype, bool mx, bool quant, hipStream_t st) {
-  if (!quant && mm_ok(a, OP, mx)) {
+static int run_product(const LinArgs& a, int dtype, bool mx, hipStream_t st) {
+  if (mm_ok(a, OP, mx)) {
     if constexpr (OP != LIN_WEIGHT_GRAD) {
-      if (mx) return run_mm<OP, true>(a, dtype, st);
+      if (mx) return run_mm<OP, W_MX>(a, dtype, st);
     }
-    return run_mm<OP, false>(a, dtype, st);
-  }
-  if constexpr (OP == LIN_FORWARD) {
-    if (quant) return dtype == LM_F16 ? run_general<F16, true, true, OP>(a, st) : run_general<BF16, true, true, OP>(a, st);
+    return run_mm<OP, W_DENSE>(a, dtype, st);
   }
   if constexpr (OP != LIN_WEIGHT_GRAD) {
-    if (mx) return dtype == LM_F16 ? run_general<F16, true, false, OP>(a, st) : run_general<BF16, true, false, OP>(a, st);
+    if (mx) return dtype == LM_F16 ? run_general<F16, true, OP>(a, st) : run_general<BF16, true, OP>(a, st);
   }
-  return dtype == LM_F16 ? run_general<F16, false, false, OP>(a, st) : run_general<BF16, false, false, OP>(a, st);
+  return dtype == LM_F16 ? run_general<F16, false, OP>(a, st) : run_general<BF16, false, OP>(a, st);
 }
 
 extern "C" size_t lm_linear_workspace_size(int64_t T, int64_t N, int64_t K, int32_t experts, int32_t input_dtype) {
-  (void)N;
-  (void)experts;
-  if (T <= 0 || K <= 0) return 0;
-  return lin_ws(T, K, input_dtype == LM_E2M1).total;
+  if (T <= 0 || N <= 0 || K <= 0 || experts <= 0 || input_dtype != LM_E2M1) return 0;
+  return lin_ws(T, N, K, experts, true).total;
 }
 
 extern "C" int lm_linear(const void* x, int64_t ldx, const lm_weight* w, const void* bias, const int32_t* ends, void* y,
@@ -250,22 +297,26 @@ extern "C" int lm_linear(const void* x, int64_t ldx, const lm_weight* w, const v
   a.lda = ldx;
   a.bias = bias;
   a.out = y;
-  if (quant) {
-    const LinWs ws = lin_ws(T, a.K, true);
-    if (!workspace || workspace_bytes < ws.total)
-      return fail(LM_EWORKSPACE, "workspace too small: %zu < %zu bytes", workspace ? workspace_bytes : 0, ws.total);
-    if (((uintptr_t)workspace & 255) != 0) return fail(LM_EINVAL, "workspace must be 256-byte aligned");
-    uint8_t* q = (uint8_t*)workspace + ws.xq;
-    uint8_t* s = (uint8_t*)workspace + ws.xs;
-    a.xq = q;
-    a.xs = s;
-    const int64_t nb = (T * (a.K / 32) + 255) / 256;
-    const dim3 grid((unsigned)(nb < 65536 ? nb : 65536));
-    if (dtype == LM_F16) hipLaunchKernelGGL((k_lin_quant<F16>), grid, dim3(256), 0, st, (const uint16_t*)x, ldx, T, a.K, q, s);
-    else hipLaunchKernelGGL((k_lin_quant<BF16>), grid, dim3(256), 0, st, (const uint16_t*)x, ldx, T, a.K, q, s);
+  if (!quant) return run_product<LIN_FORWARD>(a, dtype, mx, st);
+  const LinWs ws = lin_ws(T, a.N, a.K, a.experts, ends != nullptr);
+  if (!workspace || workspace_bytes < ws.total)
+    return fail(LM_EWORKSPACE, "workspace too small: %zu < %zu bytes", workspace ? workspace_bytes : 0, ws.total);
+  if (((uintptr_t)workspace & 255) != 0) return fail(LM_EINVAL, "workspace must be 256-byte aligned");
+  uint8_t* base = (uint8_t*)workspace;
+  a.xq = base;
+  a.xs = base + ws.xs;
+  a.wsc = base + ws.wsc;
+  a.padded = ws.padded;
+  {
+    TimedLaunch timed("linear_prep", st);
+    const int64_t rows = (T + 3) / 4, pieces = (a.experts * ((a.N + 63) / 64) * ((a.K + 255) / 256) + 3) / 4;
+    if (rows + pieces > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+    const dim3 grid((unsigned)(rows + pieces));
+    if (dtype == LM_F16) hipLaunchKernelGGL((k_lin_prep4<F16>), grid, dim3(256), 0, st, a, (int)rows, base, base + ws.xs, base + ws.wsc);
+    else hipLaunchKernelGGL((k_lin_prep4<BF16>), grid, dim3(256), 0, st, a, (int)rows, base, base + ws.xs, base + ws.wsc);
     LAUNCH_CHECK();
   }
-  return run_product<LIN_FORWARD>(a, dtype, mx, quant, st);
+  return run_mm<LIN_FORWARD, W_Q4>(a, dtype, st);
 }
 
 extern "C" int lm_linear_input_grad(const void* dy, int64_t lddy, const lm_weight* w, const int32_t* ends, void* dx,
@@ -280,7 +331,7 @@ extern "C" int lm_linear_input_grad(const void* dy, int64_t lddy, const lm_weigh
   a.a = dy;
   a.lda = lddy;
   a.out = dx;
-  return run_product<LIN_INPUT_GRAD>(a, dtype, w->dtype == LM_E2M1, false, (hipStream_t)stream);
+  return run_product<LIN_INPUT_GRAD>(a, dtype, w->dtype == LM_E2M1, (hipStream_t)stream);
 }
 
 extern "C" int lm_linear_weight_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int32_t* ends,
@@ -289,6 +340,7 @@ extern "C" int lm_linear_weight_grad(const void* dy, int64_t lddy, const void* x
   int rc;
   if ((rc = check_lin(nullptr, T, dtype, ends, experts))) return rc;
   if (N <= 0 || K <= 0) return fail(LM_EINVAL, "empty weight gradient");
+  if (N >= (1 << 22) || K >= (1 << 22)) return fail(LM_EUNSUPPORTED, "products take rows and columns below 2^22");
   if (!dw || (T > 0 && (!dy || !x))) return fail(LM_EINVAL, "pointers must be non-null");
   if (lddy < N || ldx < K) return fail(LM_EINVAL, "row stride below the row length");
   LinArgs a{};
@@ -302,5 +354,5 @@ extern "C" int lm_linear_weight_grad(const void* dy, int64_t lddy, const void* x
   a.T = T;
   a.N = N;
   a.K = K;
-  return run_product<LIN_WEIGHT_GRAD>(a, dtype, false, false, (hipStream_t)stream);
+  return run_product<LIN_WEIGHT_GRAD>(a, dtype, false, (hipStream_t)stream);
 }

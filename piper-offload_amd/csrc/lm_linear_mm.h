@@ -18,6 +18,11 @@
 //   KS4   MXFP4 with the contraction strided: every code of a run of 32 shares a
 //         scale but the 8 codes of an MFMA lane do not, so these are decoded on
 //         their way into LDS and then are KS16
+// Q4: both operands MXFP4 (x quantised beforehand), multiplied as they are by the
+// scaled MFMA, 256 codes a tile, so a slot is 128 bytes here too.  Its scales
+// come packed by k_lin_prep4: per 64 slots and tile 512 bytes, which hold for
+// lane (r, g) the blocks 2g and 2g + 1 of slots r, r + 16, r + 32, r + 48 side by
+// side: one 8-byte read gives the scales of four fragments and both steps.
 // The MFMA's first operand is J, so a lane's accumulators are consecutive output
 // columns; the columns of a pair of 16-column fragments are interleaved in
 // fours, which makes them 8 in a row: one 16-byte store.
@@ -54,6 +59,7 @@ DEV int lin_jcol(int slot) { return (slot & ~31) + 8 * ((slot & 15) >> 2) + (slo
 struct LinTile {
   int group;
   int64_t r0, r1, j0;
+  int64_t pad;  // the first row among the rows padded to 64 a group
 };
 template <int BM, int BN>
 DEV bool lin_pick(const LinArgs& a, int64_t jend, LinTile& t) {
@@ -71,15 +77,40 @@ DEV bool lin_pick(const LinArgs& a, int64_t jend, LinTile& t) {
   t.j0 = (int64_t)tn * BN;
   if (!a.ends) {
     t.group = 0;
-    t.r0 = (int64_t)tm * BM;
+    t.pad = t.r0 = (int64_t)tm * BM;
     t.r1 = a.T;
     return true;
   }
-  return lin_find<BM>(a, (int)tm, t.group, t.r0, t.r1);
+  return lin_find<BM>(a, (int)tm, t.group, t.r0, t.r1, t.pad);
 }
 
-template <int DT, int OP, bool MX, int BM, int BN, int WM, int WN>
+enum : int { W_DENSE = 0, W_MX = 1, W_Q4 = 2 };
+
+template <int S, int F, int G>
+DEV v4f32 lin_mfma4_(lm_u32x4 a, lm_u32x4 b, v4f32 c, uint32_t sa, uint32_t sb) {
+  typedef int v8i32 __attribute__((ext_vector_type(8)));
+  const v8i32 x = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}, y = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, 2 * F + S, (int)sa, 2 * G + S, (int)sb);
+}
+// step s; f, g: which of a word's two fragments the scales belong to
+DEV v4f32 lin_mfma4(lm_u32x4 a, lm_u32x4 b, v4f32 c, uint32_t sa, uint32_t sb, int s, int f, int g) {
+  switch (4 * s + 2 * f + g) {
+    case 0: return lin_mfma4_<0, 0, 0>(a, b, c, sa, sb);
+    case 1: return lin_mfma4_<0, 0, 1>(a, b, c, sa, sb);
+    case 2: return lin_mfma4_<0, 1, 0>(a, b, c, sa, sb);
+    case 3: return lin_mfma4_<0, 1, 1>(a, b, c, sa, sb);
+    case 4: return lin_mfma4_<1, 0, 0>(a, b, c, sa, sb);
+    case 5: return lin_mfma4_<1, 0, 1>(a, b, c, sa, sb);
+    case 6: return lin_mfma4_<1, 1, 0>(a, b, c, sa, sb);
+    default: return lin_mfma4_<1, 1, 1>(a, b, c, sa, sb);
+  }
+}
+
+template <int DT, int OP, int W, int BM, int BN, int WM, int WN>
 struct MmTraits {
+  static constexpr bool Q4 = W == W_Q4, MX = W == W_MX;
+  static constexpr int CT = Q4 ? 256 : 64;                        // contraction of a tile
+  static constexpr int IS = Q4 ? BM * 8 : 16, JS = Q4 ? BN * 8 : 16;  // bytes of the scales of a tile
   static constexpr int NW = WM * WN, NT = NW * 64;
   static constexpr int IK = OP == LIN_WEIGHT_GRAD ? KS16 : KC16;
   static constexpr int JK = OP == LIN_FORWARD ? (MX ? KC4 : KC16) : (OP == LIN_INPUT_GRAD && MX ? KS4 : KS16);
@@ -89,8 +120,9 @@ struct MmTraits {
   static_assert(IL * 1024 * NW == IB && JL * 1024 * NW == JB, "tiles are whole loads of all waves");
   static_assert(JK != KS4 || NT * 32 == 64 * BN, "a run of 32 codes per thread");
   // chunk c of contraction 8-groups that lane group g takes in MFMA step s: with
-  // KC4 a lane reads the codes of both steps at once, so they are neighbours
-  DEV static int chunk(int s, int g) { return JK == KC4 ? 2 * g + s : 4 * s + g; }
+  // KC4 a lane reads the codes of both steps at once, with Q4 their scales, so they
+  // are neighbours
+  DEV static int chunk(int s, int g) { return JK == KC4 || Q4 ? 2 * g + s : 4 * s + g; }
 };
 
 // per-lane byte offsets of the DMA loads of one operand tile
@@ -153,12 +185,14 @@ DEV lm_u32x4 mm_decode(uint32_t codes, float scale) {
   return v;
 }
 
-template <int DT, int OP, bool MX, int BM, int BN, int WM, int WN>
+template <int DT, int OP, int W, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
-  using P = MmTraits<DT, OP, MX, BM, BN, WM, WN>;
-  constexpr bool HALF = DT == F16;
+  using P = MmTraits<DT, OP, W, BM, BN, WM, WN>;
+  constexpr bool HALF = DT == F16, Q4 = P::Q4, MX = P::MX;
+  constexpr int CT = P::CT;
   constexpr int FI = P::FI, FJ = P::FJ;
   __shared__ __attribute__((aligned(1024))) uint8_t si0[P::IB], si1[P::IB], sj0[P::JB], sj1[P::JB];
+  __shared__ __attribute__((aligned(1024))) uint8_t sis0[P::IS], sis1[P::IS], sjs0[P::JS], sjs1[P::JS];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wi = wave / WN, wj = wave % WN;
@@ -188,17 +222,24 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
   } else {
     if (!lin_pick<BM, BN>(a, jend, t)) return;
     len = t.group == a.experts ? 0 : (OP == LIN_FORWARD ? a.K : a.N);
-    ip = (const uint8_t*)a.a + t.r0 * lda * 2;
-    ibytes = ((t.r1 - t.r0 - 1) * lda + len) * 2;
+    if constexpr (Q4) {
+      lda = a.K >> 2;  // two codes a byte, in units of two bytes as the others
+      ip = a.xq + t.pad * (a.K >> 1);
+      ibytes = (t.r1 - t.r0) * (a.K >> 1);
+    } else {
+      ip = (const uint8_t*)a.a + t.r0 * lda * 2;
+      ibytes = ((t.r1 - t.r0 - 1) * lda + len) * 2;
+    }
     istep = 128;
-    ldb = a.K;
+    ldb = Q4 ? a.K >> 2 : a.K;
+    constexpr bool MX = P::MX || Q4;
     const int64_t first = OP == LIN_FORWARD ? (t.group * a.N + t.j0) * a.K : t.group * a.N * a.K + t.j0;
     const int64_t count = OP == LIN_FORWARD ? (a.N - t.j0) * a.K : a.N * a.K - t.j0;
     jp = (const uint8_t*)a.w + (MX ? first >> 1 : first * 2);
     jbytes = MX ? count >> 1 : count * 2;
-    jstep = OP == LIN_FORWARD ? (MX ? 32 : 128) : 64 * (MX ? a.K >> 1 : a.K * 2);
+    jstep = OP == LIN_FORWARD ? (P::MX ? 32 : 128) : 64 * (MX ? a.K >> 1 : a.K * 2);
   }
-  const int nk = (int)((len + 63) >> 6);
+  const int nk = (int)((len + CT - 1) / CT);
   v4f32 acc[FI][FJ] = {};
 
   if (nk > 0) {
@@ -218,21 +259,32 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
         so[f] = a.swizzled ? (uint32_t)((n >> 7) * ((nb + 3) >> 2) * 512 + (n & 31) * 16 + ((n & 127) >> 5) * 4) : (uint32_t)(n * nb);
       }
     }
+    // Q4: packed scales of this tile's 64-slot groups, nk pieces each
+    const uint8_t *isp = nullptr, *jsp = nullptr;
+    int64_t isbytes = 0, jsbytes = 0;
+    if constexpr (Q4) {
+      const int64_t gj = (a.N + 63) >> 6;
+      isp = a.xs + (t.pad >> 6) * nk * 512;
+      isbytes = (a.padded - (t.pad >> 6)) * nk * 512;
+      jsp = a.wsc + (t.group * gj + (t.j0 >> 6)) * nk * 512;
+      jsbytes = (gj - (t.j0 >> 6)) * nk * 512;
+    }
     // KS4: this thread decodes 32 codes of contraction row kr
     const int kr = tid / (BN / 32), kc = tid % (BN / 32);
     lm_u32x4 code = {};
     uint32_t code_s = 0;
 
-    auto load = [&](int kt, lds_u8* ti, lds_u8* tj) {
+    auto load = [&](int kt, lds_u8* ti, lds_u8* tj, lds_u8* tis, lds_u8* tjs) {
       const __amdgpu_buffer_rsrc_t ri = lin_rsrc(ip + kt * istep, ibytes - kt * istep);
-      const bool cut = (kt + 1) * 64 > len;
+      const bool cut = (kt + 1) * CT > len;
+      constexpr int PIECE = CT / 8;  // of the contraction in a 16-byte piece of KC16
 #pragma unroll
       for (int n = 0; n < P::IL; ++n) {
         uint32_t o = io[n];
         if (P::IK == KC16 && cut) {  // chunks past the row's end are zeros, not the next row
           const int piece = (n * P::NW + wave) * 64 + lane;
           const int c = (piece & 7) ^ ((piece >> 3) & 7);
-          if (kt * 64 + c * 8 >= len) o = 0x80000000u;
+          if (kt * CT + c * PIECE >= len) o = 0x80000000u;
         }
         lin_dma(ri, ti + (n * P::NW + wave) * 1024, o);
       }
@@ -244,10 +296,15 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
           if (P::JK != KS16 && cut) {
             const int piece = (n * P::NW + wave) * 64 + lane;
             const int c = P::JK == KC4 ? (piece & 1) * 4 : (piece & 7) ^ ((piece >> 3) & 7);
-            if (kt * 64 + c * 8 >= len) o = 0x80000000u;
+            if (kt * CT + c * PIECE >= len) o = 0x80000000u;
           }
           lin_dma(rj, tj + (n * P::NW + wave) * 1024, o);
         }
+      }
+      if constexpr (Q4) {  // 512 bytes per 64 slots: 128 slots a load, a wave each
+        const int h = wave < BM / 128 ? wave : wave - BM / 128;
+        if (wave < BM / 128) lin_dma(lin_rsrc(isp, isbytes), tis + h * 1024, ((2 * h + (lane >> 5)) * nk + kt) * 512 + (lane & 31) * 16);
+        else if (wave < BM / 128 + BN / 128) lin_dma(lin_rsrc(jsp, jsbytes), tjs + h * 1024, ((2 * h + (lane >> 5)) * nk + kt) * 512 + (lane & 31) * 16);
       }
     };
     auto load_scales = [&](int kt) {
@@ -275,7 +332,14 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
           *(lds_u32x4*)(tj + kr * (BN * 2) + (((kc * 4 + c) ^ ((kr & 3) << 2)) << 4)) = mm_decode<HALF>(code[c], s);
       }
     };
-    auto compute = [&](const lds_u8* ti, const lds_u8* tj, const float* scales) {
+    auto compute = [&](const lds_u8* ti, const lds_u8* tj, const lds_u8* tis, const lds_u8* tjs, const float* scales) {
+      lm_u32x2 isc[Q4 ? FI / 4 : 1], jsc[Q4 ? FJ / 4 : 1];
+      if constexpr (Q4) {
+#pragma unroll
+        for (int f = 0; f < FI / 4; ++f) isc[f] = *(const lds_u32x2*)(tis + (wi * (FI / 4) + f) * 512 + lane * 8);
+#pragma unroll
+        for (int f = 0; f < FJ / 4; ++f) jsc[f] = *(const lds_u32x2*)(tjs + (wj * (FJ / 4) + f) * 512 + lane * 8);
+      }
       lm_u32x2 jc[P::JK == KC4 ? FJ : 1];
       if constexpr (P::JK == KC4) {
 #pragma unroll
@@ -301,19 +365,23 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
 #pragma unroll
         for (int x = 0; x < FI; ++x)
 #pragma unroll
-          for (int y = 0; y < FJ; ++y) acc[x][y] = lin_mfma<HALF>(fj[y], fi[x], acc[x][y]);
+          for (int y = 0; y < FJ; ++y) {
+            if constexpr (Q4) acc[x][y] = lin_mfma4(fj[y], fi[x], acc[x][y], jsc[y >> 2][(y >> 1) & 1], isc[x >> 2][(x >> 1) & 1], s, y & 1, x & 1);
+            else acc[x][y] = lin_mfma<HALF>(fj[y], fi[x], acc[x][y]);
+          }
         __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
       }
     };
     lds_u8 *i0 = (lds_u8*)si0, *i1 = (lds_u8*)si1, *j0 = (lds_u8*)sj0, *j1 = (lds_u8*)sj1;
+    lds_u8 *is0 = (lds_u8*)sis0, *is1 = (lds_u8*)sis1, *js0 = (lds_u8*)sjs0, *js1 = (lds_u8*)sjs1;
     auto scales_now = [&](float(&out)[P::JK == KC4 ? FJ : 1]) {
       if constexpr (P::JK == KC4) {
 #pragma unroll
         for (int f = 0; f < FJ; ++f) out[f] = e8m0_value(sv[f]);
       }
     };
-    load(0, i0, j0);
+    load(0, i0, j0, is0, js0);
     load_scales(0);
     store_codes(j0);
     float sc[P::JK == KC4 ? FJ : 1];
@@ -321,23 +389,23 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
     for (; kt + 1 < nk; kt += 2) {  // (no way out of the middle: it would keep two copies of the accumulators)
       __syncthreads();
       scales_now(sc);
-      load(kt + 1, i1, j1);
+      load(kt + 1, i1, j1, is1, js1);
       load_scales(kt + 1);
-      compute(i0, j0, sc);
+      compute(i0, j0, is0, js0, sc);
       store_codes(j1);
       __syncthreads();
       scales_now(sc);
       if (kt + 2 < nk) {
-        load(kt + 2, i0, j0);
+        load(kt + 2, i0, j0, is0, js0);
         load_scales(kt + 2);
       }
-      compute(i1, j1, sc);
+      compute(i1, j1, is1, js1, sc);
       if (kt + 2 < nk) store_codes(j0);
     }
     if (kt < nk) {
       __syncthreads();
       scales_now(sc);
-      compute(i0, j0, sc);
+      compute(i0, j0, is0, js0, sc);
     }
   }
 
