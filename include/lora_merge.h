@@ -278,8 +278,11 @@ int lm_routed_residual(const void* x, const void* y, void* out, int64_t T, int64
  * first, as lm_mx_requant with LM_MX_FLOOR does; a block with an infinity or a
  * NaN makes its row NaN.  The input gradient passes straight through that
  * rounding.
- * Strides are in elements; outputs are contiguous.  Workspace:
- * lm_linear_workspace_size bytes, 256-byte aligned; NULL when that is 0. */
+ * Strides are in elements; outputs are contiguous; N, K < 2^22.  Workspace:
+ * lm_linear_workspace_size bytes for the call's sizes and strides (ldb: ldx of
+ * the weight gradient, else 0; aligned: the pointers of rows and weights are
+ * multiples of 16), 256-byte aligned; NULL when that is 0. */
+enum lm_linear_op { LM_LINEAR_FORWARD = 0, LM_LINEAR_INPUT_GRAD = 1, LM_LINEAR_WEIGHT_GRAD = 2 };
 #define LM_LINEAR_MAX_EXPERTS 1024
 typedef struct lm_weight {
   const void* q;
@@ -291,13 +294,15 @@ typedef struct lm_weight {
   int32_t experts;
   int32_t reserved;
 } lm_weight;
-size_t lm_linear_workspace_size(int64_t T, int64_t N, int64_t K, int32_t experts, int32_t input_dtype);
+size_t lm_linear_workspace_size(int32_t op, int64_t T, int64_t lda, int64_t ldb, int64_t N, int64_t K, int32_t experts,
+                                int32_t weight_dtype, int32_t input_dtype, int32_t aligned);
 int lm_linear(const void* x, int64_t ldx, const lm_weight* w, const void* bias, const int32_t* ends, void* y, int64_t T,
               int32_t dtype, int32_t input_dtype, void* workspace, size_t workspace_bytes, void* stream);
 int lm_linear_input_grad(const void* dy, int64_t lddy, const lm_weight* w, const int32_t* ends, void* dx, int64_t T,
-                         int32_t dtype, void* stream);
+                         int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
 int lm_linear_weight_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int32_t* ends, void* dw,
-                          int64_t T, int64_t N, int64_t K, int32_t experts, int32_t dtype, void* stream);
+                          int64_t T, int64_t N, int64_t K, int32_t experts, int32_t dtype, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 /* ---------------- stacks: many targets, one grouped launch ------------
  * `items` is a HOST array of `count` descriptors.  Each target gets its own

@@ -9,6 +9,7 @@
 // store.  An MXFP4 value is e2m1 * 2^(scale - 127); in bf16 it is exact.
 #include "lm_impl.h"
 #include "lm_linear.h"
+#include "lm_linear_few.h"
 #include "lm_linear_mm.h"
 
 // ---------------------------------------------------------------------------
@@ -28,38 +29,22 @@ __global__ __launch_bounds__(256) void k_lin_prep4(LinArgs a, int row_blocks, ui
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t nk = (a.K + 255) >> 8, nb = a.K >> 5;
   if ((int)blockIdx.x < row_blocks) {
-    const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+    const int64_t t = (int64_t)blockIdx.x * 4 + wave_index();
     if (t >= a.T) return;
     int64_t p = t;
     if (a.ends) {
-      int g;
-      if (!lin_row(a, (int)t, g, p) || g == a.experts) return;  // a row of no group
+      int g = a.experts;
+      lin_row(a, (int)t, g, p);
+      if (g == a.experts) return;  // a row of no group
     }
     const uint16_t* x = (const uint16_t*)a.a + t * a.lda;
     const int64_t units = a.K >> 3, padded = nk * 32;
     for (int64_t u = lane; u < padded; u += 64) {
-      float v[8] = {};
-      if (u < units) {
-        const lm_u32x4 w = *(const LM_GLOBAL lm_u32x4_any*)(x + u * 8);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = val_dt<DT>(j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu);
-      }
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t b = f2u(v[j]) & 0x7fffffffu;
-        top = b > top ? b : top;
-      }
-#pragma unroll
-      for (int d = 1; d <= 2; ++d) {
-        const uint32_t o = (uint32_t)(d == 1 ? __builtin_amdgcn_update_dpp((int)top, (int)top, 0xB1, 0xf, 0xf, false)
-                                             : __builtin_amdgcn_update_dpp((int)top, (int)top, 0x4E, 0xf, 0xf, false));
-        top = o > top ? o : top;
-      }
-      float inv;
-      const uint32_t s = lin_scale4(top, inv);
-      const uint32_t w = lin_codes8(v, inv);
-      if (u < units) *(LM_GLOBAL uint32_t*)(xq + p * (a.K >> 1) + u * 4) = w;
+      lm_u32x4 w = {};
+      if (u < units) w = *(const LM_GLOBAL lm_u32x4_any*)(x + u * 8);
+      uint32_t s;
+      const uint32_t c = lin_quant8<DT>(w, s);
+      if (u < units) *(LM_GLOBAL uint32_t*)(xq + p * (a.K >> 1) + u * 4) = c;
       // (blocks past K are zeros with the smallest scale)
       if ((lane & 3) == 0) *(LM_GLOBAL uint8_t*)(xs + lin_packed(p, u >> 2, nk)) = (uint8_t)(u < units ? s : 0);
     }
@@ -80,87 +65,6 @@ __global__ __launch_bounds__(256) void k_lin_prep4(LinArgs a, int row_blocks, ui
       }
     }
     *(LM_GLOBAL lm_u32x2*)(wsc + piece * 512 + lane * 8) = lm_u32x2{s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16};
-  }
-}
-
-// ---------------------------------------------------------------------------
-// the general product: any sizes, strides and alignment, 64 x 64 tiles
-// ---------------------------------------------------------------------------
-template <int DT, bool MX>
-struct LinOps {
-  static constexpr bool HALF = DT == F16;
-  DEV static uint16_t bits(float v) { return HALF ? f16_bits(v) : bf16_bits(v); }
-  DEV static uint16_t act(const LinArgs& a, int64_t m, int64_t c) {
-    return ((const uint16_t*)a.a)[m * a.lda + c];
-  }
-  DEV static uint16_t weight(const LinArgs& a, int64_t e, int64_t n, int64_t k) {
-    if constexpr (MX) {
-      const uint32_t code = ((const uint8_t*)a.w)[(e * a.N + n) * (a.K >> 1) + (k >> 1)] >> (4 * (k & 1));
-      const uint8_t s = a.scale[e * a.scale_stride + blocked_offset(n, k >> 5, a.K >> 5, a.swizzled)];
-      return bits(e2m1_value(code) * e8m0_value(s));
-    } else {
-      return ((const uint16_t*)a.w)[(e * a.N + n) * a.K + k];
-    }
-  }
-};
-
-template <int DT, bool MX, int OP>
-__global__ __launch_bounds__(256) void k_lin_general(LinArgs a) {
-  using O = LinOps<DT, MX>;
-  __shared__ __attribute__((aligned(16))) uint16_t la[64 * 40], lb[64 * 40];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int64_t e, m0, m1, i0, iend, c0 = 0, cend;
-  const int64_t j0 = (int64_t)blockIdx.x * 64, jend = OP == LIN_FORWARD ? a.N : a.K;
-  if constexpr (OP == LIN_WEIGHT_GRAD) {
-    e = blockIdx.z;
-    lin_group(a, (int)e, m0, m1);
-    i0 = (int64_t)blockIdx.y * 64;
-    iend = a.N;
-    c0 = m0;
-    cend = m1;
-  } else {
-    int eg;
-    if (!lin_tile<64>(a, blockIdx.y, eg, i0, iend)) return;
-    e = eg;
-    cend = e == a.experts ? 0 : (OP == LIN_FORWARD ? a.K : a.N);  // rows of no group: zeros
-  }
-  v4f32 acc[4] = {};
-  for (int64_t c = c0; c < cend; c += 32) {
-    for (int u = tid; u < 64 * 32; u += 256) {
-      const int r = u >> 5, k = u & 31;
-      const int64_t i = i0 + r, j = j0 + r, cc = c + k;
-      uint16_t va = 0, vb = 0;
-      if (cc < cend) {
-        if (i < iend) va = OP == LIN_WEIGHT_GRAD ? O::act(a, cc, i) : O::act(a, i, cc);
-        if (j < jend)
-          vb = OP == LIN_FORWARD ? O::weight(a, e, j, cc)
-                                 : (OP == LIN_INPUT_GRAD ? O::weight(a, e, cc, j) : ((const uint16_t*)a.b)[cc * a.ldb + j]);
-      }
-      la[r * 40 + k] = va;
-      lb[r * 40 + k] = vb;
-    }
-    __syncthreads();
-    const lm_u32x4 fa = *(const lm_u32x4*)(la + (wave * 16 + (lane & 15)) * 40 + (lane >> 4) * 8);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const lm_u32x4 fb = *(const lm_u32x4*)(lb + (t * 16 + (lane & 15)) * 40 + (lane >> 4) * 8);
-      acc[t] = lin_mfma<O::HALF>(fa, fb, acc[t]);
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int64_t j = j0 + t * 16 + (lane & 15);
-    if (j >= jend) continue;
-    const float bias = OP == LIN_FORWARD && a.bias && e < a.experts ? val_dt<DT>(((const uint16_t*)a.bias)[j]) : 0.0f;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t i = i0 + wave * 16 + (lane >> 4) * 4 + r;
-      if (i < iend) {
-        const int64_t row = OP == LIN_WEIGHT_GRAD ? e * a.N + i : i;
-        ((uint16_t*)a.out)[row * jend + j] = bits_dt<DT>(acc[t][r] + bias);
-      }
-    }
   }
 }
 
@@ -201,82 +105,211 @@ static LinArgs lin_args(const lm_weight* w, const int32_t* ends, int64_t T) {
   return a;
 }
 
-// workspace of 4-bit inputs; padded: 64-row pieces that the rows of T rows in
-// `experts` groups can fill
-struct LinWs {
-  int64_t padded;
-  size_t xs, wsc, total;
-};
-static LinWs lin_ws(int64_t T, int64_t N, int64_t K, int64_t experts, bool grouped) {
-  LinWs w;
-  const int64_t nk = (K + 255) / 256;
-  w.padded = (T + 63) / 64 + (grouped ? experts : 0);
-  w.xs = align256((size_t)(w.padded * 64) * (size_t)(K / 2));
-  w.wsc = w.xs + (size_t)(w.padded * nk) * 512;
-  w.total = w.wsc + (size_t)(experts * ((N + 63) / 64) * nk) * 512;
-  return w;
+// ---- how a product is run: a rule on its sizes, types and alignment ----------
+// k_lin_few reads the operands once per 16 to 64 rows or columns and spreads over
+// all CUs by splitting the contraction inside workgroups; k_lin_mm shares tiles
+// of 128 or 256 and needs many of them.  Measured, us few / mm: MXFP4 [14336,
+// 4096] at 64 rows 28 / 34, at 128 rows 52 / 40; [4096, 4096] at 128 rows 24 / 26,
+// at 256 rows 27 / 29, 4-bit inputs 23 / 25; 32 experts [2816, 2048] at 16 rows each
+// 36 / 68, at 32 rows 58 / 70 (4-bit inputs 58 / 47), at 64 rows 96 / 73; dense
+// [16, 4096] of 24 adapters at 2048 rows 13 / 18, [64, 4096] 24 / 18.
+static bool lin_few(int64_t T, int64_t N, int64_t E, bool mx, bool quant) {
+  const int64_t rows = (T + E - 1) / E;
+  return N <= 16 || rows <= 16 || T * N < (mx ? 1 << 20 : 1 << 17) || (mx && !quant && E >= 8 && rows <= 32);
 }
 
-template <int DT, bool MX, int OP>
-static int run_general(const LinArgs& a, hipStream_t st) {
-  TimedLaunch timed("linear", st);
-  const int64_t J = OP == LIN_FORWARD ? a.N : a.K;
-  const int64_t gx = (J + 63) / 64;
-  const int64_t gy = OP == LIN_WEIGHT_GRAD ? (a.N + 63) / 64 : lin_tiles<64>(a.T, a.experts, a.ends != nullptr);
-  if (gx > 0x7fffffff || gy > 65535) return fail(LM_EUNSUPPORTED, "product too large for one launch");
-  hipLaunchKernelGGL((k_lin_general<DT, MX, OP>), dim3((unsigned)gx, (unsigned)gy, OP == LIN_WEIGHT_GRAD ? a.experts : 1),
-                     dim3(256), 0, st, a);
+struct LinPlan {
+  bool few;                       // k_lin_few, else k_lin_mm
+  int tile, splits;               // of k_lin_mm
+  bool copy_a, copy_b, copy_w;    // rows realigned in the workspace first
+  int64_t lda, ldb, ldw, len;
+  int64_t padded;                 // 4-bit inputs: 64-row pieces
+  size_t a, b, w, part, xq, xs, wsc, total;
+};
+static int64_t round8(int64_t x) { return (x + 7) & ~(int64_t)7; }
+
+static LinPlan lin_plan(int op, int64_t T, int64_t lda, int64_t ldb, int64_t N, int64_t K, int64_t E, bool mx, bool quant,
+                        bool aligned) {
+  LinPlan p{};
+  const int64_t rows = (T + E - 1) / E;  // of an average group
+  p.few = op == LIN_FORWARD && lin_few(T, N, E, mx, quant);
+  const int64_t inner = op == LIN_FORWARD ? K : N;  // elements of a row of a
+  const bool whole = aligned && lda % 8 == 0 && lda < (1 << 22);
+  const bool wwhole = aligned && K % 8 == 0;
+  p.lda = lda;
+  p.ldb = ldb;
+  p.ldw = K;
+  p.len = op == LIN_WEIGHT_GRAD ? 0 : inner;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += align256(bytes);
+    return o;
+  };
+  if (p.few) {
+    p.copy_a = lda >= (1 << 22);
+  } else if (!quant) {
+    p.copy_a = !whole || (op != LIN_WEIGHT_GRAD && inner % 8);
+    p.copy_b = op == LIN_WEIGHT_GRAD && (!aligned || ldb % 8 || ldb >= (1 << 22));
+    p.copy_w = op != LIN_WEIGHT_GRAD && !mx && !wwhole;
+    if (op != LIN_WEIGHT_GRAD) p.len = round8(inner);
+  }
+  if (p.copy_a) {
+    p.lda = round8(inner);
+    p.a = take((size_t)T * p.lda * 2);
+  }
+  if (p.copy_b) {
+    p.ldb = round8(K);
+    p.b = take((size_t)T * p.ldb * 2);
+  }
+  if (p.copy_w) {
+    p.ldw = round8(K);
+    p.w = take((size_t)E * N * p.ldw * 2);
+  }
+  if (quant) {
+    const int64_t nk = (K + 255) / 256;
+    p.padded = (T + 63) / 64 + E;
+    p.xq = take((size_t)(p.padded * 64) * (size_t)(K / 2));
+    p.xs = take((size_t)(p.padded * nk) * 512);
+    p.wsc = take((size_t)(E * ((N + 63) / 64) * nk) * 512);
+  }
+  p.splits = 1;
+  if (!p.few) {
+    const int64_t I = op == LIN_WEIGHT_GRAD ? N : T, J = op == LIN_FORWARD ? N : K;
+    const int64_t big = I / 256 * ((J + 255) / 256) * (op == LIN_WEIGHT_GRAD ? E : 1);
+    p.tile = big >= 192 && (op == LIN_WEIGHT_GRAD || rows >= 256) ? 256 : 128;
+    // Fewer tiles than CUs: the contraction is split so that two workgroups a CU
+    // run, into parts of 4 tiles and more (8 of 4-bit inputs, whose tiles are four
+    // times as deep).  [4096, 4096] at 64 rows, us whole / split: forward 61 / 20,
+    // input gradient 69 / 21.
+    const int64_t gi = op == LIN_WEIGHT_GRAD ? (N + 127) / 128 * E : (T + 127) / 128 + (E - 1) / 2;
+    const int64_t tiles = gi * ((J + 127) / 128);
+    const int64_t nk = ((op == LIN_WEIGHT_GRAD ? rows : p.len) + (quant ? 255 : 63)) / (quant ? 256 : 64);
+    if (p.tile == 128 && tiles < 256) {
+      int64_t s = 512 / tiles;
+      const int64_t most = nk / (quant ? 8 : 4);
+      if (s > most) s = most;
+      if (s > 16) s = 16;
+      if (s > 1) {
+        p.splits = (int)s;
+        p.part = take((size_t)s * (op == LIN_WEIGHT_GRAD ? E * N : T) * J * 4);
+      }
+    }
+  }
+  p.total = at;
+  return p;
+}
+
+static int launch_align(const void* src, int64_t lds, int64_t rows, int64_t cols, uint8_t* dst, int64_t ldd, hipStream_t st) {
+  TimedLaunch timed("linear_prep", st);
+  const int64_t n = (rows * (ldd / 8) + 255) / 256;
+  if (n == 0) return LM_OK;
+  if (n > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+  hipLaunchKernelGGL(k_lin_align, dim3((unsigned)n), dim3(256), 0, st, (const uint16_t*)src, lds, rows, cols, (uint16_t*)dst, ldd);
   LAUNCH_CHECK();
   return LM_OK;
 }
-// Whole 16-byte pieces along every row that is read, offsets inside a tile below
-// 2^31, fewer tiles than a grid holds.
-static bool mm_ok(const LinArgs& a, int op, bool mx) {
-  const int64_t len = op == LIN_FORWARD ? a.K : a.N;
-  if (a.lda % 8 || ((uintptr_t)a.a & 15) || a.lda >= (1 << 22)) return false;
-  if (op == LIN_WEIGHT_GRAD) return a.ldb % 8 == 0 && ((uintptr_t)a.b & 15) == 0 && a.ldb < (1 << 22);
-  if (len % 8) return false;
-  return mx || (a.K % 8 == 0 && ((uintptr_t)a.w & 15) == 0);
-}
 
-template <int DT, int OP, int MX, int B, int WM, int WN>
-static int launch_mm(const LinArgs& a, hipStream_t st) {
+template <int DT, int OP, int W, int B, int WM, int WN>
+static int launch_mm(const LinArgs& a, const LinPlan& p, hipStream_t st) {
   TimedLaunch timed("linear", st);
   const int64_t J = OP == LIN_FORWARD ? a.N : a.K, gj = (J + B - 1) / B;
   const int64_t gi = OP == LIN_WEIGHT_GRAD ? (a.N + B - 1) / B : lin_tiles<B>(a.T, a.experts, a.ends != nullptr);
   if (gi * gj > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
-  hipLaunchKernelGGL((k_lin_mm<DT, OP, MX, B, B, WM, WN>), dim3((unsigned)(gi * gj), OP == LIN_WEIGHT_GRAD ? a.experts : 1),
-                     dim3(WM * WN * 64), 0, st, a);
+  const dim3 grid((unsigned)(gi * gj), OP == LIN_WEIGHT_GRAD ? a.experts : p.splits, OP == LIN_WEIGHT_GRAD ? p.splits : 1);
+  hipLaunchKernelGGL((k_lin_mm<DT, OP, W, B, B, WM, WN>), grid, dim3(WM * WN * 64), 0, st, a);
+  LAUNCH_CHECK();
+  if (p.splits > 1) {
+    const int64_t n = (OP == LIN_WEIGHT_GRAD ? a.experts * a.N : a.T) * J, blocks = (n + 1023) / 1024;
+    if (blocks > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+    hipLaunchKernelGGL((k_lin_join<DT>), dim3((unsigned)blocks), dim3(256), 0, st, a.part, p.splits, n, J, (const uint16_t*)a.bias,
+                       (uint16_t*)a.out);
+    LAUNCH_CHECK();
+  }
+  return LM_OK;
+}
+template <int OP, int W>
+static int run_mm(const LinArgs& a, const LinPlan& p, int dtype, hipStream_t st) {
+  if (dtype == LM_F16)
+    return p.tile == 256 ? launch_mm<F16, OP, W, 256, 2, 4>(a, p, st) : launch_mm<F16, OP, W, 128, 2, 2>(a, p, st);
+  return p.tile == 256 ? launch_mm<BF16, OP, W, 256, 2, 4>(a, p, st) : launch_mm<BF16, OP, W, 128, 2, 2>(a, p, st);
+}
+
+template <int DT, int W, int MF, int CF, int NW, int UN, bool EDGE = false>
+static int launch_few(const LinArgs& a, hipStream_t st) {
+  TimedLaunch timed("linear_few", st);
+  const int64_t n = lin_tiles<16 * MF>(a.T, a.experts, a.ends != nullptr) * ((a.N + 16 * CF - 1) / (16 * CF));
+  if (n > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+  hipLaunchKernelGGL((k_lin_few<DT, W, MF, CF, NW, UN, EDGE>), dim3((unsigned)n), dim3(NW * 64), 0, st, a);
   LAUNCH_CHECK();
   return LM_OK;
 }
-template <int OP, int MX>
-static int run_mm(const LinArgs& a, int dtype, hipStream_t st) {
-  const int64_t J = OP == LIN_FORWARD ? a.N : a.K, I = OP == LIN_WEIGHT_GRAD ? a.N : a.T;
-  const int64_t big = I / 256 * ((J + 255) / 256) * (OP == LIN_WEIGHT_GRAD ? a.experts : 1);
-  const bool wide = big >= 192 && (OP == LIN_WEIGHT_GRAD || a.T / a.experts >= 256);
-  if (dtype == LM_F16)
-    return wide ? launch_mm<F16, OP, MX, 256, 2, 4>(a, st) : launch_mm<F16, OP, MX, 128, 2, 2>(a, st);
-  return wide ? launch_mm<BF16, OP, MX, 256, 2, 4>(a, st) : launch_mm<BF16, OP, MX, 128, 2, 2>(a, st);
+// Workgroups of 16 columns spread a small weight over the most CUs; wider ones
+// read the rows less often.  `wgs`: workgroups at 16 rows x 16 columns.
+template <int DT, int W>
+static int run_few_dt(const LinArgs& a, hipStream_t st) {
+  if constexpr (W == W_DENSE) {
+    if (a.K % 8) return launch_few<DT, W, 2, 1, 8, 1, true>(a, st);
+  }
+  const int64_t rows = (a.T + a.experts - 1) / a.experts, units = (a.K + 127) / 128;
+  const int64_t wgs = lin_tiles<16>(a.T, a.experts, a.experts > 1) * ((a.N + 15) / 16);
+  if (rows > 32 && wgs > 2048) return launch_few<DT, W, 4, 4, 8, 1>(a, st);
+  if constexpr (W == W_Q4) {
+    if (wgs <= 256 || (rows <= 8 && units >= 32)) return launch_few<DT, W, 1, 1, 8, 4>(a, st);
+    if (wgs <= 512 || units < 32) return launch_few<DT, W, 1, 2, 8, 2>(a, st);
+    return launch_few<DT, W, 1, 4, 8, 4>(a, st);
+  } else {
+    if (wgs <= 256) return launch_few<DT, W, 1, 1, 16, 2>(a, st);
+    if (wgs <= 512) return launch_few<DT, W, 1, 2, 16, 2>(a, st);
+    if (wgs <= 2048) return launch_few<DT, W, 1, 4, 16, 2>(a, st);
+    return launch_few<DT, W, 1, 4, 8, 2>(a, st);
+  }
+}
+template <int W>
+static int run_few(const LinArgs& a, int dtype, hipStream_t st) {
+  return dtype == LM_F16 ? run_few_dt<F16, W>(a, st) : run_few_dt<BF16, W>(a, st);
 }
 
-template <int OP>
-static int run_product(const LinArgs& a, int dtype, bool mx, hipStream_t st) {
-  if (mm_ok(a, OP, mx)) {
-    if constexpr (OP != LIN_WEIGHT_GRAD) {
-      if (mx) return run_mm<OP, W_MX>(a, dtype, st);
-    }
-    return run_mm<OP, W_DENSE>(a, dtype, st);
+// copies of rows that are not whole 16-byte pieces, and the pointers of the plan
+static int lin_setup(LinArgs& a, const LinPlan& p, int op, void* workspace, size_t workspace_bytes, hipStream_t st) {
+  if (p.total > 0) {
+    if (!workspace || workspace_bytes < p.total)
+      return fail(LM_EWORKSPACE, "workspace too small: %zu < %zu bytes", workspace ? workspace_bytes : 0, p.total);
+    if (((uintptr_t)workspace & 255) != 0) return fail(LM_EINVAL, "workspace must be 256-byte aligned");
   }
-  if constexpr (OP != LIN_WEIGHT_GRAD) {
-    if (mx) return dtype == LM_F16 ? run_general<F16, true, OP>(a, st) : run_general<BF16, true, OP>(a, st);
+  uint8_t* base = (uint8_t*)workspace;
+  const int64_t inner = op == LIN_FORWARD ? a.K : a.N;
+  int rc;
+  if (p.copy_a) {
+    if ((rc = launch_align(a.a, a.lda, a.T, inner, base + p.a, p.lda, st))) return rc;
+    a.a = base + p.a;
   }
-  return dtype == LM_F16 ? run_general<F16, false, OP>(a, st) : run_general<BF16, false, OP>(a, st);
+  if (p.copy_b) {
+    if ((rc = launch_align(a.b, a.ldb, a.T, a.K, base + p.b, p.ldb, st))) return rc;
+    a.b = base + p.b;
+  }
+  if (p.copy_w) {
+    if ((rc = launch_align(a.w, a.K, a.experts * a.N, a.K, base + p.w, p.ldw, st))) return rc;
+    a.w = base + p.w;
+  }
+  a.lda = p.lda;
+  a.ldb = p.ldb;
+  a.ldw = p.ldw;
+  a.len = p.len;
+  a.padded = p.padded;
+  a.part = p.splits > 1 ? (float*)(base + p.part) : nullptr;
+  a.xq = base + p.xq;
+  a.xs = base + p.xs;
+  a.wsc = base + p.wsc;
+  return LM_OK;
 }
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-extern "C" size_t lm_linear_workspace_size(int64_t T, int64_t N, int64_t K, int32_t experts, int32_t input_dtype) {
-  if (T <= 0 || N <= 0 || K <= 0 || experts <= 0 || input_dtype != LM_E2M1) return 0;
-  return lin_ws(T, N, K, experts, true).total;
+extern "C" size_t lm_linear_workspace_size(int32_t op, int64_t T, int64_t lda, int64_t ldb, int64_t N, int64_t K,
+                                           int32_t experts, int32_t weight_dtype, int32_t input_dtype, int32_t aligned) {
+  if (T <= 0 || N <= 0 || K <= 0 || experts <= 0 || op < LM_LINEAR_FORWARD || op > LM_LINEAR_WEIGHT_GRAD) return 0;
+  return lin_plan(op, T, lda, ldb, N, K, experts, weight_dtype == LM_E2M1, op == LIN_FORWARD && input_dtype == LM_E2M1, aligned != 0)
+      .total;
 }
 
 extern "C" int lm_linear(const void* x, int64_t ldx, const lm_weight* w, const void* bias, const int32_t* ends, void* y,
@@ -297,52 +330,61 @@ extern "C" int lm_linear(const void* x, int64_t ldx, const lm_weight* w, const v
   a.lda = ldx;
   a.bias = bias;
   a.out = y;
-  if (!quant) return run_product<LIN_FORWARD>(a, dtype, mx, st);
-  const LinWs ws = lin_ws(T, a.N, a.K, a.experts, ends != nullptr);
-  if (!workspace || workspace_bytes < ws.total)
-    return fail(LM_EWORKSPACE, "workspace too small: %zu < %zu bytes", workspace ? workspace_bytes : 0, ws.total);
-  if (((uintptr_t)workspace & 255) != 0) return fail(LM_EINVAL, "workspace must be 256-byte aligned");
-  uint8_t* base = (uint8_t*)workspace;
-  a.xq = base;
-  a.xs = base + ws.xs;
-  a.wsc = base + ws.wsc;
-  a.padded = ws.padded;
+  const LinPlan p = lin_plan(LIN_FORWARD, T, ldx, 0, a.N, a.K, a.experts, mx, quant, aligned16(x) && aligned16(w->q));
+  if ((rc = lin_setup(a, p, LIN_FORWARD, workspace, workspace_bytes, st))) return rc;
+  if (!quant) {
+    if (p.few) return mx ? run_few<W_MX>(a, dtype, st) : run_few<W_DENSE>(a, dtype, st);
+    return mx ? run_mm<LIN_FORWARD, W_MX>(a, p, dtype, st) : run_mm<LIN_FORWARD, W_DENSE>(a, p, dtype, st);
+  }
+  uint8_t *xq = (uint8_t*)a.xq, *xs = (uint8_t*)a.xs, *wsc = (uint8_t*)a.wsc;
   {
     TimedLaunch timed("linear_prep", st);
-    const int64_t rows = (T + 3) / 4, pieces = (a.experts * ((a.N + 63) / 64) * ((a.K + 255) / 256) + 3) / 4;
+    const int segs = (int)((a.K + 2047) / 2048);
+    const int64_t rows = (p.few ? T * segs : T + 3) / 4 + (p.few ? 1 : 0);
+    const int64_t pieces = p.few ? 0 : (a.experts * ((a.N + 63) / 64) * ((a.K + 255) / 256) + 3) / 4;
     if (rows + pieces > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
     const dim3 grid((unsigned)(rows + pieces));
-    if (dtype == LM_F16) hipLaunchKernelGGL((k_lin_prep4<F16>), grid, dim3(256), 0, st, a, (int)rows, base, base + ws.xs, base + ws.wsc);
-    else hipLaunchKernelGGL((k_lin_prep4<BF16>), grid, dim3(256), 0, st, a, (int)rows, base, base + ws.xs, base + ws.wsc);
+    if (p.few) {
+      if (dtype == LM_F16) hipLaunchKernelGGL((k_lin_quant<F16>), grid, dim3(256), 0, st, a, segs, xq, xs);
+      else hipLaunchKernelGGL((k_lin_quant<BF16>), grid, dim3(256), 0, st, a, segs, xq, xs);
+    } else {
+      if (dtype == LM_F16) hipLaunchKernelGGL((k_lin_prep4<F16>), grid, dim3(256), 0, st, a, (int)rows, xq, xs, wsc);
+      else hipLaunchKernelGGL((k_lin_prep4<BF16>), grid, dim3(256), 0, st, a, (int)rows, xq, xs, wsc);
+    }
     LAUNCH_CHECK();
   }
-  return run_mm<LIN_FORWARD, W_Q4>(a, dtype, st);
+  return p.few ? run_few<W_Q4>(a, dtype, st) : run_mm<LIN_FORWARD, W_Q4>(a, p, dtype, st);
 }
 
 extern "C" int lm_linear_input_grad(const void* dy, int64_t lddy, const lm_weight* w, const int32_t* ends, void* dx,
-                                    int64_t T, int32_t dtype, void* stream) {
+                                    int64_t T, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream) {
   int rc;
   if (!w) return fail(LM_EINVAL, "lm_linear_input_grad requires a weight");
   if ((rc = check_lin(w, T, dtype, ends, w->experts))) return rc;
   if (T == 0) return LM_OK;
   if (!dy || !dx) return fail(LM_EINVAL, "row pointers must be non-null");
   if (lddy < w->N) return fail(LM_EINVAL, "row stride below the row length");
+  hipStream_t st = (hipStream_t)stream;
+  const bool mx = w->dtype == LM_E2M1;
   LinArgs a = lin_args(w, ends, T);
   a.a = dy;
   a.lda = lddy;
   a.out = dx;
-  return run_product<LIN_INPUT_GRAD>(a, dtype, w->dtype == LM_E2M1, (hipStream_t)stream);
+  const LinPlan p = lin_plan(LIN_INPUT_GRAD, T, lddy, 0, a.N, a.K, a.experts, mx, false, aligned16(dy) && aligned16(w->q));
+  if ((rc = lin_setup(a, p, LIN_INPUT_GRAD, workspace, workspace_bytes, st))) return rc;
+  return mx ? run_mm<LIN_INPUT_GRAD, W_MX>(a, p, dtype, st) : run_mm<LIN_INPUT_GRAD, W_DENSE>(a, p, dtype, st);
 }
 
 extern "C" int lm_linear_weight_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int32_t* ends,
                                      void* dw, int64_t T, int64_t N, int64_t K, int32_t experts, int32_t dtype,
-                                     void* stream) {
+                                     void* workspace, size_t workspace_bytes, void* stream) {
   int rc;
   if ((rc = check_lin(nullptr, T, dtype, ends, experts))) return rc;
   if (N <= 0 || K <= 0) return fail(LM_EINVAL, "empty weight gradient");
   if (N >= (1 << 22) || K >= (1 << 22)) return fail(LM_EUNSUPPORTED, "products take rows and columns below 2^22");
   if (!dw || (T > 0 && (!dy || !x))) return fail(LM_EINVAL, "pointers must be non-null");
   if (lddy < N || ldx < K) return fail(LM_EINVAL, "row stride below the row length");
+  hipStream_t st = (hipStream_t)stream;
   LinArgs a{};
   a.a = dy;
   a.lda = lddy;
@@ -354,5 +396,7 @@ extern "C" int lm_linear_weight_grad(const void* dy, int64_t lddy, const void* x
   a.T = T;
   a.N = N;
   a.K = K;
-  return run_product<LIN_WEIGHT_GRAD>(a, dtype, false, (hipStream_t)stream);
+  const LinPlan p = lin_plan(LIN_WEIGHT_GRAD, T, lddy, ldx, N, K, experts, false, false, aligned16(dy) && aligned16(x));
+  if ((rc = lin_setup(a, p, LIN_WEIGHT_GRAD, workspace, workspace_bytes, st))) return rc;
+  return run_mm<LIN_WEIGHT_GRAD, W_DENSE>(a, p, dtype, st);
 }

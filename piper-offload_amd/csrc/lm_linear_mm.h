@@ -36,14 +36,6 @@ typedef __attribute__((address_space(3))) lm_u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) lm_u32x2 lds_u32x2;
 typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
 
-// Where a product's rows are too far apart for 32-bit offsets inside a tile the
-// general kernel runs instead.
-constexpr int64_t LIN_SPAN = 0x7fffffff;
-
-DEV __amdgpu_buffer_rsrc_t lin_rsrc(const void* p, int64_t bytes) {
-  const uint32_t n = bytes < 0 ? 0u : (bytes > LIN_SPAN ? (uint32_t)LIN_SPAN : (uint32_t)bytes);
-  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, n, 0x00027000);
-}
 // 16 bytes per lane to LDS at base + 16 lane; past the resource's end: zeros
 DEV void lin_dma(__amdgpu_buffer_rsrc_t r, lds_u8* base, uint32_t off) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)base, 16, (int)off, 0, 0, 0);
@@ -82,28 +74,6 @@ DEV bool lin_pick(const LinArgs& a, int64_t jend, LinTile& t) {
     return true;
   }
   return lin_find<BM>(a, (int)tm, t.group, t.r0, t.r1, t.pad);
-}
-
-enum : int { W_DENSE = 0, W_MX = 1, W_Q4 = 2 };
-
-template <int S, int F, int G>
-DEV v4f32 lin_mfma4_(lm_u32x4 a, lm_u32x4 b, v4f32 c, uint32_t sa, uint32_t sb) {
-  typedef int v8i32 __attribute__((ext_vector_type(8)));
-  const v8i32 x = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}, y = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, 2 * F + S, (int)sa, 2 * G + S, (int)sb);
-}
-// step s; f, g: which of a word's two fragments the scales belong to
-DEV v4f32 lin_mfma4(lm_u32x4 a, lm_u32x4 b, v4f32 c, uint32_t sa, uint32_t sb, int s, int f, int g) {
-  switch (4 * s + 2 * f + g) {
-    case 0: return lin_mfma4_<0, 0, 0>(a, b, c, sa, sb);
-    case 1: return lin_mfma4_<0, 0, 1>(a, b, c, sa, sb);
-    case 2: return lin_mfma4_<0, 1, 0>(a, b, c, sa, sb);
-    case 3: return lin_mfma4_<0, 1, 1>(a, b, c, sa, sb);
-    case 4: return lin_mfma4_<1, 0, 0>(a, b, c, sa, sb);
-    case 5: return lin_mfma4_<1, 0, 1>(a, b, c, sa, sb);
-    case 6: return lin_mfma4_<1, 1, 0>(a, b, c, sa, sb);
-    default: return lin_mfma4_<1, 1, 1>(a, b, c, sa, sb);
-  }
 }
 
 template <int DT, int OP, int W, int BM, int BN, int WM, int WN>
@@ -167,24 +137,6 @@ DEV lm_u32x4 mm_frag_tr(const lds_u8* t, int col0, int f, int lane, int s) {
                   __builtin_bit_cast(lm_u32x2, hi)[0], __builtin_bit_cast(lm_u32x2, hi)[1]};
 }
 
-// 8 codes -> 8 values of 16 bits
-template <bool HALF>
-DEV lm_u32x4 mm_decode(uint32_t codes, float scale) {
-  lm_u32x4 v;
-  if constexpr (HALF) {
-    v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0));
-    v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1));
-    v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 2));
-    v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3));
-  } else {
-    v[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
-    v[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1));
-    v[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2));
-    v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
-  }
-  return v;
-}
-
 template <int DT, int OP, int W, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
   using P = MmTraits<DT, OP, W, BM, BN, WM, WN>;
@@ -221,7 +173,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
     jstep = 128 * ldb;
   } else {
     if (!lin_pick<BM, BN>(a, jend, t)) return;
-    len = t.group == a.experts ? 0 : (OP == LIN_FORWARD ? a.K : a.N);
+    len = t.group == a.experts ? 0 : a.len;
     if constexpr (Q4) {
       lda = a.K >> 2;  // two codes a byte, in units of two bytes as the others
       ip = a.xq + t.pad * (a.K >> 1);
@@ -231,18 +183,22 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
       ibytes = ((t.r1 - t.r0 - 1) * lda + len) * 2;
     }
     istep = 128;
-    ldb = Q4 ? a.K >> 2 : a.K;
     constexpr bool MX = P::MX || Q4;
-    const int64_t first = OP == LIN_FORWARD ? (t.group * a.N + t.j0) * a.K : t.group * a.N * a.K + t.j0;
-    const int64_t count = OP == LIN_FORWARD ? (a.N - t.j0) * a.K : a.N * a.K - t.j0;
+    const int64_t ldw = MX ? a.K : a.ldw;
+    ldb = Q4 ? a.K >> 2 : ldw;
+    const int64_t first = OP == LIN_FORWARD ? (t.group * a.N + t.j0) * ldw : t.group * a.N * ldw + t.j0;
+    const int64_t count = OP == LIN_FORWARD ? (a.N - t.j0) * ldw : a.N * ldw - t.j0;
     jp = (const uint8_t*)a.w + (MX ? first >> 1 : first * 2);
     jbytes = MX ? count >> 1 : count * 2;
-    jstep = OP == LIN_FORWARD ? (P::MX ? 32 : 128) : 64 * (MX ? a.K >> 1 : a.K * 2);
+    jstep = OP == LIN_FORWARD ? (P::MX ? 32 : 128) : 64 * (MX ? ldw >> 1 : ldw * 2);
   }
+  // tiles [kb, ke) of nk: this workgroup's part where the contraction is split
   const int nk = (int)((len + CT - 1) / CT);
+  const int splits = OP == LIN_WEIGHT_GRAD ? gridDim.z : gridDim.y, split = OP == LIN_WEIGHT_GRAD ? blockIdx.z : blockIdx.y;
+  const int per = (nk + splits - 1) / splits, kb = split * per, ke = kb + per < nk ? kb + per : nk;
   v4f32 acc[FI][FJ] = {};
 
-  if (nk > 0) {
+  if (kb < ke) {
     uint32_t io[P::IL], jo[P::JL];
     mm_offsets<P::IK, BM, P::IL, P::NW, false>(io, wave, lane, lda);
     if constexpr (P::JK != KS4) mm_offsets<P::JK, BN, P::JL, P::NW, true>(jo, wave, lane, ldb);
@@ -318,7 +274,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
         const int64_t n = (int64_t)kt * 64 + kr, k = t.j0 + kc * 32;
         code = lm_u32x4{};
         code_s = 0;
-        if (n < len && k < a.K) {
+        if (n < a.N && k < a.K) {
           code = *(const LM_GLOBAL lm_u32x4*)(jp + n * (a.K >> 1) + kc * 16);
           code_s = sp[blocked_offset(n, k >> 5, nb, a.swizzled)];
         }
@@ -329,7 +285,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
         const float s = e8m0_value(code_s);
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          *(lds_u32x4*)(tj + kr * (BN * 2) + (((kc * 4 + c) ^ ((kr & 3) << 2)) << 4)) = mm_decode<HALF>(code[c], s);
+          *(lds_u32x4*)(tj + kr * (BN * 2) + (((kc * 4 + c) ^ ((kr & 3) << 2)) << 4)) = lin_decode8<HALF>(code[c], s);
       }
     };
     auto compute = [&](const lds_u8* ti, const lds_u8* tj, const lds_u8* tis, const lds_u8* tjs, const float* scales) {
@@ -351,7 +307,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
         lm_u32x4 fi[FI], fj[FJ];
 #pragma unroll
         for (int f = 0; f < FJ; ++f) {
-          if constexpr (P::JK == KC4) fj[f] = mm_decode<HALF>(jc[f][s], scales[f]);
+          if constexpr (P::JK == KC4) fj[f] = lin_decode8<HALF>(jc[f][s], scales[f]);
           else if constexpr (P::JK == KC16) fj[f] = mm_frag<KC16, BN>(tj, wj * (FJ * 16), f, lane, s, P::chunk(s, g));
           else fj[f] = mm_frag_tr<BN, true>(tj, wj * (FJ * 16), f, lane, s);
         }
@@ -381,12 +337,12 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
         for (int f = 0; f < FJ; ++f) out[f] = e8m0_value(sv[f]);
       }
     };
-    load(0, i0, j0, is0, js0);
-    load_scales(0);
+    load(kb, i0, j0, is0, js0);
+    load_scales(kb);
     store_codes(j0);
     float sc[P::JK == KC4 ? FJ : 1];
-    int kt = 0;
-    for (; kt + 1 < nk; kt += 2) {  // (no way out of the middle: it would keep two copies of the accumulators)
+    int kt = kb;
+    for (; kt + 1 < ke; kt += 2) {  // (no way out of the middle: it would keep two copies of the accumulators)
       __syncthreads();
       scales_now(sc);
       load(kt + 1, i1, j1, is1, js1);
@@ -395,21 +351,43 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
       store_codes(j1);
       __syncthreads();
       scales_now(sc);
-      if (kt + 2 < nk) {
+      if (kt + 2 < ke) {
         load(kt + 2, i0, j0, is0, js0);
         load_scales(kt + 2);
       }
       compute(i1, j1, is1, js1, sc);
-      if (kt + 2 < nk) store_codes(j0);
+      if (kt + 2 < ke) store_codes(j0);
     }
-    if (kt < nk) {
+    if (kt < ke) {
       __syncthreads();
       scales_now(sc);
       compute(i0, j0, is0, js0, sc);
     }
   }
 
-  uint16_t* out = (uint16_t*)a.out + (OP == LIN_WEIGHT_GRAD ? t.group * a.N * a.K : 0);
+  const int64_t rows0 = OP == LIN_WEIGHT_GRAD ? t.group * a.N : 0;  // of the output above this group's
+  if (a.part) {  // a part of the sums: k_lin_join adds them up
+    float* part = a.part + (split * (OP == LIN_WEIGHT_GRAD ? a.experts * a.N : a.T) + rows0) * jend;
+#pragma unroll
+    for (int x = 0; x < FI; ++x) {
+      const int64_t i = t.r0 + wi * (FI * 16) + x * 16 + (lane & 15);
+#pragma unroll
+      for (int y = 0; y < FJ; ++y) {
+        const int64_t j = t.j0 + wj * (FJ * 16) + (y >> 1) * 32 + 8 * g + 4 * (y & 1);
+        if (i < t.r1) {
+          if (j + 4 <= jend) {
+            *(LM_GLOBAL lm_u32x4_any*)(part + i * jend + j) = __builtin_bit_cast(lm_u32x4, acc[x][y]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+              if (j + e < jend) ((LM_GLOBAL float*)part)[i * jend + j + e] = acc[x][y][e];
+          }
+        }
+      }
+    }
+    return;
+  }
+  uint16_t* out = (uint16_t*)a.out + rows0 * jend;
 #pragma unroll
   for (int y = 0; y < FJ; y += 2) {
     const int64_t j = t.j0 + wj * (FJ * 16) + y * 16 + 8 * g;
@@ -440,4 +418,41 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
       }
     }
   }
+}
+
+// the sum of the parts of a split contraction, in their order, rounded
+template <int DT>
+__global__ __launch_bounds__(256) void k_lin_join(const float* part, int splits, int64_t n, int64_t J, const uint16_t* bias,
+                                                  uint16_t* out) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  float s[4] = {};
+  for (int k = 0; k < splits; ++k) {
+    const LM_GLOBAL float* p = (const LM_GLOBAL float*)part + k * n + i;
+    if (i + 4 <= n) {
+      const v4f32 v = __builtin_bit_cast(v4f32, *(const LM_GLOBAL lm_u32x4_any*)p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] += v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (i + e < n) s[e] += p[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (i + e < n) {
+      if (bias) s[e] += val_dt<DT>(((const LM_GLOBAL uint16_t*)bias)[(i + e) % J]);
+      ((LM_GLOBAL uint16_t*)out)[i + e] = bits_dt<DT>(s[e]);
+    }
+}
+
+// rows of any stride and alignment, copied to a stride of whole 16-byte pieces
+// and filled up with zeros
+__global__ __launch_bounds__(256) void k_lin_align(const uint16_t* src, int64_t lds, int64_t rows, int64_t cols, uint16_t* dst,
+                                                   int64_t ldd) {
+  const int64_t pieces = ldd >> 3, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * pieces) return;
+  const int64_t r = i / pieces, c = (i - r * pieces) * 8;
+  store_b128_guarded((LM_GLOBAL lm_u32x4*)(dst + r * ldd + c), lin_chunk(src + r * lds + c, cols - c));
 }

@@ -101,10 +101,10 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lm_routed_workspace_size": (_SZ, [_I64, _I64, ctypes.POINTER(RoutedFactor), _I32]),
     "lm_routed_residual": (_I32, [_P, _P, _P, _I64, _I64, _I64, _I32, ctypes.POINTER(RoutedFactor), _I32, _P, _SZ,
                                   _P]),
-    "lm_linear_workspace_size": (_SZ, [_I64, _I64, _I64, _I32, _I32]),
+    "lm_linear_workspace_size": (_SZ, [_I32, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _I32]),
     "lm_linear": (_I32, [_P, _I64, _W, _P, _P, _P, _I64, _I32, _I32, _P, _SZ, _P]),
-    "lm_linear_input_grad": (_I32, [_P, _I64, _W, _P, _P, _I64, _I32, _P]),
-    "lm_linear_weight_grad": (_I32, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _P]),
+    "lm_linear_input_grad": (_I32, [_P, _I64, _W, _P, _P, _I64, _I32, _P, _SZ, _P]),
+    "lm_linear_weight_grad": (_I32, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _P, _SZ, _P]),
     "lm_timer_enable": (_I32, [_I32]),
     "lm_timer_read": (_I32, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int64)]),
 }
@@ -188,6 +188,12 @@ def torch_dtype_id(dtype: torch.dtype) -> int:
 def workspace_size(rows: int, cols: int, rank: int) -> int:
     """``lm_workspace_size``, a function of the three numbers alone."""
     return load_library().lm_workspace_size(rows, cols, rank)
+
+
+@functools.lru_cache(maxsize=4096)
+def linear_workspace_size(*sizes: int) -> int:
+    """``lm_linear_workspace_size``, a function of its numbers alone."""
+    return load_library().lm_linear_workspace_size(*sizes)
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

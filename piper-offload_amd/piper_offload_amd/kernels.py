@@ -639,20 +639,21 @@ def merge_dense_lora_(weight: torch.Tensor, b: torch.Tensor, a: torch.Tensor, st
 _MAX_EXPERTS = 1024
 
 
-def _rows(label: str, x: torch.Tensor, cols: int) -> torch.Tensor:
-    """``x`` [..., cols] as [rows, cols] whose rows are contiguous (their stride is free)."""
-    if x.ndim < 1 or x.shape[-1] != cols:
-        raise ValueError(f"{label}: expected rows of {cols} elements, got shape {tuple(x.shape)}.")
+def _rows(label: str, x: torch.Tensor, cols: int) -> tuple[torch.Tensor, int, int]:
+    """``x`` [..., cols] as [rows, cols] whose rows are contiguous, the number of rows, and their stride."""
+    shape = x.shape
+    if not shape or shape[-1] != cols:
+        raise ValueError(f"{label}: expected rows of {cols} elements, got shape {tuple(shape)}.")
     if x.dtype not in _FACTOR_DTYPES:
         raise ValueError(f"{label} supports bfloat16 and float16 rows, got {x.dtype}.")
-    x = x.reshape(-1, cols)
-    if (cols > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < cols):
+    if len(shape) != 2:
+        x = x.reshape(-1, cols)
+    rows = x.shape[0]
+    stride, step = x.stride()
+    if (cols > 1 and step != 1) or (rows > 1 and stride < cols):
         x = x.contiguous()
-    return x
-
-
-def _stride(x: torch.Tensor) -> int:
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]  # (the stride of a single row may be anything)
+        stride = cols
+    return x, rows, stride if rows > 1 else cols  # (the stride of a single row may be anything)
 
 
 def _ends(label: str, ends: torch.Tensor, experts: int) -> torch.Tensor:
@@ -688,7 +689,7 @@ def _mx_stack(label: str, qdata: torch.Tensor, scale: torch.Tensor, swizzled: bo
 def _linear_forward(label: str, x: torch.Tensor, weight: L.WeightStruct, bias: torch.Tensor | None,
                     ends: torch.Tensor | None, activation_dtype: torch.dtype | None, device: torch.device) -> torch.Tensor:
     n, k = weight.N, weight.K
-    x2 = _rows(label, x, k)
+    x2, t, ldx = _rows(label, x, k)
     dtype_id = L.torch_dtype_id(x.dtype)
     input_id = dtype_id
     if activation_dtype is not None:
@@ -699,34 +700,37 @@ def _linear_forward(label: str, x: torch.Tensor, weight: L.WeightStruct, bias: t
         if bias.dtype is not x.dtype or tuple(bias.shape) != (n,):
             raise ValueError(f"{label}: bias must be {x.dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}.")
         bias = bias.contiguous()
-    t = x2.shape[0]
-    y = torch.empty((t, n), dtype=x.dtype, device=device)
+    y = x2.new_empty((t, n))
     if t:
         handle = L.lib()
-        ws_bytes = handle.lm_linear_workspace_size(t, n, k, weight.experts, input_id)
+        px = x2.data_ptr()
+        ws_bytes = L.linear_workspace_size(0, t, ldx, 0, n, k, weight.experts, weight.dtype, input_id, not (px | weight.q) & 15)
         with L.on_device(device):
             ws = L.workspace(ws_bytes, device) if ws_bytes else None
-            rc = handle.lm_linear(x2.data_ptr(), _stride(x2), ctypes.byref(weight), _ptr(bias), _ptr(ends), y.data_ptr(), t,
-                                  dtype_id, input_id, None if ws is None else L.aligned_ptr(ws), ws_bytes,
-                                  L.stream_ptr(device))
+            rc = handle.lm_linear(px, ldx, ctypes.byref(weight), _ptr(bias), _ptr(ends), y.data_ptr(), t, dtype_id, input_id,
+                                  None if ws is None else L.aligned_ptr(ws), ws_bytes, L.stream_ptr(device))
         if rc:
             L.check(rc)
-    return y.view(*x.shape[:-1], n)
+    return y if x.ndim == 2 else y.view(*x.shape[:-1], n)
 
 
 def _linear_input_grad(label: str, dy: torch.Tensor, weight: L.WeightStruct, ends: torch.Tensor | None,
                        device: torch.device) -> torch.Tensor:
-    dy2 = _rows(label, dy, weight.N)
-    t = dy2.shape[0]
-    dx = torch.empty((t, weight.K), dtype=dy.dtype, device=device)
+    dy2, t, ldy = _rows(label, dy, weight.N)
+    dx = dy2.new_empty((t, weight.K))
     if t:
         handle = L.lib()
+        py = dy2.data_ptr()
+        dtype_id = L.torch_dtype_id(dy.dtype)
+        ws_bytes = L.linear_workspace_size(1, t, ldy, 0, weight.N, weight.K, weight.experts, weight.dtype, dtype_id,
+                                           not (py | weight.q) & 15)
         with L.on_device(device):
-            rc = handle.lm_linear_input_grad(dy2.data_ptr(), _stride(dy2), ctypes.byref(weight), _ptr(ends), dx.data_ptr(),
-                                             t, L.torch_dtype_id(dy.dtype), L.stream_ptr(device))
+            ws = L.workspace(ws_bytes, device) if ws_bytes else None
+            rc = handle.lm_linear_input_grad(py, ldy, ctypes.byref(weight), _ptr(ends), dx.data_ptr(), t, dtype_id,
+                                             None if ws is None else L.aligned_ptr(ws), ws_bytes, L.stream_ptr(device))
         if rc:
             L.check(rc)
-    return dx.view(*dy.shape[:-1], weight.K)
+    return dx if dy.ndim == 2 else dx.view(*dy.shape[:-1], weight.K)
 
 
 def mx_matmul(x: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, *, swizzled: bool = False,
@@ -794,15 +798,17 @@ def grouped_matmul_weight_grad(dy: torch.Tensor, x: torch.Tensor, ends: torch.Te
     n, k = dy.shape[-1], x.shape[-1]
     if n == 0 or k == 0:
         raise ValueError(f"{label} requires non-empty rows.")
-    dy2, x2 = _rows(label, dy, n), _rows(label, x, k)
+    (dy2, t, ldy), (x2, _, ldx) = _rows(label, dy, n), _rows(label, x, k)
     ends = _ends(label, ends, ends.shape[0] if ends.ndim == 1 else -1)
     e = ends.shape[0]
     dw = torch.empty((e, n, k), dtype=x.dtype, device=device)
     handle = L.lib()
+    py, px, dtype_id = dy2.data_ptr(), x2.data_ptr(), L.torch_dtype_id(x.dtype)
+    ws_bytes = L.linear_workspace_size(2, t, ldy, ldx, n, k, e, dtype_id, dtype_id, not (py | px) & 15)
     with L.on_device(device):
-        rc = handle.lm_linear_weight_grad(dy2.data_ptr(), _stride(dy2), x2.data_ptr(), _stride(x2), ends.data_ptr(),
-                                          dw.data_ptr(), x2.shape[0], n, k, e, L.torch_dtype_id(x.dtype),
-                                          L.stream_ptr(device))
+        ws = L.workspace(ws_bytes, device) if ws_bytes else None
+        rc = handle.lm_linear_weight_grad(py, ldy, px, ldx, ends.data_ptr(), dw.data_ptr(), t, n, k, e, dtype_id,
+                                          None if ws is None else L.aligned_ptr(ws), ws_bytes, L.stream_ptr(device))
     if rc:
         L.check(rc)
     return dw

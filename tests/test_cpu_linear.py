@@ -51,7 +51,7 @@ def test_c_entries_refuse_bad_arguments(over, args):
                             None) in (L.LM_EINVAL, L.LM_EUNSUPPORTED)
     assert handle.lm_last_error()
     if a["ldx"] == 128:
-        assert handle.lm_linear_input_grad(a["x"], a["ldx"], ctypes.byref(w), None, a["y"], a["T"], a["dtype"],
+        assert handle.lm_linear_input_grad(a["x"], a["ldx"], ctypes.byref(w), None, a["y"], a["T"], a["dtype"], None, 0,
                                            None) in (L.LM_EINVAL, L.LM_EUNSUPPORTED)
 
 
@@ -65,7 +65,7 @@ def test_c_entries_refuse_more():
     dense = _weight(dtype=L.LM_BF16)
     assert handle.lm_linear(4096, 128, ctypes.byref(dense), None, None, 4096, 4, L.LM_BF16, L.LM_E2M1, None, 0,
                             None) == L.LM_EUNSUPPORTED
-    need = handle.lm_linear_workspace_size(300, 64, 128, 1, L.LM_E2M1)
+    need = handle.lm_linear_workspace_size(0, 300, 128, 0, 64, 128, 1, L.LM_E2M1, L.LM_E2M1, 1)
     assert need >= 300 * (64 + 4)
     assert handle.lm_linear(4096, 128, ctypes.byref(w), None, None, 4096, 300, L.LM_BF16, L.LM_E2M1, 4096, need - 256,
                             None) == L.LM_EWORKSPACE
@@ -73,7 +73,8 @@ def test_c_entries_refuse_more():
                             None) == L.LM_EINVAL
     for n, k, e, lddy, ldx in ((0, 8, 1, 8, 8), (8, 0, 1, 8, 8), (8, 8, 0, 8, 8), (8, 8, 2, 8, 8), (8, 8, 1, 7, 8),
                                (8, 8, 1, 8, 7)):
-        assert handle.lm_linear_weight_grad(4096, lddy, 4096, ldx, None, 4096, 4, n, k, e, L.LM_BF16, None) == L.LM_EINVAL
+        assert handle.lm_linear_weight_grad(4096, lddy, 4096, ldx, None, 4096, 4, n, k, e, L.LM_BF16, None, 0,
+                                            None) == L.LM_EINVAL
 
 
 def test_cpu_tensors_are_refused():
