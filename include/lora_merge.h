@@ -278,7 +278,7 @@ int lm_routed_residual(const void* x, const void* y, void* out, int64_t T, int64
  * first, as lm_mx_requant with LM_MX_FLOOR does; a block with an infinity or a
  * NaN makes its row NaN.  The input gradient passes straight through that
  * rounding.
- * Strides are in elements; outputs are contiguous; N, K < 2^22.  Workspace:
+ * Strides are in elements; outputs are contiguous; N, K < 2^21.  Workspace:
  * lm_linear_workspace_size bytes for the call's sizes and strides (ldb: ldx of
  * the weight gradient, else 0; aligned: the pointers of rows and weights are
  * multiples of 16), 256-byte aligned; NULL when that is 0. */

@@ -34,6 +34,7 @@ static inline int64_t lin_scale_bytes(int64_t N, int64_t K, int swizzled) {
 }
 
 constexpr int64_t LIN_SPAN = 0x7fffffff;
+constexpr uint32_t LIN_OUT = 0x80000000u;  // an offset past any resource
 
 // a buffer resource over `bytes` bytes: offsets past them (any offset from 2^31
 // on) read zeros
@@ -54,6 +55,9 @@ DEV lm_u32x4 lin_chunk(const uint16_t* p, int64_t left) {
   }
   return v;
 }
+typedef uint32_t lm_u32_any __attribute__((aligned(1)));
+typedef uint32_t lm_u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+
 // ---- groups of rows --------------------------------------------------------
 // Ends that fall, are negative or pass T are clamped to what came before and to
 // T, so no index leaves the tensors whatever the caller's memory holds.  A wave
@@ -248,22 +252,28 @@ DEV lm_u32x4 lin_decode8(uint32_t codes, float scale) {
 
 enum : int { W_DENSE = 0, W_MX = 1, W_Q4 = 2 };
 
-template <int S, int F, int G>
+// byte FA of sa and byte FB of sb are the operands' scales
+template <int FA, int FB>
 DEV v4f32 lin_mfma4_(lm_u32x4 a, lm_u32x4 b, v4f32 c, uint32_t sa, uint32_t sb) {
   typedef int v8i32 __attribute__((ext_vector_type(8)));
   const v8i32 x = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}, y = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, 2 * F + S, (int)sa, 2 * G + S, (int)sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, FA, (int)sa, FB, (int)sb);
 }
-// step s; f, g: which of a word's two fragments the scales belong to
-DEV v4f32 lin_mfma4(lm_u32x4 a, lm_u32x4 b, v4f32 c, uint32_t sa, uint32_t sb, int s, int f, int g) {
-  switch (4 * s + 2 * f + g) {
-    case 0: return lin_mfma4_<0, 0, 0>(a, b, c, sa, sb);
-    case 1: return lin_mfma4_<0, 0, 1>(a, b, c, sa, sb);
-    case 2: return lin_mfma4_<0, 1, 0>(a, b, c, sa, sb);
-    case 3: return lin_mfma4_<0, 1, 1>(a, b, c, sa, sb);
-    case 4: return lin_mfma4_<1, 0, 0>(a, b, c, sa, sb);
-    case 5: return lin_mfma4_<1, 0, 1>(a, b, c, sa, sb);
-    case 6: return lin_mfma4_<1, 1, 0>(a, b, c, sa, sb);
-    default: return lin_mfma4_<1, 1, 1>(a, b, c, sa, sb);
+template <int FA>
+DEV v4f32 lin_mfma4_(lm_u32x4 a, lm_u32x4 b, v4f32 c, uint32_t sa, uint32_t sb, int fb) {
+  switch (fb) {
+    case 0: return lin_mfma4_<FA, 0>(a, b, c, sa, sb);
+    case 1: return lin_mfma4_<FA, 1>(a, b, c, sa, sb);
+    case 2: return lin_mfma4_<FA, 2>(a, b, c, sa, sb);
+    default: return lin_mfma4_<FA, 3>(a, b, c, sa, sb);
+  }
+}
+// (fa, fb known at compile time once the callers' loops are unrolled)
+DEV v4f32 lin_mfma4(lm_u32x4 a, lm_u32x4 b, v4f32 c, uint32_t sa, uint32_t sb, int fa, int fb) {
+  switch (fa) {
+    case 0: return lin_mfma4_<0>(a, b, c, sa, sb, fb);
+    case 1: return lin_mfma4_<1>(a, b, c, sa, sb, fb);
+    case 2: return lin_mfma4_<2>(a, b, c, sa, sb, fb);
+    default: return lin_mfma4_<3>(a, b, c, sa, sb, fb);
   }
 }

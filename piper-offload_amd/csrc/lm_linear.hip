@@ -19,15 +19,15 @@
 // wave (8 values a lane: 16 bytes in, 4 out, a block's maximum over 4 lanes
 // by DPP), the others one packed piece of weight scales per wave.
 // ---------------------------------------------------------------------------
-// byte of (slot, block) in the packed scales: pieces of 64 slots x 8 blocks
+// byte of (slot, block) in the packed scales: pieces of 64 slots x 4 blocks
 DEV int64_t lin_packed(int64_t slot, int64_t block, int64_t nk) {
-  const int f = (int)(slot >> 4) & 3, r = (int)slot & 15, g = (int)(block & 7) >> 1;
-  return ((slot >> 6) * nk + (block >> 3)) * 512 + (16 * g + r) * 8 + 2 * f + (block & 1);
+  const int f = (int)(slot >> 4) & 3, r = (int)slot & 15, g = (int)block & 3;
+  return ((slot >> 6) * nk + (block >> 2)) * 256 + (16 * g + r) * 4 + f;
 }
 template <int DT>
 __global__ __launch_bounds__(256) void k_lin_prep4(LinArgs a, int row_blocks, uint8_t* xq, uint8_t* xs, uint8_t* wsc) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t nk = (a.K + 255) >> 8, nb = a.K >> 5;
+  const int64_t nk = (a.K + 127) >> 7, nb = a.K >> 5;
   if ((int)blockIdx.x < row_blocks) {
     const int64_t t = (int64_t)blockIdx.x * 4 + wave_index();
     if (t >= a.T) return;
@@ -38,7 +38,7 @@ __global__ __launch_bounds__(256) void k_lin_prep4(LinArgs a, int row_blocks, ui
       if (g == a.experts) return;  // a row of no group
     }
     const uint16_t* x = (const uint16_t*)a.a + t * a.lda;
-    const int64_t units = a.K >> 3, padded = nk * 32;
+    const int64_t units = a.K >> 3, padded = nk * 16;
     for (int64_t u = lane; u < padded; u += 64) {
       lm_u32x4 w = {};
       if (u < units) w = *(const LM_GLOBAL lm_u32x4_any*)(x + u * 8);
@@ -52,19 +52,14 @@ __global__ __launch_bounds__(256) void k_lin_prep4(LinArgs a, int row_blocks, ui
     const int64_t gj = (a.N + 63) >> 6, piece = (int64_t)(blockIdx.x - row_blocks) * 4 + wave;
     if (piece >= gj * nk * a.experts) return;
     const int64_t kt = piece % nk, eg = piece / nk, e = eg / gj, n0 = (eg % gj) * 64;
-    const int g = lane >> 4;
-    uint16_t s[4];
+    const int64_t b = kt * 4 + (lane >> 4);
+    uint32_t s = 0;
 #pragma unroll
     for (int f = 0; f < 4; ++f) {
-      const int64_t n = n0 + lin_jcol(16 * f + (lane & 15));
-      s[f] = 0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t b = kt * 8 + 2 * g + h;
-        if (n < a.N && b < nb) s[f] |= (uint16_t)(a.scale[e * a.scale_stride + blocked_offset(n, b, nb, a.swizzled)] << (8 * h));
-      }
+      const int64_t n = n0 + 16 * f + (lane & 15);
+      if (n < a.N && b < nb) s |= (uint32_t)a.scale[e * a.scale_stride + blocked_offset(n, b, nb, a.swizzled)] << (8 * f);
     }
-    *(LM_GLOBAL lm_u32x2*)(wsc + piece * 512 + lane * 8) = lm_u32x2{s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16};
+    *(LM_GLOBAL uint32_t*)(wsc + piece * 256 + lane * 4) = s;
   }
 }
 
@@ -80,7 +75,7 @@ static int check_lin(const lm_weight* w, int64_t T, int32_t dtype, const int32_t
   if (!w) return LM_OK;
   if (!w->q) return fail(LM_EINVAL, "weight pointer must be non-null");
   if (w->N <= 0 || w->K <= 0) return fail(LM_EINVAL, "empty weight");
-  if (w->N >= (1 << 22) || w->K >= (1 << 22)) return fail(LM_EUNSUPPORTED, "products take rows and columns below 2^22");
+  if (w->N >= (1 << 21) || w->K >= (1 << 21)) return fail(LM_EUNSUPPORTED, "products take rows and columns below 2^21");
   if (w->dtype == LM_E2M1) {
     if (!w->scale) return fail(LM_EINVAL, "MXFP4 weight without scales");
     if (w->K % 32 != 0) return fail(LM_EINVAL, "MXFP4 requires columns divisible by 32, got %lld", (long long)w->K);
@@ -134,7 +129,7 @@ static LinPlan lin_plan(int op, int64_t T, int64_t lda, int64_t ldb, int64_t N, 
   const int64_t rows = (T + E - 1) / E;  // of an average group
   p.few = op == LIN_FORWARD && lin_few(T, N, E, mx, quant);
   const int64_t inner = op == LIN_FORWARD ? K : N;  // elements of a row of a
-  const bool whole = aligned && lda % 8 == 0 && lda < (1 << 22);
+  const bool whole = aligned && lda % 8 == 0 && lda < (1 << 21);
   const bool wwhole = aligned && K % 8 == 0;
   p.lda = lda;
   p.ldb = ldb;
@@ -147,10 +142,10 @@ static LinPlan lin_plan(int op, int64_t T, int64_t lda, int64_t ldb, int64_t N, 
     return o;
   };
   if (p.few) {
-    p.copy_a = lda >= (1 << 22);
+    p.copy_a = lda >= (1 << 21);
   } else if (!quant) {
     p.copy_a = !whole || (op != LIN_WEIGHT_GRAD && inner % 8);
-    p.copy_b = op == LIN_WEIGHT_GRAD && (!aligned || ldb % 8 || ldb >= (1 << 22));
+    p.copy_b = op == LIN_WEIGHT_GRAD && (!aligned || ldb % 8 || ldb >= (1 << 21));
     p.copy_w = op != LIN_WEIGHT_GRAD && !mx && !wwhole;
     if (op != LIN_WEIGHT_GRAD) p.len = round8(inner);
   }
@@ -167,11 +162,11 @@ static LinPlan lin_plan(int op, int64_t T, int64_t lda, int64_t ldb, int64_t N, 
     p.w = take((size_t)E * N * p.ldw * 2);
   }
   if (quant) {
-    const int64_t nk = (K + 255) / 256;
+    const int64_t nk = (K + 127) / 128;
     p.padded = (T + 63) / 64 + E;
     p.xq = take((size_t)(p.padded * 64) * (size_t)(K / 2));
-    p.xs = take((size_t)(p.padded * nk) * 512);
-    p.wsc = take((size_t)(E * ((N + 63) / 64) * nk) * 512);
+    p.xs = take((size_t)(p.padded * nk) * 256);
+    p.wsc = take((size_t)(E * ((N + 63) / 64) * nk) * 256);
   }
   p.splits = 1;
   if (!p.few) {
@@ -179,15 +174,15 @@ static LinPlan lin_plan(int op, int64_t T, int64_t lda, int64_t ldb, int64_t N, 
     const int64_t big = I / 256 * ((J + 255) / 256) * (op == LIN_WEIGHT_GRAD ? E : 1);
     p.tile = big >= 192 && (op == LIN_WEIGHT_GRAD || rows >= 256) ? 256 : 128;
     // Fewer tiles than CUs: the contraction is split so that two workgroups a CU
-    // run, into parts of 4 tiles and more (8 of 4-bit inputs, whose tiles are four
+    // run, into parts of 8 stages and more (16 of 4-bit inputs, whose stages are four
     // times as deep).  [4096, 4096] at 64 rows, us whole / split: forward 61 / 20,
     // input gradient 69 / 21.
     const int64_t gi = op == LIN_WEIGHT_GRAD ? (N + 127) / 128 * E : (T + 127) / 128 + (E - 1) / 2;
     const int64_t tiles = gi * ((J + 127) / 128);
-    const int64_t nk = ((op == LIN_WEIGHT_GRAD ? rows : p.len) + (quant ? 255 : 63)) / (quant ? 256 : 64);
+    const int64_t nk = ((op == LIN_WEIGHT_GRAD ? rows : p.len) + (quant ? 127 : 31)) / (quant ? 128 : 32);
     if (p.tile == 128 && tiles < 256) {
       int64_t s = 512 / tiles;
-      const int64_t most = nk / (quant ? 8 : 4);
+      const int64_t most = nk / (quant ? 16 : 8);
       if (s > most) s = most;
       if (s > 16) s = 16;
       if (s > 1) {
@@ -341,7 +336,7 @@ extern "C" int lm_linear(const void* x, int64_t ldx, const lm_weight* w, const v
     TimedLaunch timed("linear_prep", st);
     const int segs = (int)((a.K + 2047) / 2048);
     const int64_t rows = (p.few ? T * segs : T + 3) / 4 + (p.few ? 1 : 0);
-    const int64_t pieces = p.few ? 0 : (a.experts * ((a.N + 63) / 64) * ((a.K + 255) / 256) + 3) / 4;
+    const int64_t pieces = p.few ? 0 : (a.experts * ((a.N + 63) / 64) * ((a.K + 127) / 128) + 3) / 4;
     if (rows + pieces > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
     const dim3 grid((unsigned)(rows + pieces));
     if (p.few) {
@@ -381,7 +376,7 @@ extern "C" int lm_linear_weight_grad(const void* dy, int64_t lddy, const void* x
   int rc;
   if ((rc = check_lin(nullptr, T, dtype, ends, experts))) return rc;
   if (N <= 0 || K <= 0) return fail(LM_EINVAL, "empty weight gradient");
-  if (N >= (1 << 22) || K >= (1 << 22)) return fail(LM_EUNSUPPORTED, "products take rows and columns below 2^22");
+  if (N >= (1 << 21) || K >= (1 << 21)) return fail(LM_EUNSUPPORTED, "products take rows and columns below 2^21");
   if (!dw || (T > 0 && (!dy || !x))) return fail(LM_EINVAL, "pointers must be non-null");
   if (lddy < N || ldx < K) return fail(LM_EINVAL, "row stride below the row length");
   hipStream_t st = (hipStream_t)stream;

@@ -33,13 +33,9 @@ DEV void lin_transpose4(lm_u32x4& d) {
   const auto q = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
   d = lm_u32x4{p[0], p[1], q[0], q[1]};
 }
-typedef uint32_t lm_u32_any __attribute__((aligned(1)));
-typedef uint32_t lm_u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
-
 DEV lm_u32x4 few_load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
   return __builtin_bit_cast(lm_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
 }
-constexpr uint32_t FEW_OUT = 0x80000000u;  // past any resource (lin_rsrc)
 
 // rows of x to MXFP4 in row order: codes [T, K/2], scales [T, padded to 4]
 template <int DT>
@@ -124,7 +120,7 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few(LinArgs a) {
             } else {
               const uint32_t o = wo[c] + u * (W == W_DENSE ? 256 : 64) + 64 * j;
               const bool in = W == W_DENSE ? u * 128 + 32 * j + 8 * g < a.K : u * 4 + g < nb;
-              wv[i][c][j] = few_load16(rw, TAIL && !in ? FEW_OUT : o);
+              wv[i][c][j] = few_load16(rw, TAIL && !in ? LIN_OUT : o);
             }
           }
           if constexpr (W != W_DENSE) {  // scales of blocks 4u .. 4u + 3, zeros past the last
@@ -165,11 +161,11 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few(LinArgs a) {
             } else {
               const uint32_t o = xo[m] + u * (Q4 ? 64 : 256) + 64 * j;
               const bool in = Q4 ? u * 4 + g < nb : u * 128 + 32 * j + 8 * g < a.K;
-              xv[i][m][j] = few_load16(rx, TAIL && !in ? FEW_OUT : o);
+              xv[i][m][j] = few_load16(rx, TAIL && !in ? LIN_OUT : o);
             }
           }
           if constexpr (Q4)
-            xs[i][m] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rxs, (int)(TAIL && u * 4 >= nb ? FEW_OUT : xso[m] + u * 4), 0, 0);
+            xs[i][m] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rxs, (int)(TAIL && u * 4 >= nb ? LIN_OUT : xso[m] + u * 4), 0, 0);
         }
       }
 #pragma unroll
@@ -179,7 +175,7 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few(LinArgs a) {
           for (int c = 0; c < CF; ++c)
 #pragma unroll
             for (int m = 0; m < MF; ++m)
-              acc[i % AC][m][c] = lin_mfma4(wv[i][c][0], xv[i][m][0], acc[i % AC][m][c], sv[i][c] >> (8 * g), xs[i][m] >> (8 * g), 0, 0, 0);
+              acc[i % AC][m][c] = lin_mfma4(wv[i][c][0], xv[i][m][0], acc[i % AC][m][c], sv[i][c] >> (8 * g), xs[i][m] >> (8 * g), 0, 0);
         } else {
 #pragma unroll
           for (int c = 0; c < CF; ++c) {

@@ -1,53 +1,95 @@
 // lm_linear_mm.h -- products of many rows: LDS-tiled MFMA kernels.
 //
-// An output tile of BM rows x BN columns per workgroup, the contraction in
-// tiles of 64, two LDS buffers: while the waves multiply tile k out of one, the
-// loads of tile k + 1 are on their way into the other (buffer loads straight
-// to LDS, no registers in between).  One barrier a tile.
+// An output tile of BM rows x BN columns per workgroup.  The contraction goes by
+// in stages of one MFMA step (32 values; 128 with 4-bit inputs), four LDS
+// buffers deep: a stage's loads (buffer loads straight to LDS, no registers in
+// between) are issued three stages before its multiplication.
 //
 // Operands are named by the output index they carry: I (rows) and J
 // (columns).  Their tiles lie in LDS as
-//   KC16  contraction contiguous in memory: a slot of 128 bytes per I/J index,
-//         its eight 16-byte chunks rotated by XOR with slot & 7, so that the
-//         16 lanes that read one chunk of 16 slots hit all banks
+//   KC16  contraction contiguous in memory: a slot of 64 bytes per I/J index,
+//         its four 16-byte chunks in an order that depends on the slot (mm_key)
 //   KS16  contraction strided (the index contiguous): a row per contraction
-//         step; read transposed (ds_read_b64_tr_b16); chunks XORed with
-//         4 (row & 3) for the same reason
-//   KC4   MXFP4 codes as they are stored, 32 bytes per slot, decoded to 16 bits
+//         step; read transposed (ds_read_b64_tr_b16); chunks XORed with a key
+//         of the row (mm_row_key)
+//   KC4   MXFP4 codes as they are stored, 16 bytes per slot, decoded to 16 bits
 //         after the read (v_cvt_scalef32_pk: exact products in bf16)
 //   KS4   MXFP4 with the contraction strided: every code of a run of 32 shares a
 //         scale but the 8 codes of an MFMA lane do not, so these are decoded on
 //         their way into LDS and then are KS16
 // Q4: both operands MXFP4 (x quantised beforehand), multiplied as they are by the
-// scaled MFMA, 256 codes a tile, so a slot is 128 bytes here too.  Its scales
-// come packed by k_lin_prep4: per 64 slots and tile 512 bytes, which hold for
-// lane (r, g) the blocks 2g and 2g + 1 of slots r, r + 16, r + 32, r + 48 side by
-// side: one 8-byte read gives the scales of four fragments and both steps.
-// The MFMA's first operand is J, so a lane's accumulators are consecutive output
-// columns; the columns of a pair of 16-column fragments are interleaved in
-// fours, which makes them 8 in a row: one 16-byte store.
+// scaled MFMA, 128 codes a stage, so a slot is 64 bytes here too.  Its scales
+// come packed by k_lin_prep4: per 64 slots and stage 256 bytes, which hold for
+// lane (r, g) block g of slots r, r + 16, r + 32, r + 48: one 4-byte read gives
+// the scales of four fragments.
+// The MFMA's first operand is J, so a lane's four accumulators are consecutive
+// output columns; before the store two neighbouring fragments trade halves
+// between lane groups, which makes them 8 in a row: one 16-byte store.
+//
+// Eight waves (256 x 256): two on a SIMD.  If both read their fragments at the
+// same time and then both multiply, LDS and the matrix unit take turns
+// (measured: 1.24 PFLOP/s at most).  So the waves of the second half run one
+// barrier behind those of the first: while one wave of a SIMD reads, the other
+// multiplies.  Four waves (128 x 128): the two workgroups of a CU do that by
+// themselves.
 #pragma once
 #include "lm_linear.h"
 
 enum : int { KC16, KS16, KC4, KS4 };
 
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef __attribute__((address_space(3))) uint32_t lds_u32;
 typedef __attribute__((address_space(3))) lm_u32x4 lds_u32x4;
-typedef __attribute__((address_space(3))) lm_u32x2 lds_u32x2;
 typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
 
 // 16 bytes per lane to LDS at base + 16 lane; past the resource's end: zeros
 DEV void lin_dma(__amdgpu_buffer_rsrc_t r, lds_u8* base, uint32_t off) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)base, 16, (int)off, 0, 0, 0);
 }
+// a barrier of the workgroup that waits for no memory by itself
+DEV void lin_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+// wait until at most N vector-memory operations and no LDS operation are left
+template <int N>
+DEV void lin_wait() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
 
-// Slot of a J tile -> column: pairs of fragments of 16 interleaved in fours
-DEV int lin_jcol(int slot) { return (slot & ~31) + 8 * ((slot & 15) >> 2) + (slot & 3) + 4 * ((slot >> 4) & 1); }
+// LDS serves a 16-byte read of a wave 16 lanes at a time, lanes 0-3, 12-15 and
+// 20-27 first, then 4-11, 16-19 and 28-31, and the same in the upper half.  A slot
+// is a quarter of the 64 banks, so four slots (p & 3) share them out and the
+// four groups of slots (p >> 2) that are served together have to find their
+// chunks in four different places: chunk c lies at c ^ (2 (p >> 2) in GF(4)).
+// With c ^ (p >> 2), right for lanes taken in order, half the cycles are
+// conflicts (SQ_LDS_BANK_CONFLICT).
+DEV int mm_key(int slot) { return (((slot >> 2) << 1) & 2) ^ (((slot >> 3) & 1) * 3); }
+// A transposed read takes 32 bytes each of rows 0-3 and 8-11 (then 16-19 and
+// 24-27) together: eight pairs of chunks, one of each in all 64 banks.
+DEV int mm_row_key(int row) { return ((row & 3) | ((row >> 1) & 4)) << 1; }
 
-// The tile of this workgroup: group, first row, end of the group's rows, number of
-// the column tile.  Tiles of up to 8 row tiles x all columns, row tiles
-// first, are neighbours; each XCD takes a contiguous part of them, so its L2
-// holds the weight tiles that several row tiles share.
+// Tiles of up to 8 row tiles x all columns, row tiles first, are neighbours, and
+// each XCD takes a contiguous part of them, so its L2 holds the tiles of the
+// other operand that several row tiles share.
+DEV bool lin_order(uint32_t b, uint32_t tm, uint32_t tn, uint32_t& m, uint32_t& n) {
+  const uint32_t total = tm * tn;
+  if (b >= total) return false;
+  const uint32_t u = (uint32_t)xcd_unit(b, total), band = u / (8 * tn), in = u - band * 8 * tn;
+  const uint32_t left = tm - band * 8, h = left < 8 ? left : 8;
+  m = band * 8 + in % h;
+  n = in / h;
+  return true;
+}
+// The tile of this workgroup: group, first row, end of the group's rows, first
+// column.
 struct LinTile {
   int group;
   int64_t r0, r1, j0;
@@ -55,111 +97,100 @@ struct LinTile {
 };
 template <int BM, int BN>
 DEV bool lin_pick(const LinArgs& a, int64_t jend, LinTile& t) {
-  const int gn = (int)((jend + BN - 1) / BN);
-  int tiles;
-  if (!a.ends) tiles = (int)((a.T + BM - 1) / BM);
-  else tiles = lin_count<BM>(a);
-  const uint32_t total = (uint32_t)tiles * (uint32_t)gn;
-  if (blockIdx.x >= total) return false;
-  const uint32_t u = xcd_unit(blockIdx.x, total);
-  constexpr uint32_t GM = 8;
-  const uint32_t band = u / (GM * gn), in = u - band * GM * gn;
-  const uint32_t left = (uint32_t)tiles - band * GM, h = left < GM ? left : GM;
-  const uint32_t tm = band * GM + in % h, tn = in / h;
-  t.j0 = (int64_t)tn * BN;
-  if (!a.ends) {
-    t.group = 0;
-    t.pad = t.r0 = (int64_t)tm * BM;
-    t.r1 = a.T;
-    return true;
-  }
-  return lin_find<BM>(a, (int)tm, t.group, t.r0, t.r1, t.pad);
+  uint32_t m, n;
+  const uint32_t tiles = a.ends ? (uint32_t)lin_count<BM>(a) : (uint32_t)((a.T + BM - 1) / BM);
+  if (!lin_order(blockIdx.x, tiles, (uint32_t)((jend + BN - 1) / BN), m, n)) return false;
+  t.j0 = (int64_t)n * BN;
+  if (a.ends) return lin_find<BM>(a, (int)m, t.group, t.r0, t.r1, t.pad);
+  t.group = 0;
+  t.pad = t.r0 = (int64_t)m * BM;
+  t.r1 = a.T;
+  return true;
 }
 
 template <int DT, int OP, int W, int BM, int BN, int WM, int WN>
 struct MmTraits {
   static constexpr bool Q4 = W == W_Q4, MX = W == W_MX;
-  static constexpr int CT = Q4 ? 256 : 64;                        // contraction of a tile
-  static constexpr int IS = Q4 ? BM * 8 : 16, JS = Q4 ? BN * 8 : 16;  // bytes of the scales of a tile
   static constexpr int NW = WM * WN, NT = NW * 64;
+  static constexpr int CS = Q4 ? 128 : 32;  // contraction of a stage
   static constexpr int IK = OP == LIN_WEIGHT_GRAD ? KS16 : KC16;
   static constexpr int JK = OP == LIN_FORWARD ? (MX ? KC4 : KC16) : (OP == LIN_INPUT_GRAD && MX ? KS4 : KS16);
   static constexpr int FI = BM / WM / 16, FJ = BN / WN / 16;
-  static constexpr int IB = BM * 128, JB = JK == KC4 ? BN * 32 : BN * 128;  // bytes of a tile
-  static constexpr int IL = IB / 1024 / NW, JL = JB / 1024 / NW;            // loads per wave
-  static_assert(IL * 1024 * NW == IB && JL * 1024 * NW == JB, "tiles are whole loads of all waves");
-  static_assert(JK != KS4 || NT * 32 == 64 * BN, "a run of 32 codes per thread");
-  // chunk c of contraction 8-groups that lane group g takes in MFMA step s: with
-  // KC4 a lane reads the codes of both steps at once, with Q4 their scales, so they
-  // are neighbours
-  DEV static int chunk(int s, int g) { return JK == KC4 || Q4 ? 2 * g + s : 4 * s + g; }
+  static constexpr int IB = BM * 64, JB = JK == KC4 ? BN * 16 : BN * 64;  // bytes of a stage
+  static constexpr int IL = IB / 1024 / NW;                               // loads per wave
+  static constexpr int JL = JK == KS4 ? 2 : (JB / 1024 + NW - 1) / NW;
+  static constexpr int SB = Q4 ? NW * 256 : 16;  // bytes of a stage's scales: I's, then J's
+  static_assert(!Q4 || BM / 64 + BN / 64 == NW, "a piece of scales per wave");
+  static_assert(IL * 1024 * NW == IB, "tiles are whole loads of all waves");
+  static_assert(JK != KC4 || JB == NW * 512, "KC4: half a load per wave");
+  static_assert(JK != KS4 || NT * 16 == 32 * BN, "KS4: half a run of 32 codes per thread");
 };
 
-// per-lane byte offsets of the DMA loads of one operand tile
-template <int KIND, int B, int L, int NW, bool PERM>
+// per-lane byte offsets of the DMA loads of one operand's stage
+template <int KIND, int B, int L, int NW>
 DEV void mm_offsets(uint32_t (&off)[L], int wave, int lane, int64_t ld) {
 #pragma unroll
   for (int n = 0; n < L; ++n) {
     const int piece = (n * NW + wave) * 64 + lane;  // 16-byte piece of the tile
-    if constexpr (KIND == KC16) {
-      const int slot = piece >> 3, c = (piece & 7) ^ (slot & 7);
-      off[n] = (uint32_t)((PERM ? lin_jcol(slot) : slot) * ld * 2) + c * 16;
-    } else if constexpr (KIND == KC4) {
-      const int slot = piece >> 1;
-      off[n] = (uint32_t)(lin_jcol(slot) * (ld >> 1)) + (piece & 1) * 16;
-    } else {  // KS16
-      const int row = piece / (B / 8), c = (piece % (B / 8)) ^ ((row & 3) << 2);
-      off[n] = (uint32_t)(row * ld * 2) + c * 16;
-    }
+    if constexpr (KIND == KC16) off[n] = (uint32_t)((piece >> 2) * ld * 2) + ((piece & 3) ^ mm_key(piece >> 2)) * 16;
+    else if constexpr (KIND == KC4) off[n] = (uint32_t)((wave * 32 + (lane & 31)) * (ld >> 1));
+    else off[n] = (uint32_t)(piece / (B / 8) * ld * 2) + ((piece % (B / 8)) ^ mm_row_key(piece / (B / 8))) * 16;
   }
 }
 
+// The fragments of a stage: per lane one LDS offset (mm_at), and 8 contraction
+// steps (chunk g) of this lane's index of fragment f from there.  KS16 reads
+// transposed, two loads of 4 steps: lane p of 16 points at 4 indices of row p >> 2.
 template <int KIND, int B>
-DEV lm_u32x4 mm_frag(const lds_u8* t, int slot0, int f, int lane, int s, int c) {
-  if constexpr (KIND == KC16) {
-    const int slot = slot0 + f * 16 + (lane & 15);
-    return *(const lds_u32x4*)(t + slot * 128 + ((c ^ (slot & 7)) << 4));
-  } else {
-    return lm_u32x4{};
-  }
+DEV uint32_t mm_at(int slot0, int lane) {
+  const int p = lane & 15, g = lane >> 4;
+  if constexpr (KIND == KC16) return (slot0 + p) * 64 + ((g ^ mm_key(p)) << 4);
+  else if constexpr (KIND == KC4) return (slot0 + p) * 16 + g * 4;
+  const int row = 8 * g + (p >> 2), chunk = (slot0 >> 3) + ((p >> 1) & 1);
+  return row * (B * 2) + ((chunk ^ mm_row_key(row)) << 4 | (p & 1) << 3);
 }
-// 8 contraction steps x this lane's index, read transposed: two loads of 4 steps
-// each.  Lane p of 16 points at 4 indices of row p >> 2.
-template <int B, bool PERM>
-DEV lm_u32x4 mm_frag_tr(const lds_u8* t, int col0, int f, int lane, int s) {
-  const int p = lane & 15, g = lane >> 4, q = p & 3;
-  const int row = 32 * s + 8 * g + (p >> 2);
-  const int col = col0 + (PERM ? (f >> 1) * 32 + 8 * q + 4 * (f & 1) : f * 16 + 4 * q);
-  const int at = row * (B * 2) + ((((col >> 3) ^ ((row & 3) << 2)) << 4) | ((col & 4) << 1));
-  const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(t + at));
-  const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(t + at + 4 * (B * 2)));  // row + 4: same XOR
+template <int KIND, int B>
+DEV lm_u32x4 mm_frag(const lds_u8* t, uint32_t at, int f) {
+  if constexpr (KIND == KC16) return *(const lds_u32x4*)(t + at + f * 1024);
+  const uint32_t o = at ^ (f << 5);  // two chunks on
+  const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(t + o));
+  const v4i16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(t + o + 4 * (B * 2)));  // row + 4: same key
   return lm_u32x4{__builtin_bit_cast(lm_u32x2, lo)[0], __builtin_bit_cast(lm_u32x2, lo)[1],
                   __builtin_bit_cast(lm_u32x2, hi)[0], __builtin_bit_cast(lm_u32x2, hi)[1]};
+}
+// The compiler would keep this value plus every buffer's address in a register
+// of its own across the loop; like this it adds the buffer's offset in the read.
+DEV uint32_t mm_hide(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 template <int DT, int OP, int W, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
   using P = MmTraits<DT, OP, W, BM, BN, WM, WN>;
-  constexpr bool HALF = DT == F16, Q4 = P::Q4, MX = P::MX;
-  constexpr int CT = P::CT;
-  constexpr int FI = P::FI, FJ = P::FJ;
-  __shared__ __attribute__((aligned(1024))) uint8_t si0[P::IB], si1[P::IB], sj0[P::JB], sj1[P::JB];
-  __shared__ __attribute__((aligned(1024))) uint8_t sis0[P::IS], sis1[P::IS], sjs0[P::JS], sjs1[P::JS];
+  constexpr bool HALF = DT == F16, Q4 = P::Q4, PP = P::NW == 8;
+  constexpr int CS = P::CS, FI = P::FI, FJ = P::FJ, IK = P::IK, JK = P::JK;
+  // (separate arrays: the compiler then knows that a read of one stage need not
+  // wait for the loads of another)
+  __shared__ __attribute__((aligned(1024))) uint8_t si0[P::IB], si1[P::IB], si2[P::IB], si3[P::IB];
+  __shared__ __attribute__((aligned(1024))) uint8_t sj0[P::JB], sj1[P::JB], sj2[P::JB], sj3[P::JB];
+  __shared__ __attribute__((aligned(1024))) uint8_t ss0[P::SB], ss1[P::SB], ss2[P::SB], ss3[P::SB];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = wave_index();
   const int wi = wave / WN, wj = wave % WN;
   const int64_t jend = OP == LIN_FORWARD ? a.N : a.K;
   LinTile t;
   int64_t len;  // of the contraction
   const uint8_t *ip, *jp;
-  int64_t ibytes, jbytes, istep, jstep;  // bytes of the resources, and per tile of 64
+  int64_t ibytes, jbytes, istep, jstep;  // bytes of the resources, and per stage
   int64_t lda = a.lda, ldb;
   if constexpr (OP == LIN_WEIGHT_GRAD) {
-    const int gm = (int)((a.N + BM - 1) / BM);
+    uint32_t m, n;
+    if (!lin_order(blockIdx.x, (uint32_t)((a.N + BM - 1) / BM), (uint32_t)((a.K + BN - 1) / BN), m, n)) return;
     t.group = blockIdx.y;
-    t.r0 = (int64_t)(blockIdx.x % gm) * BM;
+    t.r0 = (int64_t)m * BM;
     t.r1 = a.N;
-    t.j0 = (int64_t)(blockIdx.x / gm) * BN;
+    t.j0 = (int64_t)n * BN;
     int64_t b, e;
     lin_group(a, t.group, b, e);
     len = e - b;
@@ -169,8 +200,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
     // (whole pieces of 16 bytes: what a piece holds past the row's end goes to columns that are not stored)
     ibytes = (((len - 1) * lda + a.N - t.r0) * 2 + 15) & ~(int64_t)15;
     jbytes = (((len - 1) * ldb + a.K - t.j0) * 2 + 15) & ~(int64_t)15;
-    istep = 128 * lda;
-    jstep = 128 * ldb;
+    istep = 2 * CS * lda;
+    jstep = 2 * CS * ldb;
   } else {
     if (!lin_pick<BM, BN>(a, jend, t)) return;
     len = t.group == a.experts ? 0 : a.len;
@@ -182,7 +213,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
       ip = (const uint8_t*)a.a + t.r0 * lda * 2;
       ibytes = ((t.r1 - t.r0 - 1) * lda + len) * 2;
     }
-    istep = 128;
+    istep = 64;
     constexpr bool MX = P::MX || Q4;
     const int64_t ldw = MX ? a.K : a.ldw;
     ldb = Q4 ? a.K >> 2 : ldw;
@@ -190,179 +221,246 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
     const int64_t count = OP == LIN_FORWARD ? (a.N - t.j0) * ldw : a.N * ldw - t.j0;
     jp = (const uint8_t*)a.w + (MX ? first >> 1 : first * 2);
     jbytes = MX ? count >> 1 : count * 2;
-    jstep = OP == LIN_FORWARD ? (P::MX ? 32 : 128) : 64 * (MX ? ldw >> 1 : ldw * 2);
+    jstep = OP == LIN_FORWARD ? (P::MX ? 16 : 64) : CS * (MX ? ldw >> 1 : ldw * 2);
   }
-  // tiles [kb, ke) of nk: this workgroup's part where the contraction is split
-  const int nk = (int)((len + CT - 1) / CT);
+  // stages [kb, ke) of nk: this workgroup's part where the contraction is split
+  const int nk = (int)((len + CS - 1) / CS);
   const int splits = OP == LIN_WEIGHT_GRAD ? gridDim.z : gridDim.y, split = OP == LIN_WEIGHT_GRAD ? blockIdx.z : blockIdx.y;
-  const int per = (nk + splits - 1) / splits, kb = split * per, ke = kb + per < nk ? kb + per : nk;
+  const int per = ((nk + splits - 1) / splits + 3) & ~3, kb = split * per, ke = kb + per < nk ? kb + per : nk;
   v4f32 acc[FI][FJ] = {};
 
   if (kb < ke) {
     uint32_t io[P::IL], jo[P::JL];
-    mm_offsets<P::IK, BM, P::IL, P::NW, false>(io, wave, lane, lda);
-    if constexpr (P::JK != KS4) mm_offsets<P::JK, BN, P::JL, P::NW, true>(jo, wave, lane, ldb);
-    // scales of KC4: per fragment column, the byte of block 2 kt + (g >> 1)
-    const uint8_t* sp = MX ? a.scale + t.group * a.scale_stride : nullptr;
-    uint32_t so[P::JK == KC4 ? FJ : 1];
-    uint32_t sv[P::JK == KC4 ? FJ : 1];
-    const int64_t nb = a.K >> 5;
-    if constexpr (P::JK == KC4) {
+    mm_offsets<IK, BM, P::IL, P::NW>(io, wave, lane, lda);
+    if constexpr (JK != KS4) mm_offsets<JK, BN, P::JL, P::NW>(jo, wave, lane, ldb);
+    const int nb = (int)(a.K >> 5);
+    const uint8_t* sp = P::MX ? a.scale + t.group * a.scale_stride : nullptr;
+    // KC4: the scales of four stages, one word per fragment column
+    uint32_t so[JK == KC4 ? FJ : 1], sv[JK == KC4 ? FJ : 1], sn[JK == KC4 ? FJ : 1];
+    const int64_t stile = a.swizzled ? (t.j0 >> 7) * ((nb + 3) >> 2) * 512 : t.j0 * nb;
+    const uint32_t sleft = a.scale_stride - stile > LIN_SPAN ? (uint32_t)LIN_SPAN : (uint32_t)(a.scale_stride - stile);
+    if constexpr (JK == KC4) {
 #pragma unroll
       for (int f = 0; f < FJ; ++f) {
-        int64_t n = t.j0 + wj * (FJ * 16) + lin_jcol(f * 16 + (lane & 15));
-        if (n >= a.N) n = a.N - 1;
+        int n = wj * (FJ * 16) + f * 16 + (lane & 15);
+        if (t.j0 + n >= a.N) n = (int)(a.N - 1 - t.j0);
         so[f] = a.swizzled ? (uint32_t)((n >> 7) * ((nb + 3) >> 2) * 512 + (n & 31) * 16 + ((n & 127) >> 5) * 4) : (uint32_t)(n * nb);
       }
     }
-    // Q4: packed scales of this tile's 64-slot groups, nk pieces each
-    const uint8_t *isp = nullptr, *jsp = nullptr;
-    int64_t isbytes = 0, jsbytes = 0;
-    if constexpr (Q4) {
-      const int64_t gj = (a.N + 63) >> 6;
-      isp = a.xs + (t.pad >> 6) * nk * 512;
-      isbytes = (a.padded - (t.pad >> 6)) * nk * 512;
-      jsp = a.wsc + (t.group * gj + (t.j0 >> 6)) * nk * 512;
-      jsbytes = (gj - (t.j0 >> 6)) * nk * 512;
-    }
-    // KS4: this thread decodes 32 codes of contraction row kr
-    const int kr = tid / (BN / 32), kc = tid % (BN / 32);
-    lm_u32x4 code = {};
-    uint32_t code_s = 0;
-
-    auto load = [&](int kt, lds_u8* ti, lds_u8* tj, lds_u8* tis, lds_u8* tjs) {
-      const __amdgpu_buffer_rsrc_t ri = lin_rsrc(ip + kt * istep, ibytes - kt * istep);
-      const bool cut = (kt + 1) * CT > len;
-      constexpr int PIECE = CT / 8;  // of the contraction in a 16-byte piece of KC16
-#pragma unroll
-      for (int n = 0; n < P::IL; ++n) {
-        uint32_t o = io[n];
-        if (P::IK == KC16 && cut) {  // chunks past the row's end are zeros, not the next row
-          const int piece = (n * P::NW + wave) * 64 + lane;
-          const int c = (piece & 7) ^ ((piece >> 3) & 7);
-          if (kt * CT + c * PIECE >= len) o = 0x80000000u;
-        }
-        lin_dma(ri, ti + (n * P::NW + wave) * 1024, o);
-      }
-      if constexpr (P::JK != KS4) {
-        const __amdgpu_buffer_rsrc_t rj = lin_rsrc(jp + kt * jstep, jbytes - kt * jstep);
-#pragma unroll
-        for (int n = 0; n < P::JL; ++n) {
-          uint32_t o = jo[n];
-          if (P::JK != KS16 && cut) {
-            const int piece = (n * P::NW + wave) * 64 + lane;
-            const int c = P::JK == KC4 ? (piece & 1) * 4 : (piece & 7) ^ ((piece >> 3) & 7);
-            if (kt * CT + c * PIECE >= len) o = 0x80000000u;
-          }
-          lin_dma(rj, tj + (n * P::NW + wave) * 1024, o);
-        }
-      }
-      if constexpr (Q4) {  // 512 bytes per 64 slots: 128 slots a load, a wave each
-        const int h = wave < BM / 128 ? wave : wave - BM / 128;
-        if (wave < BM / 128) lin_dma(lin_rsrc(isp, isbytes), tis + h * 1024, ((2 * h + (lane >> 5)) * nk + kt) * 512 + (lane & 31) * 16);
-        else if (wave < BM / 128 + BN / 128) lin_dma(lin_rsrc(jsp, jsbytes), tjs + h * 1024, ((2 * h + (lane >> 5)) * nk + kt) * 512 + (lane & 31) * 16);
-      }
-    };
-    auto load_scales = [&](int kt) {
-      if constexpr (P::JK == KC4) {
-        int64_t kb = 2 * kt + (g >> 1);
-        if (kb >= nb) kb = nb - 1;
-        const uint32_t at = a.swizzled ? (uint32_t)((kb >> 2) * 512 + (kb & 3)) : (uint32_t)kb;
-#pragma unroll
-        for (int f = 0; f < FJ; ++f) sv[f] = sp[so[f] + at];
-      } else if constexpr (P::JK == KS4) {
-        const int64_t n = (int64_t)kt * 64 + kr, k = t.j0 + kc * 32;
-        code = lm_u32x4{};
-        code_s = 0;
-        if (n < a.N && k < a.K) {
-          code = *(const LM_GLOBAL lm_u32x4*)(jp + n * (a.K >> 1) + kc * 16);
-          code_s = sp[blocked_offset(n, k >> 5, nb, a.swizzled)];
-        }
-      }
-    };
-    auto store_codes = [&](lds_u8* tj) {
-      if constexpr (P::JK == KS4) {
-        const float s = e8m0_value(code_s);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          *(lds_u32x4*)(tj + kr * (BN * 2) + (((kc * 4 + c) ^ ((kr & 3) << 2)) << 4)) = lin_decode8<HALF>(code[c], s);
-      }
-    };
-    auto compute = [&](const lds_u8* ti, const lds_u8* tj, const lds_u8* tis, const lds_u8* tjs, const float* scales) {
-      lm_u32x2 isc[Q4 ? FI / 4 : 1], jsc[Q4 ? FJ / 4 : 1];
-      if constexpr (Q4) {
-#pragma unroll
-        for (int f = 0; f < FI / 4; ++f) isc[f] = *(const lds_u32x2*)(tis + (wi * (FI / 4) + f) * 512 + lane * 8);
-#pragma unroll
-        for (int f = 0; f < FJ / 4; ++f) jsc[f] = *(const lds_u32x2*)(tjs + (wj * (FJ / 4) + f) * 512 + lane * 8);
-      }
-      lm_u32x2 jc[P::JK == KC4 ? FJ : 1];
-      if constexpr (P::JK == KC4) {
-#pragma unroll
-        for (int f = 0; f < FJ; ++f)
-          jc[f] = *(const lds_u32x2*)(tj + (wj * (FJ * 16) + f * 16 + (lane & 15)) * 32 + g * 8);
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        lm_u32x4 fi[FI], fj[FJ];
+    auto load_scales = [&](int st) {  // of stages st .. st + 3: always FJ loads
+      if constexpr (JK == KC4) {
+        const __amdgpu_buffer_rsrc_t rs = lin_rsrc(sp + stile, sleft);
 #pragma unroll
         for (int f = 0; f < FJ; ++f) {
-          if constexpr (P::JK == KC4) fj[f] = lin_decode8<HALF>(jc[f][s], scales[f]);
-          else if constexpr (P::JK == KC16) fj[f] = mm_frag<KC16, BN>(tj, wj * (FJ * 16), f, lane, s, P::chunk(s, g));
-          else fj[f] = mm_frag_tr<BN, true>(tj, wj * (FJ * 16), f, lane, s);
+          uint32_t o = so[f] + (a.swizzled ? st * 128 : st);
+          if (o > sleft - 4) o = sleft - 4;  // (the last word of all: next_scales shifts)
+          sn[f] = __builtin_amdgcn_raw_buffer_load_b32(rs, (int)o, 0, 0);
         }
+      }
+    };
+    auto next_scales = [&](int st) {  // zeros past the row's last block
+      if constexpr (JK == KC4) {
+        const int have = nb - st;
+        const uint32_t mask = have >= 4 ? 0xffffffffu : (have <= 0 ? 0u : (1u << (8 * have)) - 1);
 #pragma unroll
-        for (int f = 0; f < FI; ++f) {
-          if constexpr (P::IK == KC16) fi[f] = mm_frag<KC16, BM>(ti, wi * (FI * 16), f, lane, s, P::chunk(s, g));
-          else fi[f] = mm_frag_tr<BM, false>(ti, wi * (FI * 16), f, lane, s);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int x = 0; x < FI; ++x)
-#pragma unroll
-          for (int y = 0; y < FJ; ++y) {
-            if constexpr (Q4) acc[x][y] = lin_mfma4(fj[y], fi[x], acc[x][y], jsc[y >> 2][(y >> 1) & 1], isc[x >> 2][(x >> 1) & 1], s, y & 1, x & 1);
-            else acc[x][y] = lin_mfma<HALF>(fj[y], fi[x], acc[x][y]);
+        for (int f = 0; f < FJ; ++f) {
+          sv[f] = sn[f] & mask;
+          if (have < 4) {
+            const uint32_t o = so[f] + (a.swizzled ? st * 128 : st);
+            const uint32_t by = o > sleft - 4 ? o - (sleft - 4) : 0;
+            sv[f] = by < 4 ? (sn[f] >> (8 * by)) & mask : 0u;
           }
-        __builtin_amdgcn_s_setprio(0);
-        __builtin_amdgcn_sched_barrier(0);
+        }
       }
     };
-    lds_u8 *i0 = (lds_u8*)si0, *i1 = (lds_u8*)si1, *j0 = (lds_u8*)sj0, *j1 = (lds_u8*)sj1;
-    lds_u8 *is0 = (lds_u8*)sis0, *is1 = (lds_u8*)sis1, *js0 = (lds_u8*)sjs0, *js1 = (lds_u8*)sjs1;
-    auto scales_now = [&](float(&out)[P::JK == KC4 ? FJ : 1]) {
-      if constexpr (P::JK == KC4) {
+    // Q4: the packed scales of one 64-slot group of this tile, nk pieces of 256
+    // bytes, are this wave's to load
+    const uint8_t* scp = nullptr;
+    int64_t scleft = 0;
+    if constexpr (Q4) {
+      const int64_t gj = (a.N + 63) >> 6, ig = (t.pad >> 6) + wave, jg = (t.j0 >> 6) + wave - BM / 64;
+      if (wave < BM / 64) {
+        scp = a.xs + ig * nk * 256;
+        scleft = ig < a.padded ? (int64_t)nk * 256 : 0;
+      } else {
+        scp = a.wsc + (t.group * gj + jg) * nk * 256;
+        scleft = jg < gj ? (int64_t)nk * 256 : 0;
+      }
+    }
+    const __amdgpu_buffer_rsrc_t rsc = lin_rsrc(scp, scleft);
+    // Contraction contiguous: one resource for the tile (its offsets stay below
+    // 2^31), the offset runs along, and from this value of st * CS on the lane's
+    // chunk is past the end (of the row or of this workgroup's part) and reads
+    // zeros, not the next row.  Strided: the resource runs along; rows past
+    // the end are past its end.  Every stage has the same number of loads, the
+    // ones past the last too, which is what the waits below count.
+    const int end = ke * CS < len ? ke * CS : (int)len;
+    const int last = end - ((lane & 3) ^ mm_key(lane >> 2)) * (CS / 4);
+    const uint8_t *ir = ip + kb * istep, *jr = jp + kb * jstep;
+    int64_t il = ibytes - kb * istep, jl = jbytes - kb * jstep;
+    auto left32 = [&](int64_t left, bool none) {  // (scalar instructions only)
+      const int hi = (int)(left >> 32);
+      const uint32_t lo = (uint32_t)left < (uint32_t)LIN_SPAN ? (uint32_t)left : (uint32_t)LIN_SPAN;
+      const uint32_t n = hi > 0 ? (uint32_t)LIN_SPAN : (hi < 0 ? 0u : lo);
+      return none ? 0u : n;
+    };
+    const uint32_t in = left32(il, false), jn = left32(jl, false);
+    // KS4: this thread decodes 16 codes of contraction row kr.  (Its loads are
+    // issued for every stage, inside the weight or not: the waits count them.)
+    const int kr = tid / (BN / 16), kc = tid % (BN / 16);
+    lm_u32x2 code[2];
+    uint32_t code_s[2];
+    const uint32_t co = t.j0 + kc * 16 < a.K ? (uint32_t)(kr * (a.K >> 1) + kc * 8) : LIN_OUT;
+    const uint32_t cb = (uint32_t)((t.j0 + kc * 16) >> 5);  // block of the row
+    const uint32_t cso = a.swizzled ? (cb >> 2) * 512 + (kr & 31) * 16 + (cb & 3) : (uint32_t)(kr * nb) + cb;
+    auto load_codes = [&](int st, int set) {
+      if constexpr (JK == KS4) {
+        const int64_t sbase = a.swizzled ? (int64_t)(st >> 2) * ((nb + 3) >> 2) * 512 + (st & 3) * 4 : (int64_t)st * CS * nb;
+        const bool none = st >= ke;
+        const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)jr, 0, left32(jl, none), 0x00027000);
+        jr += jstep;
+        jl -= jstep;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(sp + sbase), 0, left32(a.scale_stride - sbase, none), 0x00027000);
+        code[set] = __builtin_bit_cast(lm_u32x2, __builtin_amdgcn_raw_buffer_load_b64(rc, (int)co, 0, 0));
+        code_s[set] = __builtin_amdgcn_raw_buffer_load_b8(rs, (int)(co == LIN_OUT ? LIN_OUT : cso), 0, 0);
+      }
+    };
+    auto store_codes = [&](lds_u8* tj, int set) {
+      if constexpr (JK == KS4) {
+        const float s = e8m0_value(code_s[set]);
 #pragma unroll
-        for (int f = 0; f < FJ; ++f) out[f] = e8m0_value(sv[f]);
+        for (int c = 0; c < 2; ++c)
+          *(lds_u32x4*)(tj + kr * (BN * 2) + (((kc * 2 + c) ^ mm_row_key(kr)) << 4)) = lin_decode8<HALF>(code[set][c], s);
       }
     };
-    load(kb, i0, j0, is0, js0);
-    load_scales(kb);
-    store_codes(j0);
-    float sc[P::JK == KC4 ? FJ : 1];
-    int kt = kb;
-    for (; kt + 1 < ke; kt += 2) {  // (no way out of the middle: it would keep two copies of the accumulators)
-      __syncthreads();
-      scales_now(sc);
-      load(kt + 1, i1, j1, is1, js1);
-      load_scales(kt + 1);
-      compute(i0, j0, is0, js0, sc);
-      store_codes(j1);
-      __syncthreads();
-      scales_now(sc);
-      if (kt + 2 < ke) {
-        load(kt + 2, i0, j0, is0, js0);
-        load_scales(kt + 2);
+    auto load = [&](int st, lds_u8* ti, lds_u8* tj, lds_u8* ts) {  // (called for every stage, in order)
+      const bool none = st >= ke, out = st * CS >= last;
+      const __amdgpu_buffer_rsrc_t ri = __builtin_amdgcn_make_buffer_rsrc((void*)ir, 0, IK == KC16 ? in : left32(il, none), 0x00027000);
+#pragma unroll
+      for (int n = 0; n < P::IL; ++n) {
+        lin_dma(ri, ti + (n * P::NW + wave) * 1024, IK == KC16 && out ? LIN_OUT : io[n]);
+        if constexpr (IK == KC16) io[n] += 64;
       }
-      compute(i1, j1, is1, js1, sc);
-      if (kt + 2 < ke) store_codes(j0);
+      if constexpr (IK != KC16) {
+        ir += istep;
+        il -= istep;
+      }
+      if constexpr (JK != KS4) {
+        const __amdgpu_buffer_rsrc_t rj =
+            __builtin_amdgcn_make_buffer_rsrc((void*)jr, 0, JK == KC16 ? jn : (JK == KC4 ? (none ? 0u : jn) : left32(jl, none)), 0x00027000);
+        if constexpr (JK == KC4) {  // 32 slots a wave: half a load
+          if (lane < 32) lin_dma(rj, tj + wave * 512, jo[0]);
+          jo[0] += 16;
+        } else {
+#pragma unroll
+          for (int n = 0; n < P::JL; ++n) {
+            lin_dma(rj, tj + (n * P::NW + wave) * 1024, JK == KC16 && out ? LIN_OUT : jo[n]);
+            if constexpr (JK == KC16) jo[n] += 64;
+          }
+          if constexpr (JK != KC16) {
+            jr += jstep;
+            jl -= jstep;
+          }
+        }
+      }
+      if constexpr (Q4) {
+        if (lane < 16) lin_dma(rsc, ts + wave * 256, st * 256 + lane * 16);
+      }
+    };
+    const uint32_t ati = mm_at<IK, BM>(wi * (FI * 16), lane), atj = mm_at<JK == KS4 ? KS16 : JK, BN>(wj * (FJ * 16), lane);
+    lm_u32x4 fi[FI], fj[FJ];
+    uint32_t isc[Q4 ? FI / 4 : 1], jsc[Q4 ? FJ / 4 : 1], jc[JK == KC4 ? FJ : 1];
+    auto read = [&](const lds_u8* ti, const lds_u8* tj, const lds_u8* ts) {
+      const uint32_t ai = mm_hide(ati), aj = mm_hide(atj);
+#pragma unroll
+      for (int f = 0; f < FJ; ++f) {
+        if constexpr (JK == KC4) jc[f] = *(const lds_u32*)(tj + aj + f * 256);
+        else fj[f] = mm_frag<JK == KC16 ? KC16 : KS16, BN>(tj, aj, f);
+      }
+#pragma unroll
+      for (int f = 0; f < FI; ++f) fi[f] = mm_frag<IK, BM>(ti, ai, f);
+      if constexpr (Q4) {
+        const uint32_t as = mm_hide(lane * 4);
+#pragma unroll
+        for (int f = 0; f < FI / 4; ++f) isc[f] = *(const lds_u32*)(ts + as + (wi * (FI / 4) + f) * 256);
+#pragma unroll
+        for (int f = 0; f < FJ / 4; ++f) jsc[f] = *(const lds_u32*)(ts + as + (BM / 64 + wj * (FJ / 4) + f) * 256);
+      }
+    };
+    auto decode = [&](int b) {
+      if constexpr (JK == KC4) {
+#pragma unroll
+        for (int f = 0; f < FJ; ++f) fj[f] = lin_decode8<HALF>(jc[f], e8m0_value((sv[f] >> (8 * b)) & 255u));
+      }
+    };
+    auto multiply = [&]() {
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int x = 0; x < FI; ++x)
+#pragma unroll
+        for (int y = 0; y < FJ; ++y) {
+          if constexpr (Q4) acc[x][y] = lin_mfma4(fj[y], fi[x], acc[x][y], jsc[y >> 2], isc[x >> 2], y & 3, x & 3);
+          else acc[x][y] = lin_mfma<HALF>(fj[y], fi[x], acc[x][y]);
+        }
+      // (the products have no side effects: nothing else keeps them from moving
+      // past the barriers, the fragments of several stages with them)
+#pragma unroll
+      for (int x = 0; x < FI; ++x)
+#pragma unroll
+        for (int y = 0; y < FJ; ++y) asm volatile("" : "+v"(acc[x][y]));
+      __builtin_amdgcn_s_setprio(0);
+    };
+    lds_u8* const ti[4] = {(lds_u8*)si0, (lds_u8*)si1, (lds_u8*)si2, (lds_u8*)si3};
+    lds_u8* const tj[4] = {(lds_u8*)sj0, (lds_u8*)sj1, (lds_u8*)sj2, (lds_u8*)sj3};
+    lds_u8* const ts[4] = {(lds_u8*)ss0, (lds_u8*)ss1, (lds_u8*)ss2, (lds_u8*)ss3};
+    // loads of a stage per wave
+    constexpr int L = P::IL + P::JL + (Q4 ? 1 : 0);
+
+    load_scales(kb);
+#pragma unroll
+    for (int b = 0; b < 3; ++b) load(kb + b, ti[b], tj[b], ts[b]);
+    if constexpr (JK == KS4) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        load_codes(kb + b, 0);
+        store_codes(tj[b], 0);
+      }
+      load_codes(kb + 2, 0);
     }
-    if (kt < ke) {
-      __syncthreads();
-      scales_now(sc);
-      compute(i0, j0, is0, js0, sc);
+    lin_wait<JK == KS4 ? 0 : 2 * L>();  // stage kb is in LDS
+    lin_barrier();
+    if (PP && wave >= 4) lin_barrier();  // the second half runs one barrier behind
+    for (int st = kb; st < ke; st += 4) {
+      next_scales(st);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        read(ti[b], tj[b], ts[b]);
+        __builtin_amdgcn_sched_barrier(0);
+        // (while the reads are on their way)  Buffer b + 3 was read for stage
+        // st + b - 1, and all waves are past that.
+        if (b == 0) load_scales(st + 4);
+        load_codes(st + b + 3, (b + 1) & 1);
+        load(st + b + 3, ti[(b + 3) & 3], tj[(b + 3) & 3], ts[(b + 3) & 3]);
+        decode(b);
+        // stage st + b + 1 is in LDS, and this one in registers: what may be left
+        // are the loads of stages st + b + 2 and st + b + 3, with KC4 the scales that
+        // were asked for among them
+        if constexpr (JK == KC4) {
+          if (b < 2) lin_wait<2 * L + FJ>();
+          else lin_wait<2 * L>();
+        } else {
+          lin_wait<2 * L>();
+        }
+        lin_barrier();
+        multiply();
+        store_codes(tj[(b + 2) & 3], b & 1);
+        if constexpr (PP) lin_barrier();
+      }
     }
+    if constexpr (PP) {
+      if (wave < 4) lin_barrier();
+    }
+    lin_wait<0>();  // no load may reach LDS after the workgroup
   }
 
   const int64_t rows0 = OP == LIN_WEIGHT_GRAD ? t.group * a.N : 0;  // of the output above this group's
@@ -373,7 +471,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
       const int64_t i = t.r0 + wi * (FI * 16) + x * 16 + (lane & 15);
 #pragma unroll
       for (int y = 0; y < FJ; ++y) {
-        const int64_t j = t.j0 + wj * (FJ * 16) + (y >> 1) * 32 + 8 * g + 4 * (y & 1);
+        const int64_t j = t.j0 + wj * (FJ * 16) + y * 16 + 4 * g;
         if (i < t.r1) {
           if (j + 4 <= jend) {
             *(LM_GLOBAL lm_u32x4_any*)(part + i * jend + j) = __builtin_bit_cast(lm_u32x4, acc[x][y]);
@@ -390,7 +488,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
   uint16_t* out = (uint16_t*)a.out + rows0 * jend;
 #pragma unroll
   for (int y = 0; y < FJ; y += 2) {
-    const int64_t j = t.j0 + wj * (FJ * 16) + y * 16 + 8 * g;
+    const int64_t j = t.j0 + wj * (FJ * 16) + (y + (g & 1)) * 16 + 8 * (g >> 1);
     float bias[8] = {};
     if (OP == LIN_FORWARD && a.bias && t.group < a.experts) {
 #pragma unroll
@@ -400,10 +498,19 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
 #pragma unroll
     for (int x = 0; x < FI; ++x) {
       const int64_t i = t.r0 + wi * (FI * 16) + x * 16 + (lane & 15);
+      // lane groups 0, 2 keep fragment y and get columns 4 .. 7 (12 .. 15) of it
+      // from groups 1, 3, which get columns 0 .. 3 (8 .. 11) of fragment y + 1
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const auto r = __builtin_amdgcn_permlane16_swap(f2u(acc[x][y][e]), f2u(acc[x][y + 1][e]), false, false);
+        v[e] = u2f(r[0]);
+        v[4 + e] = u2f(r[1]);
+      }
       lm_u32x4 w;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float lo = acc[x][y + (e >> 1)][2 * (e & 1)] + bias[2 * e], hi = acc[x][y + (e >> 1)][2 * (e & 1) + 1] + bias[2 * e + 1];
+        const float lo = v[2 * e] + bias[2 * e], hi = v[2 * e + 1] + bias[2 * e + 1];
         w[e] = DT == F16 ? (uint32_t)f16_bits(lo) | (uint32_t)f16_bits(hi) << 16 : pack_bf16x2(lo, hi);
       }
       uint16_t* p = out + i * jend + j;
