@@ -233,6 +233,11 @@ DEV v4f32 lin_mfma(lm_u32x4 a, lm_u32x4 b, v4f32 c) {
 }
 
 // 8 codes -> 8 values of 16 bits
+// Byte b of a word of e8m0 scales, as the conversion below takes it: it reads the
+// exponent field alone (0 is 2^-127, 255 NaN), whatever sign and mantissa are.
+DEV float lin_e8m0(uint32_t word, int b) {
+  return u2f(b == 3 ? word >> 1 : word << (23 - 8 * b));
+}
 template <bool HALF>
 DEV lm_u32x4 lin_decode8(uint32_t codes, float scale) {
   lm_u32x4 v;

@@ -183,7 +183,7 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few(LinArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               lm_u32x4 f;
-              if constexpr (MX) f = lin_decode8<HALF>(wv[i][c][0][j], e8m0_value((sv[i][c] >> (8 * j)) & 255u));
+              if constexpr (MX) f = lin_decode8<HALF>(wv[i][c][0][j], lin_e8m0(sv[i][c], j));
               else f = wv[i][c][j];
 #pragma unroll
               for (int m = 0; m < MF; ++m) acc[j % AC][m][c] = lin_mfma<HALF>(f, xv[i][m][j], acc[j % AC][m][c]);

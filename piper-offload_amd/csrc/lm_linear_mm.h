@@ -12,8 +12,9 @@
 //   KS16  contraction strided (the index contiguous): a row per contraction
 //         step; read transposed (ds_read_b64_tr_b16); chunks XORed with a key
 //         of the row (mm_row_key)
-//   KC4   MXFP4 codes as they are stored, 16 bytes per slot, decoded to 16 bits
-//         after the read (v_cvt_scalef32_pk: exact products in bf16)
+//   KC4   MXFP4 codes as they are stored, decoded to 16 bits after the read
+//         (v_cvt_scalef32_pk: exact products in bf16).  A stage is 16 bytes of a
+//         row, so four stages are loaded together, in whole runs of 64 bytes
 //   KS4   MXFP4 with the contraction strided: every code of a run of 32 shares a
 //         scale but the 8 codes of an MFMA lane do not, so these are decoded on
 //         their way into LDS and then are KS16
@@ -116,13 +117,15 @@ struct MmTraits {
   static constexpr int IK = OP == LIN_WEIGHT_GRAD ? KS16 : KC16;
   static constexpr int JK = OP == LIN_FORWARD ? (MX ? KC4 : KC16) : (OP == LIN_INPUT_GRAD && MX ? KS4 : KS16);
   static constexpr int FI = BM / WM / 16, FJ = BN / WN / 16;
-  static constexpr int IB = BM * 64, JB = JK == KC4 ? BN * 16 : BN * 64;  // bytes of a stage
+  static constexpr int US = JK == KC4 ? 8 : 4;       // stages of a turn of the loop
+  static constexpr int IB = BM * 64, JB = BN * 64;  // bytes of a stage (KC4: of four)
   static constexpr int IL = IB / 1024 / NW;                               // loads per wave
-  static constexpr int JL = JK == KS4 ? 2 : (JB / 1024 + NW - 1) / NW;
+  static constexpr int JL = JK == KS4 ? 2 : JB / 1024 / NW;
   static constexpr int SB = Q4 ? NW * 256 : 16;  // bytes of a stage's scales: I's, then J's
   static_assert(!Q4 || BM / 64 + BN / 64 == NW, "a piece of scales per wave");
   static_assert(IL * 1024 * NW == IB, "tiles are whole loads of all waves");
-  static_assert(JK != KC4 || JB == NW * 512, "KC4: half a load per wave");
+  static_assert(JK == KS4 || JL * 1024 * NW == JB, "tiles are whole loads of all waves");
+  static_assert(JK != KC4 || JL == 2, "KC4: a load in each of two stages");
   static_assert(JK != KS4 || NT * 16 == 32 * BN, "KS4: half a run of 32 codes per thread");
 };
 
@@ -133,7 +136,7 @@ DEV void mm_offsets(uint32_t (&off)[L], int wave, int lane, int64_t ld) {
   for (int n = 0; n < L; ++n) {
     const int piece = (n * NW + wave) * 64 + lane;  // 16-byte piece of the tile
     if constexpr (KIND == KC16) off[n] = (uint32_t)((piece >> 2) * ld * 2) + ((piece & 3) ^ mm_key(piece >> 2)) * 16;
-    else if constexpr (KIND == KC4) off[n] = (uint32_t)((wave * 32 + (lane & 31)) * (ld >> 1));
+    else if constexpr (KIND == KC4) off[n] = (uint32_t)((piece >> 2) * (ld >> 1)) + ((piece & 3) ^ ((piece >> 4) & 3)) * 16;
     else off[n] = (uint32_t)(piece / (B / 8) * ld * 2) + ((piece % (B / 8)) ^ mm_row_key(piece / (B / 8))) * 16;
   }
 }
@@ -145,7 +148,7 @@ template <int KIND, int B>
 DEV uint32_t mm_at(int slot0, int lane) {
   const int p = lane & 15, g = lane >> 4;
   if constexpr (KIND == KC16) return (slot0 + p) * 64 + ((g ^ mm_key(p)) << 4);
-  else if constexpr (KIND == KC4) return (slot0 + p) * 16 + g * 4;
+  else if constexpr (KIND == KC4) return (slot0 + p) * 64 + ((p >> 2) << 4) + g * 4;  // ^ 16 times the stage
   const int row = 8 * g + (p >> 2), chunk = (slot0 >> 3) + ((p >> 1) & 1);
   return row * (B * 2) + ((chunk ^ mm_row_key(row)) << 4 | (p & 1) << 3);
 }
@@ -173,7 +176,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
   // (separate arrays: the compiler then knows that a read of one stage need not
   // wait for the loads of another)
   __shared__ __attribute__((aligned(1024))) uint8_t si0[P::IB], si1[P::IB], si2[P::IB], si3[P::IB];
-  __shared__ __attribute__((aligned(1024))) uint8_t sj0[P::JB], sj1[P::JB], sj2[P::JB], sj3[P::JB];
+  __shared__ __attribute__((aligned(1024))) uint8_t sj0[P::JB], sj1[P::JB], sj2[JK == KC4 ? 16 : P::JB], sj3[JK == KC4 ? 16 : P::JB];
   __shared__ __attribute__((aligned(1024))) uint8_t ss0[P::SB], ss1[P::SB], ss2[P::SB], ss3[P::SB];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
   const int wave = wave_index();
@@ -226,7 +229,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
   // stages [kb, ke) of nk: this workgroup's part where the contraction is split
   const int nk = (int)((len + CS - 1) / CS);
   const int splits = OP == LIN_WEIGHT_GRAD ? gridDim.z : gridDim.y, split = OP == LIN_WEIGHT_GRAD ? blockIdx.z : blockIdx.y;
-  const int per = ((nk + splits - 1) / splits + 3) & ~3, kb = split * per, ke = kb + per < nk ? kb + per : nk;
+  const int per = ((nk + splits - 1) / splits + P::US - 1) / P::US * P::US, kb = split * per, ke = kb + per < nk ? kb + per : nk;
   v4f32 acc[FI][FJ] = {};
 
   if (kb < ke) {
@@ -296,6 +299,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
     // ones past the last too, which is what the waits below count.
     const int end = ke * CS < len ? ke * CS : (int)len;
     const int last = end - ((lane & 3) ^ mm_key(lane >> 2)) * (CS / 4);
+    const int lastj = end - ((lane & 3) ^ ((lane >> 4) & 3)) * CS;  // KC4: a chunk is a stage
     const uint8_t *ir = ip + kb * istep, *jr = jp + kb * jstep;
     int64_t il = ibytes - kb * istep, jl = jbytes - kb * jstep;
     auto left32 = [&](int64_t left, bool none) {  // (scalar instructions only)
@@ -327,14 +331,22 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
     };
     auto store_codes = [&](lds_u8* tj, int set) {
       if constexpr (JK == KS4) {
-        const float s = e8m0_value(code_s[set]);
+        const float s = lin_e8m0(code_s[set], 0);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
           *(lds_u32x4*)(tj + kr * (BN * 2) + (((kc * 2 + c) ^ mm_row_key(kr)) << 4)) = lin_decode8<HALF>(code[set][c], s);
       }
     };
-    auto load = [&](int st, lds_u8* ti, lds_u8* tj, lds_u8* ts) {  // (called for every stage, in order)
+    // (called for every stage, in order; KC4: half says which half of the codes, tj where they go)
+    auto load = [&](int st, int jst, int half, lds_u8* ti, lds_u8* tj, lds_u8* ts) {
       const bool none = st >= ke, out = st * CS >= last;
+      if constexpr (JK == KC4) {  // half of the codes of stages jst .. jst + 3
+        if (half >= 0) {
+          lin_dma(__builtin_amdgcn_make_buffer_rsrc((void*)jr, 0, jn, 0x00027000), tj + (half * P::NW + wave) * 1024,
+                  jst * CS >= lastj ? LIN_OUT : jo[half]);
+          jo[half] += 64;
+        }
+      }
       const __amdgpu_buffer_rsrc_t ri = __builtin_amdgcn_make_buffer_rsrc((void*)ir, 0, IK == KC16 ? in : left32(il, none), 0x00027000);
 #pragma unroll
       for (int n = 0; n < P::IL; ++n) {
@@ -345,22 +357,16 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
         ir += istep;
         il -= istep;
       }
-      if constexpr (JK != KS4) {
-        const __amdgpu_buffer_rsrc_t rj =
-            __builtin_amdgcn_make_buffer_rsrc((void*)jr, 0, JK == KC16 ? jn : (JK == KC4 ? (none ? 0u : jn) : left32(jl, none)), 0x00027000);
-        if constexpr (JK == KC4) {  // 32 slots a wave: half a load
-          if (lane < 32) lin_dma(rj, tj + wave * 512, jo[0]);
-          jo[0] += 16;
-        } else {
+      if constexpr (JK == KC16 || JK == KS16) {
+        const __amdgpu_buffer_rsrc_t rj = __builtin_amdgcn_make_buffer_rsrc((void*)jr, 0, JK == KS16 ? left32(jl, none) : jn, 0x00027000);
 #pragma unroll
-          for (int n = 0; n < P::JL; ++n) {
-            lin_dma(rj, tj + (n * P::NW + wave) * 1024, JK == KC16 && out ? LIN_OUT : jo[n]);
-            if constexpr (JK == KC16) jo[n] += 64;
-          }
-          if constexpr (JK != KC16) {
-            jr += jstep;
-            jl -= jstep;
-          }
+        for (int n = 0; n < P::JL; ++n) {
+          lin_dma(rj, tj + (n * P::NW + wave) * 1024, JK == KC16 && out ? LIN_OUT : jo[n]);
+          if constexpr (JK == KC16) jo[n] += 64;
+        }
+        if constexpr (JK != KC16) {
+          jr += jstep;
+          jl -= jstep;
         }
       }
       if constexpr (Q4) {
@@ -370,11 +376,11 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
     const uint32_t ati = mm_at<IK, BM>(wi * (FI * 16), lane), atj = mm_at<JK == KS4 ? KS16 : JK, BN>(wj * (FJ * 16), lane);
     lm_u32x4 fi[FI], fj[FJ];
     uint32_t isc[Q4 ? FI / 4 : 1], jsc[Q4 ? FJ / 4 : 1], jc[JK == KC4 ? FJ : 1];
-    auto read = [&](const lds_u8* ti, const lds_u8* tj, const lds_u8* ts) {
+    auto read = [&](int b, const lds_u8* ti, const lds_u8* tj, const lds_u8* ts) {
       const uint32_t ai = mm_hide(ati), aj = mm_hide(atj);
 #pragma unroll
       for (int f = 0; f < FJ; ++f) {
-        if constexpr (JK == KC4) jc[f] = *(const lds_u32*)(tj + aj + f * 256);
+        if constexpr (JK == KC4) jc[f] = *(const lds_u32*)(tj + (aj ^ ((b & 3) << 4)) + f * 1024);
         else fj[f] = mm_frag<JK == KC16 ? KC16 : KS16, BN>(tj, aj, f);
       }
 #pragma unroll
@@ -390,7 +396,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
     auto decode = [&](int b) {
       if constexpr (JK == KC4) {
 #pragma unroll
-        for (int f = 0; f < FJ; ++f) fj[f] = lin_decode8<HALF>(jc[f], e8m0_value((sv[f] >> (8 * b)) & 255u));
+        for (int f = 0; f < FJ; ++f) fj[f] = lin_decode8<HALF>(jc[f], lin_e8m0(sv[f], b & 3));
       }
     };
     auto multiply = [&]() {
@@ -414,11 +420,13 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
     lds_u8* const tj[4] = {(lds_u8*)sj0, (lds_u8*)sj1, (lds_u8*)sj2, (lds_u8*)sj3};
     lds_u8* const ts[4] = {(lds_u8*)ss0, (lds_u8*)ss1, (lds_u8*)ss2, (lds_u8*)ss3};
     // loads of a stage per wave
-    constexpr int L = P::IL + P::JL + (Q4 ? 1 : 0);
+    constexpr int L = P::IL + (JK == KC4 ? 0 : P::JL) + (Q4 ? 1 : 0);
 
     load_scales(kb);
+    // KC4: the first four stages' codes; the loop asks for the next four in the
+    // first two of every four stages
 #pragma unroll
-    for (int b = 0; b < 3; ++b) load(kb + b, ti[b], tj[b], ts[b]);
+    for (int b = 0; b < 3; ++b) load(kb + b, kb, b < 2 ? b : -1, ti[b], JK == KC4 ? tj[0] : tj[b], ts[b]);
     if constexpr (JK == KS4) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -430,23 +438,26 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
     lin_wait<JK == KS4 ? 0 : 2 * L>();  // stage kb is in LDS
     lin_barrier();
     if (PP && wave >= 4) lin_barrier();  // the second half runs one barrier behind
-    for (int st = kb; st < ke; st += 4) {
-      next_scales(st);
+    for (int st = kb; st < ke; st += P::US) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        read(ti[b], tj[b], ts[b]);
+      for (int b = 0; b < P::US; ++b) {
+        const int n = (b + 3) & 3;  // the buffer of stage st + b + 3
+        if (b % 4 == 0) next_scales(st + b);
+        read(b, ti[b & 3], JK == KC4 ? tj[(b >> 2) & 1] : tj[b & 3], ts[b & 3]);
         __builtin_amdgcn_sched_barrier(0);
-        // (while the reads are on their way)  Buffer b + 3 was read for stage
+        // (while the reads are on their way)  Buffer n was read for stage
         // st + b - 1, and all waves are past that.
-        if (b == 0) load_scales(st + 4);
+        if (b % 4 == 0) load_scales(st + b + 4);
         load_codes(st + b + 3, (b + 1) & 1);
-        load(st + b + 3, ti[(b + 3) & 3], tj[(b + 3) & 3], ts[(b + 3) & 3]);
+        load(st + b + 3, st + (b & ~3) + 4, b % 4 < 2 ? b % 4 : -1, ti[n], JK == KC4 ? tj[~(b >> 2) & 1] : tj[n], ts[n]);
         decode(b);
-        // stage st + b + 1 is in LDS, and this one in registers: what may be left
-        // are the loads of stages st + b + 2 and st + b + 3, with KC4 the scales that
-        // were asked for among them
+        // Stage st + b + 1 is in LDS, and this one in registers: what may be left
+        // are the loads of stages st + b + 2 and st + b + 3, with KC4 the scales and
+        // codes that were asked for since.
         if constexpr (JK == KC4) {
-          if (b < 2) lin_wait<2 * L + FJ>();
+          if (b % 4 == 0) lin_wait<2 * L + FJ + 1>();
+          else if (b % 4 == 1) lin_wait<2 * L + FJ + 2>();
+          else if (b % 4 == 2) lin_wait<2 * L + 1>();
           else lin_wait<2 * L>();
         } else {
           lin_wait<2 * L>();
