@@ -30,6 +30,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from typing import Any
 
 import torch
 
@@ -639,6 +640,7 @@ def merge_dense_lora_(weight: torch.Tensor, b: torch.Tensor, a: torch.Tensor, st
 _MAX_EXPERTS = 1024
 
 
+# (These calls are as short as 5 us on the GPU: the checks below look at each tensor once.)
 def _rows(label: str, x: torch.Tensor, cols: int) -> tuple[torch.Tensor, int, int]:
     """``x`` [..., cols] as [rows, cols] whose rows are contiguous, the number of rows, and their stride."""
     shape = x.shape
@@ -648,12 +650,24 @@ def _rows(label: str, x: torch.Tensor, cols: int) -> tuple[torch.Tensor, int, in
         raise ValueError(f"{label} supports bfloat16 and float16 rows, got {x.dtype}.")
     if len(shape) != 2:
         x = x.reshape(-1, cols)
-    rows = x.shape[0]
+        shape = x.shape
+    rows = shape[0]
+    if x.is_contiguous():
+        return x, rows, cols
     stride, step = x.stride()
     if (cols > 1 and step != 1) or (rows > 1 and stride < cols):
-        x = x.contiguous()
-        stride = cols
+        return x.contiguous(), rows, cols
     return x, rows, stride if rows > 1 else cols  # (the stride of a single row may be anything)
+
+
+def _on_gpu(label: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    """All tensors on the GPU of the first."""
+    if not first.is_cuda:
+        raise ValueError(f"{label} requires GPU tensors.")
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{label} requires all tensors on one GPU device.")
 
 
 def _ends(label: str, ends: torch.Tensor, experts: int) -> torch.Tensor:
@@ -665,33 +679,46 @@ def _ends(label: str, ends: torch.Tensor, experts: int) -> torch.Tensor:
     return ends.contiguous()
 
 
-def _mx_stack(label: str, qdata: torch.Tensor, scale: torch.Tensor, swizzled: bool, experts: int | None) -> tuple[int, int]:
-    """Check MXFP4 storage ([rows, cols/2], or [experts, rows, cols/2]); returns (rows, cols)."""
-    ndim = 2 if experts is None else 3
-    if qdata.ndim != ndim or scale.ndim != ndim:
-        raise ValueError(f"{label} expects rank-{'two' if ndim == 2 else 'three'} MXFP4 codes and scales.")
+def _mx_weight(label: str, qdata: torch.Tensor, scale: torch.Tensor, swizzled: bool, stacked: bool) -> L.WeightStruct:
+    """Check MXFP4 storage ([rows, cols/2], stacked: [groups, rows, cols/2]) and describe it."""
+    shape, sshape = qdata.shape, scale.shape
+    if len(shape) != 2 + stacked or len(sshape) != 2 + stacked:
+        raise ValueError(f"{label} expects rank-{'three' if stacked else 'two'} MXFP4 codes and scales.")
     if qdata.dtype is not torch.uint8 and qdata.dtype is not _FP4_DTYPE:
         raise ValueError(f"{label} expects packed uint8 MXFP4 codes, got {qdata.dtype}.")
     if scale.dtype is not torch.uint8 and scale.dtype is not _E8M0_DTYPE:
         raise ValueError(f"{label} expects E8M0 scales, got {scale.dtype}.")
     if not qdata.is_contiguous() or not scale.is_contiguous():
         raise ValueError(f"{label} requires contiguous MXFP4 storage.")
-    rows, cols = qdata.shape[-2], qdata.shape[-1] * 2
+    rows, cols, groups = shape[-2], shape[-1] * 2, shape[0] if stacked else 1
     if rows == 0 or cols == 0:
         raise ValueError(f"{label} requires a non-empty weight.")
     if cols % 32 != 0:
         raise ValueError(f"{label} requires columns divisible by 32.")
-    if tuple(scale.shape) != qdata.shape[:-2] + _mx_scale_shape(rows, cols, swizzled):
-        raise ValueError(f"{label}: the scale shape {tuple(scale.shape)} does not match its block layout.")
-    return rows, cols
+    if sshape[-2:] != _mx_scale_shape(rows, cols, swizzled) or (stacked and sshape[0] != groups):
+        raise ValueError(f"{label}: the scale shape {tuple(sshape)} does not match its block layout.")
+    return L.WeightStruct(qdata.data_ptr(), scale.data_ptr(), rows, cols, L.LM_E2M1, swizzled, groups, 0)
+
+
+def _launch(entry: Any, index: int, ws_bytes: int, device: torch.device, *args: object) -> None:
+    """Call one C entry on GPU ``index`` with a workspace on the current stream."""
+    if torch._C._cuda_getDevice() != index:
+        with L.on_device(device):
+            _launch(entry, index, ws_bytes, device, *args)
+        return
+    ws = L.aligned_ptr(keep := L.workspace(ws_bytes, device)) if ws_bytes else None
+    rc = entry(*args, ws, ws_bytes, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        L.check(rc)
+    if ws_bytes:
+        del keep  # released in stream order
 
 
 def _linear_forward(label: str, x: torch.Tensor, weight: L.WeightStruct, bias: torch.Tensor | None,
-                    ends: torch.Tensor | None, activation_dtype: torch.dtype | None, device: torch.device) -> torch.Tensor:
+                    ends: torch.Tensor | None, activation_dtype: torch.dtype | None) -> torch.Tensor:
     n, k = weight.N, weight.K
     x2, t, ldx = _rows(label, x, k)
-    dtype_id = L.torch_dtype_id(x.dtype)
-    input_id = dtype_id
+    dtype_id = input_id = L.torch_dtype_id(x.dtype)
     if activation_dtype is not None:
         if activation_dtype is not _FP4_DTYPE or _FP4_DTYPE is None:
             raise ValueError(f"{label} quantises its input to float4_e2m1fn_x2 only, got {activation_dtype}.")
@@ -702,35 +729,24 @@ def _linear_forward(label: str, x: torch.Tensor, weight: L.WeightStruct, bias: t
         bias = bias.contiguous()
     y = x2.new_empty((t, n))
     if t:
-        handle = L.lib()
         px = x2.data_ptr()
         ws_bytes = L.linear_workspace_size(0, t, ldx, 0, n, k, weight.experts, weight.dtype, input_id, not (px | weight.q) & 15)
-        with L.on_device(device):
-            ws = L.workspace(ws_bytes, device) if ws_bytes else None
-            rc = handle.lm_linear(px, ldx, ctypes.byref(weight), _ptr(bias), _ptr(ends), y.data_ptr(), t, dtype_id, input_id,
-                                  None if ws is None else L.aligned_ptr(ws), ws_bytes, L.stream_ptr(device))
-        if rc:
-            L.check(rc)
+        _launch(L.lib().lm_linear, x2.get_device(), ws_bytes, x2.device, px, ldx, weight, _ptr(bias), _ptr(ends), y.data_ptr(), t,
+                dtype_id, input_id)
     return y if x.ndim == 2 else y.view(*x.shape[:-1], n)
 
 
-def _linear_input_grad(label: str, dy: torch.Tensor, weight: L.WeightStruct, ends: torch.Tensor | None,
-                       device: torch.device) -> torch.Tensor:
-    dy2, t, ldy = _rows(label, dy, weight.N)
-    dx = dy2.new_empty((t, weight.K))
+def _linear_input_grad(label: str, dy: torch.Tensor, weight: L.WeightStruct, ends: torch.Tensor | None) -> torch.Tensor:
+    n, k = weight.N, weight.K
+    dy2, t, ldy = _rows(label, dy, n)
+    dx = dy2.new_empty((t, k))
     if t:
-        handle = L.lib()
         py = dy2.data_ptr()
         dtype_id = L.torch_dtype_id(dy.dtype)
-        ws_bytes = L.linear_workspace_size(1, t, ldy, 0, weight.N, weight.K, weight.experts, weight.dtype, dtype_id,
-                                           not (py | weight.q) & 15)
-        with L.on_device(device):
-            ws = L.workspace(ws_bytes, device) if ws_bytes else None
-            rc = handle.lm_linear_input_grad(py, ldy, ctypes.byref(weight), _ptr(ends), dx.data_ptr(), t, dtype_id,
-                                             None if ws is None else L.aligned_ptr(ws), ws_bytes, L.stream_ptr(device))
-        if rc:
-            L.check(rc)
-    return dx if dy.ndim == 2 else dx.view(*dy.shape[:-1], weight.K)
+        ws_bytes = L.linear_workspace_size(1, t, ldy, 0, n, k, weight.experts, weight.dtype, dtype_id, not (py | weight.q) & 15)
+        _launch(L.lib().lm_linear_input_grad, dy2.get_device(), ws_bytes, dy2.device, py, ldy, weight, _ptr(ends), dx.data_ptr(),
+                t, dtype_id)
+    return dx if dy.ndim == 2 else dx.view(*dy.shape[:-1], k)
 
 
 def mx_matmul(x: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, *, swizzled: bool = False,
@@ -741,31 +757,27 @@ def mx_matmul(x: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, *, swiz
     ``activation_dtype=torch.float4_e2m1fn_x2`` ``x`` is quantised first, as :func:`requantize_mx` does it.
     """
     label = "MX product"
-    device = _same_device(label, x, qdata, scale, bias)
-    n, k = _mx_stack(label, qdata, scale, swizzled, None)
-    weight = L.WeightStruct(qdata.data_ptr(), scale.data_ptr(), n, k, L.LM_E2M1, int(swizzled), 1, 0)
-    return _linear_forward(label, x, weight, bias, None, activation_dtype, device)
+    _on_gpu(label, x, qdata, scale, bias)
+    return _linear_forward(label, x, _mx_weight(label, qdata, scale, swizzled, False), bias, None, activation_dtype)
 
 
 def mx_matmul_input_grad(dy: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, *,
                          swizzled: bool = False) -> torch.Tensor:
     """``dy @ W``: the input gradient of :func:`mx_matmul` (straight through a quantised input)."""
     label = "MX product gradient"
-    device = _same_device(label, dy, qdata, scale)
-    n, k = _mx_stack(label, qdata, scale, swizzled, None)
-    weight = L.WeightStruct(qdata.data_ptr(), scale.data_ptr(), n, k, L.LM_E2M1, int(swizzled), 1, 0)
-    return _linear_input_grad(label, dy, weight, None, device)
+    _on_gpu(label, dy, qdata, scale)
+    return _linear_input_grad(label, dy, _mx_weight(label, qdata, scale, swizzled, False), None)
 
 
-def _dense_stack(label: str, rows: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> L.WeightStruct:
-    if weight.ndim != 3 or 0 in weight.shape:
-        raise ValueError(f"{label} expects a weight [groups, out, in], got {tuple(weight.shape)}.")
+def _dense_stack(label: str, rows: torch.Tensor, weight: torch.Tensor) -> L.WeightStruct:
+    shape = weight.shape
+    if len(shape) != 3 or 0 in shape:
+        raise ValueError(f"{label} expects a weight [groups, out, in], got {tuple(shape)}.")
     if weight.dtype is not rows.dtype:
         raise ValueError(f"{label} requires the weight in the rows' dtype {rows.dtype}, got {weight.dtype}.")
     if not weight.is_contiguous():
         raise ValueError(f"{label} requires a contiguous weight.")
-    e, n, k = weight.shape
-    return L.WeightStruct(weight.data_ptr(), None, n, k, L.torch_dtype_id(weight.dtype), 0, e, 0)
+    return L.WeightStruct(weight.data_ptr(), None, shape[1], shape[2], L.torch_dtype_id(weight.dtype), 0, shape[0], 0)
 
 
 def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
@@ -774,23 +786,23 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) ->
     ``ends`` int32 [groups] stays on the GPU (no synchronization); rows past the last end give zeros.
     """
     label = "Grouped product"
-    device = _same_device(label, x, weight, ends)
-    w = _dense_stack(label, x, weight, ends)
-    return _linear_forward(label, x, w, None, _ends(label, ends, w.experts), None, device)
+    _on_gpu(label, x, weight, ends)
+    w = _dense_stack(label, x, weight)
+    return _linear_forward(label, x, w, None, _ends(label, ends, w.experts), None)
 
 
 def grouped_matmul_input_grad(dy: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
     """The gradient of :func:`grouped_matmul` to ``x``; zeros for rows of no group."""
     label = "Grouped product gradient"
-    device = _same_device(label, dy, weight, ends)
-    w = _dense_stack(label, dy, weight, ends)
-    return _linear_input_grad(label, dy, w, _ends(label, ends, w.experts), device)
+    _on_gpu(label, dy, weight, ends)
+    w = _dense_stack(label, dy, weight)
+    return _linear_input_grad(label, dy, w, _ends(label, ends, w.experts))
 
 
 def grouped_matmul_weight_grad(dy: torch.Tensor, x: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
     """The gradient of :func:`grouped_matmul` to ``weight``: ``dy[group].T @ x[group]``, zeros for empty groups."""
     label = "Grouped product weight gradient"
-    device = _same_device(label, dy, x, ends)
+    _on_gpu(label, dy, x, ends)
     if dy.ndim < 1 or x.ndim < 1 or dy.shape[:-1] != x.shape[:-1]:
         raise ValueError(f"{label}: dy {tuple(dy.shape)} and x {tuple(x.shape)} differ in their rows.")
     if dy.dtype is not x.dtype:
@@ -801,16 +813,11 @@ def grouped_matmul_weight_grad(dy: torch.Tensor, x: torch.Tensor, ends: torch.Te
     (dy2, t, ldy), (x2, _, ldx) = _rows(label, dy, n), _rows(label, x, k)
     ends = _ends(label, ends, ends.shape[0] if ends.ndim == 1 else -1)
     e = ends.shape[0]
-    dw = torch.empty((e, n, k), dtype=x.dtype, device=device)
-    handle = L.lib()
+    dw = x2.new_empty((e, n, k))
     py, px, dtype_id = dy2.data_ptr(), x2.data_ptr(), L.torch_dtype_id(x.dtype)
     ws_bytes = L.linear_workspace_size(2, t, ldy, ldx, n, k, e, dtype_id, dtype_id, not (py | px) & 15)
-    with L.on_device(device):
-        ws = L.workspace(ws_bytes, device) if ws_bytes else None
-        rc = handle.lm_linear_weight_grad(py, ldy, px, ldx, ends.data_ptr(), dw.data_ptr(), t, n, k, e, dtype_id,
-                                          None if ws is None else L.aligned_ptr(ws), ws_bytes, L.stream_ptr(device))
-    if rc:
-        L.check(rc)
+    _launch(L.lib().lm_linear_weight_grad, x2.get_device(), ws_bytes, x2.device, py, ldy, px, ldx, ends.data_ptr(), dw.data_ptr(),
+            t, n, k, e, dtype_id)
     return dw
 
 
@@ -818,21 +825,15 @@ def grouped_mx_matmul(x: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor,
                       swizzled: bool = False, activation_dtype: torch.dtype | None = None) -> torch.Tensor:
     """:func:`grouped_matmul` with MXFP4 weights: ``qdata`` [groups, out, in/2], scales of each group's weight."""
     label = "Grouped MX product"
-    device = _same_device(label, x, qdata, scale, ends)
-    experts = qdata.shape[0] if qdata.ndim else 0
-    n, k = _mx_stack(label, qdata, scale, swizzled, experts)
-    ends = _ends(label, ends, experts)
-    weight = L.WeightStruct(qdata.data_ptr(), scale.data_ptr(), n, k, L.LM_E2M1, int(swizzled), experts, 0)
-    return _linear_forward(label, x, weight, None, ends, activation_dtype, device)
+    _on_gpu(label, x, qdata, scale, ends)
+    w = _mx_weight(label, qdata, scale, swizzled, True)
+    return _linear_forward(label, x, w, None, _ends(label, ends, w.experts), activation_dtype)
 
 
 def grouped_mx_matmul_input_grad(dy: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, ends: torch.Tensor, *,
                                  swizzled: bool = False) -> torch.Tensor:
     """The gradient of :func:`grouped_mx_matmul` to ``x``; zeros for rows of no group."""
     label = "Grouped MX product gradient"
-    device = _same_device(label, dy, qdata, scale, ends)
-    experts = qdata.shape[0] if qdata.ndim else 0
-    n, k = _mx_stack(label, qdata, scale, swizzled, experts)
-    ends = _ends(label, ends, experts)
-    weight = L.WeightStruct(qdata.data_ptr(), scale.data_ptr(), n, k, L.LM_E2M1, int(swizzled), experts, 0)
-    return _linear_input_grad(label, dy, weight, ends, device)
+    _on_gpu(label, dy, qdata, scale, ends)
+    w = _mx_weight(label, qdata, scale, swizzled, True)
+    return _linear_input_grad(label, dy, w, _ends(label, ends, w.experts))
