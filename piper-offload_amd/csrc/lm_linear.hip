@@ -102,15 +102,20 @@ static LinArgs lin_args(const lm_weight* w, const int32_t* ends, int64_t T) {
 
 // ---- how a product is run: a rule on its sizes, types and alignment ----------
 // k_lin_few reads the operands once per 16 to 64 rows or columns and spreads over
-// all CUs by splitting the contraction inside workgroups; k_lin_mm shares tiles
-// of 128 or 256 and needs many of them.  Measured, us few / mm: MXFP4 [14336,
-// 4096] at 64 rows 28 / 34, at 128 rows 52 / 40; [4096, 4096] at 128 rows 24 / 26,
-// at 256 rows 27 / 29, 4-bit inputs 23 / 25; 32 experts [2816, 2048] at 16 rows each
-// 36 / 68, at 32 rows 58 / 70 (4-bit inputs 58 / 47), at 64 rows 96 / 73; dense
-// [16, 4096] of 24 adapters at 2048 rows 13 / 18, [64, 4096] 24 / 18.
-static bool lin_few(int64_t T, int64_t N, int64_t E, bool mx, bool quant) {
+// all CUs by splitting the contraction inside workgroups; k_lin_mm shares tiles.
+// The first wins while the product is small, which is a matter of its volume T N
+// K more than of any one size.  Measured, us few / mm: MXFP4 [4096, 4096] at 64 rows
+// 13 / 15, at 96 rows 23 / 17; [1024, 4096] at 200 rows 12 / 14; [64, 4096] of 24
+// groups at 2048 rows 13 / 18; [1000, 8192] at 300 rows 41 / 22.  4-bit inputs pay
+// for the packing of the weight's scales in k_lin_mm: [4096, 14336] at 64 rows
+// 31 / 37, at 128 rows 52 / 39; 32 groups [2816, 2048] of 16 rows 36 / 46, of 32 rows
+// 58 / 42.  Dense: [4096, 4096] at 32 rows 14 / 15, at 64 rows 21 / 18; [64, 4096] of 24
+// groups at 2048 rows 24 / 17.
+static bool lin_few(int64_t T, int64_t N, int64_t K, int64_t E, bool mx, bool quant) {
   const int64_t rows = (T + E - 1) / E;
-  return N <= 16 || rows <= 16 || T * N < (mx ? 1 << 20 : 1 << 17) || (mx && !quant && E >= 8 && rows <= 32);
+  const double volume = (double)T * (double)N * (double)K;
+  if (!mx) return T <= 16 || volume <= 5e8;
+  return rows <= 16 || volume <= 1.1e9 || (quant && T <= 64);
 }
 
 struct LinPlan {
@@ -123,11 +128,49 @@ struct LinPlan {
 };
 static int64_t round8(int64_t x) { return (x + 7) & ~(int64_t)7; }
 
+// Tile and splits of k_lin_mm: the least of a model of its time.  A CU's time for
+// a stage, us, by the tiles that it works on in turn (measured, bf16, 4096 columns
+// at 256 to 4096 rows; a stage of 4-bit inputs, four times as deep, takes 1.65
+// times as long): 256 x 256 0.78 a tile, 0.56 where less than half of the CUs have
+// one; 128 x 128 two at a time in 0.58, one in 0.30; 64 x 128 three in 0.60, two
+// in 0.41, one in 0.22.  Groups end in a part of a tile, half of one on
+// average.  A split contraction writes and reads its sums in fp32 (4.5 TB/s) and
+// has one launch more; its parts have 8 stages and more.  Groups' weights are read
+// again for every row tile, from memory where they are large: forward, the 256
+// rows of a tile count for 0.7 (32 groups [2816, 2048] at 8192 rows 98 us, 128 x
+// 128 124; dense 126, 156; 16 groups [4096, 2048] at 2048 rows 48, 57).  [4096, 4096], us: 512
+// rows 64 x 128 29, 128 x 128 whole 36, in four parts 35, 256 x 256 68; 4096
+// rows 103, 145, 103 (64, 128, 256: 210).
+static void lin_tiling(LinPlan& p, int op, int64_t I, int64_t J, int64_t len, int64_t E, bool quant) {
+  const int64_t nk = (len + (quant ? 127 : 31)) / (quant ? 128 : 32);
+  const double stage = quant ? 1.65 : 1.0;
+  double best = 1e30;
+  for (int tile = 256; tile >= 64; tile /= 2) {
+    const int64_t bn = tile == 256 ? 256 : 128;
+    const int64_t gi = op == LIN_WEIGHT_GRAD ? (I + tile - 1) / tile * E : (E > 1 ? I / tile + (E < I ? E : I) / 2 + 1 : (I + tile - 1) / tile);
+    const int64_t tiles = gi * ((J + bn - 1) / bn);
+    int64_t most = tiles < 256 ? nk / 8 : 1;
+    if (most > 16) most = 16;
+    for (int64_t s = 1; s == 1 || s <= most; ++s) {
+      const int64_t per = s == 1 ? nk : ((nk + s - 1) / s + 3) & ~(int64_t)3, n = (tiles * s + 255) / 256;  // tiles a CU
+      const double c64[3] = {0.0, 0.22, 0.41};
+      const double c = tile == 256 ? (tiles * s <= 128 ? 0.56 : 0.78 * n) : tile == 128 ? n / 2 * 0.58 + n % 2 * 0.30 : n / 3 * 0.60 + c64[n % 3];
+      double t = c * stage * per * (tile == 256 && E > 1 && op == LIN_FORWARD ? 0.7 : 1.0) + 5.0;
+      if (s > 1) t += 4.0 + (double)(s * I * (op == LIN_WEIGHT_GRAD ? E : 1) * J) * 8.0 / 4.5e6;
+      if (t < best) {
+        best = t;
+        p.tile = tile;
+        p.splits = (int)s;
+      }
+    }
+  }
+}
+
 static LinPlan lin_plan(int op, int64_t T, int64_t lda, int64_t ldb, int64_t N, int64_t K, int64_t E, bool mx, bool quant,
                         bool aligned) {
   LinPlan p{};
   const int64_t rows = (T + E - 1) / E;  // of an average group
-  p.few = op == LIN_FORWARD && lin_few(T, N, E, mx, quant);
+  p.few = op == LIN_FORWARD && lin_few(T, N, K, E, mx, quant);
   const int64_t inner = op == LIN_FORWARD ? K : N;  // elements of a row of a
   const bool whole = aligned && lda % 8 == 0 && lda < (1 << 21);
   const bool wwhole = aligned && K % 8 == 0;
@@ -171,25 +214,8 @@ static LinPlan lin_plan(int op, int64_t T, int64_t lda, int64_t ldb, int64_t N, 
   p.splits = 1;
   if (!p.few) {
     const int64_t I = op == LIN_WEIGHT_GRAD ? N : T, J = op == LIN_FORWARD ? N : K;
-    const int64_t big = I / 256 * ((J + 255) / 256) * (op == LIN_WEIGHT_GRAD ? E : 1);
-    p.tile = big >= 192 && (op == LIN_WEIGHT_GRAD || rows >= 256) ? 256 : 128;
-    // Fewer tiles than CUs: the contraction is split so that two workgroups a CU
-    // run, into parts of 8 stages and more (16 of 4-bit inputs, whose stages are four
-    // times as deep).  [4096, 4096] at 64 rows, us whole / split: forward 61 / 20,
-    // input gradient 69 / 21.
-    const int64_t gi = op == LIN_WEIGHT_GRAD ? (N + 127) / 128 * E : (T + 127) / 128 + (E - 1) / 2;
-    const int64_t tiles = gi * ((J + 127) / 128);
-    const int64_t nk = ((op == LIN_WEIGHT_GRAD ? rows : p.len) + (quant ? 127 : 31)) / (quant ? 128 : 32);
-    if (p.tile == 128 && tiles < 256) {
-      int64_t s = 512 / tiles;
-      const int64_t most = nk / (quant ? 16 : 8);
-      if (s > most) s = most;
-      if (s > 16) s = 16;
-      if (s > 1) {
-        p.splits = (int)s;
-        p.part = take((size_t)s * (op == LIN_WEIGHT_GRAD ? E * N : T) * J * 4);
-      }
-    }
+    lin_tiling(p, op, I, J, op == LIN_WEIGHT_GRAD ? rows : p.len, E, quant);
+    if (p.splits > 1) p.part = take((size_t)p.splits * (op == LIN_WEIGHT_GRAD ? E * N : T) * J * 4);
   }
   p.total = at;
   return p;
@@ -205,14 +231,14 @@ static int launch_align(const void* src, int64_t lds, int64_t rows, int64_t cols
   return LM_OK;
 }
 
-template <int DT, int OP, int W, int B, int WM, int WN>
+template <int DT, int OP, int W, int BM, int BN, int WM, int WN>
 static int launch_mm(const LinArgs& a, const LinPlan& p, hipStream_t st) {
   TimedLaunch timed("linear", st);
-  const int64_t J = OP == LIN_FORWARD ? a.N : a.K, gj = (J + B - 1) / B;
-  const int64_t gi = OP == LIN_WEIGHT_GRAD ? (a.N + B - 1) / B : lin_tiles<B>(a.T, a.experts, a.ends != nullptr);
+  const int64_t J = OP == LIN_FORWARD ? a.N : a.K, gj = (J + BN - 1) / BN;
+  const int64_t gi = OP == LIN_WEIGHT_GRAD ? (a.N + BM - 1) / BM : lin_tiles<BM>(a.T, a.experts, a.ends != nullptr);
   if (gi * gj > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
   const dim3 grid((unsigned)(gi * gj), OP == LIN_WEIGHT_GRAD ? a.experts : p.splits, OP == LIN_WEIGHT_GRAD ? p.splits : 1);
-  hipLaunchKernelGGL((k_lin_mm<DT, OP, W, B, B, WM, WN>), grid, dim3(WM * WN * 64), 0, st, a);
+  hipLaunchKernelGGL((k_lin_mm<DT, OP, W, BM, BN, WM, WN>), grid, dim3(WM * WN * 64), 0, st, a);
   LAUNCH_CHECK();
   if (p.splits > 1) {
     const int64_t n = (OP == LIN_WEIGHT_GRAD ? a.experts * a.N : a.T) * J, blocks = (n + 1023) / 1024;
@@ -223,11 +249,15 @@ static int launch_mm(const LinArgs& a, const LinPlan& p, hipStream_t st) {
   }
   return LM_OK;
 }
+template <int DT, int OP, int W>
+static int run_mm_dt(const LinArgs& a, const LinPlan& p, hipStream_t st) {
+  if (p.tile == 256) return launch_mm<DT, OP, W, 256, 256, 2, 4>(a, p, st);
+  if (p.tile == 64) return launch_mm<DT, OP, W, 64, 128, 1, 4>(a, p, st);
+  return launch_mm<DT, OP, W, 128, 128, 2, 2>(a, p, st);
+}
 template <int OP, int W>
 static int run_mm(const LinArgs& a, const LinPlan& p, int dtype, hipStream_t st) {
-  if (dtype == LM_F16)
-    return p.tile == 256 ? launch_mm<F16, OP, W, 256, 2, 4>(a, p, st) : launch_mm<F16, OP, W, 128, 2, 2>(a, p, st);
-  return p.tile == 256 ? launch_mm<BF16, OP, W, 256, 2, 4>(a, p, st) : launch_mm<BF16, OP, W, 128, 2, 2>(a, p, st);
+  return dtype == LM_F16 ? run_mm_dt<F16, OP, W>(a, p, st) : run_mm_dt<BF16, OP, W>(a, p, st);
 }
 
 template <int DT, int W, int MF, int CF, int NW, int UN, bool EDGE = false>

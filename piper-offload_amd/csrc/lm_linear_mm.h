@@ -34,6 +34,8 @@
 // multiplies.  Four waves (128 x 128): the two workgroups of a CU do that by
 // themselves.
 #pragma once
+#include <type_traits>
+
 #include "lm_linear.h"
 
 enum : int { KC16, KS16, KC4, KS4 };
@@ -74,8 +76,13 @@ DEV void lin_wait() {
 // conflicts (SQ_LDS_BANK_CONFLICT).
 DEV int mm_key(int slot) { return (((slot >> 2) << 1) & 2) ^ (((slot >> 3) & 1) * 3); }
 // A transposed read takes 32 bytes each of rows 0-3 and 8-11 (then 16-19 and
-// 24-27) together: eight pairs of chunks, one of each in all 64 banks.
-DEV int mm_row_key(int row) { return ((row & 3) | ((row >> 1) & 4)) << 1; }
+// 24-27) together: eight pairs of chunks, one of each in all 64 banks.  (Rows of
+// 64 indices are half of the banks, two neighbours all of them.)
+template <int B>
+DEV int mm_row_key(int row) {
+  if constexpr (B == 64) return (((row >> 1) & 1) | ((row >> 2) & 2)) << 1;
+  return ((row & 3) | ((row >> 1) & 4)) << 1;
+}
 
 // Tiles of up to 8 row tiles x all columns, row tiles first, are neighbours, and
 // each XCD takes a contiguous part of them, so its L2 holds the tiles of the
@@ -117,12 +124,11 @@ struct MmTraits {
   static constexpr int IK = OP == LIN_WEIGHT_GRAD ? KS16 : KC16;
   static constexpr int JK = OP == LIN_FORWARD ? (MX ? KC4 : KC16) : (OP == LIN_INPUT_GRAD && MX ? KS4 : KS16);
   static constexpr int FI = BM / WM / 16, FJ = BN / WN / 16;
-  static constexpr int US = JK == KC4 ? 8 : 4;       // stages of a turn of the loop
   static constexpr int IB = BM * 64, JB = BN * 64;  // bytes of a stage (KC4: of four)
   static constexpr int IL = IB / 1024 / NW;                               // loads per wave
   static constexpr int JL = JK == KS4 ? 2 : JB / 1024 / NW;
   static constexpr int SB = Q4 ? NW * 256 : 16;  // bytes of a stage's scales: I's, then J's
-  static_assert(!Q4 || BM / 64 + BN / 64 == NW, "a piece of scales per wave");
+  static_assert(!Q4 || BM / 64 + BN / 64 <= NW, "at most a piece of scales per wave");
   static_assert(IL * 1024 * NW == IB, "tiles are whole loads of all waves");
   static_assert(JK == KS4 || JL * 1024 * NW == JB, "tiles are whole loads of all waves");
   static_assert(JK != KC4 || JL == 2, "KC4: a load in each of two stages");
@@ -137,7 +143,7 @@ DEV void mm_offsets(uint32_t (&off)[L], int wave, int lane, int64_t ld) {
     const int piece = (n * NW + wave) * 64 + lane;  // 16-byte piece of the tile
     if constexpr (KIND == KC16) off[n] = (uint32_t)((piece >> 2) * ld * 2) + ((piece & 3) ^ mm_key(piece >> 2)) * 16;
     else if constexpr (KIND == KC4) off[n] = (uint32_t)((piece >> 2) * (ld >> 1)) + ((piece & 3) ^ ((piece >> 4) & 3)) * 16;
-    else off[n] = (uint32_t)(piece / (B / 8) * ld * 2) + ((piece % (B / 8)) ^ mm_row_key(piece / (B / 8))) * 16;
+    else off[n] = (uint32_t)(piece / (B / 8) * ld * 2) + ((piece % (B / 8)) ^ mm_row_key<B>(piece / (B / 8))) * 16;
   }
 }
 
@@ -150,7 +156,7 @@ DEV uint32_t mm_at(int slot0, int lane) {
   if constexpr (KIND == KC16) return (slot0 + p) * 64 + ((g ^ mm_key(p)) << 4);
   else if constexpr (KIND == KC4) return (slot0 + p) * 64 + ((p >> 2) << 4) + g * 4;  // ^ 16 times the stage
   const int row = 8 * g + (p >> 2), chunk = (slot0 >> 3) + ((p >> 1) & 1);
-  return row * (B * 2) + ((chunk ^ mm_row_key(row)) << 4 | (p & 1) << 3);
+  return row * (B * 2) + ((chunk ^ mm_row_key<B>(row)) << 4 | (p & 1) << 3);
 }
 template <int KIND, int B>
 DEV lm_u32x4 mm_frag(const lds_u8* t, uint32_t at, int f) {
@@ -229,7 +235,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
   // stages [kb, ke) of nk: this workgroup's part where the contraction is split
   const int nk = (int)((len + CS - 1) / CS);
   const int splits = OP == LIN_WEIGHT_GRAD ? gridDim.z : gridDim.y, split = OP == LIN_WEIGHT_GRAD ? blockIdx.z : blockIdx.y;
-  const int per = ((nk + splits - 1) / splits + P::US - 1) / P::US * P::US, kb = split * per, ke = kb + per < nk ? kb + per : nk;
+  const int per = ((nk + splits - 1) / splits + 3) & ~3, kb = split * per, ke = kb + per < nk ? kb + per : nk;
   v4f32 acc[FI][FJ] = {};
 
   if (kb < ke) {
@@ -285,7 +291,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
       if (wave < BM / 64) {
         scp = a.xs + ig * nk * 256;
         scleft = ig < a.padded ? (int64_t)nk * 256 : 0;
-      } else {
+      } else if (wave < BM / 64 + BN / 64) {
         scp = a.wsc + (t.group * gj + jg) * nk * 256;
         scleft = jg < gj ? (int64_t)nk * 256 : 0;
       }
@@ -334,7 +340,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
         const float s = lin_e8m0(code_s[set], 0);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
-          *(lds_u32x4*)(tj + kr * (BN * 2) + (((kc * 2 + c) ^ mm_row_key(kr)) << 4)) = lin_decode8<HALF>(code[set][c], s);
+          *(lds_u32x4*)(tj + kr * (BN * 2) + (((kc * 2 + c) ^ mm_row_key<BN>(kr)) << 4)) = lin_decode8<HALF>(code[set][c], s);
       }
     };
     // (called for every stage, in order; KC4: half says which half of the codes, tj where they go)
@@ -375,7 +381,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
     };
     const uint32_t ati = mm_at<IK, BM>(wi * (FI * 16), lane), atj = mm_at<JK == KS4 ? KS16 : JK, BN>(wj * (FJ * 16), lane);
     lm_u32x4 fi[FI], fj[FJ];
-    uint32_t isc[Q4 ? FI / 4 : 1], jsc[Q4 ? FJ / 4 : 1], jc[JK == KC4 ? FJ : 1];
+    constexpr int IW = (FI + 3) / 4, JW = (FJ + 3) / 4;  // words of scales
+    uint32_t isc[IW], jsc[JW], jc[JK == KC4 ? FJ : 1];
     auto read = [&](int b, const lds_u8* ti, const lds_u8* tj, const lds_u8* ts) {
       const uint32_t ai = mm_hide(ati), aj = mm_hide(atj);
 #pragma unroll
@@ -388,9 +395,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
       if constexpr (Q4) {
         const uint32_t as = mm_hide(lane * 4);
 #pragma unroll
-        for (int f = 0; f < FI / 4; ++f) isc[f] = *(const lds_u32*)(ts + as + (wi * (FI / 4) + f) * 256);
+        for (int f = 0; f < IW; ++f) isc[f] = *(const lds_u32*)(ts + as + (wi * FI / 4 + f) * 256) >> (FI < 4 ? 8 * (wi * FI & 3) : 0);
 #pragma unroll
-        for (int f = 0; f < FJ / 4; ++f) jsc[f] = *(const lds_u32*)(ts + as + (BM / 64 + wj * (FJ / 4) + f) * 256);
+        for (int f = 0; f < JW; ++f) jsc[f] = *(const lds_u32*)(ts + as + (BM / 64 + wj * FJ / 4 + f) * 256) >> (FJ < 4 ? 8 * (wj * FJ & 3) : 0);
       }
     };
     auto decode = [&](int b) {
@@ -438,26 +445,27 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
     lin_wait<JK == KS4 ? 0 : 2 * L>();  // stage kb is in LDS
     lin_barrier();
     if (PP && wave >= 4) lin_barrier();  // the second half runs one barrier behind
-    for (int st = kb; st < ke; st += P::US) {
+    auto four = [&](int st, auto half) {  // stages st .. st + 3; KC4: their codes are in buffer `half`
+      constexpr int H = decltype(half)::value;
 #pragma unroll
-      for (int b = 0; b < P::US; ++b) {
+      for (int b = 0; b < 4; ++b) {
         const int n = (b + 3) & 3;  // the buffer of stage st + b + 3
-        if (b % 4 == 0) next_scales(st + b);
-        read(b, ti[b & 3], JK == KC4 ? tj[(b >> 2) & 1] : tj[b & 3], ts[b & 3]);
+        if (b == 0) next_scales(st);
+        read(b, ti[b], JK == KC4 ? tj[H] : tj[b], ts[b]);
         __builtin_amdgcn_sched_barrier(0);
         // (while the reads are on their way)  Buffer n was read for stage
         // st + b - 1, and all waves are past that.
-        if (b % 4 == 0) load_scales(st + b + 4);
+        if (b == 0) load_scales(st + 4);
         load_codes(st + b + 3, (b + 1) & 1);
-        load(st + b + 3, st + (b & ~3) + 4, b % 4 < 2 ? b % 4 : -1, ti[n], JK == KC4 ? tj[~(b >> 2) & 1] : tj[n], ts[n]);
+        load(st + b + 3, st + 4, b < 2 ? b : -1, ti[n], JK == KC4 ? tj[1 - H] : tj[n], ts[n]);
         decode(b);
         // Stage st + b + 1 is in LDS, and this one in registers: what may be left
         // are the loads of stages st + b + 2 and st + b + 3, with KC4 the scales and
         // codes that were asked for since.
         if constexpr (JK == KC4) {
-          if (b % 4 == 0) lin_wait<2 * L + FJ + 1>();
-          else if (b % 4 == 1) lin_wait<2 * L + FJ + 2>();
-          else if (b % 4 == 2) lin_wait<2 * L + 1>();
+          if (b == 0) lin_wait<2 * L + FJ + 1>();
+          else if (b == 1) lin_wait<2 * L + FJ + 2>();
+          else if (b == 2) lin_wait<2 * L + 1>();
           else lin_wait<2 * L>();
         } else {
           lin_wait<2 * L>();
@@ -466,6 +474,12 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
         multiply();
         store_codes(tj[(b + 2) & 3], b & 1);
         if constexpr (PP) lin_barrier();
+      }
+    };
+    for (int st = kb; st < ke; st += JK == KC4 ? 8 : 4) {
+      four(st, std::integral_constant<int, 0>{});
+      if constexpr (JK == KC4) {
+        if (st + 4 < ke) four(st + 4, std::integral_constant<int, 1>{});
       }
     }
     if constexpr (PP) {
