@@ -15,51 +15,91 @@
 // ---------------------------------------------------------------------------
 // 4-bit inputs: x quantised to MXFP4 (blocks of 32 along K, scale
 // 2^(floor(log2 max) - 2)), and its scales and the weight's in the order the
-// scaled MFMA takes them.  One launch: the first workgroups take a row of x per
-// wave (8 values a lane: 16 bytes in, 4 out, a block's maximum over 4 lanes
-// by DPP), the others one packed piece of weight scales per wave.
+// scaled MFMA takes them.  One launch: the first workgroups take 2048 values of a
+// row of x per wave (8 a lane and load: 16 bytes in, 4 out, a block's maximum over
+// 4 lanes by DPP), the others 64 rows x 16 blocks of weight scales per wave.
 // ---------------------------------------------------------------------------
 // byte of (slot, block) in the packed scales: pieces of 64 slots x 4 blocks
 DEV int64_t lin_packed(int64_t slot, int64_t block, int64_t nk) {
   const int f = (int)(slot >> 4) & 3, r = (int)slot & 15, g = (int)block & 3;
   return ((slot >> 6) * nk + (block >> 2)) * 256 + (16 * g + r) * 4 + f;
 }
-template <int DT>
-__global__ __launch_bounds__(256) void k_lin_prep4(LinArgs a, int row_blocks, uint8_t* xq, uint8_t* xs, uint8_t* wsc) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t nk = (a.K + 127) >> 7, nb = a.K >> 5;
-  if ((int)blockIdx.x < row_blocks) {
-    const int64_t t = (int64_t)blockIdx.x * 4 + wave_index();
+// PACK: rows in the padded order of their groups, packed scales (k_lin_mm); else
+// both in row order (k_lin_few)
+template <int DT, bool PACK>
+__global__ __launch_bounds__(256) void k_lin_prep4(LinArgs a, uint32_t row_blocks, uint32_t segs, uint8_t* xq, uint8_t* xs, uint8_t* wsc) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t nk = (uint32_t)((a.K + 127) >> 7), nb = (uint32_t)(a.K >> 5);
+  if (!PACK || blockIdx.x < row_blocks) {
+    const uint32_t item = blockIdx.x * 4 + wave_index(), t = item / segs, units = (uint32_t)(a.K >> 3);
     if (t >= a.T) return;
+    const uint32_t u0 = (item - t * segs) * 256 + lane;
+    const LM_GLOBAL uint16_t* x = (const LM_GLOBAL uint16_t*)a.a + t * a.lda;
+    lm_u32x4 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = lm_u32x4{};
+      if (u0 + 64 * i < units) w[i] = *(const LM_GLOBAL lm_u32x4_any*)(x + (u0 + 64 * i) * 8);
+    }
     int64_t p = t;
-    if (a.ends) {
+    if (PACK && a.ends) {
       int g = a.experts;
       lin_row(a, (int)t, g, p);
       if (g == a.experts) return;  // a row of no group
     }
-    const uint16_t* x = (const uint16_t*)a.a + t * a.lda;
-    const int64_t units = a.K >> 3, padded = nk * 16;
-    for (int64_t u = lane; u < padded; u += 64) {
-      lm_u32x4 w = {};
-      if (u < units) w = *(const LM_GLOBAL lm_u32x4_any*)(x + u * 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = u0 + 64 * i;
       uint32_t s;
-      const uint32_t c = lin_quant8<DT>(w, s);
+      const uint32_t c = lin_quant8<DT>(w[i], s);
       if (u < units) *(LM_GLOBAL uint32_t*)(xq + p * (a.K >> 1) + u * 4) = c;
-      // (blocks past K are zeros with the smallest scale)
-      if ((lane & 3) == 0) *(LM_GLOBAL uint8_t*)(xs + lin_packed(p, u >> 2, nk)) = (uint8_t)(u < units ? s : 0);
+      // (blocks past K, up to whole words of scales, are zeros with the smallest scale)
+      if ((lane & 3) == 0 && (u >> 2) < nk * 4)
+        ((LM_GLOBAL uint8_t*)xs)[PACK ? lin_packed(p, u >> 2, nk) : p * (int64_t)(nk * 4) + (u >> 2)] = (uint8_t)(u < units ? s : 0);
     }
   } else {
-    const int64_t gj = (a.N + 63) >> 6, piece = (int64_t)(blockIdx.x - row_blocks) * 4 + wave;
-    if (piece >= gj * nk * a.experts) return;
-    const int64_t kt = piece % nk, eg = piece / nk, e = eg / gj, n0 = (eg % gj) * 64;
-    const int64_t b = kt * 4 + (lane >> 4);
-    uint32_t s = 0;
+    // Lane 16f + r has the row of slot (f, r) and four words w[j], blocks 4j .. 4j + 3
+    // of it.  The transpose of words between the lane groups gives lane group j the
+    // words of all four f for piece j; a transpose of their bytes makes them the
+    // words (g, r) of the piece.
+    const uint32_t gj = (uint32_t)((a.N + 63) >> 6), quads = (nk + 3) >> 2;
+    const int64_t item = (int64_t)(blockIdx.x - row_blocks) * 4 + wave_index(), eg = item / quads;
+    if (eg >= (int64_t)gj * a.experts) return;
+    const uint32_t q = (uint32_t)(item - eg * quads);
+    const int64_t e = eg / gj, n = (eg - e * gj) * 64 + lane;
+    const LM_GLOBAL uint8_t* src = (const LM_GLOBAL uint8_t*)a.scale + e * a.scale_stride;
+    lm_u32x4 w = {};
+    if (n < a.N) {
+      if (a.swizzled) {
+        src += blocked_offset(n, 0, nb, true);
 #pragma unroll
-    for (int f = 0; f < 4; ++f) {
-      const int64_t n = n0 + 16 * f + (lane & 15);
-      if (n < a.N && b < nb) s |= (uint32_t)a.scale[e * a.scale_stride + blocked_offset(n, b, nb, a.swizzled)] << (8 * f);
+        for (int j = 0; j < 4; ++j)
+          if (4 * q + j < nk) w[j] = *(const LM_GLOBAL uint32_t*)(src + (4 * q + j) * (int64_t)512);
+      } else if (16 * q + 16 <= nb) {
+        w = *(const LM_GLOBAL lm_u32x4_any*)(src + n * nb + 16 * q);
+      } else {
+#pragma unroll
+        for (int b = 0; b < 15; ++b)
+          if (16 * q + b < nb) w[b >> 2] |= (uint32_t)src[n * nb + 16 * q + b] << (8 * (b & 3));
+      }
     }
-    *(LM_GLOBAL uint32_t*)(wsc + piece * 256 + lane * 4) = s;
+    if (a.swizzled && 16 * q + 16 > nb) {  // what the padding of the last tile holds
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int have = (int)nb - (int)(16 * q + 4 * j);
+        if (have < 4) w[j] = have <= 0 ? 0u : w[j] & ((1u << (8 * have)) - 1);
+      }
+    }
+    lin_transpose4(w);
+    // bytes: v[g] = byte g of w[0], w[1], w[2], w[3]
+    const uint32_t a0 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400), a1 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602);
+    const uint32_t b0 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400), b1 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602);
+    const uint32_t v[4] = {(a0 & 0xffffu) | b0 << 16, a0 >> 16 | (b0 & 0xffff0000u), (a1 & 0xffffu) | b1 << 16, a1 >> 16 | (b1 & 0xffff0000u)};
+    const uint32_t piece = 4 * q + (lane >> 4);
+    if (piece < nk) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) *(LM_GLOBAL uint32_t*)(wsc + (eg * nk + piece) * 256 + (16 * g + (lane & 15)) * 4) = v[g];
+    }
   }
 }
 
@@ -364,18 +404,19 @@ extern "C" int lm_linear(const void* x, int64_t ldx, const lm_weight* w, const v
   uint8_t *xq = (uint8_t*)a.xq, *xs = (uint8_t*)a.xs, *wsc = (uint8_t*)a.wsc;
   {
     TimedLaunch timed("linear_prep", st);
-    const int segs = (int)((a.K + 2047) / 2048);
-    const int64_t rows = (p.few ? T * segs : T + 3) / 4 + (p.few ? 1 : 0);
-    const int64_t pieces = p.few ? 0 : (a.experts * ((a.N + 63) / 64) * ((a.K + 127) / 128) + 3) / 4;
-    if (rows + pieces > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+    const int64_t segs = (a.K + 2047) / 2048, rows = (T * segs + 3) / 4;
+    const int64_t pieces = p.few ? 0 : (a.experts * ((a.N + 63) / 64) * ((a.K + 511) / 512) + 3) / 4;
+    if (T * segs > 0x7fffffff || rows + pieces > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
     const dim3 grid((unsigned)(rows + pieces));
+#define PREP(DT, PACK) hipLaunchKernelGGL((k_lin_prep4<DT, PACK>), grid, dim3(256), 0, st, a, (uint32_t)rows, (uint32_t)segs, xq, xs, wsc)
     if (p.few) {
-      if (dtype == LM_F16) hipLaunchKernelGGL((k_lin_quant<F16>), grid, dim3(256), 0, st, a, segs, xq, xs);
-      else hipLaunchKernelGGL((k_lin_quant<BF16>), grid, dim3(256), 0, st, a, segs, xq, xs);
+      if (dtype == LM_F16) PREP(F16, false);
+      else PREP(BF16, false);
     } else {
-      if (dtype == LM_F16) hipLaunchKernelGGL((k_lin_prep4<F16>), grid, dim3(256), 0, st, a, (int)rows, xq, xs, wsc);
-      else hipLaunchKernelGGL((k_lin_prep4<BF16>), grid, dim3(256), 0, st, a, (int)rows, xq, xs, wsc);
+      if (dtype == LM_F16) PREP(F16, true);
+      else PREP(BF16, true);
     }
+#undef PREP
     LAUNCH_CHECK();
   }
   return p.few ? run_few<W_Q4>(a, dtype, st) : run_mm<LIN_FORWARD, W_Q4>(a, p, dtype, st);

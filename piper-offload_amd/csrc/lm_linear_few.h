@@ -14,7 +14,7 @@
 // transpose of dwords between the lane groups (4 lane swaps) brings them to
 // the same order.  With 4-bit inputs both sides are codes and the scaled MFMA
 // takes them as they lie; the rows are quantised by a launch of their own
-// (k_lin_quant): every workgroup needs all of them, and quantising them in each
+// (k_lin_prep4): every workgroup needs all of them, and quantising them in each
 // costs more than the launch ([14336, 4096] at 1 row: 34 us in one launch).
 //
 // All loads are buffer loads: 32-bit offsets, and what lies past the end of the
@@ -35,31 +35,6 @@ DEV void lin_transpose4(lm_u32x4& d) {
 }
 DEV lm_u32x4 few_load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
   return __builtin_bit_cast(lm_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
-}
-
-// rows of x to MXFP4 in row order: codes [T, K/2], scales [T, padded to 4]
-template <int DT>
-__global__ __launch_bounds__(256) void k_lin_quant(LinArgs a, int segs, uint8_t* xq, uint8_t* xs) {
-  const int lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * 4 + wave_index();
-  const int64_t t = item / segs, units = a.K >> 3, nb4 = ((a.K >> 5) + 3) & ~(int64_t)3;
-  if (t >= a.T) return;
-  const uint16_t* x = (const uint16_t*)a.a + t * a.lda;
-  const int64_t u0 = (item % segs) * 256 + lane;
-  lm_u32x4 w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[i] = lm_u32x4{};
-    if (u0 + 64 * i < units) w[i] = *(const LM_GLOBAL lm_u32x4_any*)(x + (u0 + 64 * i) * 8);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t u = u0 + 64 * i;
-    uint32_t s;
-    const uint32_t c = lin_quant8<DT>(w[i], s);
-    if (u < units) *(LM_GLOBAL uint32_t*)(xq + t * (a.K >> 1) + u * 4) = c;
-    if ((lane & 3) == 0 && (u >> 2) < nb4) ((LM_GLOBAL uint8_t*)xs)[t * nb4 + (u >> 2)] = (uint8_t)(u < units ? s : 0);
-  }
 }
 
 // EDGE: dense rows whose length is no multiple of 8
