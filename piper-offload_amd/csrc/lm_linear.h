@@ -18,6 +18,7 @@ struct LinArgs {
   int64_t padded;  // 64-row pieces of xq
   int64_t ldw;     // row stride of a dense w
   int64_t len;     // contraction (with zeros up to whole 16-byte pieces)
+  int rounds;      // 256 x 256 tiles: whole rounds in one launch, the rest in another (lin_rounds)
   float* part;     // split contraction: fp32 sums [splits, rows, columns], or null
   const void* w;  // [experts, N, K] dense or [experts, N, K/2] codes
   const uint8_t* scale;
@@ -121,13 +122,12 @@ DEV void lin_group(const LinArgs& a, int g, int64_t& b, int64_t& e) {
 // row.  Finds tile t: its group and rows [r0, r1), false past the last tile;
 // t < 0 counts the tiles into g.  pad: r0 if every group's rows were padded to a
 // multiple of 64.
-template <int BM>
-DEV bool lin_find(const LinArgs& a, int t, int& g, int64_t& r0, int64_t& r1, int64_t& pad) {
+DEV bool lin_find(const LinArgs& a, int BM, int t, int& g, int64_t& r0, int64_t& r1, int64_t& pad) {
   int before = 0, tiles = 0, pieces = 0;
   for (int c = 0; c <= a.experts; c += 64) {
     int b, e;
     lin_groups64(a, c, before, b, e);
-    const int n = (e - b + BM - 1) / BM, n64 = (e - b + 63) >> 6;
+    const int n = (int)((uint32_t)(e - b + BM - 1) / (uint32_t)BM), n64 = (e - b + 63) >> 6;
     const int sum = lin_scan_add(n), sum64 = lin_scan_add(n64);
     const uint64_t hit = __ballot(t >= tiles && t < tiles + sum);
     if (hit) {
@@ -165,17 +165,16 @@ DEV void lin_row(const LinArgs& a, int t, int& g, int64_t& p) {
 template <int BM>
 DEV bool lin_tile(const LinArgs& a, int64_t t, int& g, int64_t& r0, int64_t& r1) {
   int64_t pad;
-  if (a.ends) return lin_find<BM>(a, (int)t, g, r0, r1, pad);
+  if (a.ends) return lin_find(a, BM, (int)t, g, r0, r1, pad);
   g = 0;
   r0 = t * BM;
   r1 = a.T;
   return r0 < a.T;
 }
-template <int BM>
-DEV int lin_count(const LinArgs& a) {
+DEV int lin_count(const LinArgs& a, int BM) {
   int g;
   int64_t r0, r1, pad;
-  lin_find<BM>(a, -1, g, r0, r1, pad);
+  lin_find(a, BM, -1, g, r0, r1, pad);
   return g;
 }
 // at most this many tiles: every group may end in a part of one

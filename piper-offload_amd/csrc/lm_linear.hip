@@ -154,6 +154,7 @@ static LinArgs lin_args(const lm_weight* w, const int32_t* ends, int64_t T) {
 static bool lin_few(int64_t T, int64_t N, int64_t K, int64_t E, bool mx, bool quant) {
   const int64_t rows = (T + E - 1) / E;
   const double volume = (double)T * (double)N * (double)K;
+  if (K < 512 && T > 64) return false;  // too few units for the waves: [4096, 16] of 24 groups at 2048 rows 39 / 13
   if (!mx) return T <= 16 || volume <= 5e8;
   return rows <= 16 || volume <= 1.1e9 || (quant && T <= 64);
 }
@@ -161,6 +162,7 @@ static bool lin_few(int64_t T, int64_t N, int64_t K, int64_t E, bool mx, bool qu
 struct LinPlan {
   bool few;                       // k_lin_few, else k_lin_mm
   int tile, splits;               // of k_lin_mm
+  bool rounds;                    // 256 x 256 tiles in whole rounds, the rest in smaller ones
   bool copy_a, copy_b, copy_w;    // rows realigned in the workspace first
   int64_t lda, ldb, ldw, len;
   int64_t padded;                 // 4-bit inputs: 64-row pieces
@@ -168,39 +170,64 @@ struct LinPlan {
 };
 static int64_t round8(int64_t x) { return (x + 7) & ~(int64_t)7; }
 
-// Tile and splits of k_lin_mm: the least of a model of its time.  A CU's time for
-// a stage, us, by the tiles that it works on in turn (measured, bf16, 4096 columns
-// at 256 to 4096 rows; a stage of 4-bit inputs, four times as deep, takes 1.65
-// times as long): 256 x 256 0.78 a tile, 0.56 where less than half of the CUs have
-// one; 128 x 128 two at a time in 0.58, one in 0.30; 64 x 128 three in 0.60, two
-// in 0.41, one in 0.22.  Groups end in a part of a tile, half of one on
-// average.  A split contraction writes and reads its sums in fp32 (4.5 TB/s) and
-// has one launch more; its parts have 8 stages and more.  Groups' weights are read
-// again for every row tile, from memory where they are large: forward, the 256
-// rows of a tile count for 0.7 (32 groups [2816, 2048] at 8192 rows 98 us, 128 x
-// 128 124; dense 126, 156; 16 groups [4096, 2048] at 2048 rows 48, 57).  [4096, 4096], us: 512
-// rows 64 x 128 29, 128 x 128 whole 36, in four parts 35, 256 x 256 68; 4096
-// rows 103, 145, 103 (64, 128, 256: 210).
+// Tile and splits of k_lin_mm: the least of a model of its time.  What a CU takes
+// for the tiles that it works on in turn, us per stage and per tile (measured,
+// bf16, [4096, 4096] at 256 to 4096 rows, and weight gradients of few stages; a
+// stage of 4-bit inputs, four times as deep, takes 1.65 times as long): 256 x 256
+// 0.70 and 8 (its store is not covered by another workgroup's work), 0.50 a
+// stage where less than half of the CUs have one; 128 x 128 two at a time in 0.55
+// and 2.5, one in 0.28 and 2; 64 x 128 three in 0.58 and 2, two in 0.40 and 1.5, one
+// in 0.21 and 1.  Groups end in a part of a tile, half of one on average.  A split
+// contraction writes and reads its sums in fp32 (4.5 TB/s) and has one launch more;
+// its parts have 8 stages and more.  Groups' weights are read again for every
+// row tile, from memory where they are large: forward, the 256 rows of a tile
+// count for 0.7 (32 groups [2816, 2048] at 8192 rows 98 us, 128 x 128 124; dense
+// 126, 156; 16 groups [4096, 2048] at 2048 rows 48, 57).  [4096, 4096], us: 512 rows
+// 64 x 128 29, 128 x 128 whole 36, in four parts 35, 256 x 256 68; 4096 rows 103 on
+// 256 x 256, 145 on 128 x 128.
+// Whole rounds and the rest apart (lin_rounds) where the rest's share of a round
+// is more than the second launch, 5 us: always known for one weight, likely for
+// groups with 48 stages and more (8 groups [4096, 2048] at 4096 rows 119 -> 97 us).
 static void lin_tiling(LinPlan& p, int op, int64_t I, int64_t J, int64_t len, int64_t E, bool quant) {
   const int64_t nk = (len + (quant ? 127 : 31)) / (quant ? 128 : 32);
   const double stage = quant ? 1.65 : 1.0;
+  const bool wgrad = op == LIN_WEIGHT_GRAD;
   double best = 1e30;
   for (int tile = 256; tile >= 64; tile /= 2) {
     const int64_t bn = tile == 256 ? 256 : 128;
-    const int64_t gi = op == LIN_WEIGHT_GRAD ? (I + tile - 1) / tile * E : (E > 1 ? I / tile + (E < I ? E : I) / 2 + 1 : (I + tile - 1) / tile);
+    const int64_t gi = wgrad ? (I + tile - 1) / tile * E : (E > 1 ? I / tile + (E < I ? E : I) / 2 + 1 : (I + tile - 1) / tile);
     const int64_t tiles = gi * ((J + bn - 1) / bn);
     int64_t most = tiles < 256 ? nk / 8 : 1;
     if (most > 16) most = 16;
     for (int64_t s = 1; s == 1 || s <= most; ++s) {
       const int64_t per = s == 1 ? nk : ((nk + s - 1) / s + 3) & ~(int64_t)3, n = (tiles * s + 255) / 256;  // tiles a CU
-      const double c64[3] = {0.0, 0.22, 0.41};
-      const double c = tile == 256 ? (tiles * s <= 128 ? 0.56 : 0.78 * n) : tile == 128 ? n / 2 * 0.58 + n % 2 * 0.30 : n / 3 * 0.60 + c64[n % 3];
-      double t = c * stage * per * (tile == 256 && E > 1 && op == LIN_FORWARD ? 0.7 : 1.0) + 5.0;
-      if (s > 1) t += 4.0 + (double)(s * I * (op == LIN_WEIGHT_GRAD ? E : 1) * J) * 8.0 / 4.5e6;
+      double c, fixed;
+      bool rounds = false;
+      if (tile == 256) {
+        const int64_t rest = tiles % 256;
+        c = tiles * s <= 128 ? 0.50 : 0.70 * (double)n;
+        fixed = 8.0 * (double)n;
+        rounds = s == 1 && !wgrad && tiles >= 256 && (E > 1 ? (double)nk * stage >= 48.0 : rest > 0 && rest <= 64);
+        if (rounds) c -= E > 1 ? 0.15 : 0.42;
+        if (E > 1 && op == LIN_FORWARD) {
+          c *= 0.7;
+          fixed *= 0.7;
+        }
+      } else if (tile == 128) {
+        c = (double)(n / 2) * 0.55 + (double)(n % 2) * 0.28;
+        fixed = (double)(n / 2) * 2.5 + (double)(n % 2) * 2.0;
+      } else {
+        const double c64[3] = {0.0, 0.21, 0.40}, f64[3] = {0.0, 1.0, 1.5};
+        c = (double)(n / 3) * 0.58 + c64[n % 3];
+        fixed = (double)(n / 3) * 2.0 + f64[n % 3];
+      }
+      double t = c * stage * (double)per + fixed;
+      if (s > 1) t += 4.0 + (double)(s * I * (wgrad ? E : 1) * J) * 8.0 / 4.5e6;
       if (t < best) {
         best = t;
         p.tile = tile;
         p.splits = (int)s;
+        p.rounds = rounds;
       }
     }
   }
@@ -277,7 +304,9 @@ static int launch_mm(const LinArgs& a, const LinPlan& p, hipStream_t st) {
   const int64_t J = OP == LIN_FORWARD ? a.N : a.K, gj = (J + BN - 1) / BN;
   const int64_t gi = OP == LIN_WEIGHT_GRAD ? (a.N + BM - 1) / BM : lin_tiles<BM>(a.T, a.experts, a.ends != nullptr);
   if (gi * gj > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
-  const dim3 grid((unsigned)(gi * gj), OP == LIN_WEIGHT_GRAD ? a.experts : p.splits, OP == LIN_WEIGHT_GRAD ? p.splits : 1);
+  // (the rest of whole rounds: at most 128 tiles, four workgroups each)
+  const int64_t n0 = BM == 128 && a.rounds ? 512 : gi * gj;
+  const dim3 grid((unsigned)n0, OP == LIN_WEIGHT_GRAD ? a.experts : p.splits, OP == LIN_WEIGHT_GRAD ? p.splits : 1);
   hipLaunchKernelGGL((k_lin_mm<DT, OP, W, BM, BN, WM, WN>), grid, dim3(WM * WN * 64), 0, st, a);
   LAUNCH_CHECK();
   if (p.splits > 1) {
@@ -291,7 +320,12 @@ static int launch_mm(const LinArgs& a, const LinPlan& p, hipStream_t st) {
 }
 template <int DT, int OP, int W>
 static int run_mm_dt(const LinArgs& a, const LinPlan& p, hipStream_t st) {
-  if (p.tile == 256) return launch_mm<DT, OP, W, 256, 256, 2, 4>(a, p, st);
+  if (p.tile == 256) {
+    LinArgs b = a;
+    b.rounds = p.rounds;
+    const int rc = launch_mm<DT, OP, W, 256, 256, 2, 4>(b, p, st);
+    return rc || !p.rounds ? rc : launch_mm<DT, OP, W, 128, 128, 2, 2>(b, p, st);
+  }
   if (p.tile == 64) return launch_mm<DT, OP, W, 64, 128, 1, 4>(a, p, st);
   return launch_mm<DT, OP, W, 128, 128, 2, 2>(a, p, st);
 }

@@ -87,14 +87,16 @@ DEV int mm_row_key(int row) {
 // Tiles of up to 8 row tiles x all columns, row tiles first, are neighbours, and
 // each XCD takes a contiguous part of them, so its L2 holds the tiles of the
 // other operand that several row tiles share.
-DEV bool lin_order(uint32_t b, uint32_t tm, uint32_t tn, uint32_t& m, uint32_t& n) {
-  const uint32_t total = tm * tn;
-  if (b >= total) return false;
-  const uint32_t u = (uint32_t)xcd_unit(b, total), band = u / (8 * tn), in = u - band * 8 * tn;
-  const uint32_t left = tm - band * 8, h = left < 8 ? left : 8;
+DEV void lin_order(uint32_t u, uint32_t tm, uint32_t tn, uint32_t& m, uint32_t& n) {
+  const uint32_t band = u / (8 * tn), in = u - band * 8 * tn, left = tm - band * 8, h = left < 8 ? left : 8;
   m = band * 8 + in % h;
   n = in / h;
-  return true;
+}
+// Of 256 x 256 tiles, those of whole rounds over the 256 CUs.  The rest, where it
+// is less than half a round, is left to a second launch of 128 x 128 tiles, which
+// has something for every CU: 8 groups [4096, 2048] at 4096 rows have 312 tiles.
+DEV uint32_t lin_rounds(uint32_t total) {
+  return total >= 256 && total % 256 <= 128 ? total - total % 256 : total;
 }
 // The tile of this workgroup: group, first row, end of the group's rows, first
 // column.
@@ -105,15 +107,28 @@ struct LinTile {
 };
 template <int BM, int BN>
 DEV bool lin_pick(const LinArgs& a, int64_t jend, LinTile& t) {
-  uint32_t m, n;
-  const uint32_t tiles = a.ends ? (uint32_t)lin_count<BM>(a) : (uint32_t)((a.T + BM - 1) / BM);
-  if (!lin_order(blockIdx.x, tiles, (uint32_t)((jend + BN - 1) / BN), m, n)) return false;
-  t.j0 = (int64_t)n * BN;
-  if (a.ends) return lin_find<BM>(a, (int)m, t.group, t.r0, t.r1, t.pad);
-  t.group = 0;
-  t.pad = t.r0 = (int64_t)m * BM;
-  t.r1 = a.T;
-  return true;
+  const bool rest = BM == 128 && a.rounds;  // quarters of the 256 x 256 tiles that are left
+  const int bm = rest ? 256 : BM, bn = rest ? 256 : BN;
+  const uint32_t tm = a.ends ? (uint32_t)lin_count(a, bm) : (uint32_t)((a.T + bm - 1) / bm), tn = (uint32_t)((jend + bn - 1) / bn);
+  const uint32_t total = tm * tn, whole = a.rounds ? lin_rounds(total) : total;
+  uint32_t b = blockIdx.x, m, n;
+  if (b >= (rest ? 4 * (total - whole) : whole)) return false;
+  b = (uint32_t)xcd_unit(b, rest ? 4 * (total - whole) : whole);
+  lin_order(rest ? whole + (b >> 2) : b, tm, tn, m, n);
+  t.j0 = (int64_t)n * bn;
+  if (a.ends) {
+    if (!lin_find(a, bm, (int)m, t.group, t.r0, t.r1, t.pad)) return false;
+  } else {
+    t.group = 0;
+    t.pad = t.r0 = (int64_t)m * bm;
+    t.r1 = a.T;
+  }
+  if (rest) {
+    t.r0 += (b >> 1 & 1) * 128;
+    t.pad += (b >> 1 & 1) * 128;
+    t.j0 += (b & 1) * 128;
+  }
+  return t.r0 < t.r1 && t.j0 < jend;
 }
 
 template <int DT, int OP, int W, int BM, int BN, int WM, int WN>
@@ -195,7 +210,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
   int64_t lda = a.lda, ldb;
   if constexpr (OP == LIN_WEIGHT_GRAD) {
     uint32_t m, n;
-    if (!lin_order(blockIdx.x, (uint32_t)((a.N + BM - 1) / BM), (uint32_t)((a.K + BN - 1) / BN), m, n)) return;
+    const uint32_t tm = (uint32_t)((a.N + BM - 1) / BM), tn = (uint32_t)((a.K + BN - 1) / BN);
+    lin_order((uint32_t)xcd_unit(blockIdx.x, tm * tn), tm, tn, m, n);
     t.group = blockIdx.y;
     t.r0 = (int64_t)m * BM;
     t.r1 = a.N;
