@@ -343,8 +343,21 @@ static int launch_few(const LinArgs& a, hipStream_t st) {
   LAUNCH_CHECK();
   return LM_OK;
 }
-// Workgroups of 16 columns spread a small weight over the most CUs; wider ones
-// read the rows less often.  `wgs`: workgroups at 16 rows x 16 columns.
+// Workgroups of 16 columns spread a small weight over the most CUs, wider ones read
+// the rows less often; loads in flight want many units a wave, short contractions
+// fewer waves, so that none is left without a unit.  `wgs`: workgroups at 16 rows x
+// 16 columns.  Measured, us (weights out of memory, waves x units a wave x columns):
+//   MXFP4 weight [4096, 4096], 1 row      8x4x16 5.4   8x4x32 6.3    16x2x16 5.5
+//   [14336, 4096], 16 rows                8x4x64 13.3  16x2x64 14.0  8x4x32 16.7
+//   32 groups [2816, 2048], 16 rows       4x2x32 16.5  8x2x64 18.6   8x4x64 20.5
+//   32 groups [2048, 1408], 512 rows      4x2x64 22.8  4x2x32 25.8   8x4x64 31.3
+//   4-bit inputs: [14336, 4096], 1 row    8x4x16 12.6  8x4x32 13.6   8x4x64 14.0
+//   [4096, 14336], 24 rows                8x4x32 21.8  8x4x16 26.4
+//   [14336, 4096], 64 rows                8x1x64 on 64 rows 25.7, 8x2x64 37.0
+//   32 groups [2816, 2048], 16 rows       4x4x32 18.3  4x2x32 19.9   8x2x32 20.3
+//   dense [2048, 4096], 1 row             16x2x16 8.2  8x2x16 8.6    4x2x16 10.0
+//   [4096, 4096], 16 rows                 8x2x32 16.3  8x2x16 18.8   4x2x32 18.2
+//   64 groups [2048, 1408], 100 rows      4x2x16 52.9  8x2x32 56.5   16x2x64 71.3
 template <int DT, int W>
 static int run_few_dt(const LinArgs& a, hipStream_t st) {
   if constexpr (W == W_DENSE) {
@@ -353,15 +366,14 @@ static int run_few_dt(const LinArgs& a, hipStream_t st) {
   const int64_t rows = (a.T + a.experts - 1) / a.experts, units = (a.K + 127) / 128;
   const int64_t wgs = lin_tiles<16>(a.T, a.experts, a.experts > 1) * ((a.N + 15) / 16);
   if (rows > 32 && wgs > 2048) return launch_few<DT, W, 4, 4, 8, 1>(a, st);
-  if constexpr (W == W_Q4) {
-    if (wgs <= 256 || (rows <= 8 && units >= 32)) return launch_few<DT, W, 1, 1, 8, 4>(a, st);
-    if (wgs <= 512 || units < 32) return launch_few<DT, W, 1, 2, 8, 2>(a, st);
-    return launch_few<DT, W, 1, 4, 8, 4>(a, st);
-  } else {
+  if constexpr (W == W_DENSE) {
     if (wgs <= 256) return launch_few<DT, W, 1, 1, 16, 2>(a, st);
-    if (wgs <= 512) return launch_few<DT, W, 1, 2, 16, 2>(a, st);
-    if (wgs <= 2048) return launch_few<DT, W, 1, 4, 16, 2>(a, st);
-    return launch_few<DT, W, 1, 4, 8, 2>(a, st);
+    return units < 32 ? launch_few<DT, W, 1, 1, 4, 2>(a, st) : launch_few<DT, W, 1, 2, 8, 2>(a, st);
+  } else {
+    if (wgs <= 256 || (W == W_Q4 && rows <= 8 && units >= 32)) return launch_few<DT, W, 1, 1, 8, 4>(a, st);
+    if (units >= 32) return wgs <= 512 ? launch_few<DT, W, 1, 2, 8, 4>(a, st) : launch_few<DT, W, 1, 4, 8, 4>(a, st);
+    if constexpr (W == W_Q4) return launch_few<DT, W, 1, 2, 4, 4>(a, st);
+    else return rows > 8 ? launch_few<DT, W, 1, 4, 4, 2>(a, st) : launch_few<DT, W, 1, 2, 4, 2>(a, st);
   }
 }
 template <int W>

@@ -46,11 +46,14 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few(LinArgs a) {
   constexpr int AC = MF * CF <= 2 ? 2 : 1;                   // accumulators in turn: the MFMAs of a fragment depend on each other
   __shared__ __attribute__((aligned(16))) float red[NW * ROWS * PITCH];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, wave = wave_index();
-  const uint32_t gn = (uint32_t)((a.N + COLS - 1) / COLS);
-  const int64_t n0 = (int64_t)(blockIdx.x % gn) * COLS;
+  // Row tiles first, and each XCD a contiguous part: the row tiles of a group read
+  // the same columns of its weight out of one L2.
+  const uint32_t gn = (uint32_t)((a.N + COLS - 1) / COLS), u = (uint32_t)xcd_unit(blockIdx.x, gridDim.x);
+  const uint32_t tiles = gridDim.x / gn;
+  const int64_t n0 = (int64_t)(u / tiles) * COLS;
   int group;
   int64_t r0, r1;
-  if (!lin_tile<ROWS>(a, blockIdx.x / gn, group, r0, r1)) return;
+  if (!lin_tile<ROWS>(a, u % tiles, group, r0, r1)) return;
   const bool some = group < a.experts;
   v4f32 acc[AC][MF][CF] = {};
   if (some) {
