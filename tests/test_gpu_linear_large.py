@@ -62,7 +62,7 @@ def _check(got, a, b):
 # tiles: 64, 128 and 256 rows, whole rounds of 256 tiles and a rest, contractions split over workgroups
 MX_SHAPES = [(1, 4112, 4128), (3, 8208, 4128), (9, 4112, 4160), (12, 8208, 4256), (16, 4112, 1056), (50, 8200, 512),
              (60, 16400, 544), (150, 2064, 4128), (257, 4112, 2080), (520, 1040, 8224), (1030, 2064, 1056),
-             (2050, 2320, 544), (4100, 4352, 1056), (4090, 4112, 288)]
+             (2050, 2320, 544), (4100, 4352, 1056), (4090, 4112, 288), (4100, 4112, 4128)]
 
 
 @pytest.mark.parametrize("shape", MX_SHAPES, ids=str)
@@ -113,7 +113,8 @@ def test_grouped_mx(case, swizzled):
 
 
 DENSE = [(s, n, k + d) for (s, n, k), d in zip(GROUPS, (0, 8, 0, 7, 0, 1, 4))] + \
-    [([0, 4000], 130, 264), ([1], 4112, 4128), ([16], 2048, 4096), ([7000], 96, 64), ([64] * 130, 64, 256)]
+    [([0, 4000], 130, 264), ([1], 4112, 4128), ([16], 2048, 4096), ([7000], 96, 64), ([64] * 130, 64, 256), ([40], 16400, 520),
+     ([1000, 0, 5100, 2100], 2040, 2024)]
 
 
 @pytest.mark.parametrize("case", DENSE, ids=[f"{'-'.join(map(str, s[:4]))}:{n}x{k}" for s, n, k in DENSE])
