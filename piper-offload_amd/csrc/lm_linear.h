@@ -177,10 +177,11 @@ DEV int lin_count(const LinArgs& a, int BM) {
   lin_find(a, BM, -1, g, r0, r1, pad);
   return g;
 }
-// at most this many tiles: every group may end in a part of one
+// at most this many tiles: of all groups with rows (the rows of none are one more
+// group, but there are no more groups than rows) but one may end in a part of one
 template <int BM>
 static inline int64_t lin_tiles(int64_t T, int experts, bool grouped) {
-  return (T + BM - 1) / BM + (grouped ? experts : 0);
+  return (T + BM - 1) / BM + (!grouped || T < 1 ? 0 : experts < T - 1 ? experts : T - 1);
 }
 
 // The e8m0 scale of a block whose largest magnitude has these bits, and its

@@ -155,12 +155,15 @@ static bool lin_few(int64_t T, int64_t N, int64_t K, int64_t E, bool mx, bool qu
   const int64_t rows = (T + E - 1) / E;
   const double volume = (double)T * (double)N * (double)K;
   if (K < 512 && T > 64) return false;  // too few units for the waves: [4096, 16] of 24 groups at 2048 rows 39 / 13
+  // (k_lin_mm<SHORT>: [14336, 64] of 16 groups at 16 rows 16.5 / 5.5; [4096, 16] at one row 3.3 / 3.8)
+  if (!mx && K <= 64 && T > 1) return false;
   if (!mx) return T <= 16 || volume <= 5e8;
   return rows <= 16 || volume <= 1.1e9 || (quant && T <= 64);
 }
 
 struct LinPlan {
   bool few;                       // k_lin_few, else k_lin_mm
+  bool brief;                     // k_lin_mm<SHORT>
   int tile, splits;               // of k_lin_mm
   bool rounds;                    // 256 x 256 tiles in whole rounds, the rest in smaller ones
   bool copy_a, copy_b, copy_w;    // rows realigned in the workspace first
@@ -279,7 +282,11 @@ static LinPlan lin_plan(int op, int64_t T, int64_t lda, int64_t ldb, int64_t N, 
     p.wsc = take((size_t)(E * ((N + 63) / 64) * nk) * 256);
   }
   p.splits = 1;
-  if (!p.few) {
+  // Contractions of at most two stages, the ranks of adapters: a write of the
+  // output.  [16, 4096] of 24 groups at 2048 rows 14.8 -> 9.9 us (input gradient,
+  // 1.7 TB/s), [16, 14336] of 8 groups at 4096 rows 53.5 -> 28.8 (4.1 TB/s).
+  p.brief = !p.few && !mx && op != LIN_WEIGHT_GRAD && p.len <= 64;
+  if (!p.few && !p.brief) {
     const int64_t I = op == LIN_WEIGHT_GRAD ? N : T, J = op == LIN_FORWARD ? N : K;
     lin_tiling(p, op, I, J, op == LIN_WEIGHT_GRAD ? rows : p.len, E, quant);
     if (p.splits > 1) p.part = take((size_t)p.splits * (op == LIN_WEIGHT_GRAD ? E * N : T) * J * 4);
@@ -298,7 +305,7 @@ static int launch_align(const void* src, int64_t lds, int64_t rows, int64_t cols
   return LM_OK;
 }
 
-template <int DT, int OP, int W, int BM, int BN, int WM, int WN>
+template <int DT, int OP, int W, int BM, int BN, int WM, int WN, bool SHORT = false>
 static int launch_mm(const LinArgs& a, const LinPlan& p, hipStream_t st) {
   TimedLaunch timed("linear", st);
   const int64_t J = OP == LIN_FORWARD ? a.N : a.K, gj = (J + BN - 1) / BN;
@@ -307,7 +314,7 @@ static int launch_mm(const LinArgs& a, const LinPlan& p, hipStream_t st) {
   // (the rest of whole rounds: at most 128 tiles, four workgroups each)
   const int64_t n0 = BM == 128 && a.rounds ? 512 : gi * gj;
   const dim3 grid((unsigned)n0, OP == LIN_WEIGHT_GRAD ? a.experts : p.splits, OP == LIN_WEIGHT_GRAD ? p.splits : 1);
-  hipLaunchKernelGGL((k_lin_mm<DT, OP, W, BM, BN, WM, WN>), grid, dim3(WM * WN * 64), 0, st, a);
+  hipLaunchKernelGGL((k_lin_mm<DT, OP, W, BM, BN, WM, WN, SHORT>), grid, dim3(WM * WN * 64), 0, st, a);
   LAUNCH_CHECK();
   if (p.splits > 1) {
     const int64_t n = (OP == LIN_WEIGHT_GRAD ? a.experts * a.N : a.T) * J, blocks = (n + 1023) / 1024;
@@ -325,6 +332,9 @@ static int run_mm_dt(const LinArgs& a, const LinPlan& p, hipStream_t st) {
     b.rounds = p.rounds;
     const int rc = launch_mm<DT, OP, W, 256, 256, 2, 4>(b, p, st);
     return rc || !p.rounds ? rc : launch_mm<DT, OP, W, 128, 128, 2, 2>(b, p, st);
+  }
+  if constexpr (W == W_DENSE && OP != LIN_WEIGHT_GRAD) {
+    if (p.brief) return launch_mm<DT, OP, W, 64, 128, 1, 4, true>(a, p, st);
   }
   if (p.tile == 64) return launch_mm<DT, OP, W, 64, 128, 1, 4>(a, p, st);
   return launch_mm<DT, OP, W, 128, 128, 2, 2>(a, p, st);
@@ -367,7 +377,8 @@ static int run_few_dt(const LinArgs& a, hipStream_t st) {
   const int64_t wgs = lin_tiles<16>(a.T, a.experts, a.experts > 1) * ((a.N + 15) / 16);
   if (rows > 32 && wgs > 2048) return launch_few<DT, W, 4, 4, 8, 1>(a, st);
   if constexpr (W == W_DENSE) {
-    if (wgs <= 256) return launch_few<DT, W, 1, 1, 16, 2>(a, st);
+    // (16 waves with nothing to do for most of them: [4096, 16] 4.9, 4 waves 3.3)
+    if (wgs <= 256 && units > 8) return launch_few<DT, W, 1, 1, 16, 2>(a, st);
     return units < 32 ? launch_few<DT, W, 1, 1, 4, 2>(a, st) : launch_few<DT, W, 1, 2, 8, 2>(a, st);
   } else {
     if (wgs <= 256 || (W == W_Q4 && rows <= 8 && units >= 32)) return launch_few<DT, W, 1, 1, 8, 4>(a, st);

@@ -189,15 +189,18 @@ DEV uint32_t mm_hide(uint32_t x) {
   return x;
 }
 
-template <int DT, int OP, int W, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
+// SHORT: a contraction of at most two stages (a LoRA's rank).  All of it is loaded
+// at once, so two buffers do and twice as many workgroups fit on a CU: such a
+// product is a write of its output, and a workgroup mostly waits.
+template <int DT, int OP, int W, int BM, int BN, int WM, int WN, bool SHORT = false>
+__global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a) {
   using P = MmTraits<DT, OP, W, BM, BN, WM, WN>;
   constexpr bool HALF = DT == F16, Q4 = P::Q4, PP = P::NW == 8;
   constexpr int CS = P::CS, FI = P::FI, FJ = P::FJ, IK = P::IK, JK = P::JK;
   // (separate arrays: the compiler then knows that a read of one stage need not
   // wait for the loads of another)
-  __shared__ __attribute__((aligned(1024))) uint8_t si0[P::IB], si1[P::IB], si2[P::IB], si3[P::IB];
-  __shared__ __attribute__((aligned(1024))) uint8_t sj0[P::JB], sj1[P::JB], sj2[JK == KC4 ? 16 : P::JB], sj3[JK == KC4 ? 16 : P::JB];
+  __shared__ __attribute__((aligned(1024))) uint8_t si0[P::IB], si1[P::IB], si2[SHORT ? 16 : P::IB], si3[SHORT ? 16 : P::IB];
+  __shared__ __attribute__((aligned(1024))) uint8_t sj0[P::JB], sj1[P::JB], sj2[JK == KC4 || SHORT ? 16 : P::JB], sj3[JK == KC4 || SHORT ? 16 : P::JB];
   __shared__ __attribute__((aligned(1024))) uint8_t ss0[P::SB], ss1[P::SB], ss2[P::SB], ss3[P::SB];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
   const int wave = wave_index();
@@ -445,63 +448,77 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_lin_mm(LinArgs a) {
     // loads of a stage per wave
     constexpr int L = P::IL + (JK == KC4 ? 0 : P::JL) + (Q4 ? 1 : 0);
 
-    load_scales(kb);
-    // KC4: the first four stages' codes; the loop asks for the next four in the
-    // first two of every four stages
-#pragma unroll
-    for (int b = 0; b < 3; ++b) load(kb + b, kb, b < 2 ? b : -1, ti[b], JK == KC4 ? tj[0] : tj[b], ts[b]);
-    if constexpr (JK == KS4) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        load_codes(kb + b, 0);
-        store_codes(tj[b], 0);
-      }
-      load_codes(kb + 2, 0);
-    }
-    lin_wait<JK == KS4 ? 0 : 2 * L>();  // stage kb is in LDS
-    lin_barrier();
-    if (PP && wave >= 4) lin_barrier();  // the second half runs one barrier behind
-    auto four = [&](int st, auto half) {  // stages st .. st + 3; KC4: their codes are in buffer `half`
-      constexpr int H = decltype(half)::value;
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int n = (b + 3) & 3;  // the buffer of stage st + b + 3
-        if (b == 0) next_scales(st);
-        read(b, ti[b], JK == KC4 ? tj[H] : tj[b], ts[b]);
-        __builtin_amdgcn_sched_barrier(0);
-        // (while the reads are on their way)  Buffer n was read for stage
-        // st + b - 1, and all waves are past that.
-        if (b == 0) load_scales(st + 4);
-        load_codes(st + b + 3, (b + 1) & 1);
-        load(st + b + 3, st + 4, b < 2 ? b : -1, ti[n], JK == KC4 ? tj[1 - H] : tj[n], ts[n]);
-        decode(b);
-        // Stage st + b + 1 is in LDS, and this one in registers: what may be left
-        // are the loads of stages st + b + 2 and st + b + 3, with KC4 the scales and
-        // codes that were asked for since.
-        if constexpr (JK == KC4) {
-          if (b == 0) lin_wait<2 * L + FJ + 1>();
-          else if (b == 1) lin_wait<2 * L + FJ + 2>();
-          else if (b == 2) lin_wait<2 * L + 1>();
-          else lin_wait<2 * L>();
-        } else {
-          lin_wait<2 * L>();
-        }
-        lin_barrier();
+    if constexpr (SHORT) {
+      static_assert(W == W_DENSE && !PP, "short contractions: dense weights");
+      load(0, 0, -1, ti[0], tj[0], ts[0]);
+      if (nk > 1) load(1, 0, -1, ti[1], tj[1], ts[1]);
+      lin_wait<0>();
+      lin_barrier();
+      read(0, ti[0], tj[0], ts[0]);
+      multiply();
+      if (nk > 1) {
+        read(1, ti[1], tj[1], ts[1]);
         multiply();
-        store_codes(tj[(b + 2) & 3], b & 1);
-        if constexpr (PP) lin_barrier();
       }
-    };
-    for (int st = kb; st < ke; st += JK == KC4 ? 8 : 4) {
-      four(st, std::integral_constant<int, 0>{});
-      if constexpr (JK == KC4) {
-        if (st + 4 < ke) four(st + 4, std::integral_constant<int, 1>{});
+    } else {
+      load_scales(kb);
+      // KC4: the first four stages' codes; the loop asks for the next four in the
+      // first two of every four stages
+#pragma unroll
+      for (int b = 0; b < 3; ++b) load(kb + b, kb, b < 2 ? b : -1, ti[b], JK == KC4 ? tj[0] : tj[b], ts[b]);
+      if constexpr (JK == KS4) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          load_codes(kb + b, 0);
+          store_codes(tj[b], 0);
+        }
+        load_codes(kb + 2, 0);
       }
+      lin_wait<JK == KS4 ? 0 : 2 * L>();  // stage kb is in LDS
+      lin_barrier();
+      if (PP && wave >= 4) lin_barrier();  // the second half runs one barrier behind
+      auto four = [&](int st, auto half) {  // stages st .. st + 3; KC4: their codes are in buffer `half`
+        constexpr int H = decltype(half)::value;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int n = (b + 3) & 3;  // the buffer of stage st + b + 3
+          if (b == 0) next_scales(st);
+          read(b, ti[b], JK == KC4 ? tj[H] : tj[b], ts[b]);
+          __builtin_amdgcn_sched_barrier(0);
+          // (while the reads are on their way)  Buffer n was read for stage
+          // st + b - 1, and all waves are past that.
+          if (b == 0) load_scales(st + 4);
+          load_codes(st + b + 3, (b + 1) & 1);
+          load(st + b + 3, st + 4, b < 2 ? b : -1, ti[n], JK == KC4 ? tj[1 - H] : tj[n], ts[n]);
+          decode(b);
+          // Stage st + b + 1 is in LDS, and this one in registers: what may be left
+          // are the loads of stages st + b + 2 and st + b + 3, with KC4 the scales and
+          // codes that were asked for since.
+          if constexpr (JK == KC4) {
+            if (b == 0) lin_wait<2 * L + FJ + 1>();
+            else if (b == 1) lin_wait<2 * L + FJ + 2>();
+            else if (b == 2) lin_wait<2 * L + 1>();
+            else lin_wait<2 * L>();
+          } else {
+            lin_wait<2 * L>();
+          }
+          lin_barrier();
+          multiply();
+          store_codes(tj[(b + 2) & 3], b & 1);
+          if constexpr (PP) lin_barrier();
+        }
+      };
+      for (int st = kb; st < ke; st += JK == KC4 ? 8 : 4) {
+        four(st, std::integral_constant<int, 0>{});
+        if constexpr (JK == KC4) {
+          if (st + 4 < ke) four(st + 4, std::integral_constant<int, 1>{});
+        }
+      }
+      if constexpr (PP) {
+        if (wave < 4) lin_barrier();
+      }
+      lin_wait<0>();  // no load may reach LDS after the workgroup
     }
-    if constexpr (PP) {
-      if (wave < 4) lin_barrier();
-    }
-    lin_wait<0>();  // no load may reach LDS after the workgroup
   }
 
   const int64_t rows0 = OP == LIN_WEIGHT_GRAD ? t.group * a.N : 0;  // of the output above this group's
