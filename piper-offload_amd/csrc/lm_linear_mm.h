@@ -544,42 +544,48 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
     return;
   }
   uint16_t* out = (uint16_t*)a.out + rows0 * jend;
+  auto column = [&](int y) { return t.j0 + wj * (FJ * 16) + (y + (g & 1)) * 16 + 8 * (g >> 1); };
+  float bias[FJ / 2][8] = {};
+  if (OP == LIN_FORWARD && a.bias && t.group < a.experts) {
 #pragma unroll
-  for (int y = 0; y < FJ; y += 2) {
-    const int64_t j = t.j0 + wj * (FJ * 16) + (y + (g & 1)) * 16 + 8 * (g >> 1);
-    float bias[8] = {};
-    if (OP == LIN_FORWARD && a.bias && t.group < a.experts) {
+    for (int y = 0; y < FJ; y += 2) {
+      const int64_t j = column(y);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        bias[e] = val_dt<DT>(((const LM_GLOBAL uint16_t*)a.bias)[j + e < jend ? j + e : jend - 1]);
+        bias[y / 2][e] = val_dt<DT>(((const LM_GLOBAL uint16_t*)a.bias)[j + e < jend ? j + e : jend - 1]);
     }
+  }
+  // A row's columns one store after the other: the halves of a 128-byte line reach
+  // the L2 together, which otherwise writes many of them to memory by themselves
+  // (dense weight gradient, 134 MB: 165 -> 137 MB written, 2% fewer cycles).  KS4 has no
+  // register left for this order and takes a column's rows.
 #pragma unroll
-    for (int x = 0; x < FI; ++x) {
-      const int64_t i = t.r0 + wi * (FI * 16) + x * 16 + (lane & 15);
-      // lane groups 0, 2 keep fragment y and get columns 4 .. 7 (12 .. 15) of it
-      // from groups 1, 3, which get columns 0 .. 3 (8 .. 11) of fragment y + 1
-      float v[8];
+  for (int n = 0; n < FI * FJ / 2; ++n) {
+    const int x = JK == KS4 ? n % FI : n / (FJ / 2), y = 2 * (JK == KS4 ? n / FI : n % (FJ / 2));
+    const int64_t i = t.r0 + wi * (FI * 16) + x * 16 + (lane & 15), j = column(y);
+    // lane groups 0, 2 keep fragment y and get columns 4 .. 7 (12 .. 15) of it
+    // from groups 1, 3, which get columns 0 .. 3 (8 .. 11) of fragment y + 1
+    float v[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const auto r = __builtin_amdgcn_permlane16_swap(f2u(acc[x][y][e]), f2u(acc[x][y + 1][e]), false, false);
-        v[e] = u2f(r[0]);
-        v[4 + e] = u2f(r[1]);
-      }
-      lm_u32x4 w;
+    for (int e = 0; e < 4; ++e) {
+      const auto r = __builtin_amdgcn_permlane16_swap(f2u(acc[x][y][e]), f2u(acc[x][y + 1][e]), false, false);
+      v[e] = u2f(r[0]);
+      v[4 + e] = u2f(r[1]);
+    }
+    lm_u32x4 w;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float lo = v[2 * e] + bias[2 * e], hi = v[2 * e + 1] + bias[2 * e + 1];
-        w[e] = DT == F16 ? (uint32_t)f16_bits(lo) | (uint32_t)f16_bits(hi) << 16 : pack_bf16x2(lo, hi);
-      }
-      uint16_t* p = out + i * jend + j;
-      if (i < t.r1) {
-        if (j + 8 <= jend) {
-          *(LM_GLOBAL lm_u32x4_any*)p = w;
-        } else {
+    for (int e = 0; e < 4; ++e) {
+      const float lo = v[2 * e] + bias[y / 2][2 * e], hi = v[2 * e + 1] + bias[y / 2][2 * e + 1];
+      w[e] = DT == F16 ? (uint32_t)f16_bits(lo) | (uint32_t)f16_bits(hi) << 16 : pack_bf16x2(lo, hi);
+    }
+    uint16_t* p = out + i * jend + j;
+    if (i < t.r1) {
+      if (j + 8 <= jend) {
+        *(LM_GLOBAL lm_u32x4_any*)p = w;
+      } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (j + e < jend) ((LM_GLOBAL uint16_t*)p)[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-        }
+        for (int e = 0; e < 8; ++e)
+          if (j + e < jend) ((LM_GLOBAL uint16_t*)p)[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
       }
     }
   }
