@@ -21,6 +21,9 @@
  *                      P/_torchao_mx.py:143-207) as single fused kernels
  *   lm_*_merge_stack <- the per-target loop of merge_lora()
  *                      (P/merge.py:121-125) as one grouped launch
+ *   lm_linear, lm_linear_*_grad <- (no reference counterpart: products with
+ *                      the merged MXFP4 weights, and with one weight per
+ *                      group of rows)
  *
  * Conventions
  *  - All pointers are device pointers unless noted; tensors are row-major
@@ -334,7 +337,8 @@ int lm_nvfp4_merge_stack(const lm_stack_item* items, int32_t count, int32_t swiz
  * No reference counterpart.  When enabled, every entry point brackets its
  * main kernel launches with hipEvents on the caller's stream, keyed by kernel
  * family ("rows", "rows_stack", "blocks_full", "blocks_amax",
- * "blocks_quant", "todense", "prep", "nvfp4", "mx", "q8", "gguf").  lm_timer_read synchronizes the
+ * "blocks_quant", "todense", "prep", "nvfp4", "mx", "q8", "gguf", "linear",
+ * "linear_few", "linear_prep").  lm_timer_read synchronizes the
  * recorded events and returns the summed milliseconds and launch count of one
  * family.  Enabling (or re-enabling) clears the record. */
 int lm_timer_enable(int32_t enable);
