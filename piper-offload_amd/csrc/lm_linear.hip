@@ -7,6 +7,8 @@
 //
 // Sums are kept in fp32 by the matrix instructions and rounded once, on the
 // store.  An MXFP4 value is e2m1 * 2^(scale - 127); in bf16 it is exact.
+#include <algorithm>
+
 #include "lm_impl.h"
 #include "lm_linear.h"
 #include "lm_linear_few.h"
@@ -173,58 +175,65 @@ struct LinPlan {
 };
 static int64_t round8(int64_t x) { return (x + 7) & ~(int64_t)7; }
 
-// Tile and splits of k_lin_mm: the least of a model of its time.  What a CU takes
-// for the tiles that it works on in turn, us per stage and per tile (measured,
-// bf16, [4096, 4096] at 256 to 4096 rows, and weight gradients of few stages; a
-// stage of 4-bit inputs, four times as deep, takes 1.65 times as long): 256 x 256
-// 0.70 and 8 (its store is not covered by another workgroup's work), 0.50 a
-// stage where less than half of the CUs have one; 128 x 128 two at a time in 0.55
-// and 2.5, one in 0.28 and 2; 64 x 128 three in 0.58 and 2, two in 0.40 and 1.5, one
-// in 0.21 and 1.  Groups end in a part of a tile, half of one on average.  A split
-// contraction writes and reads its sums in fp32 (4.5 TB/s) and has one launch more;
-// its parts have 8 stages and more.  Groups' weights are read again for every
-// row tile, from memory where they are large: forward, the 256 rows of a tile
-// count for 0.7 (32 groups [2816, 2048] at 8192 rows 98 us, 128 x 128 124; dense
-// 126, 156; 16 groups [4096, 2048] at 2048 rows 48, 57).  [4096, 4096], us: 512 rows
-// 64 x 128 29, 128 x 128 whole 36, in four parts 35, 256 x 256 68; 4096 rows 103 on
-// 256 x 256, 145 on 128 x 128.
-// Whole rounds and the rest apart (lin_rounds) where the rest's share of a round
-// is more than the second launch, 5 us: always known for one weight, likely for
-// groups with 48 stages and more (8 groups [4096, 2048] at 4096 rows 119 -> 97 us).
-static void lin_tiling(LinPlan& p, int op, int64_t I, int64_t J, int64_t len, int64_t E, bool quant) {
+// Tile and splits of k_lin_mm: the least of a model of its time.  A CU works on
+// its tiles in turn; LinCost has the microseconds per stage, measured at 300 to
+// 4096 rows of [4096, 4096], [14336, 4096] and [4096, 14336] and of 4 to 32 groups:
+// 256 x 256 tiles alone, where less than half of the CUs have one, 128 x 128 two at
+// a time and one, 64 x 128 three, two and one.  A stage of 4-bit inputs, four times
+// as deep, takes 1.65 times as long as a dense one.  Per tile there are 8, 2.5 / 2
+// and 2 / 1.5 / 1 us besides (the store of a 256 x 256 tile is not covered by
+// another workgroup's work).  A split contraction writes and reads its sums in fp32
+// (4.5 TB/s) and has one launch more; its parts have 8 stages and more.  Groups end
+// in a part of a tile, 0.4 of one on average, and one in ten has no rows.
+// Whole rounds and the rest apart (lin_rounds): the rest in 128 x 128 tiles after a
+// second launch, 5 us, which groups with fewer than 48 stages do not wait for.
+// Measured, us at 256 x 256 / 128 x 128 / 64 x 128: MXFP4 [14336, 4096] at 300 rows
+// 81 / 68 / 56, [4096, 4096] at 2048 rows 90 / 78 / 83 (input gradient 96 / 77 / 103),
+// 4 groups [4096, 4096] at 1024 rows 83 / 76 / 63, 32 groups [2816, 2048] at 2048 rows
+// 73 / 57 / 46, at 8192 114 / 137 / 134; dense, 8 groups [4096, 2048] at 4096 rows in
+// rounds 84, whole 99 / 103 / 128.
+struct LinCost {
+  double full, alone, pair, one, three, two, single;
+};
+static void lin_tiling(LinPlan& p, int op, int64_t I, int64_t J, int64_t len, int64_t E, bool mx, bool quant) {
+  static const LinCost dense{0.70, 0.50, 0.55, 0.28, 0.58, 0.40, 0.21}, forward{0.72, 0.64, 0.60, 0.38, 0.48, 0.36, 0.26},
+      input_grad{0.72, 0.69, 0.60, 0.39, 0.60, 0.42, 0.32};
+  const LinCost& k = !mx || quant ? dense : op == LIN_FORWARD ? forward : input_grad;
   const int64_t nk = (len + (quant ? 127 : 31)) / (quant ? 128 : 32);
   const double stage = quant ? 1.65 : 1.0;
   const bool wgrad = op == LIN_WEIGHT_GRAD;
+  auto pairs = [&](int64_t n, double stages) {  // n 128 x 128 tiles on a CU
+    return ((double)(n / 2) * k.pair + (double)(n % 2) * k.one) * stages + (double)(n / 2) * 2.5 + (double)(n % 2) * 2.0;
+  };
   double best = 1e30;
   for (int tile = 256; tile >= 64; tile /= 2) {
-    const int64_t bn = tile == 256 ? 256 : 128;
-    const int64_t gi = wgrad ? (I + tile - 1) / tile * E : (E > 1 ? I / tile + (E < I ? E : I) / 2 + 1 : (I + tile - 1) / tile);
-    const int64_t tiles = gi * ((J + bn - 1) / bn);
+    const int64_t bn = tile == 256 ? 256 : 128, gj = (J + bn - 1) / bn, groups = E < I ? E : I;
+    int64_t gi = (I + tile - 1) / tile;
+    if (wgrad) gi *= E;
+    else if (E > 1) gi = std::max((groups * 9 + 9) / 10, (I * 10 + groups * tile * 4 + tile * 10 - 1) / (tile * 10));
+    const int64_t tiles = gi * gj;
     int64_t most = tiles < 256 ? nk / 8 : 1;
     if (most > 16) most = 16;
     for (int64_t s = 1; s == 1 || s <= most; ++s) {
       const int64_t per = s == 1 ? nk : ((nk + s - 1) / s + 3) & ~(int64_t)3, n = (tiles * s + 255) / 256;  // tiles a CU
-      double c, fixed;
+      const double stages = stage * (double)per;
+      double t;
       bool rounds = false;
       if (tile == 256) {
+        t = (double)n * (k.full * stages + 8.0);
+        if (tiles * s <= 128) t = k.alone * stages + 8.0;
         const int64_t rest = tiles % 256;
-        c = tiles * s <= 128 ? 0.50 : 0.70 * (double)n;
-        fixed = 8.0 * (double)n;
-        rounds = s == 1 && !wgrad && tiles >= 256 && (E > 1 ? (double)nk * stage >= 48.0 : rest > 0 && rest <= 64);
-        if (rounds) c -= E > 1 ? 0.15 : 0.42;
-        if (E > 1 && op == LIN_FORWARD) {
-          c *= 0.7;
-          fixed *= 0.7;
+        if (s == 1 && !wgrad && tiles >= 256 && (E > 1 ? (double)nk * stage >= 48.0 && rest <= 128 : rest > 0 && rest <= 64)) {
+          const double apart = (double)(tiles / 256) * (k.full * stages + 8.0) + 5.0 + pairs((4 * rest + 255) / 256, stages);
+          rounds = apart < t;
+          if (rounds) t = apart;
         }
       } else if (tile == 128) {
-        c = (double)(n / 2) * 0.55 + (double)(n % 2) * 0.28;
-        fixed = (double)(n / 2) * 2.5 + (double)(n % 2) * 2.0;
+        t = pairs(n, stages);
       } else {
-        const double c64[3] = {0.0, 0.21, 0.40}, f64[3] = {0.0, 1.0, 1.5};
-        c = (double)(n / 3) * 0.58 + c64[n % 3];
-        fixed = (double)(n / 3) * 2.0 + f64[n % 3];
+        const double c64[3] = {0.0, k.single, k.two}, f64[3] = {0.0, 1.0, 1.5};
+        t = ((double)(n / 3) * k.three + c64[n % 3]) * stages + (double)(n / 3) * 2.0 + f64[n % 3];
       }
-      double t = c * stage * (double)per + fixed;
       if (s > 1) t += 4.0 + (double)(s * I * (wgrad ? E : 1) * J) * 8.0 / 4.5e6;
       if (t < best) {
         best = t;
@@ -288,7 +297,7 @@ static LinPlan lin_plan(int op, int64_t T, int64_t lda, int64_t ldb, int64_t N, 
   p.brief = !p.few && !mx && op != LIN_WEIGHT_GRAD && p.len <= 64;
   if (!p.few && !p.brief) {
     const int64_t I = op == LIN_WEIGHT_GRAD ? N : T, J = op == LIN_FORWARD ? N : K;
-    lin_tiling(p, op, I, J, op == LIN_WEIGHT_GRAD ? rows : p.len, E, quant);
+    lin_tiling(p, op, I, J, op == LIN_WEIGHT_GRAD ? rows : p.len, E, mx, quant);
     if (p.splits > 1) p.part = take((size_t)p.splits * (op == LIN_WEIGHT_GRAD ? E * N : T) * J * 4);
   }
   p.total = at;
