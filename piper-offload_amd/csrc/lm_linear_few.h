@@ -7,6 +7,9 @@
 // the contraction, 128 a unit, and add their sums up through LDS in a fixed
 // order.  With 16 columns a workgroup even a 1024-row weight spreads over 64 CUs;
 // every wave has UN units of loads in flight at once.
+// MXFP4 [14336, 4096] at one row: 10.0 us, 3.1 TB/s of codes and scales with the
+// launch's ends (5.0 us for [1024, 4096], which is latency alone); 64 groups
+// [2048, 1408] at 100 rows with 4-bit inputs 18 us, 4.1 TB/s.
 //
 // Both operands are read in whole runs of a row: access j of a unit gives lane
 // group g (lane >> 4) 16 bytes, chunk 4j + g of 8 values, and that is what MFMA
