@@ -275,8 +275,8 @@ int lm_routed_residual(const void* x, const void* y, void* out, int64_t T, int64
  * weight rounded to fp16, bf16 rows see it exactly.  Otherwise a dense weight
  * [experts, N, K] of `dtype`.
  * `ends`: device int32[experts]; group e's rows are [ends[e-1], ends[e]).  Rows
- * past ends[experts-1] get zeros.  NULL with one expert: all T rows.  Ends
- * that fall or pass T are clamped.
+ * past ends[experts-1] get zeros, without the bias.  NULL with one expert: all
+ * T rows.  Ends that fall or pass T are clamped.
  * input_dtype: `dtype`, or LM_E2M1 (MXFP4 weights): x is quantised to MXFP4
  * first, as lm_mx_requant with LM_MX_FLOOR does; a block with an infinity or a
  * NaN makes its row NaN.  The input gradient passes straight through that

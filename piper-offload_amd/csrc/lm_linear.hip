@@ -329,8 +329,7 @@ static int launch_mm(const LinArgs& a, const LinPlan& p, hipStream_t st) {
   if (p.splits > 1) {
     const int64_t n = (OP == LIN_WEIGHT_GRAD ? a.experts * a.N : a.T) * J, blocks = (n + 1023) / 1024;
     if (blocks > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
-    hipLaunchKernelGGL((k_lin_join<DT>), dim3((unsigned)blocks), dim3(256), 0, st, a.part, p.splits, n, J, (const uint16_t*)a.bias,
-                       (uint16_t*)a.out);
+    hipLaunchKernelGGL((k_lin_join<DT>), dim3((unsigned)blocks), dim3(256), 0, st, a, p.splits, n, J);
     LAUNCH_CHECK();
   }
   return LM_OK;

@@ -596,17 +596,23 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
   }
 }
 
-// The sum of the parts of a split contraction, in their order, rounded.  Bound by
+// The sum of the parts of a split contraction, in their order, rounded.  Rows of no
+// group have no bias (`ends` is read only where there is one).  Bound by
 // memory: two parts of [2048, 4096], 84 MB moved, 14 us (6 TB/s, much of it from the
 // last-level cache).
 template <int DT>
-__global__ __launch_bounds__(256) void k_lin_join(const float* part, int splits, int64_t n, int64_t J, const uint16_t* bias,
-                                                  uint16_t* out) {
+__global__ __launch_bounds__(256) void k_lin_join(LinArgs a, int splits, int64_t n, int64_t J) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  int64_t biased = n;  // of the sums, those before this one
+  if (a.bias && a.ends) {
+    int64_t b, e;
+    lin_group(a, a.experts - 1, b, e);
+    biased = e * J;
+  }
   if (i >= n) return;
   float s[4] = {};
   for (int k = 0; k < splits; ++k) {
-    const LM_GLOBAL float* p = (const LM_GLOBAL float*)part + k * n + i;
+    const LM_GLOBAL float* p = (const LM_GLOBAL float*)a.part + k * n + i;
     if (i + 4 <= n) {
       const v4f32 v = __builtin_bit_cast(v4f32, *(const LM_GLOBAL lm_u32x4_any*)p);
 #pragma unroll
@@ -620,8 +626,8 @@ __global__ __launch_bounds__(256) void k_lin_join(const float* part, int splits,
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (i + e < n) {
-      if (bias) s[e] += val_dt<DT>(((const LM_GLOBAL uint16_t*)bias)[(i + e) % J]);
-      ((LM_GLOBAL uint16_t*)out)[i + e] = bits_dt<DT>(s[e]);
+      if (a.bias && i + e < biased) s[e] += val_dt<DT>(((const LM_GLOBAL uint16_t*)a.bias)[(i + e) % J]);
+      ((LM_GLOBAL uint16_t*)a.out)[i + e] = bits_dt<DT>(s[e]);
     }
 }
 

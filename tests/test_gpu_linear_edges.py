@@ -1,0 +1,107 @@
+"""Products with MXFP4 weights and grouped products where a tile, a group or the stored scales end, against sums in 64 bits.
+
+Tolerance of one output: half a unit in the last place of its type (up to 2^-8 of it in bfloat16, 2^-11 in float16) and, for
+an fp32 sum of n products in any order, at most n + 2 roundings of 2^-23 of the sum of magnitudes.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from piper_offload_amd import _lib as L
+
+pytestmark = pytest.mark.gpu
+
+K = pytest.importorskip("piper_offload_amd.kernels")
+
+DEV = "cuda"
+FP4 = getattr(torch, "float4_e2m1fn_x2", None)
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def _normal(seed, *shape, std=1.0, dtype=BF16):
+    return (torch.randn(*shape, generator=torch.Generator(DEV).manual_seed(seed), device=DEV) * std).to(dtype)
+
+
+def _scale_places(n, blocks):
+    """Byte of (row, block) in swizzled scales."""
+    r, c = torch.arange(n, device=DEV)[:, None], torch.arange(blocks, device=DEV)[None]
+    return ((r // 128) * (-(-blocks // 4)) + c // 4) * 512 + (r % 32) * 16 + (r % 128) // 32 * 4 + c % 4
+
+
+def _decode(q, s, swizzled=False):
+    n, blocks = q.shape[0], q.shape[1] // 16
+    s = s.reshape(-1)[_scale_places(n, blocks)] if swizzled else s
+    grid = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, 0, -0.5, -1, -1.5, -2, -3, -4, -6], dtype=torch.float64, device=DEV)
+    v = grid[torch.stack((q & 15, q >> 4), -1).reshape(n, -1).int()]
+    return v * torch.pow(2.0, s.double() - 127).repeat_interleave(32, 1)
+
+
+def _weight(seed, n, k, swizzled=False):
+    q, s = K.requantize_mx(_normal(seed, n, k, std=0.02), FP4, swizzled=swizzled)
+    return q, s, _decode(q, s, swizzled)
+
+
+def _quantised(x):
+    """x on the MXFP4 grid: scale 2^(floor(log2 max) - 2), nearest (ties to even), up to 6."""
+    b = x.double().reshape(x.shape[0], -1, 32)
+    scale = torch.pow(2.0, (torch.frexp(b.abs().amax(-1, keepdim=True))[1] - 3).double())
+    v = b / scale
+    step = torch.where(v.abs() < 2, 0.5, torch.where(v.abs() < 4, 1.0, 2.0)).double()
+    return (torch.sign(v) * (torch.round(v.abs() / step) * step).clamp(max=6) * scale).reshape(x.shape)
+
+
+def _check(got, a, b, bias=None):
+    """got against a @ b + bias in 64 bits."""
+    a, b = a.double().contiguous(), b.double().contiguous()
+    want, size = a @ b, a.abs() @ b.abs()
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    half, tiny = (2.0**-8, 1e-38) if got.dtype is BF16 else (2.0**-11, 2.0**-25)
+    tol = (1 + 2.0**-8) * half * want.abs() + (a.shape[1] + 2) * 2.0**-23 * size + tiny
+    off = (got.double() - want).abs()
+    assert torch.isfinite(got).all()
+    assert (off <= tol).all(), f"{int((off > tol).sum())} of {off.numel()} off, worst {(off / tol).max():.3g} tolerances"
+
+
+def _spans(sizes):
+    end = 0
+    for e, size in enumerate(sizes):
+        yield e, end, end + size
+        end += size
+
+
+# rows of the groups, rows after the last of them, N, K; whether the sums are split over workgroups.  The last row of a group
+# times an odd N ends inside the four sums that a thread adds up.
+BIASED = [([9], 11, 64, 512, False), ([100], 29, 1000, 128, False), ([2000, 0, 7], 60, 2001, 544, False),
+          ([200], 100, 1024, 8192, True), ([199, 0, 33], 68, 1021, 8224, True), ([0], 300, 1021, 8192, True)]
+
+
+@pytest.mark.parametrize("case", BIASED, ids=[f"{'-'.join(map(str, s))}+{r}:{n}x{k}" for s, r, n, k, _ in BIASED])
+@pytest.mark.parametrize("kind", ["mxfp4", "fp4-inputs", "dense"])
+def test_bias_leaves_rows_of_no_group_zero(case, kind):
+    sizes, rest, n, k, split = case
+    t, groups = sum(sizes) + rest, len(sizes)
+    x, bias, ends = _normal(1, t, k), _normal(2, n), torch.tensor(sizes).cumsum(0).to(torch.int32).to(DEV)
+    if kind == "dense":
+        w = _normal(3, groups, n, k, std=k**-0.5)
+        scale, stored = None, list(w.double())
+    else:
+        made = [_weight(e, n, k) for e in range(groups)]
+        w, scale, stored = torch.stack([m[0] for m in made]), torch.stack([m[1] for m in made]), [m[2] for m in made]
+    weight = L.WeightStruct(w.data_ptr(), None if scale is None else scale.data_ptr(), n, k,
+                            L.LM_BF16 if kind == "dense" else L.LM_E2M1, 0, groups, 0)
+    input_id = L.LM_E2M1 if kind == "fp4-inputs" else L.LM_BF16
+    need = L.lib().lm_linear_workspace_size(0, t, k, 0, n, k, groups, weight.dtype, input_id, 1)
+    if kind == "mxfp4":
+        assert (need > 0) == split
+    space, y = L.workspace(need, x.device), torch.full((t, n), float("nan"), dtype=BF16, device=DEV)
+    L.check(L.lib().lm_linear(x.data_ptr(), k, ctypes.byref(weight), bias.data_ptr(), ends.data_ptr(), y.data_ptr(), t,
+                              L.LM_BF16, input_id, L.aligned_ptr(space), need, torch.cuda.current_stream().cuda_stream))
+    for e, b, end in _spans(sizes):
+        if end > b:
+            _check(y[b:end], _quantised(x[b:end]) if kind == "fp4-inputs" else x[b:end], stored[e].t(), bias)
+    assert not y[t - rest:].any()
