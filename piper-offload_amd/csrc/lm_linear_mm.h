@@ -351,12 +351,14 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
       if constexpr (JK == KS4) {
         const int64_t sbase = a.swizzled ? (int64_t)(st >> 2) * ((nb + 3) >> 2) * 512 + (st & 3) * 4 : (int64_t)st * CS * nb;
         const bool none = st >= ke;
-        const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)jr, 0, left32(jl, none), 0x00027000);
+        const uint32_t left = left32(jl, none);
+        const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)jr, 0, left, 0x00027000);
         jr += jstep;
         jl -= jstep;
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(sp + sbase), 0, left32(a.scale_stride - sbase, none), 0x00027000);
         code[set] = __builtin_bit_cast(lm_u32x2, __builtin_amdgcn_raw_buffer_load_b64(rc, (int)co, 0, 0));
-        code_s[set] = __builtin_amdgcn_raw_buffer_load_b8(rs, (int)(co == LIN_OUT ? LIN_OUT : cso), 0, 0);
+        // (a scale only where there are codes: past row N swizzled scales have padding, which may hold a NaN)
+        code_s[set] = __builtin_amdgcn_raw_buffer_load_b8(rs, (int)(co < left ? cso : LIN_OUT), 0, 0);
       }
     };
     auto store_codes = [&](lds_u8* tj, int set) {

@@ -105,3 +105,45 @@ def test_bias_leaves_rows_of_no_group_zero(case, kind):
         if end > b:
             _check(y[b:end], _quantised(x[b:end]) if kind == "fp4-inputs" else x[b:end], stored[e].t(), bias)
     assert not y[t - rest:].any()
+
+
+def _pad(s, n, blocks, value):
+    """Swizzled scales with `value` in every byte that belongs to no row or no block."""
+    out = torch.full_like(s, value)
+    at = _scale_places(n, blocks).reshape(-1)
+    out.view(-1)[at] = s.reshape(-1)[at]
+    return out
+
+
+# few rows, tiles of 64, 128 and 256 rows, split sums (40 and 150 rows); N a part of a run of 32 rows, K of four blocks
+PADDED = [(3, 1, 64), (40, 33, 96), (20, 100, 4128), (70, 100, 160), (150, 1100, 4128), (300, 257, 416), (300, 130, 32),
+          (1030, 2050, 1056), (2050, 2325, 544)]
+
+
+@pytest.mark.parametrize("shape", PADDED, ids=str)
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("groups", [1, 3])
+def test_padding_of_swizzled_scales_is_not_read(shape, dtype, groups):
+    """The padding may hold anything, the code of NaN too: the results are those with zeros there, bit for bit."""
+    t, n, k = shape
+    made = [_weight(e, n, k, True) for e in range(groups)]
+    q = torch.stack([m[0] for m in made])
+    zeros, nans = (torch.stack([_pad(m[1], n, k // 32, v) for m in made]) for v in (0, 255))
+    x, dy = _normal(1, t, k, dtype=dtype), _normal(2, t, n, dtype=dtype)
+    ends = torch.tensor([t // 3, t // 3, t][-groups:], dtype=torch.int32, device=DEV)
+    for quant in (None, FP4):
+        if groups == 1:
+            y = [K.mx_matmul(x, q[0], s[0], swizzled=True, activation_dtype=quant) for s in (zeros, nans)]
+        else:
+            y = [K.grouped_mx_matmul(x, q, s, ends, swizzled=True, activation_dtype=quant) for s in (zeros, nans)]
+        assert torch.equal(y[0], y[1])
+    if groups == 1:
+        dx = [K.mx_matmul_input_grad(dy, q[0], s[0], swizzled=True) for s in (zeros, nans)]
+    else:
+        dx = [K.grouped_mx_matmul_input_grad(dy, q, s, ends, swizzled=True) for s in (zeros, nans)]
+    assert torch.equal(dx[0], dx[1])
+    b = 0
+    for e, end in enumerate(ends.tolist()):
+        if end > b:
+            _check(dx[1][b:end], dy[b:end], made[e][2])
+        b = end
