@@ -272,6 +272,7 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
     uint32_t so[JK == KC4 ? FJ : 1], sv[JK == KC4 ? FJ : 1], sn[JK == KC4 ? FJ : 1];
     const int64_t stile = a.swizzled ? (t.j0 >> 7) * ((nb + 3) >> 2) * 512 : t.j0 * nb;
     const uint32_t sleft = a.scale_stride - stile > LIN_SPAN ? (uint32_t)LIN_SPAN : (uint32_t)(a.scale_stride - stile);
+    const uint32_t slast = sleft < 4 ? LIN_OUT : sleft - 4;  // the last whole word, if there is one
     if constexpr (JK == KC4) {
 #pragma unroll
       for (int f = 0; f < FJ; ++f) {
@@ -286,8 +287,21 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
 #pragma unroll
         for (int f = 0; f < FJ; ++f) {
           uint32_t o = so[f] + (a.swizzled ? st * 128 : st);
-          if (o > sleft - 4) o = sleft - 4;  // (the last word of all: next_scales shifts)
+          if (o > slast) o = slast;  // (the last word of all: next_scales shifts)
           sn[f] = __builtin_amdgcn_raw_buffer_load_b32(rs, (int)o, 0, 0);
+        }
+      }
+    };
+    // Fewer than 4 bytes in all: rows of at most 3 blocks, so these are all stages'.
+    // A word would end past the resource, and reads past the tensor or as zeros.
+    auto load_bytes = [&]() {
+      if constexpr (JK == KC4) {
+        const __amdgpu_buffer_rsrc_t rs = lin_rsrc(sp + stile, sleft);
+#pragma unroll
+        for (int f = 0; f < FJ; ++f) {
+          sn[f] = 0;
+#pragma unroll
+          for (int b = 0; b < 3; ++b) sn[f] |= (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(rs, (int)so[f] + b, 0, 0) << (8 * b);
         }
       }
     };
@@ -300,7 +314,7 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
           sv[f] = sn[f] & mask;
           if (have < 4) {
             const uint32_t o = so[f] + (a.swizzled ? st * 128 : st);
-            const uint32_t by = o > sleft - 4 ? o - (sleft - 4) : 0;
+            const uint32_t by = o > slast ? o - slast : 0;
             sv[f] = by < 4 ? (sn[f] >> (8 * by)) & mask : 0u;
           }
         }
@@ -468,7 +482,8 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
         multiply();
       }
     } else {
-      load_scales(kb);
+      if (JK == KC4 && sleft < 4) load_bytes();
+      else load_scales(kb);
       // KC4: the first four stages' codes; the loop asks for the next four in the
       // first two of every four stages
 #pragma unroll

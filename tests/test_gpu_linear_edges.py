@@ -147,3 +147,20 @@ def test_padding_of_swizzled_scales_is_not_read(shape, dtype, groups):
         if end > b:
             _check(dx[1][b:end], dy[b:end], made[e][2])
         b = end
+
+
+@pytest.mark.parametrize("k", [32, 64, 96])
+@pytest.mark.parametrize("n", [1, 2, 3, 129, 130, 131, 257])
+@pytest.mark.parametrize("t", [65, 100, 300])
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_last_columns_with_fewer_than_four_scales(t, n, k, dtype):
+    """The last column tile has 1 to 9 bytes of scales, not always a whole word: of one weight, and of each in a stack."""
+    made = [_weight(10 * e + k, n, k) for e in range(3)]
+    x = _normal(t, t, k, dtype=dtype)
+    _check(K.mx_matmul(x, made[0][0], made[0][1]), x, made[0][2].t())
+    ends = torch.tensor([t // 2, t - 20, t], dtype=torch.int32, device=DEV)
+    y = K.grouped_mx_matmul(x, torch.stack([m[0] for m in made]), torch.stack([m[1] for m in made]), ends)
+    b = 0
+    for e, end in enumerate(ends.tolist()):
+        _check(y[b:end], x[b:end], made[e][2].t())
+        b = end
