@@ -14,7 +14,7 @@ the C ABI:
 * :func:`dequantize_gguf`   <- P/gguf_dequant.py:303-331 (all 15 dispatched types)
 
 Products with weights as they are stored (no reference counterpart; with
-autograd in :mod:`.linear`):
+autograd in :mod:`.linear`, these refuse to lose a gradient):
 
 * :func:`mx_matmul`, :func:`mx_matmul_input_grad` -- one MXFP4 weight
 * :func:`grouped_matmul`, :func:`grouped_matmul_input_grad`,
@@ -641,6 +641,13 @@ _MAX_EXPERTS = 1024
 
 
 # (These calls are as short as 5 us on the GPU: the checks below look at each tensor once.)
+def _raw(label: str, *tensors: torch.Tensor) -> None:
+    """Refuse what would lose a gradient: the result has no graph, the layers of :mod:`.linear` give it one."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise NotImplementedError(f"{label} records no gradient; call mx_linear or grouped_linear, or run it under "
+                                  "torch.no_grad().")
+
+
 def _rows(label: str, x: torch.Tensor, cols: int) -> tuple[torch.Tensor, int, int]:
     """``x`` [..., cols] as [rows, cols] whose rows are contiguous, the number of rows, and their stride."""
     shape = x.shape
@@ -648,6 +655,8 @@ def _rows(label: str, x: torch.Tensor, cols: int) -> tuple[torch.Tensor, int, in
         raise ValueError(f"{label}: expected rows of {cols} elements, got shape {tuple(shape)}.")
     if x.dtype not in _FACTOR_DTYPES:
         raise ValueError(f"{label} supports bfloat16 and float16 rows, got {x.dtype}.")
+    if x.requires_grad:
+        _raw(label, x)
     if len(shape) != 2:
         x = x.reshape(-1, cols)
         shape = x.shape
@@ -726,6 +735,7 @@ def _linear_forward(label: str, x: torch.Tensor, weight: L.WeightStruct, bias: t
     if bias is not None:
         if bias.dtype is not x.dtype or tuple(bias.shape) != (n,):
             raise ValueError(f"{label}: bias must be {x.dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}.")
+        _raw(label, bias)
         bias = bias.contiguous()
     y = x2.new_empty((t, n))
     if t:
@@ -777,6 +787,7 @@ def _dense_stack(label: str, rows: torch.Tensor, weight: torch.Tensor) -> L.Weig
         raise ValueError(f"{label} requires the weight in the rows' dtype {rows.dtype}, got {weight.dtype}.")
     if not weight.is_contiguous():
         raise ValueError(f"{label} requires a contiguous weight.")
+    _raw(label, weight)
     return L.WeightStruct(weight.data_ptr(), None, shape[1], shape[2], L.torch_dtype_id(weight.dtype), 0, shape[0], 0)
 
 

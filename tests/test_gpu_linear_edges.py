@@ -164,3 +164,27 @@ def test_last_columns_with_fewer_than_four_scales(t, n, k, dtype):
     for e, end in enumerate(ends.tolist()):
         _check(y[b:end], x[b:end], made[e][2].t())
         b = end
+
+
+def test_raw_products_refuse_to_lose_a_gradient():
+    """The raw operators return no graph: with gradients on they refuse what requires one, and run under no_grad."""
+    q, s, _ = _weight(1, 64, 128)
+    x, dy, bias = _normal(2, 4, 128), _normal(3, 4, 64), _normal(4, 64)
+    w, ends = _normal(5, 2, 64, 128), torch.tensor([1, 3], dtype=torch.int32, device=DEV)
+    stack = q.view(2, 32, 64), s.view(2, 32, 4)
+    calls = [(lambda x: K.mx_matmul(x, q, s), x), (lambda b: K.mx_matmul(x, q, s, bias=b), bias),
+             (lambda dy: K.mx_matmul_input_grad(dy, q, s), dy), (lambda x: K.grouped_matmul(x, w, ends), x),
+             (lambda w: K.grouped_matmul(x, w, ends), w), (lambda dy: K.grouped_matmul_input_grad(dy, w, ends), dy),
+             (lambda w: K.grouped_matmul_input_grad(dy, w, ends), w),
+             (lambda dy: K.grouped_matmul_weight_grad(dy, x, ends), dy),
+             (lambda x: K.grouped_matmul_weight_grad(dy, x, ends), x),
+             (lambda x: K.grouped_mx_matmul(x, *stack, ends), x),
+             (lambda dy: K.grouped_mx_matmul_input_grad(dy, *stack, ends), dy[:, :32].contiguous())]
+    for i, (call, tensor) in enumerate(calls):
+        want = call(tensor)
+        leaf = tensor.clone().requires_grad_()
+        with pytest.raises(NotImplementedError):
+            call(leaf)
+            pytest.fail(f"call {i} was taken")
+        with torch.no_grad():
+            assert torch.equal(call(leaf), want)
