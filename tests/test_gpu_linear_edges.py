@@ -188,3 +188,76 @@ def test_raw_products_refuse_to_lose_a_gradient():
             pytest.fail(f"call {i} was taken")
         with torch.no_grad():
             assert torch.equal(call(leaf), want)
+
+
+# tiles of 64, 128 and 256 rows, whole rounds of tiles with a rest, split sums; N a multiple of 8 and not
+MANY = [(100, 1000, 128), (128, 256, 256), (777, 2001, 2080), (150, 2064, 4128), (300, 1021, 8192), (1030, 2064, 1056),
+        (2050, 2325, 544), (4100, 4352, 1056), (4100, 4353, 1056)]
+
+
+@pytest.mark.parametrize("shape", MANY, ids=str)
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("quant", [False, True], ids=["wide", "fp4"])
+def test_bias_of_many_rows(shape, dtype, quant):
+    """Every column its own bias, of the size of the sums."""
+    t, n, k = shape
+    q, s, w = _weight(n, n, k)
+    x, bias = _normal(t, t, k, dtype=dtype), _normal(n + 1, n, dtype=dtype)
+    act = FP4 if quant else None
+    a = _quantised(x) if quant else x
+    _check(K.mx_matmul(x, q, s, bias=bias, activation_dtype=act), a, w.t(), bias)
+    _check(K.mx_matmul(x, q, s, activation_dtype=act), a, w.t())
+
+
+def _whole(seed, *shape, blocks):
+    """Whole numbers of the 4-bit grid up to 4; the first of every block of 32 is 4 (blocks: its scale is 2^0)."""
+    g = torch.Generator(DEV).manual_seed(seed)
+    v = torch.randint(-4, 5, shape, generator=g, device=DEV).double()
+    if blocks:
+        v[..., ::32] = 4
+    return v
+
+
+def _whole_weight(seed, n, k):
+    w = _whole(seed, n, k, blocks=True)
+    q, s = K.requantize_mx(w.to(BF16), FP4)
+    assert torch.equal(_decode(q, s), w)
+    return q, s, w
+
+
+def _same(got, want):
+    """want is exact, and so is a sum of whole numbers in fp32: one rounding is left, and one right value."""
+    assert want.abs().max() < 2**24 and (got.dtype is BF16 or want.abs().max() < 65504)
+    assert torch.equal(got, want.to(got.dtype))
+
+
+@pytest.mark.parametrize("shape", MANY, ids=str)
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_whole_numbers_of_many_rows_are_exact(shape, dtype):
+    t, n, k = shape
+    q, s, w = _whole_weight(n, n, k)
+    x, dy = _whole(t, t, k, blocks=True), _whole(k, t, n, blocks=False)
+    xd, wt = x.to(dtype), w.t().contiguous()
+    _same(K.mx_matmul(xd, q, s), x @ wt)
+    _same(K.mx_matmul(xd, q, s, activation_dtype=FP4), x @ wt)
+    _same(K.mx_matmul_input_grad(dy.to(dtype), q, s), dy @ w)
+
+
+@pytest.mark.parametrize("case", [([1500, 0, 1, 2000, 700], 4112, 1568), ([255, 257, 0, 512, 1], 1040, 2080),
+                                  ([130, 0, 900], 2061, 544)], ids=lambda c: f"{'-'.join(map(str, c[0]))}:{c[1]}x{c[2]}")
+def test_whole_numbers_of_groups_are_exact(case):
+    sizes, n, k = case
+    t, ends = sum(sizes) + 3, torch.tensor(sizes).cumsum(0).to(torch.int32).to(DEV)
+    made = [_whole_weight(e, n, k) for e in range(len(sizes))]
+    q, s, w = (torch.stack(m) for m in zip(*made))
+    x, dy = _whole(1, t, k, blocks=True), _whole(2, t, n, blocks=False)
+    xd, dyd, wd = x.to(BF16), dy.to(BF16), w.to(BF16)
+    y, dx, dw = x.new_zeros(t, n), x.new_zeros(t, k), torch.zeros_like(w)
+    for e, b, end in _spans(sizes):
+        y[b:end], dx[b:end], dw[e] = x[b:end] @ w[e].t().contiguous(), dy[b:end] @ w[e], dy[b:end].t().contiguous() @ x[b:end]
+    _same(K.grouped_mx_matmul(xd, q, s, ends), y)
+    _same(K.grouped_mx_matmul(xd, q, s, ends, activation_dtype=FP4), y)
+    _same(K.grouped_mx_matmul_input_grad(dyd, q, s, ends), dx)
+    _same(K.grouped_matmul(xd, wd, ends), y)
+    _same(K.grouped_matmul_input_grad(dyd, wd, ends), dx)
+    _same(K.grouped_matmul_weight_grad(dyd, xd, ends), dw)
