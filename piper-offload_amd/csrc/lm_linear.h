@@ -11,7 +11,7 @@ struct LinArgs {
   const void* b;  // x in the weight gradient: [T, ldb]
   int64_t ldb;
   // 4-bit inputs: codes [64 padded, K/2], scales and the weight's scales packed in
-  // pieces of 64 rows x 256 of K (k_lin_prep4); every group starts on a piece
+  // pieces of 64 rows x 128 of K, 256 bytes (k_lin_prep4); every group starts on a piece
   const uint8_t* xq;
   const uint8_t* xs;
   const uint8_t* wsc;
@@ -232,12 +232,13 @@ DEV v4f32 lin_mfma(lm_u32x4 a, lm_u32x4 b, v4f32 c) {
   else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf16, a), __builtin_bit_cast(v8bf16, b), c, 0, 0, 0);
 }
 
-// 8 codes -> 8 values of 16 bits
 // Byte b of a word of e8m0 scales, as the conversion below takes it: it reads the
 // exponent field alone (0 is 2^-127, 255 NaN), whatever sign and mantissa are.
 DEV float lin_e8m0(uint32_t word, int b) {
   return u2f(b == 3 ? word >> 1 : word << (23 - 8 * b));
 }
+// 8 codes -> 8 values of 16 bits.  Exact in bf16.  fp16 rows take fp16 products, so
+// the values are rounded to fp16: exact from 2^-23 to 49152, infinite above.
 template <bool HALF>
 DEV lm_u32x4 lin_decode8(uint32_t codes, float scale) {
   lm_u32x4 v;

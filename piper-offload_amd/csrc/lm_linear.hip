@@ -188,11 +188,12 @@ static int64_t round8(int64_t x) { return (x + 7) & ~(int64_t)7; }
 // in a part of a tile, 0.4 of one on average, and one in ten has no rows.
 // Whole rounds and the rest apart (lin_rounds): the rest in 128 x 128 tiles after a
 // second launch, 5 us, which groups with fewer than 48 stages do not wait for.
-// Measured, us at 256 x 256 / 128 x 128 / 64 x 128: MXFP4 [14336, 4096] at 300 rows
-// 81 / 68 / 56, [4096, 4096] at 2048 rows 90 / 78 / 83 (input gradient 96 / 77 / 103),
-// 4 groups [4096, 4096] at 1024 rows 83 / 76 / 63, 32 groups [2816, 2048] at 2048 rows
-// 73 / 57 / 46, at 8192 114 / 137 / 134; dense, 8 groups [4096, 2048] at 4096 rows in
-// rounds 84, whole 99 / 103 / 128.
+// Measured in graphs, us at 256 x 256 / 128 x 128 / 64 x 128: MXFP4 [14336, 4096] at 300
+// rows 62 / 66 / 55, [4096, 4096] at 2048 rows 76 / 77 / 82 (input gradient 78 / 77 /
+// 103), 4 groups [4096, 4096] at 1024 rows 63 / 74 / 61, 32 groups [2816, 2048] at 2048
+// rows 84 / 56 / 44, at 8192 104 / 126 / 126; dense, 8 groups [4096, 2048] at 4096 rows
+// in rounds 79, whole 92 / 99 / 121.  The worst of 48: dense, 32 groups [2816, 2048] at
+// 2048 rows, input gradient, 90 where 256 x 256 takes 72.
 struct LinCost {
   double full, alone, pair, one, three, two, single;
 };

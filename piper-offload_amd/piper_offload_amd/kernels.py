@@ -765,6 +765,8 @@ def mx_matmul(x: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, *, swiz
 
     ``x`` [..., in] bfloat16 or float16; sums in fp32, rounded once to ``x.dtype``.  With
     ``activation_dtype=torch.float4_e2m1fn_x2`` ``x`` is quantised first, as :func:`requantize_mx` does it.
+    Weights are exact for bfloat16 and for quantised inputs; float16 inputs see each weight rounded to float16
+    (exact from 2^-23 to 49152 in magnitude, infinite above).
     """
     label = "MX product"
     _on_gpu(label, x, qdata, scale, bias)
@@ -773,7 +775,10 @@ def mx_matmul(x: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, *, swiz
 
 def mx_matmul_input_grad(dy: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, *,
                          swizzled: bool = False) -> torch.Tensor:
-    """``dy @ W``: the input gradient of :func:`mx_matmul` (straight through a quantised input)."""
+    """``dy @ W``: the input gradient of :func:`mx_matmul` (straight through a quantised input).
+
+    A float16 ``dy`` sees each weight rounded to float16, as there.
+    """
     label = "MX product gradient"
     _on_gpu(label, dy, qdata, scale)
     return _linear_input_grad(label, dy, _mx_weight(label, qdata, scale, swizzled, False), None)
@@ -834,7 +839,10 @@ def grouped_matmul_weight_grad(dy: torch.Tensor, x: torch.Tensor, ends: torch.Te
 
 def grouped_mx_matmul(x: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, ends: torch.Tensor, *,
                       swizzled: bool = False, activation_dtype: torch.dtype | None = None) -> torch.Tensor:
-    """:func:`grouped_matmul` with MXFP4 weights: ``qdata`` [groups, out, in/2], scales of each group's weight."""
+    """:func:`grouped_matmul` with MXFP4 weights: ``qdata`` [groups, out, in/2], scales of each group's weight.
+
+    Roundings as in :func:`mx_matmul`.
+    """
     label = "Grouped MX product"
     _on_gpu(label, x, qdata, scale, ends)
     w = _mx_weight(label, qdata, scale, swizzled, True)
