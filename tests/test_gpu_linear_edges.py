@@ -115,7 +115,7 @@ def _pad(s, n, blocks, value):
     return out
 
 
-# few rows, tiles of 64, 128 and 256 rows, split sums (40 and 150 rows); N a part of a run of 32 rows, K of four blocks
+# one tile and many, sums split in three from 1030 rows on; N that ends inside a run of 32 rows, K with and without whole words of scales
 PADDED = [(3, 1, 64), (40, 33, 96), (20, 100, 4128), (70, 100, 160), (150, 1100, 4128), (300, 257, 416), (300, 130, 32),
           (1030, 2050, 1056), (2050, 2325, 544)]
 
