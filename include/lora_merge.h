@@ -22,8 +22,11 @@
  *   lm_*_merge_stack <- the per-target loop of merge_lora()
  *                      (P/merge.py:121-125) as one grouped launch
  *   lm_linear, lm_linear_*_grad <- (no reference counterpart: products with
- *                      the merged MXFP4 weights, and with one weight per
- *                      group of rows)
+ *                      the merged MXFP4 and INT8 weights, and with one weight
+ *                      per group of rows)
+ *   lm_route_topk, lm_dispatch_rows, lm_combine_rows, their *_grad <- (no
+ *                      reference counterpart: routing to experts, and rows to
+ *                      their experts and back)
  *
  * Conventions
  *  - All pointers are device pointers unless noted; tensors are row-major
@@ -67,7 +70,8 @@ enum lm_dtype {
   LM_E4M3 = 3, /* float8_e4m3fn */
   LM_E5M2 = 4, /* float8_e5m2 */
   LM_E2M1 = 5, /* packed fp4, even column in the low nibble */
-  LM_E8M0 = 6
+  LM_E8M0 = 6,
+  LM_I8 = 7 /* int8, of products alone */
 };
 
 /* rounding of terminal codes */
@@ -272,15 +276,22 @@ int lm_routed_residual(const void* x, const void* y, void* out, int64_t T, int64
  * `w` is a HOST struct.  dtype LM_E2M1: MXFP4, codes [experts, N, K/2]
  * (16-byte aligned, K % 32 == 0) and e8m0 scales per expert as lm_mx_merge has
  * them (plain or swizzled, one expert after the other); fp16 rows see each
- * weight rounded to fp16, bf16 rows see it exactly.  Otherwise a dense weight
- * [experts, N, K] of `dtype`.
+ * weight rounded to fp16, bf16 rows see it exactly.  dtype LM_I8: INT8 with one
+ * scale a row, codes [experts, N, K] and `scale` fp32 or bf16 [experts, N]
+ * (`reserved` says which: LM_F32 or LM_BF16); the product sees the codes
+ * exactly and multiplies its sum by the scale, the input gradient sees each
+ * weight rounded to `dtype`.  Otherwise a dense weight [experts, N, K] of
+ * `dtype`.
  * `ends`: device int32[experts]; group e's rows are [ends[e-1], ends[e]).  Rows
  * past ends[experts-1] get zeros, without the bias.  NULL with one expert: all
  * T rows.  Ends that fall or pass T are clamped.
  * input_dtype: `dtype`, or LM_E2M1 (MXFP4 weights): x is quantised to MXFP4
  * first, as lm_mx_requant with LM_MX_FLOOR does; a block with an infinity or a
- * NaN makes its row NaN.  The input gradient passes straight through that
- * rounding.
+ * NaN makes its row NaN.  Or LM_I8 (INT8 weights, K <= 132104): a row's scale is
+ * its largest magnitude / 127 in fp32, its codes are the exact quotients
+ * rounded to nearest (ties to even), their sums with the weight's codes are
+ * exact; a row with an infinity or a NaN comes out NaN.  The input gradient
+ * passes straight through either rounding.
  * Strides are in elements; outputs are contiguous; N, K < 2^21.  Workspace:
  * lm_linear_workspace_size bytes for the call's sizes and strides (ldb: ldx of
  * the weight gradient, else 0; aligned: the pointers of rows and weights are
@@ -306,6 +317,76 @@ int lm_linear_input_grad(const void* dy, int64_t lddy, const lm_weight* w, const
 int lm_linear_weight_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const int32_t* ends, void* dw,
                           int64_t T, int64_t N, int64_t K, int32_t experts, int32_t dtype, void* workspace,
                           size_t workspace_bytes, void* stream);
+
+/* ---------------- routing to experts ----------------------------------
+ * No reference counterpart.  For every row of `logits` ([T, experts], row
+ * stride ld, dtype LM_F32 / LM_BF16 / LM_F16):
+ *   p      softmax or sigmoid of the row, in fp32
+ *   c      p + bias (fp32 [experts], or NULL); an expert whose logit or c is
+ *          -inf is closed
+ *   groups `groups` runs of consecutive experts; a run's value is the sum of
+ *          its group_best (1 or 2) best c, as far as they are open; the
+ *          top_groups best runs stay open (ties: the first)
+ *   expert the top_k best c, the best first (ties: the lowest index); -1 where
+ *          none is left.  c are compared as numbers of 64 bits, without a bias
+ *          by their logits.
+ *   weight scale * p, renormalize: scale * p / sum of the chosen p; 0 for -1
+ * position [T, top_k]: the choices sorted by expert, those of one expert in the
+ * order of the tokens, those of none behind all; ends [experts]: the choices of
+ * the experts up to each, the `ends` of lm_linear.  A row with a NaN (softmax:
+ * or a +inf) has NaN weights and experts that exist.
+ * The gradient needs the logits, the settings and the experts; it writes
+ * [T, experts] of dtype.  `r` is a HOST struct.  Workspace: 256-byte aligned,
+ * NULL when lm_route_workspace_size is 0. */
+enum lm_route_score { LM_ROUTE_SOFTMAX = 0, LM_ROUTE_SIGMOID = 1 };
+#define LM_ROUTE_MAX_BEST 64
+#define LM_ROUTE_MAX_GROUPS 64
+typedef struct lm_route {
+  const void* logits;
+  const float* bias;
+  int64_t ld;
+  int64_t T;
+  int32_t experts;
+  int32_t dtype;
+  int32_t score;
+  int32_t top_k;
+  int32_t groups;
+  int32_t top_groups;
+  int32_t group_best;
+  int32_t renormalize;
+  float scale;
+  int32_t reserved;
+} lm_route;
+size_t lm_route_workspace_size(const lm_route* r);
+int lm_route_topk(const lm_route* r, float* weight, int32_t* expert, int32_t* position, int32_t* ends, void* workspace,
+                  size_t workspace_bytes, void* stream);
+int lm_route_topk_grad(const lm_route* r, const float* dweight, const int32_t* expert, void* dlogits, void* stream);
+
+/* Rows of tokens [T, N] to the places of their choices [T top_k, N], and back:
+ *   lm_dispatch_rows       out[position[t,j]] = x[t]
+ *   lm_dispatch_rows_grad  dx[t] = sum_j dy[position[t,j]]
+ *   lm_combine_rows        out[t] = sum_j weight[t,j] h[position[t,j]]
+ *   lm_combine_rows_grad   dh[position[t,j]] = weight[t,j] dy[t],
+ *                          dweight[t,j] = sum_n dy[t,n] h[position[t,j],n]
+ * Sums in fp32 in the order of j, rounded once to dtype (LM_BF16 / LM_F16).
+ * Places from ends[experts - 1] on have no expert: nothing is read there, and
+ * zeros are written.  `position` holds each place 0 .. T top_k - 1 once; a place
+ * outside is passed over.  Strides are in elements, outputs are contiguous. */
+typedef struct lm_rows {
+  const int32_t* position;
+  const int32_t* ends;
+  int64_t T;
+  int64_t N;
+  int32_t top_k;
+  int32_t experts;
+  int32_t dtype;
+  int32_t reserved;
+} lm_rows;
+int lm_dispatch_rows(const lm_rows* r, const void* x, int64_t ldx, void* out, void* stream);
+int lm_dispatch_rows_grad(const lm_rows* r, const void* dy, int64_t lddy, void* dx, void* stream);
+int lm_combine_rows(const lm_rows* r, const void* h, int64_t ldh, const float* weight, void* out, void* stream);
+int lm_combine_rows_grad(const lm_rows* r, const void* dy, int64_t lddy, const void* h, int64_t ldh, const float* weight,
+                         void* dh, float* dweight, void* stream);
 
 /* ---------------- stacks: many targets, one grouped launch ------------
  * `items` is a HOST array of `count` descriptors.  Each target gets its own
@@ -338,7 +419,7 @@ int lm_nvfp4_merge_stack(const lm_stack_item* items, int32_t count, int32_t swiz
  * main kernel launches with hipEvents on the caller's stream, keyed by kernel
  * family ("rows", "rows_stack", "blocks_full", "blocks_amax",
  * "blocks_quant", "todense", "prep", "nvfp4", "mx", "q8", "gguf", "linear",
- * "linear_few", "linear_prep").  lm_timer_read synchronizes the
+ * "linear_few", "linear_prep", "route", "rows_experts").  lm_timer_read synchronizes the
  * recorded events and returns the summed milliseconds and launch count of one
  * family.  Enabling (or re-enabling) clears the record. */
 int lm_timer_enable(int32_t enable);

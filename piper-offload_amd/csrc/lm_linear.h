@@ -23,6 +23,9 @@ struct LinArgs {
   const void* w;  // [experts, N, K] dense or [experts, N, K/2] codes
   const uint8_t* scale;
   int64_t scale_stride;  // bytes of one expert's scales
+  // INT8 weights: `scale` has one number a row, fp32 or bf16 (scale16); 8-bit inputs: one fp32 number a row of x
+  const float* row_scale;
+  int scale16;
   const void* bias;
   const int32_t* ends;  // [experts] or null: one group of all T rows
   void* out;

@@ -11,6 +11,7 @@
 
 #include "lm_impl.h"
 #include "lm_linear.h"
+#include "lm_linear8.h"
 #include "lm_linear_few.h"
 #include "lm_linear_mm.h"
 
@@ -123,6 +124,9 @@ static int check_lin(const lm_weight* w, int64_t T, int32_t dtype, const int32_t
     if (!w->scale) return fail(LM_EINVAL, "MXFP4 weight without scales");
     if (w->K % 32 != 0) return fail(LM_EINVAL, "MXFP4 requires columns divisible by 32, got %lld", (long long)w->K);
     if (((uintptr_t)w->q & 15) != 0) return fail(LM_EINVAL, "MXFP4 codes must be 16-byte aligned");
+  } else if (w->dtype == LM_I8) {
+    if (!w->scale) return fail(LM_EINVAL, "INT8 weight without scales");
+    if (w->reserved != LM_F32 && w->reserved != LM_BF16) return fail(LM_EUNSUPPORTED, "INT8 weights have fp32 or bf16 scales");
   } else if (w->dtype != dtype) {
     return fail(LM_EUNSUPPORTED, "a dense weight must have the rows' dtype");
   }
@@ -137,7 +141,12 @@ static LinArgs lin_args(const lm_weight* w, const int32_t* ends, int64_t T) {
   a.K = w->K;
   a.swizzled = w->swizzled;
   a.experts = w->experts;
-  a.scale_stride = lin_scale_bytes(w->N, w->K, w->swizzled);
+  if (w->dtype == LM_I8) {
+    a.scale16 = w->reserved == LM_BF16;
+    a.scale_stride = w->N * (a.scale16 ? 2 : 4);
+  } else {
+    a.scale_stride = lin_scale_bytes(w->N, w->K, w->swizzled);
+  }
   a.ends = ends;
   a.T = T;
   return a;
@@ -440,6 +449,7 @@ static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 extern "C" size_t lm_linear_workspace_size(int32_t op, int64_t T, int64_t lda, int64_t ldb, int64_t N, int64_t K,
                                            int32_t experts, int32_t weight_dtype, int32_t input_dtype, int32_t aligned) {
   if (T <= 0 || N <= 0 || K <= 0 || experts <= 0 || op < LM_LINEAR_FORWARD || op > LM_LINEAR_WEIGHT_GRAD) return 0;
+  if (weight_dtype == LM_I8) return op == LIN_WEIGHT_GRAD ? 0 : lin8_workspace(op, T, lda, N, K, experts, input_dtype == LM_I8, aligned != 0);
   return lin_plan(op, T, lda, ldb, N, K, experts, weight_dtype == LM_E2M1, op == LIN_FORWARD && input_dtype == LM_E2M1, aligned != 0)
       .total;
 }
@@ -450,9 +460,13 @@ extern "C" int lm_linear(const void* x, int64_t ldx, const lm_weight* w, const v
   int rc;
   if (!w) return fail(LM_EINVAL, "lm_linear requires a weight");
   if ((rc = check_lin(w, T, dtype, ends, w->experts))) return rc;
-  const bool mx = w->dtype == LM_E2M1, quant = input_dtype == LM_E2M1;
-  if (!quant && input_dtype != dtype) return fail(LM_EUNSUPPORTED, "the product's input dtype is the rows' or LM_E2M1");
+  const bool mx = w->dtype == LM_E2M1, quant = input_dtype == LM_E2M1, i8 = w->dtype == LM_I8;
+  if (!quant && input_dtype != dtype && input_dtype != LM_I8)
+    return fail(LM_EUNSUPPORTED, "the product's input dtype is the rows', LM_E2M1 or LM_I8");
   if (quant && !mx) return fail(LM_EUNSUPPORTED, "4-bit inputs need an MXFP4 weight");
+  if (input_dtype == LM_I8 && !i8) return fail(LM_EUNSUPPORTED, "8-bit inputs need an INT8 weight");
+  if (input_dtype == LM_I8 && w->K > LIN8_MAX_SUM)
+    return fail(LM_EUNSUPPORTED, "8-bit products sum up to %d columns in 32 bits, got %lld", LIN8_MAX_SUM, (long long)w->K);
   if (T == 0) return LM_OK;
   if (!x || !y) return fail(LM_EINVAL, "row pointers must be non-null");
   if (ldx < w->K) return fail(LM_EINVAL, "row stride below the row length");
@@ -462,6 +476,7 @@ extern "C" int lm_linear(const void* x, int64_t ldx, const lm_weight* w, const v
   a.lda = ldx;
   a.bias = bias;
   a.out = y;
+  if (i8) return lin8_forward(a, dtype, input_dtype == LM_I8, workspace, workspace_bytes, st);
   const LinPlan p = lin_plan(LIN_FORWARD, T, ldx, 0, a.N, a.K, a.experts, mx, quant, aligned16(x) && aligned16(w->q));
   if ((rc = lin_setup(a, p, LIN_FORWARD, workspace, workspace_bytes, st))) return rc;
   if (!quant) {
@@ -503,6 +518,7 @@ extern "C" int lm_linear_input_grad(const void* dy, int64_t lddy, const lm_weigh
   a.a = dy;
   a.lda = lddy;
   a.out = dx;
+  if (w->dtype == LM_I8) return lin8_input_grad(a, dtype, workspace, workspace_bytes, st);
   const LinPlan p = lin_plan(LIN_INPUT_GRAD, T, lddy, 0, a.N, a.K, a.experts, mx, false, aligned16(dy) && aligned16(w->q));
   if ((rc = lin_setup(a, p, LIN_INPUT_GRAD, workspace, workspace_bytes, st))) return rc;
   return mx ? run_mm<LIN_INPUT_GRAD, W_MX>(a, p, dtype, st) : run_mm<LIN_INPUT_GRAD, W_DENSE>(a, p, dtype, st);

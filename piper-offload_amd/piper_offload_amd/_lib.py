@@ -14,13 +14,13 @@ import threading
 import torch
 
 __all__ = [
-    "LM_F32", "LM_BF16", "LM_F16", "LM_E4M3", "LM_E5M2", "LM_E2M1", "LM_E8M0",
+    "LM_F32", "LM_BF16", "LM_F16", "LM_E4M3", "LM_E5M2", "LM_E2M1", "LM_E8M0", "LM_I8",
     "LM_ROUND_NEAREST", "LM_ROUND_STOCHASTIC",
-    "LoraStruct", "RoundingStruct", "RoutedFactor", "StackItem", "WeightStruct",
+    "LoraStruct", "RoundingStruct", "RouteStruct", "RoutedFactor", "RowsStruct", "StackItem", "WeightStruct",
     "check", "lib", "library_path", "torch_dtype_id", "workspace",
 ]
 
-LM_F32, LM_BF16, LM_F16, LM_E4M3, LM_E5M2, LM_E2M1, LM_E8M0 = 0, 1, 2, 3, 4, 5, 6
+LM_F32, LM_BF16, LM_F16, LM_E4M3, LM_E5M2, LM_E2M1, LM_E8M0, LM_I8 = 0, 1, 2, 3, 4, 5, 6, 7
 LM_ROUND_NEAREST, LM_ROUND_STOCHASTIC = 0, 1
 LM_OK, LM_EINVAL, LM_EUNSUPPORTED, LM_EWORKSPACE, LM_EHIP = 0, 1, 2, 3, 4
 
@@ -70,7 +70,24 @@ class WeightStruct(ctypes.Structure):
                 ("experts", _I32), ("reserved", _I32)]
 
 
+class RouteStruct(ctypes.Structure):
+    """Mirror of ``lm_route``."""
+
+    _fields_ = [("logits", _P), ("bias", _P), ("ld", _I64), ("T", _I64), ("experts", _I32), ("dtype", _I32),
+                ("score", _I32), ("top_k", _I32), ("groups", _I32), ("top_groups", _I32), ("group_best", _I32),
+                ("renormalize", _I32), ("scale", ctypes.c_float), ("reserved", _I32)]
+
+
+class RowsStruct(ctypes.Structure):
+    """Mirror of ``lm_rows``."""
+
+    _fields_ = [("position", _P), ("ends", _P), ("T", _I64), ("N", _I64), ("top_k", _I32), ("experts", _I32),
+                ("dtype", _I32), ("reserved", _I32)]
+
+
 _L = ctypes.POINTER(LoraStruct)
+_T = ctypes.POINTER(RouteStruct)
+_X = ctypes.POINTER(RowsStruct)
 _W = ctypes.POINTER(WeightStruct)
 _R = ctypes.POINTER(RoundingStruct)
 
@@ -105,6 +122,13 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lm_linear": (_I32, [_P, _I64, _W, _P, _P, _P, _I64, _I32, _I32, _P, _SZ, _P]),
     "lm_linear_input_grad": (_I32, [_P, _I64, _W, _P, _P, _I64, _I32, _P, _SZ, _P]),
     "lm_linear_weight_grad": (_I32, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _P, _SZ, _P]),
+    "lm_route_workspace_size": (_SZ, [_T]),
+    "lm_route_topk": (_I32, [_T, _P, _P, _P, _P, _P, _SZ, _P]),
+    "lm_route_topk_grad": (_I32, [_T, _P, _P, _P, _P]),
+    "lm_dispatch_rows": (_I32, [_X, _P, _I64, _P, _P]),
+    "lm_dispatch_rows_grad": (_I32, [_X, _P, _I64, _P, _P]),
+    "lm_combine_rows": (_I32, [_X, _P, _I64, _P, _P, _P]),
+    "lm_combine_rows_grad": (_I32, [_X, _P, _I64, _P, _I64, _P, _P, _P, _P]),
     "lm_timer_enable": (_I32, [_I32]),
     "lm_timer_read": (_I32, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int64)]),
 }

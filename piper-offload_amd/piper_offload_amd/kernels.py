@@ -21,6 +21,16 @@ autograd in :mod:`.linear`, these refuse to lose a gradient):
   :func:`grouped_matmul_weight_grad` -- one dense weight per group of rows
 * :func:`grouped_mx_matmul`, :func:`grouped_mx_matmul_input_grad` -- one MXFP4
   weight per group of rows
+* :func:`int8_matmul`, :func:`int8_matmul_input_grad`,
+  :func:`grouped_int8_matmul`, :func:`grouped_int8_matmul_input_grad` -- INT8
+  weights with one scale per output channel
+
+Mixtures of experts (likewise; with autograd in :mod:`.routing`):
+
+* :func:`route_topk`, :func:`route_topk_grad` -- the experts of every token,
+  their weights, and the places that bring the rows of one expert together
+* :func:`dispatch_rows`, :func:`combine_rows` and their gradients -- rows to
+  these places, and back as weighted sums
 
 The ``*_into`` variants write into caller-provided (possibly aliasing)
 outputs; the adapters use them to merge in place without a copy.
@@ -30,24 +40,33 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Any
+from typing import Any, NamedTuple
 
 import torch
 
 from . import _lib as L
 
 __all__ = [
+    "Routing",
+    "combine_rows",
+    "combine_rows_grad",
     "dequantize_float8",
     "GGUF_DEQUANT_TYPES",
     "dequantize_gguf",
     "dequantize_int8",
     "dequantize_mx",
     "dequantize_nvfp4",
+    "dispatch_rows",
+    "dispatch_rows_grad",
+    "grouped_int8_matmul",
+    "grouped_int8_matmul_input_grad",
     "grouped_matmul",
     "grouped_matmul_input_grad",
     "grouped_matmul_weight_grad",
     "grouped_mx_matmul",
     "grouped_mx_matmul_input_grad",
+    "int8_matmul",
+    "int8_matmul_input_grad",
     "merge_dense_lora_",
     "merge_float8_lora",
     "merge_float8_lora_into",
@@ -64,6 +83,8 @@ __all__ = [
     "requantize_mx",
     "requantize_nvfp4",
     "requantize_q8_0",
+    "route_topk",
+    "route_topk_grad",
 ]
 
 GGML_Q8_0 = 8
@@ -638,14 +659,17 @@ def merge_dense_lora_(weight: torch.Tensor, b: torch.Tensor, a: torch.Tensor, st
 # Products with stored weights
 # ---------------------------------------------------------------------------
 _MAX_EXPERTS = 1024
+_MAX_INT8_COLS = 132104  # products of codes, 127 * 128 each, add up below 2^31
+
+
+_LAYERS = "mx_linear, int8_linear, grouped_linear, route_experts, dispatch_experts or combine_experts"
 
 
 # (These calls are as short as 5 us on the GPU: the checks below look at each tensor once.)
 def _raw(label: str, *tensors: torch.Tensor) -> None:
     """Refuse what would lose a gradient: the result has no graph, the layers of :mod:`.linear` give it one."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise NotImplementedError(f"{label} records no gradient; call mx_linear or grouped_linear, or run it under "
-                                  "torch.no_grad().")
+        raise NotImplementedError(f"{label} records no gradient; call {_LAYERS}, or run it under torch.no_grad().")
 
 
 def _rows(label: str, x: torch.Tensor, cols: int) -> tuple[torch.Tensor, int, int]:
@@ -729,9 +753,16 @@ def _linear_forward(label: str, x: torch.Tensor, weight: L.WeightStruct, bias: t
     x2, t, ldx = _rows(label, x, k)
     dtype_id = input_id = L.torch_dtype_id(x.dtype)
     if activation_dtype is not None:
-        if activation_dtype is not _FP4_DTYPE or _FP4_DTYPE is None:
-            raise ValueError(f"{label} quantises its input to float4_e2m1fn_x2 only, got {activation_dtype}.")
-        input_id = L.LM_E2M1
+        if weight.dtype == L.LM_I8:
+            if activation_dtype is not torch.int8:
+                raise ValueError(f"{label} quantises its input to int8 only, got {activation_dtype}.")
+            if k > _MAX_INT8_COLS:
+                raise ValueError(f"{label}: 8-bit products take up to {_MAX_INT8_COLS} columns, got {k}.")
+            input_id = L.LM_I8
+        else:
+            if activation_dtype is not _FP4_DTYPE or _FP4_DTYPE is None:
+                raise ValueError(f"{label} quantises its input to float4_e2m1fn_x2 only, got {activation_dtype}.")
+            input_id = L.LM_E2M1
     if bias is not None:
         if bias.dtype is not x.dtype or tuple(bias.shape) != (n,):
             raise ValueError(f"{label}: bias must be {x.dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}.")
@@ -856,3 +887,281 @@ def grouped_mx_matmul_input_grad(dy: torch.Tensor, qdata: torch.Tensor, scale: t
     _on_gpu(label, dy, qdata, scale, ends)
     w = _mx_weight(label, qdata, scale, swizzled, True)
     return _linear_input_grad(label, dy, w, _ends(label, ends, w.experts))
+
+
+# ---- INT8 weights ----------------------------------------------------------
+def _int8_weight(label: str, qdata: torch.Tensor, scale: torch.Tensor, stacked: bool) -> L.WeightStruct:
+    """Check INT8 storage (codes [rows, cols], one scale a row; stacked: one such weight per group) and describe it."""
+    shape, sshape = qdata.shape, scale.shape
+    if len(shape) != 2 + stacked:
+        raise ValueError(f"{label} expects rank-{'three' if stacked else 'two'} INT8 codes.")
+    if qdata.dtype is not torch.int8:
+        raise ValueError(f"{label} expects int8 codes, got {qdata.dtype}.")
+    if scale.dtype is not torch.float32 and scale.dtype is not torch.bfloat16:
+        raise ValueError(f"{label} supports float32 and bfloat16 scales, got {scale.dtype}.")
+    if not qdata.is_contiguous() or not scale.is_contiguous():
+        raise ValueError(f"{label} requires contiguous INT8 storage.")
+    if 0 in shape:
+        raise ValueError(f"{label} requires a non-empty weight.")
+    if sshape != shape[:-1] and sshape != (*shape[:-1], 1):
+        raise ValueError(f"{label} takes one scale per row of the weight, got scales {tuple(sshape)} for codes {tuple(shape)}.")
+    return L.WeightStruct(qdata.data_ptr(), scale.data_ptr(), shape[-2], shape[-1], L.LM_I8, 0, shape[0] if stacked else 1,
+                          L.torch_dtype_id(scale.dtype))
+
+
+def int8_matmul(x: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, *, bias: torch.Tensor | None = None,
+                activation_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``x @ W.T + bias`` with ``W = scale * qdata`` (``qdata`` int8 [out, in], ``scale`` [out] or [out, 1]).
+
+    ``x`` [..., in] bfloat16 or float16.  The sums run over the codes, which are exact, in fp32; they are multiplied by
+    the scale and rounded once to ``x.dtype``.  With ``activation_dtype=torch.int8`` every row of ``x`` is quantised
+    first: its scale is its largest magnitude / 127 in fp32, its codes are the exact quotients rounded to nearest (ties
+    to even), and the sums of products of codes are exact.  A row with an infinity or a NaN then comes out NaN.
+    """
+    label = "INT8 product"
+    _on_gpu(label, x, qdata, scale, bias)
+    return _linear_forward(label, x, _int8_weight(label, qdata, scale, False), bias, None, activation_dtype)
+
+
+def int8_matmul_input_grad(dy: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """``dy @ W``: the input gradient of :func:`int8_matmul` (straight through a quantised input).
+
+    ``W`` is rounded to ``dy.dtype`` here: its scales lie along the sums.
+    """
+    label = "INT8 product gradient"
+    _on_gpu(label, dy, qdata, scale)
+    return _linear_input_grad(label, dy, _int8_weight(label, qdata, scale, False), None)
+
+
+def grouped_int8_matmul(x: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, ends: torch.Tensor, *,
+                        activation_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """:func:`grouped_matmul` with INT8 weights: ``qdata`` [groups, out, in], ``scale`` [groups, out] or [groups, out, 1].
+
+    Roundings as in :func:`int8_matmul`.
+    """
+    label = "Grouped INT8 product"
+    _on_gpu(label, x, qdata, scale, ends)
+    w = _int8_weight(label, qdata, scale, True)
+    return _linear_forward(label, x, w, None, _ends(label, ends, w.experts), activation_dtype)
+
+
+def grouped_int8_matmul_input_grad(dy: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor,
+                                   ends: torch.Tensor) -> torch.Tensor:
+    """The gradient of :func:`grouped_int8_matmul` to ``x``; zeros for rows of no group."""
+    label = "Grouped INT8 product gradient"
+    _on_gpu(label, dy, qdata, scale, ends)
+    w = _int8_weight(label, qdata, scale, True)
+    return _linear_input_grad(label, dy, w, _ends(label, ends, w.experts))
+
+
+# ---------------------------------------------------------------------------
+# Routing to experts
+# ---------------------------------------------------------------------------
+_SCORES = {"softmax": 0, "sigmoid": 1}
+_MAX_BEST = 64
+_MAX_GROUPS = 64
+_LOGIT_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class Routing(NamedTuple):
+    """The choices of every token, the best first.
+
+    ``weight`` float32 [tokens, top_k]; ``expert`` int32 [tokens, top_k], -1 (with weight 0) where no expert was open;
+    ``position`` int32 [tokens, top_k]: the place of each choice when the rows of one expert lie side by side, in the
+    order of the tokens (those of no expert come last); ``ends`` int32 [experts]: the end of each expert's rows.
+    """
+
+    weight: torch.Tensor
+    expert: torch.Tensor
+    position: torch.Tensor
+    ends: torch.Tensor
+
+
+def _route(label: str, logits: torch.Tensor, top_k: int, bias: torch.Tensor | None, score: str, groups: int, top_groups: int,
+           group_best: int, renormalize: bool, scale: float) -> tuple[L.RouteStruct, torch.Tensor]:
+    shape = logits.shape
+    if len(shape) != 2:
+        raise ValueError(f"{label} expects logits [tokens, experts], got {tuple(shape)}.")
+    if logits.dtype not in _LOGIT_DTYPES:
+        raise ValueError(f"{label} supports float32, bfloat16 and float16 logits, got {logits.dtype}.")
+    tokens, experts = shape
+    if not 1 <= experts <= _MAX_EXPERTS:
+        raise ValueError(f"{label} takes 1 to {_MAX_EXPERTS} experts, got {experts}.")
+    if score not in _SCORES:
+        raise ValueError(f"{label}: score must be 'softmax' or 'sigmoid', got {score!r}.")
+    if not 1 <= groups <= _MAX_GROUPS or experts % groups:
+        raise ValueError(f"{label}: {experts} experts do not divide into {groups} groups (1 to {_MAX_GROUPS}).")
+    if not 1 <= top_groups <= groups:
+        raise ValueError(f"{label}: top_groups must be 1 to {groups}, got {top_groups}.")
+    if group_best not in (1, 2) or group_best > experts // groups:
+        raise ValueError(f"{label}: group_best must be 1 or 2, and at most the experts of a group, got {group_best}.")
+    if not 1 <= top_k <= min(_MAX_BEST, top_groups * (experts // groups)):
+        raise ValueError(f"{label}: top_k must be 1 to {min(_MAX_BEST, top_groups * (experts // groups))}, got {top_k}.")
+    if tokens * top_k >= 1 << 31:
+        raise ValueError(f"{label} takes fewer than 2^31 choices, got {tokens} tokens of {top_k}.")
+    if not math.isfinite(scale) or scale == 0:
+        raise ValueError(f"{label}: scale must be finite and not zero, got {scale}.")
+    if bias is not None:
+        if bias.dtype is not torch.float32 or tuple(bias.shape) != (experts,):
+            raise ValueError(f"{label}: bias must be float32 [{experts}], got {bias.dtype} {tuple(bias.shape)}.")
+        _raw(label, bias)
+        bias = bias.contiguous()
+    ld = experts
+    if tokens > 1:
+        ld = logits.stride(0)
+        if ld < experts or (experts > 1 and logits.stride(1) != 1):
+            logits, ld = logits.contiguous(), experts
+    elif not logits.is_contiguous():
+        logits = logits.contiguous()
+    keep = logits if bias is None else (logits, bias)
+    return L.RouteStruct(logits.data_ptr(), _ptr(bias), ld, tokens, experts, L.torch_dtype_id(logits.dtype), _SCORES[score],
+                         top_k, groups, top_groups, group_best, renormalize, scale, 0), keep
+
+
+def _call(entry: Any, device: torch.device, *args: object) -> None:
+    """Call one C entry without a workspace on the device's current stream."""
+    with L.on_device(device):
+        rc = entry(*args, L.stream_ptr(device))
+    if rc:
+        L.check(rc)
+
+
+def route_topk(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | None = None, score: str = "softmax",
+               groups: int = 1, top_groups: int = 1, group_best: int = 1, renormalize: bool = True,
+               scale: float = 1.0) -> Routing:
+    """The ``top_k`` experts of every token of ``logits`` [tokens, experts], their weights and their places.
+
+    ``score`` 'softmax' or 'sigmoid' of the logits.  ``bias`` (float32 [experts]) is added for the choice alone.  With
+    ``groups`` the experts form that many runs; the ``top_groups`` runs with the largest sums of their ``group_best``
+    best choices stay open.  The weights are ``scale`` times the scores, divided by the sum of the chosen ones if
+    ``renormalize``.  Ties go to the lowest index; scores are compared as numbers of 64 bits (without a bias by their
+    logits).  An expert whose logit (or bias) is -inf is closed: so is every expert of a padding token whose row is
+    -inf.  A row with a NaN (softmax: or +inf) has NaN weights.  float32 throughout.
+    """
+    label = "Routing"
+    _on_gpu(label, logits, bias)
+    _raw(label, logits)
+    r, keep = _route(label, logits, top_k, bias, score, groups, top_groups, group_best, renormalize, scale)
+    t, e = logits.shape
+    weight = logits.new_empty((t, top_k), dtype=torch.float32)
+    expert = logits.new_empty((t, top_k), dtype=torch.int32)
+    position = logits.new_empty((t, top_k), dtype=torch.int32)
+    ends = logits.new_empty(e, dtype=torch.int32)
+    handle = L.lib()
+    _launch(handle.lm_route_topk, logits.get_device(), handle.lm_route_workspace_size(r), logits.device, r, weight.data_ptr(),
+            expert.data_ptr(), position.data_ptr(), ends.data_ptr())
+    del keep
+    return Routing(weight, expert, position, ends)
+
+
+def route_topk_grad(dweight: torch.Tensor, logits: torch.Tensor, expert: torch.Tensor, *, score: str = "softmax",
+                    renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
+    """The gradient of :func:`route_topk`'s ``weight`` to ``logits``, for the ``expert`` that it chose."""
+    label = "Routing gradient"
+    _on_gpu(label, dweight, logits, expert)
+    _raw(label, dweight, logits)
+    if expert.dtype is not torch.int32 or expert.ndim != 2 or expert.shape[0] != logits.shape[0]:
+        raise ValueError(f"{label}: expert must be int32 [tokens, top_k], got {expert.dtype} {tuple(expert.shape)}.")
+    if dweight.dtype is not torch.float32 or dweight.shape != expert.shape:
+        raise ValueError(f"{label}: dweight must be float32 {tuple(expert.shape)}, got {dweight.dtype} {tuple(dweight.shape)}.")
+    r, keep = _route(label, logits, expert.shape[1], None, score, 1, 1, 1, renormalize, scale)
+    dlogits = logits.new_empty(logits.shape)
+    dweight, expert = dweight.contiguous(), expert.contiguous()
+    if logits.shape[0]:
+        _call(L.lib().lm_route_topk_grad, logits.device, r, dweight.data_ptr(), expert.data_ptr(), dlogits.data_ptr())
+    del keep
+    return dlogits
+
+
+def _places(label: str, position: torch.Tensor, ends: torch.Tensor, cols: int, dtype: torch.dtype
+            ) -> tuple[L.RowsStruct, tuple[torch.Tensor, torch.Tensor]]:
+    if position.dtype is not torch.int32 or position.ndim != 2 or position.shape[1] < 1:
+        raise ValueError(f"{label}: position must be int32 [tokens, top_k], got {position.dtype} {tuple(position.shape)}.")
+    if position.numel() >= 1 << 31:
+        raise ValueError(f"{label} takes fewer than 2^31 choices.")
+    if cols < 1:
+        raise ValueError(f"{label} requires non-empty rows.")
+    ends = _ends(label, ends, ends.shape[0] if ends.ndim == 1 else -1)
+    position = position.contiguous()
+    return L.RowsStruct(position.data_ptr(), ends.data_ptr(), position.shape[0], cols, position.shape[1], ends.shape[0],
+                        L.torch_dtype_id(dtype), 0), (position, ends)
+
+
+def _token_rows(label: str, x: torch.Tensor, rows: int) -> tuple[torch.Tensor, int]:
+    if x.ndim != 2 or x.shape[0] != rows:
+        raise ValueError(f"{label}: expected {rows} rows, got shape {tuple(x.shape)}.")
+    x, _, ld = _rows(label, x, x.shape[1])
+    return x, ld
+
+
+def _choice_weight(label: str, weight: torch.Tensor, position: torch.Tensor) -> torch.Tensor:
+    if weight.dtype is not torch.float32 or weight.shape != position.shape:
+        raise ValueError(f"{label}: weight must be float32 {tuple(position.shape)}, got {weight.dtype} {tuple(weight.shape)}.")
+    _raw(label, weight)
+    return weight.contiguous()
+
+
+def dispatch_rows(x: torch.Tensor, position: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
+    """Rows of tokens [tokens, cols] to the places of their choices: [tokens * top_k, cols], what a grouped product takes.
+
+    ``position`` and ``ends`` as :func:`route_topk` gives them (each place once); places of no expert get zeros.
+    """
+    label = "Dispatch"
+    _on_gpu(label, x, position, ends)
+    x, ld = _token_rows(label, x, position.shape[0] if position.ndim == 2 else 0)
+    r, keep = _places(label, position, ends, x.shape[1], x.dtype)
+    out = x.new_empty((position.numel(), x.shape[1]))
+    if out.shape[0]:
+        _call(L.lib().lm_dispatch_rows, x.device, r, x.data_ptr(), ld, out.data_ptr())
+    del keep
+    return out
+
+
+def dispatch_rows_grad(dy: torch.Tensor, position: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
+    """The gradient of :func:`dispatch_rows` to ``x``: the sum over a token's choices, in fp32, rounded once."""
+    label = "Dispatch gradient"
+    _on_gpu(label, dy, position, ends)
+    dy, ld = _token_rows(label, dy, position.numel())
+    r, keep = _places(label, position, ends, dy.shape[1], dy.dtype)
+    dx = dy.new_empty((position.shape[0], dy.shape[1]))
+    if dx.shape[0]:
+        _call(L.lib().lm_dispatch_rows_grad, dy.device, r, dy.data_ptr(), ld, dx.data_ptr())
+    del keep
+    return dx
+
+
+def combine_rows(h: torch.Tensor, weight: torch.Tensor, position: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
+    """What the experts return, ``h`` [tokens * top_k, cols], as weighted sums of a token's choices: [tokens, cols].
+
+    ``weight`` float32 [tokens, top_k].  Sums in fp32 in the order of the choices, rounded once to ``h.dtype``; choices
+    of no expert are left out, whatever their rows hold.
+    """
+    label = "Combine"
+    _on_gpu(label, h, weight, position, ends)
+    h, ld = _token_rows(label, h, position.numel())
+    weight = _choice_weight(label, weight, position)
+    r, keep = _places(label, position, ends, h.shape[1], h.dtype)
+    out = h.new_empty((position.shape[0], h.shape[1]))
+    if out.shape[0]:
+        _call(L.lib().lm_combine_rows, h.device, r, h.data_ptr(), ld, weight.data_ptr(), out.data_ptr())
+    del keep
+    return out
+
+
+def combine_rows_grad(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, position: torch.Tensor, ends: torch.Tensor
+                      ) -> tuple[torch.Tensor, torch.Tensor]:
+    """The gradients of :func:`combine_rows` to ``h`` (zeros at places of no expert) and to ``weight``."""
+    label = "Combine gradient"
+    _on_gpu(label, dy, h, weight, position, ends)
+    dy, ldy = _token_rows(label, dy, position.shape[0] if position.ndim == 2 else 0)
+    h, ldh = _token_rows(label, h, position.numel())
+    if dy.dtype is not h.dtype or dy.shape[1] != h.shape[1]:
+        raise ValueError(f"{label}: dy {dy.dtype} {tuple(dy.shape)} and h {h.dtype} {tuple(h.shape)} differ.")
+    weight = _choice_weight(label, weight, position)
+    r, keep = _places(label, position, ends, h.shape[1], h.dtype)
+    dh, dweight = h.new_empty(h.shape), weight.new_empty(weight.shape)
+    if position.shape[0]:
+        _call(L.lib().lm_combine_rows_grad, h.device, r, dy.data_ptr(), ldy, h.data_ptr(), ldh, weight.data_ptr(), dh.data_ptr(),
+              dweight.data_ptr())
+    del keep
+    return dh, dweight

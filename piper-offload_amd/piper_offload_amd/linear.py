@@ -1,17 +1,20 @@
-"""Linear layers over stored weights: MXFP4 weights and one weight per group of rows, with gradients.
+"""Linear layers over stored weights: MXFP4 and INT8 weights and one weight per group of rows, with gradients.
 
 After a merge a packed weight is used as it is stored, without a dense copy:
 
 * :func:`mx_linear` -- ``x @ W.T + bias`` for an :class:`MXWeight` in MXFP4;
+* :func:`int8_linear` -- the same for an :class:`Int8Weight` with one scale per
+  row, with inputs in 16 bits or in 8;
 * :func:`grouped_linear` -- consecutive groups of rows, each with a weight of
-  its own (the experts of a mixture, one adapter per request), dense or MXFP4.
+  its own (the experts of a mixture, one adapter per request), dense, MXFP4 or
+  INT8.
 
 Gradients: to ``x`` for every weight, to the weight where it is dense.  A
 packed weight is frozen, as is a bias.  With quantised inputs the gradient
 passes straight through the rounding.
 
-The experts of a packed stack lie one below the other in one ``MXWeight`` of
-``groups * out`` rows; :func:`expert_view` gives one of them as a weight of its
+The experts of a packed stack lie one below the other in one ``MXWeight`` or
+``Int8Weight`` of ``groups * out`` rows; :func:`expert_view` gives one of them as a weight of its
 own, for a LoRA merge in place.
 """
 
@@ -20,9 +23,9 @@ from __future__ import annotations
 import torch
 
 from . import kernels as K
-from .formats import MXWeight
+from .formats import Int8Weight, MXWeight
 
-__all__ = ["expert_view", "grouped_linear", "mx_linear"]
+__all__ = ["expert_view", "grouped_linear", "int8_linear", "mx_linear"]
 
 _FP4 = getattr(torch, "float4_e2m1fn_x2", None)
 
@@ -47,11 +50,37 @@ def _stacked(label: str, weight: MXWeight, groups: int) -> tuple[torch.Tensor, t
     return q.view(groups, rows // groups, q.shape[1]), s.view(groups, s.shape[0] // groups, s.shape[1])
 
 
-def expert_view(weight: MXWeight, index: int, groups: int) -> MXWeight:
+def _int8(label: str, weight: Int8Weight) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales of a weight with one scale per row and nothing besides."""
+    q = weight.qdata
+    if q.ndim != 2 or tuple(weight.block_size) != (1, q.shape[1]) or weight.scale.numel() != q.shape[0]:
+        raise ValueError(f"{label} supports INT8 weights with one scale per row, got block size {tuple(weight.block_size)} "
+                         f"for {tuple(q.shape)}.")
+    if weight.zero_point is not None:  # (whether all are zero is known on the GPU alone, and a call waits for nothing)
+        raise ValueError(f"{label} supports symmetric INT8 weights without zero points; if all of them are zero, leave them out.")
+    if weight.act_pre_scale is not None:
+        raise ValueError(f"{label} does not apply an activation pre-scale; multiply the input by it.")
+    return q, weight.scale.reshape(-1, 1)
+
+
+def _int8_stacked(label: str, weight: Int8Weight, groups: int) -> tuple[torch.Tensor, torch.Tensor]:
+    q, s = _int8(label, weight)
+    rows = q.shape[0]
+    if groups < 1 or rows % groups:
+        raise ValueError(f"{label}: {rows} rows do not divide into {groups} weights.")
+    if not q.is_contiguous() or not s.is_contiguous():
+        raise ValueError(f"{label} requires contiguous INT8 storage.")
+    return q.view(groups, rows // groups, q.shape[1]), s.view(groups, rows // groups, 1)
+
+
+def expert_view(weight: MXWeight | Int8Weight, index: int, groups: int) -> MXWeight | Int8Weight:
     """Weight ``index`` of ``groups`` stacked along the rows of ``weight``, sharing its storage."""
-    q, s = _stacked("expert_view", weight, groups)
+    eight = isinstance(weight, Int8Weight)
+    q, s = (_int8_stacked if eight else _stacked)("expert_view", weight, groups)
     if not 0 <= index < groups:
         raise ValueError(f"expert_view: index {index} is not one of {groups}.")
+    if eight:
+        return Int8Weight(q[index], s[index], weight.block_size, weight.dtype_, reduce_range=weight.reduce_range)
     return MXWeight(q[index].view(weight.qdata.dtype), s[index].view(weight.scale.dtype), weight.elem_dtype,
                     weight.block_size, weight.orig_dtype, weight.is_swizzled_scales, weight.scaling_mode)
 
@@ -84,6 +113,30 @@ class _GroupedMx(torch.autograd.Function):
         return K.grouped_mx_matmul_input_grad(dy, qdata, scale, ends, swizzled=ctx.swizzled), None, None, None, None, None
 
 
+class _Int8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, qdata, scale, bias, activation_dtype):  # noqa: ANN001, ANN205
+        ctx.save_for_backward(qdata, scale)
+        return K.int8_matmul(x, qdata, scale, bias=bias, activation_dtype=activation_dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):  # noqa: ANN001, ANN205
+        return K.int8_matmul_input_grad(dy, *ctx.saved_tensors), None, None, None, None
+
+
+class _GroupedInt8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, qdata, scale, ends, activation_dtype):  # noqa: ANN001, ANN205
+        ctx.save_for_backward(qdata, scale, ends)
+        return K.grouped_int8_matmul(x, qdata, scale, ends, activation_dtype=activation_dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):  # noqa: ANN001, ANN205
+        return K.grouped_int8_matmul_input_grad(dy, *ctx.saved_tensors), None, None, None, None
+
+
 class _GroupedDense(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, ends):  # noqa: ANN001, ANN205
@@ -108,16 +161,32 @@ def mx_linear(x: torch.Tensor, weight: MXWeight, bias: torch.Tensor | None = Non
     return _MxLinear.apply(x, q, s, weight.is_swizzled_scales, bias, activation_dtype)
 
 
+def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None = None, *,
+                activation_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``x @ W.T + bias`` over an INT8 weight with one scale per row, as :func:`.kernels.int8_matmul`.
+
+    ``activation_dtype=torch.int8`` quantises every row of ``x`` first.  Differentiable in ``x``.
+    """
+    q, s = _int8("INT8 linear", weight)
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+        raise ValueError("INT8 linear: the bias is frozen with its packed weight; detach it.")
+    return _Int8Linear.apply(x, q, s, bias, activation_dtype)
+
+
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor, *,
                    activation_dtype: torch.dtype | None = None) -> torch.Tensor:
     """Rows ``ends[e-1] : ends[e]`` of ``x`` times weight ``e``; rows past ``ends[-1]`` give zeros.
 
-    ``weight``: dense [groups, out, in], differentiable like ``x``, or an MXFP4 ``MXWeight`` whose rows are the
-    groups' weights one below the other.  ``ends``: int32 [groups] on the GPU.
+    ``weight``: dense [groups, out, in], differentiable like ``x``, or an MXFP4 ``MXWeight`` or an ``Int8Weight`` with
+    one scale per row, whose rows are the groups' weights one below the other.  ``ends``: int32 [groups] on the GPU.
+    ``activation_dtype``: float4_e2m1fn_x2 for MXFP4 weights, int8 for INT8 ones.
     """
+    if isinstance(weight, Int8Weight):
+        q, s = _int8_stacked("Grouped linear", weight, ends.shape[0] if ends.ndim == 1 else 0)
+        return _GroupedInt8.apply(x, q, s, ends, activation_dtype)
     if isinstance(weight, MXWeight):
         q, s = _stacked("Grouped linear", weight, ends.shape[0] if ends.ndim == 1 else 0)
         return _GroupedMx.apply(x, q, s, ends, weight.is_swizzled_scales, activation_dtype)
     if activation_dtype is not None:
-        raise ValueError("Grouped linear quantises its input for MXFP4 weights only.")
+        raise ValueError("Grouped linear quantises its input for MXFP4 weights only (and INT8 ones), not for dense ones.")
     return _GroupedDense.apply(x, weight, ends)

@@ -1,0 +1,460 @@
+"""Routing to experts, and rows to their experts and back, against plain code in 64 bits.
+
+Experts, places and ends have to be equal.  Tolerances, with D the largest difference of two logits that matter to a
+weight: an exponential is off by 4 + D units of 2^-24 (2 units in its last place, and the rounding of its argument), a
+sum of at most 1024 terms by 22 (a tree of 6 levels over at most 16 terms of a lane), a sigmoid's quotient by 8, and
+3 roundings join them, above and below the fraction line: at most (60 + 2 D) 2^-24 of a weight.  A gradient is a sum of
+terms, each of which has two such factors.  Outputs in 16 bits are off by half a unit in their last place besides.
+Weighted sums of n terms are off by n + 1 roundings of 2^-24 of the sum of magnitudes.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from piper_offload_amd import combine_experts, dispatch_experts, grouped_linear, route_experts
+
+pytestmark = pytest.mark.gpu
+
+K = pytest.importorskip("piper_offload_amd.kernels")
+
+DEV = "cuda"
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+INF = math.inf
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _normal(g, *shape, std=1.0, dtype=F32):
+    return (torch.randn(*shape, generator=g) * std).to(dtype)
+
+
+def _order(row, n):
+    """Indices of the n largest entries above -inf, ties by index."""
+    return [i for i in sorted(range(len(row)), key=lambda i: (-row[i], i)) if row[i] > -INF][:n]
+
+
+def _scores(logits, score):
+    x = logits.double()
+    if score == "sigmoid":
+        return 1 / (1 + torch.exp(-x))
+    top = x.amax(-1, keepdim=True)
+    e = torch.exp(x - torch.where(top > -INF, top, 0.0))
+    return e / e.sum(-1, keepdim=True).clamp_min(1e-300)
+
+
+def _plain(logits, k, bias=None, score="softmax", groups=1, top_groups=1, group_best=1, renormalize=True, scale=1.0):
+    t, e = logits.shape
+    p = _scores(logits, score)
+    # (without a bias the scores are in the order of the logits, also where they are equal in 64 bits)
+    c = (p + bias.double() if bias is not None else p)
+    c = torch.where(logits == -INF, -INF, c)
+    rank = c if bias is not None else logits.double()
+    expert = torch.full((t, k), -1)
+    for i in range(t):
+        row, values = c[i].tolist(), rank[i].tolist()
+        if groups > 1:
+            per = e // groups
+            value = []
+            for j in range(groups):
+                best = sorted((v for v in row[j * per:(j + 1) * per] if v > -INF), reverse=True)[:group_best]
+                value.append(sum(best) if best else -INF)
+            kept = _order(value, top_groups)
+            values = [v if n // per in kept else -INF for n, v in enumerate(values)]
+        best = _order(values, k)
+        expert[i, :len(best)] = torch.tensor(best, dtype=torch.long)
+    on = expert >= 0
+    picked = torch.where(on, logits.double().gather(1, expert.clamp_min(0)), 0.0)
+    if renormalize:  # (from logarithms, for scores that are 0 in 64 bits)
+        log = picked if score == "softmax" else torch.nn.functional.logsigmoid(picked)
+        w = torch.softmax(torch.where(on, log, -INF), -1).nan_to_num(0.0)
+    else:
+        w = torch.where(on, p.gather(1, expert.clamp_min(0)), 0.0)
+    key = torch.where(on, expert, e).reshape(-1)
+    place = torch.empty_like(key)
+    place[key.argsort(stable=True)] = torch.arange(key.numel())
+    ends = torch.bincount(key, minlength=e + 1)[:e].cumsum(0)
+    return w * scale, expert, place.view(t, k), ends
+
+
+def _spread(logits):
+    x = torch.where(logits > -1e30, logits.float(), 0.0)
+    return float((x.amax(-1) - x.amin(-1)).max()) if x.numel() else 0.0
+
+
+def _check(logits, k, bias=None, **how):
+    got = K.route_topk(logits.to(DEV), k, bias=None if bias is None else bias.to(DEV), **how)
+    w, expert, place, ends = _plain(logits.cpu(), k, bias, **how)
+    assert got.weight.dtype is F32 and {got.expert.dtype, got.position.dtype, got.ends.dtype} == {torch.int32}
+    assert (got.expert.cpu() == expert).all()
+    assert (got.position.cpu() == place).all()
+    assert (got.ends.cpu() == ends).all()
+    tol = (60 + 2 * _spread(logits)) * 2.0**-24 * w.abs() + 2.0**-126
+    off = (got.weight.double().cpu() - w).abs()
+    assert (off <= tol).all(), f"worst {(off / tol).max():.3g} tolerances"
+    return got
+
+
+SIZES = [(1, 1, 1), (1, 8, 2), (3, 5, 5), (8, 32, 4), (17, 64, 6), (32, 65, 8), (33, 100, 1), (64, 128, 8), (100, 129, 7), (257, 256, 8),
+         (1000, 60, 4), (40, 300, 12), (70, 512, 64), (50, 1024, 10), (5000, 16, 2), (20000, 8, 2)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("t,e,k", SIZES)
+def test_route(t, e, k, score, dtype):
+    g = _gen(t + e + k)
+    logits = _normal(g, t, e, std=1.5, dtype=dtype)
+    _check(logits, k, score=score, renormalize=(t + k) % 2 == 0, scale=2.5 if t % 3 else 1.0)
+    _check(logits, k, _normal(g, e, std=0.1), score=score, renormalize=(t + k) % 2 == 1)
+
+
+GROUPED = [(1, 8, 2, 2, 1, 1), (9, 32, 4, 8, 3, 2), (40, 256, 8, 8, 4, 2), (33, 160, 6, 8, 3, 1), (20, 60, 5, 3, 2, 2), (31, 64, 2, 64, 5, 1),
+           (50, 1024, 8, 16, 4, 2), (300, 96, 3, 12, 12, 2), (45, 21, 6, 7, 2, 2), (12, 126, 4, 63, 9, 2)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("t,e,k,groups,top,best", GROUPED)
+def test_groups(t, e, k, groups, top, best, score, dtype):
+    g = _gen(t + e + k + groups)
+    logits = _normal(g, t, e, std=1.5, dtype=dtype)
+    logits[_normal(g, t, e) > 1.5] = -INF  # some closed ones, whole groups among them
+    how = dict(score=score, groups=groups, top_groups=top, group_best=best)
+    _check(logits, k, **how)
+    _check(logits, k, _normal(g, e, std=0.1), scale=2.5, **how)
+
+
+@pytest.mark.parametrize("bias", [None, "zero", "same", "steps"])
+def test_ties_go_to_the_lowest_index(bias):
+    """Few values of the logits, so that most choices are between equals; biases that keep them so."""
+    g = _gen(3)
+    for t, e, k, groups in ((40, 64, 8, 1), (40, 256, 8, 8), (200, 24, 5, 4)):
+        logits = torch.randint(0, 3, (t, e), generator=g).to(BF16)
+        b = None if bias is None else torch.zeros(e) if bias == "zero" else torch.full((e,), 0.25)
+        if bias == "steps":
+            b = torch.randint(0, 2, (e,), generator=g).float() / 4
+        for score in ("softmax", "sigmoid"):
+            _check(logits, k, b, score=score, groups=groups, top_groups=max(1, groups // 2), group_best=min(2, groups))
+
+
+def test_choices_between_scores_that_agree_in_32_bits():
+    """Pairs of experts whose biased scores differ by less than a rounding of 2^-24."""
+    g = _gen(8)
+    t, e = 300, 64
+    logits = _normal(g, t, e)
+    logits[:, 32:] = logits[:, :32] + _normal(g, t, 32, std=2e-7)
+    bias = _normal(g, 32, std=0.05).repeat(2)
+    for score in ("softmax", "sigmoid"):
+        _check(logits, 8, bias, score=score)
+        _check(logits, 8, bias, score=score, groups=2, top_groups=1, group_best=2)
+        _check(logits, 8, None, score=score, groups=2, top_groups=1, group_best=2)
+
+
+def test_closed_experts_and_padding():
+    g = _gen(4)
+    logits = _normal(g, 50, 40)
+    logits[10:20] = -INF
+    logits[20:25, 3:] = -INF
+    logits[25, 1:] = -INF
+    logits[26] = torch.finfo(F32).min  # (a mask of the type's lowest value closes nothing: all alike)
+    logits[27, 5:] = torch.finfo(F32).min
+    logits[28] = -200.0  # sigmoid: scores that are 0 in 32 bits
+    logits[29] = 200.0
+    for bias in (None, _normal(g, 40, std=0.1)):
+        for score in ("softmax", "sigmoid"):
+            for dtype in (F32, BF16, F16):
+                x = logits.clamp_min(torch.finfo(dtype).min).to(dtype)
+                x[logits == -INF] = -INF
+                r = _check(x, 6, bias, score=score)
+                assert (r.expert[10:20] == -1).all() and (r.weight[10:20] == 0).all()
+                assert torch.isfinite(r.weight).all()
+    b = torch.zeros(40)
+    b[7] = -INF
+    r = K.route_topk(torch.full((3, 40), 1.0, device=DEV), 40, bias=b.to(DEV))
+    want = [i for i in range(40) if i != 7] + [-1]
+    assert r.expert.tolist() == [want] * 3 and r.ends[-1] == 117
+
+
+def test_not_a_number_stays_in_its_row():
+    g = _gen(6)
+    logits = _normal(g, 20, 30)
+    logits[3, 4] = float("nan")
+    logits[9, 29] = float("nan")
+    logits[11, 2] = INF
+    for bias in (None, _normal(g, 30, std=0.1)):
+        for score in ("softmax", "sigmoid"):
+            for groups in (1, 3):
+                how = dict(score=score, groups=groups, top_groups=max(1, groups - 1), group_best=1)
+                r = K.route_topk(logits.to(DEV), 4, bias=None if bias is None else bias.to(DEV), **how)
+                bad = [3, 9] + ([11] if score == "softmax" else [])
+                assert torch.isnan(r.weight[bad]).all()
+                assert all(len(set(row)) == 4 and 0 <= min(row) and max(row) < 30 for row in r.expert.tolist())
+                rest = [i for i in range(20) if i not in bad]
+                w, expert, _, _ = _plain(logits[rest], 4, bias, **how)
+                assert (r.expert.cpu()[rest] == expert).all() and torch.isfinite(r.weight[rest]).all()
+                assert sorted(r.position.view(-1).tolist()) == list(range(80)) and int(r.ends[-1]) == 80
+
+
+def test_strides():
+    g = _gen(12)
+    big = _normal(g, 70, 99, dtype=BF16).to(DEV)
+    for x in (big[:, :64], big[:, 7:71], big[::2, :64], big[:, ::3], big[:64, :64].t(), big[:1, 3:60]):
+        _check(x, 4)
+        dw = _normal(g, x.shape[0], 4).to(DEV)
+        e = K.route_topk(x, 4).expert
+        a, b = K.route_topk_grad(dw, x, e), K.route_topk_grad(dw, x.contiguous(), e)
+        assert a.is_contiguous() and (a == b).all()
+
+
+def _grad_want(logits, expert, dw, score, renormalize, scale):
+    """By autograd in 64 bits, and the sum of the terms' magnitudes."""
+    x = logits.double().clone().requires_grad_()
+    on = expert >= 0
+    at = expert.clamp_min(0).long()
+    if renormalize:
+        log = x if score == "softmax" else torch.nn.functional.logsigmoid(x)
+        w = torch.softmax(torch.where(on, log.gather(1, at), -1e300), -1)
+    else:
+        p = torch.softmax(torch.where(x == -INF, -1e300, x), -1) if score == "softmax" else torch.sigmoid(x)
+        w = p.gather(1, at)
+    w = torch.where(on, w, 0.0) * scale
+    g = torch.where(on, dw.double(), 0.0)
+    (w * g).sum().backward()
+    total = (g * w).abs().sum(-1, keepdim=True)
+    size = torch.zeros_like(x).scatter_add(1, at, torch.where(on, (g * w).abs(), 0.0)).detach()
+    if renormalize:
+        size += torch.zeros_like(x).scatter_add(1, at, w.abs() / abs(scale) * total).detach()
+    elif score == "softmax":
+        size += (torch.softmax(torch.where(x == -INF, -1e300, x), -1) * total).detach()
+    return x.grad.nan_to_num(0.0), size
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_gradient(score, renormalize, dtype):
+    for t, e, k in ((1, 1, 1), (5, 8, 2), (40, 64, 4), (33, 130, 8), (20, 256, 6), (9, 500, 64), (7, 1024, 10)):
+        g = _gen(t + e)
+        logits = _normal(g, t, e, std=1.5, dtype=dtype)
+        if e > 8:
+            logits[2, 3:] = -INF
+            logits[3] = -INF
+        dw = _normal(g, t, k)
+        expert = K.route_topk(logits.to(DEV), k, score=score).expert
+        got = K.route_topk_grad(dw.to(DEV), logits.to(DEV), expert, score=score, renormalize=renormalize, scale=2.5)
+        want, size = _grad_want(logits, expert.cpu(), dw, score, renormalize, 2.5)
+        half, tiny = {F32: (2.0**-24, 2.0**-120), BF16: (2.0**-8, 2.0**-120), F16: (2.0**-11, 2.0**-25)}[dtype]
+        tol = (1 + 2.0**-8) * half * want.abs() + 2 * (60 + 2 * _spread(logits)) * 2.0**-24 * size + tiny
+        assert got.dtype is dtype
+        off = (got.double().cpu() - want).abs()
+        assert (off <= tol).all(), f"{t} {e} {k}: worst {(off / tol).max():.3g} tolerances"
+
+
+def test_gradient_against_differences():
+    """The loss sum(w dw) along a direction, by central differences, whose error is of the third order."""
+    g = _gen(14)
+    logits, u, dw = _normal(g, 30, 48), _normal(g, 30, 48), _normal(g, 30, 5)
+    for score in ("softmax", "sigmoid"):
+        for renormalize in (True, False):
+            how = dict(score=score, renormalize=renormalize)
+            bias = torch.where(torch.arange(48) < 5, 100.0, 0.0).to(DEV)  # (the choice does not change)
+
+            def loss(x):
+                return (K.route_topk(x.to(DEV), 5, bias=bias, **how).weight.double().cpu() * dw.double()).sum()
+
+            h = 2.0**-6
+            r = K.route_topk(logits.to(DEV), 5, bias=bias, **how)
+            along = (K.route_topk_grad(dw.to(DEV), logits.to(DEV), r.expert, **how).double().cpu() * u.double()).sum()
+            diff = (loss(logits + h * u) - loss(logits - h * u)) / (2 * h)
+            # third derivative of a weight along u: at most 6 of |u|^3, h^2 / 6 of it; fp32 weights' errors over 2 h
+            u3 = (u.abs().amax(-1, keepdim=True) ** 3 * dw.abs()).sum()
+            bound = h * h * u3 + 2 * (60 + 20) * 2.0**-24 * dw.abs().sum() / (2 * h)
+            assert abs(along - diff) <= bound, (score, renormalize, float(along), float(diff))
+
+
+def _case(g, t, e, k, cols, dtype, padded=0):
+    logits = _normal(g, t, e)
+    logits[t - padded:] = -INF
+    r = K.route_topk(logits.to(DEV), k)
+    x, dy = _normal(g, t, cols, dtype=dtype), _normal(g, t, cols, dtype=dtype)
+    h, dh = _normal(g, t * k, cols, dtype=dtype), _normal(g, t * k, cols, dtype=dtype)
+    return r, x, dy, h, dh
+
+
+ROWS = [(1, 4, 1, 1, 0), (1, 8, 2, 7, 0), (5, 8, 3, 64, 2), (16, 32, 4, 2048, 0), (33, 20, 6, 513, 5), (70, 64, 8, 1000, 70), (9, 40, 33, 129, 1),
+        (300, 16, 2, 4100, 17), (6, 64, 64, 24, 0)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("t,e,k,cols,padded", ROWS)
+def test_rows(t, e, k, cols, padded, dtype):
+    g = _gen(t + cols)
+    r, x, dy, h, dh = _case(g, t, e, k, cols, dtype, padded)
+    live = t - padded
+    if padded:  # what padding holds is not looked at
+        x[live:] = float("nan")
+        h[live * k:] = float("nan")
+        dh[live * k:] = INF
+    at = (r.position, r.ends)
+    place, w = r.position.cpu().long(), r.weight.double().cpu()
+    assert sorted(place.view(-1).tolist()) == list(range(t * k)) and int(r.ends[-1]) == live * k
+    rows = K.dispatch_rows(x.to(DEV), *at).cpu()
+    want = torch.zeros_like(rows)
+    want[place[:live].reshape(-1)] = x[:live].repeat_interleave(k, 0)
+    assert (rows == want).all()
+
+    half, tiny = (2.0**-8, 1e-38) if dtype is BF16 else (2.0**-11, 2.0**-25)
+
+    def close(got, want, size, n, half=half, tiny=tiny):
+        off = (got.double().cpu() - want).abs()
+        assert (off <= (1 + 2.0**-8) * half * want.abs() + (n + 1) * 2.0**-24 * size + tiny).all()
+
+    h64, d64, y64 = h.double(), dh.double(), dy.double()
+    y = K.combine_rows(h.to(DEV), r.weight, *at)
+    mine = torch.zeros(t, k, cols, dtype=torch.float64)
+    mine[:live] = h64[place[:live]]
+    w = torch.where((torch.arange(t) < live)[:, None], w, 0.0)
+    close(y, (w[..., None] * mine).sum(1), (w[..., None] * mine).abs().sum(1), k)
+    back = torch.zeros(t, k, cols, dtype=torch.float64)
+    back[:live] = d64[place[:live]]
+    close(K.dispatch_rows_grad(dh.to(DEV), *at), back.sum(1), back.abs().sum(1), k)
+    gh, gw = K.combine_rows_grad(dy.to(DEV), h.to(DEV), r.weight, *at)
+    wh = torch.zeros(t * k, cols, dtype=torch.float64)
+    wh[place[:live].reshape(-1)] = (w[:live, :, None] * y64[:live, None]).reshape(-1, cols)
+    close(gh, wh, wh.abs(), 1)
+    terms = y64[:, None] * mine
+    close(gw, terms.sum(-1), terms.abs().sum(-1), cols, half=2.0**-24)
+
+
+def test_rows_of_other_strides():
+    g = _gen(77)
+    r, x, dy, h, dh = _case(g, 20, 8, 3, 200, BF16)
+    at = (r.position, r.ends)
+
+    def wide(v, off):
+        out = torch.empty(v.shape[0], v.shape[1] + 11, dtype=v.dtype, device=DEV)[:, off:off + v.shape[1]]
+        return out.copy_(v.to(DEV))
+
+    for off in (0, 1, 8):
+        assert (K.dispatch_rows(wide(x, off), *at) == K.dispatch_rows(x.to(DEV), *at)).all()
+        assert (K.dispatch_rows_grad(wide(dh, off), *at) == K.dispatch_rows_grad(dh.to(DEV), *at)).all()
+        assert (K.combine_rows(wide(h, off), r.weight, *at) == K.combine_rows(h.to(DEV), r.weight, *at)).all()
+        a = K.combine_rows_grad(wide(dy, off), wide(h, off), r.weight, *at)
+        b = K.combine_rows_grad(dy.to(DEV), h.to(DEV), r.weight, *at)
+        assert (a[0] == b[0]).all() and (a[1] == b[1]).all()
+
+
+def test_places_outside_are_passed_over():
+    """Positions that are no places: nothing is read or written for them."""
+    x = torch.ones(4, 16, dtype=BF16, device=DEV)
+    ends = torch.tensor([3, 8], dtype=torch.int32, device=DEV)
+    bad = torch.tensor([[0, 1], [-5, 2], [8, 3], [4, 1 << 30]], dtype=torch.int32, device=DEV)
+    h = torch.ones(8, 16, dtype=BF16, device=DEV)
+    w = torch.ones(4, 2, device=DEV)
+    rows = K.dispatch_rows(x, bad, ends)
+    assert (rows[:5] == 1).all()
+    assert K.combine_rows(h, w, bad, ends)[:, 0].tolist() == [2, 1, 1, 1]
+    gh, gw = K.combine_rows_grad(x, h, w, bad, ends)
+    assert (gh[:5] == 1).all() and gw.tolist() == [[16, 16], [0, 16], [0, 16], [16, 0]]
+    for past in (100, -3):  # ends that are not: at most all places, at least none
+        out = K.combine_rows(h, w, bad, torch.tensor([3, past], dtype=torch.int32, device=DEV))
+        assert out[:, 0].tolist() == ([2, 1, 1, 1] if past > 0 else [0, 0, 0, 0])
+
+
+def _mixture(x, router, up, down, k, r=None):
+    r = route_experts(x @ router.t(), k) if r is None else r
+    h = grouped_linear(dispatch_experts(x, r), up, r.ends)
+    return combine_experts(grouped_linear(torch.tanh(h), down, r.ends), r)
+
+
+def test_a_mixture_of_experts_and_its_gradients():
+    """All of it together against the same in plain float64, expert by expert; roundings of every step are counted
+    as 2^-7 of the sums of magnitudes."""
+    g = _gen(99)
+    t, hidden, inner, e, k = 50, 64, 96, 6, 2
+    x, router = _normal(g, t, hidden), _normal(g, e, hidden, std=hidden**-0.5)
+    up, down = _normal(g, e, inner, hidden, std=hidden**-0.5), _normal(g, e, hidden, inner, std=inner**-0.5)
+    dy = _normal(g, t, hidden)
+    ours = [v.to(BF16).to(DEV).requires_grad_() for v in (x, router, up, down)]
+    y = _mixture(*ours, k)
+    y.backward(dy.to(BF16).to(DEV))
+    plain = [v.detach().cpu().double().requires_grad_() for v in ours]
+    px, pr, pu, pd = plain
+    logits = (ours[0] @ ours[1].t()).detach().cpu()  # the choice sees rounded logits
+    expert = K.route_topk(logits.to(DEV), k).expert.cpu().long()
+    w = torch.softmax((px @ pr.t()).gather(1, expert), -1)
+    out = torch.zeros(t, hidden, dtype=torch.float64)
+    for j in range(k):
+        hh = torch.tanh((pu[expert[:, j]] @ px[..., None])[..., 0])
+        out = out + w[:, j:j + 1] * (pd[expert[:, j]] @ hh[..., None])[..., 0]
+    out.backward(dy.to(BF16).double())
+    assert (y.detach().cpu().double() - out.detach()).abs().max() <= 2.0**-7 * 4 * out.abs().max()
+    for a, b in zip(ours, plain):
+        assert (a.grad.cpu().double() - b.grad).norm() <= 2.0**-6 * b.grad.norm()
+
+
+def test_graph_replays_and_other_streams():
+    g = _gen(101)
+    router = _normal(g, 8, 64, std=0.125, dtype=BF16).to(DEV)
+    up, down = _normal(g, 8, 96, 64, std=0.1, dtype=BF16).to(DEV), _normal(g, 8, 64, 96, std=0.1, dtype=BF16).to(DEV)
+    for t in (3, 200):
+        x = _normal(g, t, 64, dtype=BF16).to(DEV)
+        logits = (x @ router.t()).clone()
+
+        def work():
+            r = K.route_topk(logits, 2)
+            y = _mixture(x, router, up, down, 2, r)
+            return *r, y, K.route_topk_grad(r.weight, logits, r.expert)
+
+        with torch.no_grad():
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                first = work()
+            torch.cuda.current_stream().wait_stream(side)
+            for a, b in zip(first, work()):
+                assert (a == b).all()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = work()
+            for i in range(4):
+                x.copy_(_normal(g, t, 64, dtype=BF16))
+                logits.copy_(x @ router.t())
+                logits[t - min(i, t):] = -INF
+                graph.replay()
+                want = work()
+                torch.cuda.synchronize()
+                for a, b in zip(out, want):
+                    assert (a == b).all()
+
+
+def test_no_tokens():
+    for e in (3, 100):
+        r = K.route_topk(torch.empty(0, e, device=DEV), 2)
+        assert r.expert.shape == (0, 2) and r.ends.tolist() == [0] * e
+    x = torch.empty(0, 16, dtype=BF16, device=DEV)
+    assert K.dispatch_rows(x, r.position, r.ends).shape == (0, 16) and K.dispatch_rows_grad(x, r.position, r.ends).shape == (0, 16)
+    assert K.combine_rows(x, r.weight, r.position, r.ends).shape == (0, 16)
+    assert K.combine_rows_grad(x, x, r.weight, r.position, r.ends)[1].shape == (0, 2)
+    assert K.route_topk_grad(r.weight, torch.empty(0, e, device=DEV), r.expert).shape == (0, e)
+
+
+def test_gradients_are_not_lost():
+    x = torch.zeros(4, 8, device=DEV, requires_grad=True)
+    with pytest.raises(NotImplementedError):
+        K.route_topk(x, 2)
+    r = route_experts(x, 2)
+    assert r.weight.requires_grad and not r.expert.requires_grad
+    h = torch.zeros(8, 16, dtype=BF16, device=DEV)
+    with pytest.raises(NotImplementedError):
+        K.combine_rows(h, r.weight, r.position, r.ends)
+    with pytest.raises(NotImplementedError):
+        K.dispatch_rows(torch.zeros(4, 16, dtype=BF16, device=DEV, requires_grad=True), r.position, r.ends)
+    with pytest.raises(ValueError, match="detach"):
+        route_experts(x, 2, bias=torch.zeros(8, device=DEV, requires_grad=True))
