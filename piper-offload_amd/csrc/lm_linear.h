@@ -259,7 +259,35 @@ DEV lm_u32x4 lin_decode8(uint32_t codes, float scale) {
   return v;
 }
 
-enum : int { W_DENSE = 0, W_MX = 1, W_Q4 = 2 };
+// W_Q8: rows and weight are INT8 codes; W_I8: INT8 weight, rows of 16 bits
+enum : int { W_DENSE = 0, W_MX = 1, W_Q4 = 2, W_Q8 = 3, W_I8 = 4 };
+
+// the scale of row i of an INT8 weight
+DEV float lin_scale8(const LinArgs& a, int64_t i) {
+  return a.scale16 ? bf16_val(((const LM_GLOBAL uint16_t*)a.scale)[i]) : ((const LM_GLOBAL float*)a.scale)[i];
+}
+// 8 INT8 codes -> 8 values of 16 bits, times s or (exact) as they are
+template <bool HALF, bool SCALED>
+DEV lm_u32x4 lin_decode8i(uint32_t lo, uint32_t hi, float s) {
+  lm_u32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = i < 2 ? lo : hi;
+    float a = (float)(int8_t)(w >> (16 * (i & 1))), b = (float)(int8_t)(w >> (16 * (i & 1) + 8));
+    if constexpr (SCALED) {
+      a *= s;
+      b *= s;
+    }
+    v[i] = HALF ? (uint32_t)f16_bits(a) | (uint32_t)f16_bits(b) << 16 : pack_bf16x2(a, b);
+  }
+  return v;
+}
+typedef int lin_i32x4 __attribute__((ext_vector_type(4)));
+// 64 steps of whole numbers; the sums' bits lie in a v4f32
+DEV v4f32 lin_mfma8(lm_u32x4 a, lm_u32x4 b, v4f32 c) {
+  return __builtin_bit_cast(v4f32, __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(lin_i32x4, a), __builtin_bit_cast(lin_i32x4, b),
+                                                                        __builtin_bit_cast(lin_i32x4, c), 0, 0, 0));
+}
 
 // byte FA of sa and byte FB of sb are the operands' scales
 template <int FA, int FB>

@@ -1,0 +1,159 @@
+// lm_linear8_few.h -- products of few rows with INT8 weights.
+//
+// Bound by the bytes of the weight.  As k_lin_few: no LDS tiles, operands straight
+// from memory into MFMA registers; a workgroup owns 16 MF rows x 16 CF columns, its
+// NW waves split the contraction, 128 codes a unit, and add their sums up through
+// LDS in a fixed order; every wave has UN units of loads in flight.
+//
+// Lane group g (lane >> 4) reads 16 codes of a row at 64 h + 16 g, h = 0, 1.  With
+// 8-bit inputs (Q8) both sides are read so and one instruction contracts the 64 of
+// an h.  With 16-bit inputs the 16 codes are decoded (exactly) into two operands of
+// 8, steps (h, 0) and (h, 1), and x is read in the same order: lane group g has
+// elements 64 h + 16 g + 8 c at step (h, c).
+#pragma once
+#include <type_traits>
+
+#include "lm_linear.h"
+
+DEV lm_u32x4 few8_load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_bit_cast(lm_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
+}
+// 16 codes from p, of which the first `left` exist (any alignment)
+DEV lm_u32x4 few8_chunk(const uint8_t* p, int left) {
+  lm_u32x4 v = {};
+  if (left >= 16) {
+    v = *(const LM_GLOBAL lm_u32x4_any*)p;
+  } else if (left > 0) {
+    uint64_t lo = 0, hi = 0;
+    for (int b = 0; b < left; ++b) {
+      const uint64_t c = ((const LM_GLOBAL uint8_t*)p)[b];
+      if (b < 8) lo |= c << (8 * b);
+      else hi |= c << (8 * b - 64);
+    }
+    v = lm_u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+  }
+  return v;
+}
+
+template <int DT, bool Q8, int MF, int CF, int NW, int UN>
+__global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* codes, int64_t pitch) {
+  constexpr bool HALF = DT == F16;
+  constexpr int COLS = CF * 16, ROWS = MF * 16, PITCH = COLS + 4;
+  constexpr int XL = Q8 ? 2 : 4;            // 16-byte loads of x a unit
+  constexpr int AC = MF * CF <= 2 ? 2 : 1;  // accumulators in turn: the MFMAs of a fragment depend on each other
+  __shared__ __attribute__((aligned(16))) uint32_t red[NW * ROWS * PITCH];
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, wave = wave_index();
+  // (row tiles first, each XCD a contiguous part: as k_lin_few)
+  const uint32_t gn = (uint32_t)((a.N + COLS - 1) / COLS), u = (uint32_t)xcd_unit(blockIdx.x, gridDim.x);
+  const uint32_t tiles = gridDim.x / gn;
+  const int64_t n0 = (int64_t)(u / tiles) * COLS;
+  int group;
+  int64_t r0, r1;
+  if (!lin_tile<ROWS>(a, u % tiles, group, r0, r1)) return;
+  const bool some = group < a.experts;
+  v4f32 acc[AC][MF][CF] = {};
+  if (some) {
+    const int K = (int)a.K;
+    const int64_t ldx = Q8 ? pitch : a.lda * 2;  // bytes
+    const int rows = (int)(r1 - r0 < ROWS ? r1 - r0 : ROWS), cols = (int)(a.N - n0 < COLS ? a.N - n0 : COLS);
+    const uint8_t* xp = (Q8 ? codes : (const uint8_t*)a.a) + r0 * ldx;
+    const uint8_t* wp = (const uint8_t*)a.w + (group * a.N + n0) * a.K;
+    const __amdgpu_buffer_rsrc_t rx = lin_rsrc(xp, (rows - 1) * ldx + (Q8 ? pitch : a.K * 2));
+    const __amdgpu_buffer_rsrc_t rw = lin_rsrc(wp, cols * a.K);
+    uint32_t xo[MF], wo[CF];
+#pragma unroll
+    for (int m = 0; m < MF; ++m) {
+      const int t = m * 16 + (lane & 15);
+      xo[m] = (uint32_t)((t < rows ? t : rows - 1) * ldx) + (Q8 ? 16 : 32) * g;
+    }
+#pragma unroll
+    for (int c = 0; c < CF; ++c) {
+      const int n = c * 16 + (lane & 15) < cols ? c * 16 + (lane & 15) : cols - 1;
+      wo[c] = (uint32_t)(n * a.K) + 16 * g;
+    }
+    // UN units from u0; TAIL: some of them may pass the end
+    auto body = [&](int u0, auto tail) {
+      constexpr bool TAIL = decltype(tail)::value;
+      lm_u32x4 xv[UN][MF][XL], wv[UN][CF][2];
+#pragma unroll
+      for (int i = 0; i < UN; ++i) {
+        const int k0 = (u0 + i) * 128;
+#pragma unroll
+        for (int c = 0; c < CF; ++c)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if constexpr (TAIL) wv[i][c][h] = few8_chunk(wp + wo[c] + k0 + 64 * h, K - k0 - 64 * h - 16 * g);
+            else wv[i][c][h] = few8_load16(rw, wo[c] + k0 + 64 * h);
+          }
+#pragma unroll
+        for (int m = 0; m < MF; ++m)
+#pragma unroll
+          for (int j = 0; j < XL; ++j) {
+            if constexpr (Q8) {
+              xv[i][m][j] = few8_load16(rx, TAIL && k0 + 64 * j + 16 * g >= K ? LIN_OUT : xo[m] + k0 + 64 * j);
+            } else {
+              const int e = k0 + 64 * (j >> 1) + 8 * (j & 1);  // (+ 16 g)
+              if constexpr (TAIL) xv[i][m][j] = lin_chunk((const uint16_t*)(xp + xo[m]) + e, K - e - 16 * g);
+              else xv[i][m][j] = few8_load16(rx, xo[m] + 2 * e);
+            }
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < UN; ++i)
+#pragma unroll
+        for (int c = 0; c < CF; ++c) {
+          if constexpr (Q8) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int m = 0; m < MF; ++m) acc[h % AC][m][c] = lin_mfma8(wv[i][c][h], xv[i][m][h], acc[h % AC][m][c]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const lm_u32x4 w = wv[i][c][j >> 1];
+              const lm_u32x4 f = lin_decode8i<HALF, false>(j & 1 ? w[2] : w[0], j & 1 ? w[3] : w[1], 1.0f);
+#pragma unroll
+              for (int m = 0; m < MF; ++m) acc[j % AC][m][c] = lin_mfma<HALF>(f, xv[i][m][j], acc[j % AC][m][c]);
+            }
+          }
+        }
+    };
+    const int units = (K + 127) >> 7, whole = K >> 7;
+    int u0 = wave * UN;
+    for (; u0 + UN <= whole; u0 += NW * UN) body(u0, std::false_type{});
+    if (u0 < units) body(u0, std::true_type{});
+#pragma unroll
+    for (int m = 0; m < MF; ++m)
+#pragma unroll
+      for (int c = 0; c < CF; ++c) {
+        lm_u32x4 v = __builtin_bit_cast(lm_u32x4, acc[0][m][c]);
+        if constexpr (AC == 2) {
+          if constexpr (Q8) v += __builtin_bit_cast(lm_u32x4, acc[1][m][c]);
+          else v = __builtin_bit_cast(lm_u32x4, acc[0][m][c] + acc[1][m][c]);
+        }
+        *(lm_u32x4*)(red + ((wave * ROWS) + m * 16 + (lane & 15)) * PITCH + c * 16 + 4 * g) = v;
+      }
+  }
+  __syncthreads();
+  for (int i = tid; i < ROWS * COLS; i += NW * 64) {
+    const int m = i / COLS, c = i % COLS;
+    const int64_t n = n0 + c;
+    if (r0 + m >= r1 || n >= a.N) continue;
+    float s = 0.0f;
+    if (some) {
+      if constexpr (Q8) {
+        uint32_t sum = 0;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) sum += red[(k * ROWS + m) * PITCH + c];
+        // (in this order no large row overflows on the way)
+        s = (float)(int)sum * lin_scale8(a, group * a.N + n) * a.row_scale[r0 + m];
+      } else {
+#pragma unroll
+        for (int k = 0; k < NW; ++k) s += u2f(red[(k * ROWS + m) * PITCH + c]);
+        s *= lin_scale8(a, group * a.N + n);
+      }
+      if (a.bias) s += val_dt<DT>(((const LM_GLOBAL uint16_t*)a.bias)[n]);
+    }
+    ((LM_GLOBAL uint16_t*)a.out)[(r0 + m) * a.N + n] = bits_dt<DT>(s);
+  }
+}

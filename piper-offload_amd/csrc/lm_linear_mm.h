@@ -18,6 +18,11 @@
 //   KS4   MXFP4 with the contraction strided: every code of a run of 32 shares a
 //         scale but the 8 codes of an MFMA lane do not, so these are decoded on
 //         their way into LDS and then are KS16
+//   KC8   INT8 codes along the contraction, KS8 across it: decoded on their way into
+//         LDS too, and then KC16 (the codes alone: the scales come with the store)
+//         and KS16 (times their row's scale, which lies along the sum)
+// Q8: both operands INT8 codes; a slot of 64 bytes has 64 of them, and all but the
+// matrix instruction is as for 16 bits (the arguments count in pairs of codes).
 // Q4: both operands MXFP4 (x quantised beforehand), multiplied as they are by the
 // scaled MFMA, 128 codes a stage, so a slot is 64 bytes here too.  Its scales
 // come packed by k_lin_prep4: per 64 slots and stage 256 bytes, which hold for
@@ -43,7 +48,7 @@
 
 #include "lm_linear.h"
 
-enum : int { KC16, KS16, KC4, KS4 };
+enum : int { KC16, KS16, KC4, KS4, KC8, KS8 };
 
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 typedef __attribute__((address_space(3))) uint32_t lds_u32;
@@ -138,21 +143,25 @@ DEV bool lin_pick(const LinArgs& a, int64_t jend, LinTile& t) {
 
 template <int DT, int OP, int W, int BM, int BN, int WM, int WN>
 struct MmTraits {
-  static constexpr bool Q4 = W == W_Q4, MX = W == W_MX;
+  static constexpr bool Q4 = W == W_Q4, MX = W == W_MX, Q8 = W == W_Q8, I8 = W == W_I8;
   static constexpr int NW = WM * WN, NT = NW * 64;
   static constexpr int CS = Q4 ? 128 : 32;  // contraction of a stage
   static constexpr int IK = OP == LIN_WEIGHT_GRAD ? KS16 : KC16;
-  static constexpr int JK = OP == LIN_FORWARD ? (MX ? KC4 : KC16) : (OP == LIN_INPUT_GRAD && MX ? KS4 : KS16);
+  static constexpr int JK = OP == LIN_FORWARD      ? (MX ? KC4 : I8 ? KC8 : KC16)
+                            : OP == LIN_INPUT_GRAD ? (MX ? KS4 : I8 ? KS8 : KS16)
+                                                   : KS16;
+  static constexpr bool REG = JK == KS4 || JK == KC8 || JK == KS8;  // decoded on the way into LDS
+  static constexpr int LK = JK == KS4 || JK == KS8 ? KS16 : JK == KC8 ? KC16 : JK;  // J's tile in LDS
   static constexpr int FI = BM / WM / 16, FJ = BN / WN / 16;
   static constexpr int IB = BM * 64, JB = BN * 64;  // bytes of a stage (KC4: of four)
   static constexpr int IL = IB / 1024 / NW;                               // loads per wave
-  static constexpr int JL = JK == KS4 ? 2 : JB / 1024 / NW;
+  static constexpr int JL = JK == KC8 ? 1 : REG ? 2 : JB / 1024 / NW;
   static constexpr int SB = Q4 ? NW * 256 : 16;  // bytes of a stage's scales: I's, then J's
   static_assert(!Q4 || BM / 64 + BN / 64 <= NW, "at most a piece of scales per wave");
   static_assert(IL * 1024 * NW == IB, "tiles are whole loads of all waves");
-  static_assert(JK == KS4 || JL * 1024 * NW == JB, "tiles are whole loads of all waves");
+  static_assert(REG || JL * 1024 * NW == JB, "tiles are whole loads of all waves");
   static_assert(JK != KC4 || JL == 2, "KC4: a load in each of two stages");
-  static_assert(JK != KS4 || NT * 16 == 32 * BN, "KS4: half a run of 32 codes per thread");
+  static_assert(!REG || NT * 16 == 32 * BN, "16 codes of a stage per thread");
 };
 
 // per-lane byte offsets of the DMA loads of one operand's stage
@@ -200,7 +209,7 @@ DEV uint32_t mm_hide(uint32_t x) {
 template <int DT, int OP, int W, int BM, int BN, int WM, int WN, bool SHORT = false>
 __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a) {
   using P = MmTraits<DT, OP, W, BM, BN, WM, WN>;
-  constexpr bool HALF = DT == F16, Q4 = P::Q4, PP = P::NW == 8;
+  constexpr bool HALF = DT == F16, Q4 = P::Q4, Q8 = P::Q8, I8 = P::I8, REG = P::REG, PP = P::NW == 8;
   constexpr int CS = P::CS, FI = P::FI, FJ = P::FJ, IK = P::IK, JK = P::JK;
   // (separate arrays: the compiler then knows that a read of one stage need not
   // wait for the loads of another)
@@ -252,9 +261,9 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
     ldb = Q4 ? a.K >> 2 : ldw;
     const int64_t first = OP == LIN_FORWARD ? (t.group * a.N + t.j0) * ldw : t.group * a.N * ldw + t.j0;
     const int64_t count = OP == LIN_FORWARD ? (a.N - t.j0) * ldw : a.N * ldw - t.j0;
-    jp = (const uint8_t*)a.w + (MX ? first >> 1 : first * 2);
-    jbytes = MX ? count >> 1 : count * 2;
-    jstep = OP == LIN_FORWARD ? (P::MX ? 16 : 64) : CS * (MX ? ldw >> 1 : ldw * 2);
+    jp = (const uint8_t*)a.w + (MX ? first >> 1 : I8 ? first : first * 2);
+    jbytes = MX ? count >> 1 : I8 ? count : count * 2;
+    jstep = OP == LIN_FORWARD ? (P::MX ? 16 : I8 ? 32 : 64) : CS * (MX ? ldw >> 1 : I8 ? ldw : ldw * 2);
   }
   // stages [kb, ke) of nk: this workgroup's part where the contraction is split
   const int nk = (int)((len + CS - 1) / CS);
@@ -265,7 +274,7 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
   if (kb < ke) {
     uint32_t io[P::IL], jo[P::JL];
     mm_offsets<IK, BM, P::IL, P::NW>(io, wave, lane, lda);
-    if constexpr (JK != KS4) mm_offsets<JK, BN, P::JL, P::NW>(jo, wave, lane, ldb);
+    if constexpr (!REG) mm_offsets<JK, BN, P::JL, P::NW>(jo, wave, lane, ldb);
     const int nb = (int)(a.K >> 5);
     const uint8_t* sp = P::MX ? a.scale + t.group * a.scale_stride : nullptr;
     // KC4: the scales of four stages, one word per fragment column
@@ -355,13 +364,30 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
     const uint32_t in = left32(il, false), jn = left32(jl, false);
     // KS4: this thread decodes 16 codes of contraction row kr.  (Its loads are
     // issued for every stage, inside the weight or not: the waits count them.)
-    const int kr = tid / (BN / 16), kc = tid % (BN / 16);
-    lm_u32x2 code[2];
+    // KS8 does the same; KC8: 16 codes of column kr.
+    const int kr = JK == KC8 ? tid >> 1 : tid / (BN / 16), kc = JK == KC8 ? tid & 1 : tid % (BN / 16);
+    lm_u32x2 code[JK == KS4 ? 2 : 1];
+    lm_u32x4 code8[REG && JK != KS4 ? 2 : 1];
     uint32_t code_s[2];
-    const uint32_t co = t.j0 + kc * 16 < a.K ? (uint32_t)(kr * (a.K >> 1) + kc * 8) : LIN_OUT;
+    const bool cin = JK == KC8 ? t.j0 + kr < a.N : t.j0 + kc * 16 < a.K;
+    const uint32_t co = !cin ? LIN_OUT : JK == KS4 ? (uint32_t)(kr * (a.K >> 1) + kc * 8) : (uint32_t)(kr * a.ldw + kc * 16);
     const uint32_t cb = (uint32_t)((t.j0 + kc * 16) >> 5);  // block of the row
     const uint32_t cso = a.swizzled ? (cb >> 2) * 512 + (kr & 31) * 16 + (cb & 3) : (uint32_t)(kr * nb) + cb;
     auto load_codes = [&](int st, int set) {
+      if constexpr (JK == KC8 || JK == KS8) {
+        const bool none = st >= ke;
+        const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)jr, 0, left32(jl, none), 0x00027000);
+        jr += jstep;
+        jl -= jstep;
+        code8[set] = __builtin_bit_cast(lm_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, (int)co, 0, 0));
+      }
+      if constexpr (JK == KS8) {  // (rows past N: zeros, as their codes are)
+        const int sz = a.scale16 ? 2 : 4;
+        const int64_t sleft8 = st >= ke ? 0 : (a.N - (int64_t)st * CS) * sz;
+        const __amdgpu_buffer_rsrc_t rs = lin_rsrc(a.scale + (t.group * a.N + (int64_t)st * CS) * sz, sleft8);
+        if (a.scale16) code_s[set] = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rs, kr * 2, 0, 0) << 16;
+        else code_s[set] = __builtin_amdgcn_raw_buffer_load_b32(rs, kr * 4, 0, 0);
+      }
       if constexpr (JK == KS4) {
         const int64_t sbase = a.swizzled ? (int64_t)(st >> 2) * ((nb + 3) >> 2) * 512 + (st & 3) * 4 : (int64_t)st * CS * nb;
         const bool none = st >= ke;
@@ -376,6 +402,14 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
       }
     };
     auto store_codes = [&](lds_u8* tj, int set) {
+      if constexpr (JK == KC8 || JK == KS8) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const lm_u32x4 v = lin_decode8i<HALF, JK == KS8>(code8[set][2 * c], code8[set][2 * c + 1], JK == KS8 ? u2f(code_s[set]) : 1.0f);
+          if constexpr (JK == KC8) *(lds_u32x4*)(tj + kr * 64 + (((kc * 2 + c) ^ mm_key(kr)) << 4)) = v;
+          else *(lds_u32x4*)(tj + kr * (BN * 2) + (((kc * 2 + c) ^ mm_row_key<BN>(kr)) << 4)) = v;
+        }
+      }
       if constexpr (JK == KS4) {
         const float s = lin_e8m0(code_s[set], 0);
 #pragma unroll
@@ -419,7 +453,7 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
         if (lane < 16) lin_dma(rsc, ts + wave * 256, st * 256 + lane * 16);
       }
     };
-    const uint32_t ati = mm_at<IK, BM>(wi * (FI * 16), lane), atj = mm_at<JK == KS4 ? KS16 : JK, BN>(wj * (FJ * 16), lane);
+    const uint32_t ati = mm_at<IK, BM>(wi * (FI * 16), lane), atj = mm_at<P::LK, BN>(wj * (FJ * 16), lane);
     lm_u32x4 fi[FI], fj[FJ];
     constexpr int IW = (FI + 3) / 4, JW = (FJ + 3) / 4;  // words of scales
     uint32_t isc[IW], jsc[JW], jc[JK == KC4 ? FJ : 1];
@@ -428,7 +462,7 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
 #pragma unroll
       for (int f = 0; f < FJ; ++f) {
         if constexpr (JK == KC4) jc[f] = *(const lds_u32*)(tj + (aj ^ ((b & 3) << 4)) + f * 1024);
-        else fj[f] = mm_frag<JK == KC16 ? KC16 : KS16, BN>(tj, aj, f);
+        else fj[f] = mm_frag<P::LK, BN>(tj, aj, f);
       }
 #pragma unroll
       for (int f = 0; f < FI; ++f) fi[f] = mm_frag<IK, BM>(ti, ai, f);
@@ -453,6 +487,7 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
 #pragma unroll
         for (int y = 0; y < FJ; ++y) {
           if constexpr (Q4) acc[x][y] = lin_mfma4(fj[y], fi[x], acc[x][y], jsc[y >> 2], isc[x >> 2], y & 3, x & 3);
+          else if constexpr (Q8) acc[x][y] = lin_mfma8(fj[y], fi[x], acc[x][y]);
           else acc[x][y] = lin_mfma<HALF>(fj[y], fi[x], acc[x][y]);
         }
       // (the products have no side effects: nothing else keeps them from moving
@@ -488,7 +523,7 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
       // first two of every four stages
 #pragma unroll
       for (int b = 0; b < 3; ++b) load(kb + b, kb, b < 2 ? b : -1, ti[b], JK == KC4 ? tj[0] : tj[b], ts[b]);
-      if constexpr (JK == KS4) {
+      if constexpr (REG) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           load_codes(kb + b, 0);
@@ -496,7 +531,7 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
         }
         load_codes(kb + 2, 0);
       }
-      lin_wait<JK == KS4 ? 0 : 2 * L>();  // stage kb is in LDS
+      lin_wait<REG ? 0 : 2 * L>();  // stage kb is in LDS
       lin_barrier();
       if (PP && wave >= 4) lin_barrier();  // the second half runs one barrier behind
       auto four = [&](int st, auto half) {  // stages st .. st + 3; KC4: their codes are in buffer `half`
@@ -577,13 +612,24 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
         bias[y / 2][e] = val_dt<DT>(((const LM_GLOBAL uint16_t*)a.bias)[j + e < jend ? j + e : jend - 1]);
     }
   }
+  // INT8 weights: the columns' scales
+  float cs[I8 || Q8 ? FJ / 2 : 1][8];
+  if constexpr ((I8 || Q8) && OP == LIN_FORWARD) {
+#pragma unroll
+    for (int y = 0; y < FJ; y += 2) {
+      const int64_t j = column(y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) cs[y / 2][e] = t.group < a.experts ? lin_scale8(a, t.group * a.N + (j + e < jend ? j + e : jend - 1)) : 0.0f;
+    }
+  }
   // A row's columns one store after the other: the halves of a 128-byte line reach
   // the L2 together, which otherwise writes many of them to memory by themselves
-  // (dense weight gradient, 134 MB: 165 -> 137 MB written, 2% fewer cycles).  KS4 has no
-  // register left for this order and takes a column's rows.
+  // (dense weight gradient, 134 MB: 165 -> 137 MB written, 2% fewer cycles).  KS4 and KS8
+  // have no register left for this order and take a column's rows.
 #pragma unroll
   for (int n = 0; n < FI * FJ / 2; ++n) {
-    const int x = JK == KS4 ? n % FI : n / (FJ / 2), y = 2 * (JK == KS4 ? n / FI : n % (FJ / 2));
+    constexpr bool DOWN = JK == KS4 || JK == KS8;
+    const int x = DOWN ? n % FI : n / (FJ / 2), y = 2 * (DOWN ? n / FI : n % (FJ / 2));
     const int64_t i = t.r0 + wi * (FI * 16) + x * 16 + (lane & 15), j = column(y);
     // lane groups 0, 2 keep fragment y and get columns 4 .. 7 (12 .. 15) of it
     // from groups 1, 3, which get columns 0 .. 3 (8 .. 11) of fragment y + 1
@@ -593,6 +639,14 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
       const auto r = __builtin_amdgcn_permlane16_swap(f2u(acc[x][y][e]), f2u(acc[x][y + 1][e]), false, false);
       v[e] = u2f(r[0]);
       v[4 + e] = u2f(r[1]);
+    }
+    if constexpr ((I8 || Q8) && OP == LIN_FORWARD) {
+      const float rs = Q8 ? a.row_scale[i < t.r1 && t.group < a.experts ? i : 0] : 1.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = Q8 ? (float)(int)f2u(v[e]) * cs[y / 2][e] * rs : v[e] * cs[y / 2][e];
+        if (t.group >= a.experts) v[e] = 0.0f;  // (rows of no group, whatever row 0 holds)
+      }
     }
     lm_u32x4 w;
 #pragma unroll
@@ -648,10 +702,45 @@ __global__ __launch_bounds__(256) void k_lin_join(LinArgs a, int splits, int64_t
     }
 }
 
+// The same for INT8 weights, whose scales come after the sum: a wave has 256 columns
+// of a row, so its group is the wave's.  Q8: the parts are whole numbers, and so is
+// their sum.
+template <int DT, bool Q8>
+__global__ __launch_bounds__(256) void k_lin_join8(LinArgs a, int splits, uint32_t chunks) {
+  const int64_t item = (int64_t)blockIdx.x * 4 + wave_index(), t = item / chunks;
+  if (t >= a.T) return;
+  const int64_t j0 = (item - t * chunks) * 256 + (threadIdx.x & 63) * 4;
+  int group = 0;
+  int64_t place;
+  if (a.ends) lin_row(a, (int)t, group = a.experts, place);
+  const float rs = Q8 && group < a.experts ? a.row_scale[t] : 1.0f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int64_t j = j0 + e;
+    if (j < a.N) {
+      float v = 0.0f;
+      if (group < a.experts) {
+        const LM_GLOBAL uint32_t* p = (const LM_GLOBAL uint32_t*)a.part + t * a.N + j;
+        if constexpr (Q8) {
+          int sum = 0;
+          for (int k = 0; k < splits; ++k) sum += (int)p[k * a.T * a.N];
+          v = (float)sum;
+        } else {
+          for (int k = 0; k < splits; ++k) v += u2f(p[k * a.T * a.N]);
+        }
+        v *= lin_scale8(a, group * a.N + j);
+        v *= rs;
+        if (a.bias) v += val_dt<DT>(((const LM_GLOBAL uint16_t*)a.bias)[j]);
+      }
+      ((LM_GLOBAL uint16_t*)a.out)[t * a.N + j] = bits_dt<DT>(v);
+    }
+  }
+}
+
 // Rows of any stride and alignment, copied to a stride of whole 16-byte pieces
 // and filled up with zeros.  Bound by memory: 8192 rows of 4096 at a stride of 4097
 // add 21 us to a product (134 MB moved, 6.4 TB/s).
-__global__ __launch_bounds__(256) void k_lin_align(const uint16_t* src, int64_t lds, int64_t rows, int64_t cols, uint16_t* dst,
+static __global__ __launch_bounds__(256) void k_lin_align(const uint16_t* src, int64_t lds, int64_t rows, int64_t cols, uint16_t* dst,
                                                    int64_t ldd) {
   const int64_t pieces = ldd >> 3, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * pieces) return;
