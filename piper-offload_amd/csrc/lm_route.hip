@@ -59,59 +59,50 @@ DEV uint64_t route_max64(uint64_t x) {
   return x;
 }
 
-// The choice in 64 bits.  Lane j returns expert j, or -1.
-template <int P>
-DEV int route_choose64(const RouteArgs& a, const float (&v)[P], const float (&b)[P]) {
+// The choice in 64 bits, for tokens where 32 leave it open.  Lane j returns expert
+// j, or -1.  (Logits from `at` on are read again: the caller's registers stay free.)
+template <int DT, int P>
+__device__ __attribute__((noinline)) int route_choose64(const void* logits, int64_t at, const float* bias, int E, int k, int sigmoid,
+                                                       int groups, int per, int top_groups, int group_best) {
   const int lane = threadIdx.x & 63;
+  float v[P];
   double s[P];
-  route_scores<double, P>(v, a.sigmoid, s);
   uint64_t key[P];
 #pragma unroll
+  for (int i = 0; i < P; ++i) v[i] = lane + 64 * i < E ? route_load<DT>(logits, at + lane + 64 * i) : -INFINITY;
+  route_scores<double, P>(v, sigmoid, s);
+#pragma unroll
   for (int i = 0; i < P; ++i) {
-    s[i] += (double)b[i];
+    if (bias && lane + 64 * i < E) s[i] += (double)bias[lane + 64 * i];
     key[i] = v[i] == -INFINITY || s[i] == -INFINITY ? 0 : route_key64(s[i]);
   }
-  if (a.top_groups < a.groups) {
-    // one group after the other: its best, and its second
+  if (top_groups < groups) {
+    auto number = [](uint64_t k) {
+      return k == ~0ull ? (double)NAN : __longlong_as_double((long long)(k & 0x8000000000000000ull ? k ^ 0x8000000000000000ull : ~k));
+    };
     uint64_t value = 0;  // lane g: of group g
-    for (int g = 0; g < a.groups; ++g) {
+    for (int g = 0; g < groups; ++g) {  // its best, and its second: the best once more if two have it
       uint64_t best = 0, second = 0;
-      double sum = 0.0;
-      for (int n = 0; n < a.group_best; ++n) {
-        uint64_t m = 0;
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        if ((lane + 64 * i) / per == g && key[i] > best) best = key[i];
+      best = route_max64(best);
+      if (best == 0) continue;
+      if (group_best == 2) {
+        int same = 0;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          const int e = lane + 64 * i;
-          const uint64_t k = e >= g * a.per && e < (g + 1) * a.per ? key[i] : 0;
-          m = k > m ? k : m;
+          const bool in = (lane + 64 * i) / per == g;
+          same += __builtin_popcountll(__ballot(in && key[i] == best));
+          if (in && key[i] < best && key[i] > second) second = key[i];
         }
-        m = route_max64(m);
-        if (n == 0) best = m;
-        else {
-          // (the best once more if two members have it, else the best below it)
-          int same = 0;
-          uint64_t below = 0;
-#pragma unroll
-          for (int i = 0; i < P; ++i) {
-            const int e = lane + 64 * i;
-            const uint64_t k = e >= g * a.per && e < (g + 1) * a.per ? key[i] : 0;
-            same += __builtin_popcountll(__ballot(k == best && k != 0));
-            if (k < best && k > below) below = k;
-          }
-          below = route_max64(below);
-          second = same > 1 ? best : below;
-        }
+        second = route_max64(second);
+        if (same > 1) second = best;
       }
-      if (best != 0) {
-        auto number = [](uint64_t k) {
-          return k == ~0ull ? (double)NAN : __longlong_as_double((long long)(k & 0x8000000000000000ull ? k ^ 0x8000000000000000ull : ~k));
-        };
-        sum = number(best) + (second != 0 ? number(second) : 0.0);
-        if (lane == g) value = route_key64(sum);
-      }
+      if (lane == g) value = route_key64(number(best) + (second != 0 ? number(second) : 0.0));
     }
     uint64_t kept = 0;
-    for (int n = 0; n < a.top_groups; ++n) {
+    for (int n = 0; n < top_groups; ++n) {
       const uint64_t m = route_max64(value);
       if (m == 0) break;
       const int g = __builtin_ctzll(__ballot(value == m));
@@ -119,13 +110,11 @@ DEV int route_choose64(const RouteArgs& a, const float (&v)[P], const float (&b)
       if (lane == g) value = 0;
     }
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const int g = (int)((uint32_t)(lane + 64 * i) * a.per_mul >> 20);
-      if (g > 63 || !(kept >> g & 1)) key[i] = 0;
-    }
+    for (int i = 0; i < P; ++i)
+      if (lane + 64 * i < E && !(kept >> ((lane + 64 * i) / per) & 1)) key[i] = 0;
   }
   int mine = -1;
-  for (int j = 0; j < a.k; ++j) {
+  for (int j = 0; j < k; ++j) {
     uint64_t m = key[0];
 #pragma unroll
     for (int i = 1; i < P; ++i) m = key[i] > m ? key[i] : m;
@@ -145,12 +134,123 @@ DEV int route_choose64(const RouteArgs& a, const float (&v)[P], const float (&b)
   return mine;
 }
 
+// Two numbers of 32 bits whose order, as numbers of 64, they leave open: scores are
+// off by at most 2^-20 (exponentials of relative 2^-21, sums of them), a sum of two
+// and two biases by twice that and its own rounding.
+DEV bool route_close(uint32_t larger, uint32_t smaller) {
+  const float x = route_value(larger), d = x - route_value(smaller);
+  return !(d > 0x1p-18f * __builtin_fmaxf(1.0f, __builtin_fabsf(x)));
+}
+
+// The k largest of key (0: none there), the largest first, ties by index.  Lane j
+// returns index j, or -1.  CHECK: open says whether two neighbours are close.
+template <int P, bool CHECK>
+DEV int route_best(uint32_t (&key)[P], int k, bool& open) {
+  const int lane = threadIdx.x & 63;
+  int mine = -1;
+  uint32_t before = 0;
+  for (int j = 0; j < k + (CHECK ? 1 : 0); ++j) {
+    uint32_t m = key[0];
+#pragma unroll
+    for (int i = 1; i < P; ++i) m = umax(m, key[i]);
+    m = route_max(m);
+    if (m == 0) break;
+    if constexpr (CHECK) {
+      if (j > 0 && route_close(before, m)) open = true;
+      if (j == k) break;
+      before = m;
+    }
+    // (the lowest i that has it, and its lowest lane)
+    uint64_t hit = 0;
+    int at = 0;
+#pragma unroll
+    for (int i = P - 1; i >= 0; --i) {
+      const uint64_t h = __ballot(key[i] == m);
+      at = h ? i : at;
+      hit = h ? h : hit;
+    }
+    const int l = __builtin_ctzll(hit);
+#pragma unroll
+    for (int i = 0; i < P; ++i) key[i] = at == i && lane == l ? 0u : key[i];
+    mine = lane == j ? 64 * at + l : mine;
+  }
+  return mine;
+}
+
+// The choice.  Without a bias it follows the logits themselves; with one it is made
+// in 32 bits, and again in 64 where two numbers that decide are close.
 template <int DT, int P>
-__global__ __launch_bounds__(1024) void k_route(RouteArgs a) {
+DEV int route_choose(const RouteArgs& a, int64_t t, const float (&v)[P], const float (&b)[P], bool even, float* lds) {
+  const int lane = threadIdx.x & 63;
+  const bool in_groups = a.top_groups < a.groups, sums = in_groups && a.group_best == 2;
+  float c[P];
+  if (!even || sums) {
+    float s[P];
+    route_scores<float, P>(v, a.sigmoid, s);
+#pragma unroll
+    for (int i = 0; i < P; ++i) c[i] = v[i] == -INFINITY ? -INFINITY : s[i] + b[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; ++i) c[i] = v[i];
+  }
+  uint32_t key[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) key[i] = c[i] == -INFINITY ? 0u : route_key(even ? v[i] : c[i]);
+  bool open = false;
+  if (in_groups) {
+    // a.lanes lanes look at a group, each at every a.lanes-th member; its two best are joined among them
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      if (lane + 64 * i < a.E) lds[lane + 64 * i] = c[i] == c[i] ? c[i] : INFINITY;
+    __builtin_amdgcn_wave_barrier();
+    const int g = lane / a.lanes, part = lane % a.lanes;
+    float one = -INFINITY, two = -INFINITY;
+    if (g < a.groups)
+      for (int m = part; m < a.per; m += a.lanes) {
+        const float y = lds[g * a.per + m];
+        two = __builtin_fmaxf(two, __builtin_fminf(one, y));
+        one = __builtin_fmaxf(one, y);
+      }
+    __builtin_amdgcn_wave_barrier();
+    for (int m = 1; m < a.lanes; m <<= 1) {
+      const float o1 = __shfl_xor(one, m), o2 = __shfl_xor(two, m);
+      two = __builtin_fmaxf(__builtin_fmaxf(two, o2), __builtin_fminf(one, o1));
+      one = __builtin_fmaxf(one, o1);
+    }
+    const float sum = sums && two > -INFINITY ? one + two : one;
+    uint32_t value = part == 0 && one > -INFINITY ? route_key(sum) : 0u;
+    uint64_t kept = 0;
+    uint32_t last = 0;
+    for (int n = 0; n < a.top_groups; ++n) {
+      last = route_max(value);
+      if (last == 0) break;
+      const int l = __builtin_ctzll(__ballot(value == last));
+      kept |= 1ull << l;
+      value = lane == l ? 0u : value;
+    }
+    if ((!even || sums) && last != 0) {
+      const uint32_t next = route_max(value);
+      open = next != 0 && route_close(last, next);
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int of = (int)((uint32_t)(lane + 64 * i) * a.per_mul >> 20) * a.lanes;
+      if (!(kept >> (of & 63) & 1)) key[i] = 0;
+    }
+  }
+  int mine = -1;
+  if (!open) mine = even ? route_best<P, false>(key, a.k, open) : route_best<P, true>(key, a.k, open);
+  if (open) mine = route_choose64<DT, P>(a.logits, t * a.ld, a.bias, a.E, a.k, a.sigmoid, a.groups, a.per, a.top_groups, a.group_best);
+  return mine;
+}
+
+template <int DT, int P>
+__global__ __launch_bounds__(512) void k_route(RouteArgs a) {
   extern __shared__ uint32_t lds[];
   // counts of the experts, then this workgroup's choices and their ranks
   uint32_t* const count = lds;
   uint16_t* const ent = (uint16_t*)(lds + a.E + 1);
+  float* const row = (float*)(lds + a.E + 1 + a.block * a.k) + (threadIdx.x >> 6) * a.E;  // this wave's scores, if there are groups
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), waves = blockDim.x >> 6;
   const int64_t t0 = (int64_t)blockIdx.x * a.block;
   const int tokens = (int)(a.T - t0 < a.block ? a.T - t0 : a.block), n = tokens * a.k;
@@ -158,12 +258,20 @@ __global__ __launch_bounds__(1024) void k_route(RouteArgs a) {
   float b[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) b[i] = a.bias && lane + 64 * i < a.E ? a.bias[lane + 64 * i] : 0.0f;
+  // a bias that is the same for all decides nothing
+  bool even = true;
+  if (a.bias) {
+    const float b0 = u2f((uint32_t)__builtin_amdgcn_readfirstlane((int)f2u(b[0])));
+#pragma unroll
+    for (int i = 0; i < P; ++i) even = even && (lane + 64 * i >= a.E || b[i] == b0);
+    even = __ballot(even) == ~0ull && __builtin_fabsf(b0) < INFINITY;
+  }
   for (int tl = wave; tl < tokens; tl += waves) {
     const int64_t t = t0 + tl;
     float v[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) v[i] = lane + 64 * i < a.E ? route_load<DT>(a.logits, t * a.ld + lane + 64 * i) : -INFINITY;
-    const int mine = route_choose64<P>(a, v, b);
+    const int mine = route_choose<DT, P>(a, t, v, b, even, row);
     // the chosen experts' logits: e^x of softmax, e^min(x, 0) / (1 + e^-|x|) of sigmoid, so that none overflows
     float x = 0.0f;
 #pragma unroll
@@ -539,8 +647,8 @@ extern "C" int lm_route_topk(const lm_route* r, float* weight, int32_t* expert, 
   }
   hipStream_t st = (hipStream_t)stream;
   TimedLaunch timed("route", st);
-  const int threads = a.blocks > 1 ? 256 : 1024;
-  const size_t lds = (size_t)(a.E + 1) * 4 + (size_t)a.block * a.k * 4;
+  const int threads = a.blocks > 1 ? 256 : 512;
+  const size_t lds = (size_t)(a.E + 1) * 4 + (size_t)a.block * a.k * 4 + (a.top_groups < a.groups ? (size_t)threads / 64 * a.E * 4 : 0);
   ROUTE_BY_TYPE(k_route, dim3((unsigned)(a.blocks > 0 ? a.blocks : 1)), dim3(threads), lds, st, a);
   LAUNCH_CHECK();
   if (a.blocks > 1) {
