@@ -357,7 +357,7 @@ typedef struct lm_route {
   float scale;
   int32_t reserved;
 } lm_route;
-size_t lm_route_workspace_size(const lm_route* r);
+size_t lm_route_workspace_size(int64_t T, int32_t experts);
 int lm_route_topk(const lm_route* r, float* weight, int32_t* expert, int32_t* position, int32_t* ends, void* workspace,
                   size_t workspace_bytes, void* stream);
 int lm_route_topk_grad(const lm_route* r, const float* dweight, const int32_t* expert, void* dlogits, void* stream);

@@ -51,12 +51,19 @@ DEV uint64_t route_key64(double x) {
   const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0), k = u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
   return x != x ? ~0ull : k;
 }
+template <int CTRL, int ROWS>
+DEV uint64_t route_max64_step(uint64_t x) {
+  const uint64_t o = (uint64_t)route_dpp<CTRL, ROWS>((uint32_t)(x >> 32)) << 32 | route_dpp<CTRL, ROWS>((uint32_t)x);
+  return o > x ? o : x;
+}
 DEV uint64_t route_max64(uint64_t x) {
-  for (int m = 1; m < 64; m <<= 1) {
-    const uint64_t o = (uint64_t)__shfl_xor((long long)x, m);
-    x = o > x ? o : x;
-  }
-  return x;
+  x = route_max64_step<0x111, 0xf>(x);
+  x = route_max64_step<0x112, 0xf>(x);
+  x = route_max64_step<0x114, 0xf>(x);
+  x = route_max64_step<0x118, 0xf>(x);
+  x = route_max64_step<0x142, 0xa>(x);
+  x = route_max64_step<0x143, 0xc>(x);
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
 
 // The choice in 64 bits, for tokens where 32 leave it open.  Lane j returns expert
@@ -349,24 +356,42 @@ __global__ __launch_bounds__(512) void k_route(RouteArgs a) {
 }
 
 // The choices of the workgroups before each one, per expert: 16 experts a
-// workgroup, 64 threads for each, which take a run of the workgroups.
+// workgroup, 64 threads for each, which take a run of the workgroups, 16 at a time
+// in registers.
 __global__ __launch_bounds__(1024) void k_route_scan(RouteArgs a) {
-  __shared__ uint32_t part[64][16];
-  const int c = threadIdx.x & 15, seg = threadIdx.x >> 4, e = blockIdx.x * 16 + c, cols = a.E + 1;
+  __shared__ uint32_t part[16][65];
+  const int c = threadIdx.x & 15, seg = threadIdx.x >> 4, e = blockIdx.x * 16 + c, cols = a.E + 1, lane = threadIdx.x & 63;
   const int each = (a.blocks + 63) / 64, b0 = seg * each, b1 = b0 + each < a.blocks ? b0 + each : a.blocks;
-  uint32_t sum = 0;
-  if (e < cols)
-    for (int b = b0; b < b1; ++b) sum += a.counts[(int64_t)b * cols + e];
-  part[seg][c] = sum;
+  LM_GLOBAL uint32_t* const at = (LM_GLOBAL uint32_t*)a.counts + e;
+  uint32_t x[16], sum = 0;
+  auto load = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = e < cols && b + i < b1 ? at[(int64_t)(b + i) * cols] : 0u;
+  };
+  for (int b = b0; b < b1; b += 16) {
+    load(b);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += x[i];
+  }
+  part[c][seg] = sum;
   __syncthreads();
-  uint32_t before = 0;
-  for (int s = 0; s < seg; ++s) before += part[s][c];
-  if (e >= cols) return;
-  if (seg == 63) a.counts[(int64_t)a.blocks * cols + e] = before + sum;
-  for (int b = b0; b < b1; ++b) {
-    const uint32_t x = a.counts[(int64_t)b * cols + e];
-    a.counts[(int64_t)b * cols + e] = before;
-    before += x;
+  // (a wave scans an expert's 64 sums)
+  {
+    const int w = threadIdx.x >> 6;
+    const uint32_t y = part[w][lane], z = (uint32_t)lin_scan_add((int)y);
+    part[w][lane] = z - y;
+    if (lane == 63 && blockIdx.x * 16 + w < cols) ((LM_GLOBAL uint32_t*)a.counts)[(int64_t)a.blocks * cols + blockIdx.x * 16 + w] = z;
+  }
+  __syncthreads();
+  uint32_t before = part[c][seg];
+  for (int b = b0; b < b1; b += 16) {
+    if (each > 16) load(b);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (e < cols && b + i < b1) {
+        at[(int64_t)(b + i) * cols] = before;
+        before += x[i];
+      }
   }
 }
 
@@ -507,13 +532,21 @@ __global__ __launch_bounds__(256) void k_rows_back(RowsArgs a, uint32_t chunks) 
   const int64_t c = (item - t * chunks) * 512 + (threadIdx.x & 63) * 8, left = a.N - c;
   const int end = rows_end(a);
   float s[8] = {};
-  for (int j = 0; j < a.k; ++j) {
-    const int p = a.position[t * a.k + j];
-    if (p < 0 || p >= end) continue;
-    const lm_u32x4 w = lin_chunk((const uint16_t*)a.h + p * a.ldh + c, left);
-    const float by = WEIGHTS ? a.weight[t * a.k + j] : 1.0f;
+  for (int j0 = 0; j0 < a.k; j0 += 4) {  // four rows on their way at once
+    lm_u32x4 w[4];
+    float by[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = __builtin_fmaf(by, val_dt<DT>(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu), s[i]);
+    for (int n = 0; n < 4; ++n) {
+      const int j = j0 + n < a.k ? j0 + n : a.k - 1, p = a.position[t * a.k + j];
+      const bool on = j0 + n < a.k && p >= 0 && p < end;
+      by[n] = !on ? 0.0f : WEIGHTS ? a.weight[t * a.k + j] : 1.0f;
+      w[n] = lm_u32x4{};
+      if (on) w[n] = lin_chunk((const uint16_t*)a.h + p * a.ldh + c, left);
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = __builtin_fmaf(by[n], val_dt<DT>(i & 1 ? w[n][i >> 1] >> 16 : w[n][i >> 1] & 0xffffu), s[i]);
   }
   lm_u32x4 w;
 #pragma unroll
@@ -577,6 +610,14 @@ static int check_route(const lm_route* r) {
   return LM_OK;
 }
 
+// Tokens of a workgroup: all of them while they are few, so that one launch does.
+static int route_block(int64_t T) {
+  if (T <= 32) return (int)T;
+  int block = 16;
+  while (block < 64 && (T + block - 1) / block > 1024) block *= 2;
+  return block;
+}
+
 static RouteArgs route_args(const lm_route* r) {
   RouteArgs a{};
   a.logits = r->logits;
@@ -595,13 +636,7 @@ static RouteArgs route_args(const lm_route* r) {
   a.lanes = 64;
   while (a.lanes * a.groups > 64) a.lanes >>= 1;
   a.per_mul = ((1u << 20) + a.per - 1) / a.per;
-  // tokens of a workgroup: all of them while they are few, so that one launch does
-  if (a.T <= 32) {
-    a.block = (int)(a.T > 0 ? a.T : 1);
-  } else {
-    a.block = 16;
-    while (a.block < 64 && (a.T + a.block - 1) / a.block > 1024) a.block *= 2;
-  }
+  a.block = a.T > 0 ? route_block(a.T) : 1;
   a.blocks = (int)((a.T + a.block - 1) / a.block);
   a.entries = fast_div((uint32_t)(a.block * a.k));
   return a;
@@ -622,10 +657,10 @@ static RouteArgs route_args(const lm_route* r) {
     else ROUTE_BY_WIDTH(KERNEL, BF16, __VA_ARGS__);                                       \
   } while (0)
 
-extern "C" size_t lm_route_workspace_size(const lm_route* r) {
-  if (check_route(r)) return 0;
-  const RouteArgs a = route_args(r);
-  return a.blocks > 1 ? align256((size_t)(a.blocks + 1) * (a.E + 1) * 4) : 0;
+extern "C" size_t lm_route_workspace_size(int64_t T, int32_t experts) {
+  if (T <= 0 || T > 0x7fffffff || experts < 1 || experts > LM_LINEAR_MAX_EXPERTS) return 0;
+  const int64_t block = route_block(T), blocks = (T + block - 1) / block;
+  return blocks > 1 ? align256((size_t)(blocks + 1) * (size_t)(experts + 1) * 4) : 0;
 }
 
 extern "C" int lm_route_topk(const lm_route* r, float* weight, int32_t* expert, int32_t* position, int32_t* ends,
@@ -639,7 +674,7 @@ extern "C" int lm_route_topk(const lm_route* r, float* weight, int32_t* expert, 
   a.position = position;
   a.ends = ends;
   if (a.blocks > 1) {
-    const size_t need = align256((size_t)(a.blocks + 1) * (a.E + 1) * 4);
+    const size_t need = lm_route_workspace_size(a.T, a.E);
     if (!workspace || workspace_bytes < need)
       return fail(LM_EWORKSPACE, "workspace too small: %zu < %zu bytes", workspace ? workspace_bytes : 0, need);
     if (((uintptr_t)workspace & 255) != 0) return fail(LM_EINVAL, "workspace must be 256-byte aligned");
@@ -647,7 +682,7 @@ extern "C" int lm_route_topk(const lm_route* r, float* weight, int32_t* expert, 
   }
   hipStream_t st = (hipStream_t)stream;
   TimedLaunch timed("route", st);
-  const int threads = a.blocks > 1 ? 256 : 512;
+  const int threads = 512;
   const size_t lds = (size_t)(a.E + 1) * 4 + (size_t)a.block * a.k * 4 + (a.top_groups < a.groups ? (size_t)threads / 64 * a.E * 4 : 0);
   ROUTE_BY_TYPE(k_route, dim3((unsigned)(a.blocks > 0 ? a.blocks : 1)), dim3(threads), lds, st, a);
   LAUNCH_CHECK();

@@ -122,7 +122,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lm_linear": (_I32, [_P, _I64, _W, _P, _P, _P, _I64, _I32, _I32, _P, _SZ, _P]),
     "lm_linear_input_grad": (_I32, [_P, _I64, _W, _P, _P, _I64, _I32, _P, _SZ, _P]),
     "lm_linear_weight_grad": (_I32, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _P, _SZ, _P]),
-    "lm_route_workspace_size": (_SZ, [_T]),
+    "lm_route_workspace_size": (_SZ, [_I64, _I32]),
     "lm_route_topk": (_I32, [_T, _P, _P, _P, _P, _P, _SZ, _P]),
     "lm_route_topk_grad": (_I32, [_T, _P, _P, _P, _P]),
     "lm_dispatch_rows": (_I32, [_X, _P, _I64, _P, _P]),
@@ -218,6 +218,12 @@ def workspace_size(rows: int, cols: int, rank: int) -> int:
 def linear_workspace_size(*sizes: int) -> int:
     """``lm_linear_workspace_size``, a function of its numbers alone."""
     return load_library().lm_linear_workspace_size(*sizes)
+
+
+@functools.lru_cache(maxsize=4096)
+def route_workspace_size(tokens: int, experts: int) -> int:
+    """``lm_route_workspace_size``, a function of the two numbers alone."""
+    return load_library().lm_route_workspace_size(tokens, experts)
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

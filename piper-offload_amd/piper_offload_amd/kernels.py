@@ -1018,10 +1018,13 @@ def _route(label: str, logits: torch.Tensor, top_k: int, bias: torch.Tensor | No
                          top_k, groups, top_groups, group_best, renormalize, scale, 0), keep
 
 
-def _call(entry: Any, device: torch.device, *args: object) -> None:
-    """Call one C entry without a workspace on the device's current stream."""
-    with L.on_device(device):
-        rc = entry(*args, L.stream_ptr(device))
+def _enqueue(entry: Any, index: int, device: torch.device, *args: object) -> None:
+    """Call one C entry that needs no workspace on GPU ``index``."""
+    if torch._C._cuda_getDevice() != index:
+        with L.on_device(device):
+            _enqueue(entry, index, device, *args)
+        return
+    rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         L.check(rc)
 
@@ -1047,8 +1050,7 @@ def route_topk(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | None = 
     expert = logits.new_empty((t, top_k), dtype=torch.int32)
     position = logits.new_empty((t, top_k), dtype=torch.int32)
     ends = logits.new_empty(e, dtype=torch.int32)
-    handle = L.lib()
-    _launch(handle.lm_route_topk, logits.get_device(), handle.lm_route_workspace_size(r), logits.device, r, weight.data_ptr(),
+    _launch(L.lib().lm_route_topk, logits.get_device(), L.route_workspace_size(t, e), logits.device, r, weight.data_ptr(),
             expert.data_ptr(), position.data_ptr(), ends.data_ptr())
     del keep
     return Routing(weight, expert, position, ends)
@@ -1068,7 +1070,7 @@ def route_topk_grad(dweight: torch.Tensor, logits: torch.Tensor, expert: torch.T
     dlogits = logits.new_empty(logits.shape)
     dweight, expert = dweight.contiguous(), expert.contiguous()
     if logits.shape[0]:
-        _call(L.lib().lm_route_topk_grad, logits.device, r, dweight.data_ptr(), expert.data_ptr(), dlogits.data_ptr())
+        _enqueue(L.lib().lm_route_topk_grad, logits.get_device(), logits.device, r, dweight.data_ptr(), expert.data_ptr(), dlogits.data_ptr())
     del keep
     return dlogits
 
@@ -1112,7 +1114,7 @@ def dispatch_rows(x: torch.Tensor, position: torch.Tensor, ends: torch.Tensor) -
     r, keep = _places(label, position, ends, x.shape[1], x.dtype)
     out = x.new_empty((position.numel(), x.shape[1]))
     if out.shape[0]:
-        _call(L.lib().lm_dispatch_rows, x.device, r, x.data_ptr(), ld, out.data_ptr())
+        _enqueue(L.lib().lm_dispatch_rows, x.get_device(), x.device, r, x.data_ptr(), ld, out.data_ptr())
     del keep
     return out
 
@@ -1125,7 +1127,7 @@ def dispatch_rows_grad(dy: torch.Tensor, position: torch.Tensor, ends: torch.Ten
     r, keep = _places(label, position, ends, dy.shape[1], dy.dtype)
     dx = dy.new_empty((position.shape[0], dy.shape[1]))
     if dx.shape[0]:
-        _call(L.lib().lm_dispatch_rows_grad, dy.device, r, dy.data_ptr(), ld, dx.data_ptr())
+        _enqueue(L.lib().lm_dispatch_rows_grad, dy.get_device(), dy.device, r, dy.data_ptr(), ld, dx.data_ptr())
     del keep
     return dx
 
@@ -1143,7 +1145,7 @@ def combine_rows(h: torch.Tensor, weight: torch.Tensor, position: torch.Tensor, 
     r, keep = _places(label, position, ends, h.shape[1], h.dtype)
     out = h.new_empty((position.shape[0], h.shape[1]))
     if out.shape[0]:
-        _call(L.lib().lm_combine_rows, h.device, r, h.data_ptr(), ld, weight.data_ptr(), out.data_ptr())
+        _enqueue(L.lib().lm_combine_rows, h.get_device(), h.device, r, h.data_ptr(), ld, weight.data_ptr(), out.data_ptr())
     del keep
     return out
 
@@ -1161,7 +1163,7 @@ def combine_rows_grad(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, p
     r, keep = _places(label, position, ends, h.shape[1], h.dtype)
     dh, dweight = h.new_empty(h.shape), weight.new_empty(weight.shape)
     if position.shape[0]:
-        _call(L.lib().lm_combine_rows_grad, h.device, r, dy.data_ptr(), ldy, h.data_ptr(), ldh, weight.data_ptr(), dh.data_ptr(),
+        _enqueue(L.lib().lm_combine_rows_grad, h.get_device(), h.device, r, dy.data_ptr(), ldy, h.data_ptr(), ldh, weight.data_ptr(), dh.data_ptr(),
               dweight.data_ptr())
     del keep
     return dh, dweight
