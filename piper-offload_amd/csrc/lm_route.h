@@ -2,6 +2,10 @@
 #pragma once
 #include "lm_linear.h"
 
+// Up to this many tokens k_route_place adds up the counts by itself: every workgroup
+// reads those of all.  (16384 tokens, 256 experts: TODO)
+constexpr int64_t ROUTE_NEAR = 32768;
+
 struct RouteArgs {
   const void* logits;  // [T, ld]
   int64_t ld;
@@ -18,7 +22,10 @@ struct RouteArgs {
   int32_t* position;   // [T, k]
   int32_t* ends;       // [E]
   int block, blocks;   // tokens of a workgroup, workgroups
-  uint32_t* counts;    // [blocks + 1, E + 1]: choices of a workgroup per expert; the last row has all of them
+  int pitch;           // E in whole words of bytes (and of a wave's scores)
+  uint8_t* counts;     // [blocks, pitch]: choices of a workgroup per expert, at most its tokens
+  uint32_t* none;      // [blocks]: those without an expert
+  uint32_t* starts;    // [blocks + 1, E + 1], more than ROUTE_NEAR tokens: those of the workgroups before; the last row has all
   FastDiv entries;     // choices of a workgroup
 };
 

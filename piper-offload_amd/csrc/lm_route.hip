@@ -18,12 +18,24 @@ DEV float route_load(const void* p, int64_t i) {
   else return val_dt<DT>(((const LM_GLOBAL uint16_t*)p)[i]);
 }
 
+// e^x.  Rough: v_exp_f32 of x log2(e), off by 2^-22 of it and x 2^-23 more.
+template <typename F, bool ROUGH>
+DEV F route_exp(F x) {
+  if constexpr (sizeof(F) == 8) return exp(x);
+  else if constexpr (ROUGH) return __builtin_amdgcn_exp2f(x * 1.44269504f);
+  else return expf(x);
+}
+
 // The scores of a token: lane l has experts l, l + 64, ...; those there are not have logit -inf.
-template <typename F, int P>
+template <typename F, bool ROUGH, int P>
 DEV void route_scores(const float (&v)[P], bool sigmoid, F (&s)[P]) {
   if (sigmoid) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) s[i] = F(1) / (F(1) + (sizeof(F) == 8 ? (F)exp(-(double)v[i]) : (F)expf(-v[i])));
+    for (int i = 0; i < P; ++i) {
+      const F d = F(1) + route_exp<F, ROUGH>(-(F)v[i]);
+      if constexpr (ROUGH) s[i] = __builtin_amdgcn_rcpf(d);
+      else s[i] = F(1) / d;
+    }
     return;
   }
   float top = v[0];
@@ -33,8 +45,7 @@ DEV void route_scores(const float (&v)[P], bool sigmoid, F (&s)[P]) {
   F sum = 0;
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    const F d = (F)v[i] - (F)top;
-    s[i] = v[i] == -INFINITY ? F(0) : (sizeof(F) == 8 ? (F)exp((double)d) : (F)expf((float)d));
+    s[i] = v[i] == -INFINITY ? F(0) : route_exp<F, ROUGH>((F)v[i] - (F)top);
     sum += s[i];
   }
   if constexpr (sizeof(F) == 8) {
@@ -66,21 +77,17 @@ DEV uint64_t route_max64(uint64_t x) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
 
-// The choice in 64 bits, for tokens where 32 leave it open.  Lane j returns expert
-// j, or -1.  (Logits from `at` on are read again: the caller's registers stay free.)
-template <int DT, int P>
-__device__ __attribute__((noinline)) int route_choose64(const void* logits, int64_t at, const float* bias, int E, int k, int sigmoid,
-                                                       int groups, int per, int top_groups, int group_best) {
+// The choice in 64 bits.  Lane j returns expert j, or -1.
+template <int P>
+DEV int route_choose64(const float (&v)[P], const float (&b)[P], bool even, int E, int k, int sigmoid, int groups, int per, int top_groups,
+                       int group_best) {
   const int lane = threadIdx.x & 63;
-  float v[P];
   double s[P];
   uint64_t key[P];
-#pragma unroll
-  for (int i = 0; i < P; ++i) v[i] = lane + 64 * i < E ? route_load<DT>(logits, at + lane + 64 * i) : -INFINITY;
-  route_scores<double, P>(v, sigmoid, s);
+  route_scores<double, false, P>(v, sigmoid, s);
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    if (bias && lane + 64 * i < E) s[i] += (double)bias[lane + 64 * i];
+    s[i] += (double)b[i];
     key[i] = v[i] == -INFINITY || s[i] == -INFINITY ? 0 : route_key64(s[i]);
   }
   if (top_groups < groups) {
@@ -120,6 +127,11 @@ __device__ __attribute__((noinline)) int route_choose64(const void* logits, int6
     for (int i = 0; i < P; ++i)
       if (lane + 64 * i < E && !(kept >> ((lane + 64 * i) / per) & 1)) key[i] = 0;
   }
+  if (even) {
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      if (key[i] != 0) key[i] = route_key64((double)v[i]);
+  }
   int mine = -1;
   for (int j = 0; j < k; ++j) {
     uint64_t m = key[0];
@@ -141,59 +153,109 @@ __device__ __attribute__((noinline)) int route_choose64(const void* logits, int6
   return mine;
 }
 
-// Two numbers of 32 bits whose order, as numbers of 64, they leave open: scores are
-// off by at most 2^-20 (exponentials of relative 2^-21, sums of them), a sum of two
-// and two biases by twice that and its own rounding.
+// Two numbers of 32 bits whose order, as numbers of 64, they leave open.  A sigmoid
+// is off by 2^-22 (its exponential's error counts a quarter at most, the sum, the
+// reciprocal and the bias come to it), the scores of a softmax, which add up to 1,
+// by 2^-20 all together; a sum of two scores and two biases by twice that and its
+// own rounding.
 DEV bool route_close(uint32_t larger, uint32_t smaller) {
   const float x = route_value(larger), d = x - route_value(smaller);
   return !(d > 0x1p-18f * __builtin_fmaxf(1.0f, __builtin_fabsf(x)));
 }
 
 // The k largest of key (0: none there), the largest first, ties by index.  Lane j
-// returns index j, or -1.  CHECK: open says whether two neighbours are close.
-template <int P, bool CHECK>
-DEV int route_best(uint32_t (&key)[P], int k, bool& open) {
-  const int lane = threadIdx.x & 63;
+// returns index j, or -1.  MORE: and those after them, up to the first that is not
+// close to the one before; n of them, lane j has the key too; n = 65 if 64 do not end.
+template <int P, bool MORE>
+DEV int route_best(uint32_t (&key)[P], int k, uint32_t& has, int& n) {
   int mine = -1;
   uint32_t before = 0;
-  for (int j = 0; j < k + (CHECK ? 1 : 0); ++j) {
+  has = 0;
+  for (n = 0; MORE || n < k; ++n) {
     uint32_t m = key[0];
 #pragma unroll
     for (int i = 1; i < P; ++i) m = umax(m, key[i]);
     m = route_max(m);
     if (m == 0) break;
-    if constexpr (CHECK) {
-      if (j > 0 && route_close(before, m)) open = true;
-      if (j == k) break;
+    if constexpr (MORE) {
+      if (n >= k && !route_close(before, m)) break;
+      if (n == 64) {
+        n = 65;
+        break;
+      }
       before = m;
     }
     // (the lowest i that has it, and its lowest lane)
-    uint64_t hit = 0;
-    int at = 0;
+    uint64_t hit = __ballot(key[P - 1] == m);
+    int at = P - 1;
 #pragma unroll
-    for (int i = P - 1; i >= 0; --i) {
+    for (int i = P - 2; i >= 0; --i) {
       const uint64_t h = __ballot(key[i] == m);
       at = h ? i : at;
       hit = h ? h : hit;
     }
     const int l = __builtin_ctzll(hit);
+    const uint64_t one = 1ull << l, me = 1ull << n;
 #pragma unroll
-    for (int i = 0; i < P; ++i) key[i] = at == i && lane == l ? 0u : key[i];
-    mine = lane == j ? 64 * at + l : mine;
+    for (int i = 0; i < P; ++i) key[i] = __builtin_amdgcn_inverse_ballot_w64(at == i ? one : 0ull) ? 0u : key[i];
+    mine = __builtin_amdgcn_inverse_ballot_w64(me) ? 64 * at + l : mine;
+    if constexpr (MORE) has = __builtin_amdgcn_inverse_ballot_w64(me) ? m : has;
   }
   return mine;
 }
 
-// The choice.  Without a bias it follows the logits themselves; with one it is made
-// in 32 bits, and again in 64 where two numbers that decide are close.
+// The first n experts in the order of 64 bits: lane j has one, and gets the one of place j.
 template <int DT, int P>
-DEV int route_choose(const RouteArgs& a, int64_t t, const float (&v)[P], const float (&b)[P], bool even, float* lds) {
+DEV int route_settle(const RouteArgs& a, int64_t t, const float (&v)[P], int mine, int n) {
+  const int lane = threadIdx.x & 63;
+  const bool on = lane < n;
+  const double x = on ? (double)route_load<DT>(a.logits, t * a.ld + mine) : 0.0;
+  double c;
+  if (a.sigmoid) {
+    c = 1.0 / (1.0 + exp(-x));
+  } else {
+    float top = v[0];
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 1; i < P; ++i) top = __builtin_fmaxf(top, v[i]);
+    top = route_fmax(top);
+#pragma unroll
+    for (int i = 0; i < P; ++i) sum += v[i] == -INFINITY ? 0.0 : exp((double)v[i] - (double)top);
+    for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
+    c = exp(x - (double)top) * (1.0 / sum);
+  }
+  if (a.bias && on) c += (double)a.bias[mine];
+  const uint64_t key = route_key64(c);
+  int place = 0;
+  for (int i = 0; i < n; ++i) {
+    const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)key, i);
+    const int e = __builtin_amdgcn_readlane(mine, i);
+    place += o > key || (o == key && e < mine);
+  }
+  return __builtin_amdgcn_ds_permute((on ? place : lane) * 4, mine);
+}
+
+// best and second best of a group, joined with those of the lanes that CTRL reads
+template <int CTRL>
+DEV void route_two(float& one, float& two) {
+  const float o1 = u2f(route_dpp<CTRL, 0xf>(f2u(one))), o2 = u2f(route_dpp<CTRL, 0xf>(f2u(two)));
+  two = __builtin_fmaxf(__builtin_fmaxf(two, o2), __builtin_fminf(one, o1));
+  one = __builtin_fmaxf(one, o1);
+}
+
+// The choice.  Without a bias it follows the logits themselves; with one it is made
+// in 32 bits, and where numbers that decide are close (`open`), in 64: among the chosen
+// and those next to them, or, where groups are close, all of it.  That is what LATE
+// does, and does it apart from the rest: with its registers the kernel runs 5 waves a
+// SIMD instead of 8, and one token in 300 needs it.
+template <int DT, int P, bool LATE>
+DEV int route_choose(const RouteArgs& a, int64_t t, const float (&v)[P], const float (&b)[P], bool even, float* lds, bool& open) {
   const int lane = threadIdx.x & 63;
   const bool in_groups = a.top_groups < a.groups, sums = in_groups && a.group_best == 2;
   float c[P];
   if (!even || sums) {
     float s[P];
-    route_scores<float, P>(v, a.sigmoid, s);
+    route_scores<float, true, P>(v, a.sigmoid, s);
 #pragma unroll
     for (int i = 0; i < P; ++i) c[i] = v[i] == -INFINITY ? -INFINITY : s[i] + b[i];
   } else {
@@ -203,23 +265,36 @@ DEV int route_choose(const RouteArgs& a, int64_t t, const float (&v)[P], const f
   uint32_t key[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) key[i] = c[i] == -INFINITY ? 0u : route_key(even ? v[i] : c[i]);
-  bool open = false;
+  open = false;
   if (in_groups) {
-    // a.lanes lanes look at a group, each at every a.lanes-th member; its two best are joined among them
+    // a.lanes lanes look at a group, each at a part of its members; its two best are joined among them
 #pragma unroll
     for (int i = 0; i < P; ++i)
       if (lane + 64 * i < a.E) lds[lane + 64 * i] = c[i] == c[i] ? c[i] : INFINITY;
     __builtin_amdgcn_wave_barrier();
-    const int g = lane / a.lanes, part = lane % a.lanes;
+    const int g = lane / a.lanes, part = lane & (a.lanes - 1);
     float one = -INFINITY, two = -INFINITY;
-    if (g < a.groups)
-      for (int m = part; m < a.per; m += a.lanes) {
-        const float y = lds[g * a.per + m];
-        two = __builtin_fmaxf(two, __builtin_fminf(one, y));
-        one = __builtin_fmaxf(one, y);
+    auto take = [&](float y) {
+      two = __builtin_fmaxf(two, __builtin_fminf(one, y));
+      one = __builtin_fmaxf(one, y);
+    };
+    if (g < a.groups) {
+      if (a.per % 4 == 0) {
+        for (int m = part * 4; m < a.per; m += a.lanes * 4) {
+          const v4f32 y = *(const v4f32*)(lds + g * a.per + m);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) take(y[i]);
+        }
+      } else {
+        for (int m = part; m < a.per; m += a.lanes) take(lds[g * a.per + m]);
       }
+    }
     __builtin_amdgcn_wave_barrier();
-    for (int m = 1; m < a.lanes; m <<= 1) {
+    if (a.lanes > 1) route_two<0xB1>(one, two);   // lane xor 1
+    if (a.lanes > 2) route_two<0x4E>(one, two);   // lane xor 2
+    if (a.lanes > 4) route_two<0x141>(one, two);  // 7 - lane, of 8 lanes
+    if (a.lanes > 8) route_two<0x140>(one, two);  // 15 - lane, of 16
+    for (int m = 16; m < a.lanes; m <<= 1) {
       const float o1 = __shfl_xor(one, m), o2 = __shfl_xor(two, m);
       two = __builtin_fmaxf(__builtin_fmaxf(two, o2), __builtin_fminf(one, o1));
       one = __builtin_fmaxf(one, o1);
@@ -231,9 +306,9 @@ DEV int route_choose(const RouteArgs& a, int64_t t, const float (&v)[P], const f
     for (int n = 0; n < a.top_groups; ++n) {
       last = route_max(value);
       if (last == 0) break;
-      const int l = __builtin_ctzll(__ballot(value == last));
-      kept |= 1ull << l;
-      value = lane == l ? 0u : value;
+      const uint64_t l = __ballot(value == last), first = l & (0 - l);
+      kept |= first;
+      value = __builtin_amdgcn_inverse_ballot_w64(first) ? 0u : value;
     }
     if ((!even || sums) && last != 0) {
       const uint32_t next = route_max(value);
@@ -245,100 +320,141 @@ DEV int route_choose(const RouteArgs& a, int64_t t, const float (&v)[P], const f
       if (!(kept >> (of & 63) & 1)) key[i] = 0;
     }
   }
-  int mine = -1;
-  if (!open) mine = even ? route_best<P, false>(key, a.k, open) : route_best<P, true>(key, a.k, open);
-  if (open) mine = route_choose64<DT, P>(a.logits, t * a.ld, a.bias, a.E, a.k, a.sigmoid, a.groups, a.per, a.top_groups, a.group_best);
-  return mine;
+  uint32_t has;
+  int n, mine = -1;
+  if (!open && even) return route_best<P, false>(key, a.k, has, n);
+  bool close = false;
+  if (!open) {
+    mine = route_best<P, true>(key, a.k, has, n);
+    const uint32_t before = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)has, 0x138, 0xf, 0xf, false);  // of the lane below
+    open = n > 64;
+    close = __ballot(lane > 0 && lane < n && route_close(before, has)) != 0;
+  }
+  if constexpr (LATE) {
+    if (open) mine = route_choose64<P>(v, b, even, a.E, a.k, a.sigmoid, a.groups, a.per, a.top_groups, a.group_best);
+    else if (close) mine = route_settle<DT, P>(a, t, v, mine, n);
+  }
+  open = open || close;
+  return lane < a.k ? mine : -1;
 }
 
-template <int DT, int P>
-__global__ __launch_bounds__(512) void k_route(RouteArgs a) {
-  extern __shared__ uint32_t lds[];
-  // counts of the experts, then this workgroup's choices and their ranks
-  uint32_t* const count = lds;
-  uint16_t* const ent = (uint16_t*)(lds + a.E + 1);
-  float* const row = (float*)(lds + a.E + 1 + a.block * a.k) + (threadIdx.x >> 6) * a.E;  // this wave's scores, if there are groups
-  const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), waves = blockDim.x >> 6;
-  const int64_t t0 = (int64_t)blockIdx.x * a.block;
-  const int tokens = (int)(a.T - t0 < a.block ? a.T - t0 : a.block), n = tokens * a.k;
-  for (int i = tid; i <= a.E; i += blockDim.x) count[i] = 0;
-  float b[P];
+// One token: its choice, weights, and in ent its choice once more (E: none).  False,
+// and nothing done, where the choice is left to LATE.
+template <int DT, int P, bool LATE>
+DEV bool route_token(const RouteArgs& a, int64_t t, const float (&b)[P], bool even, float* row, uint16_t* ent) {
+  const int lane = threadIdx.x & 63;
+  float v[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) v[i] = lane + 64 * i < a.E ? route_load<DT>(a.logits, t * a.ld + lane + 64 * i) : -INFINITY;
+  bool open;
+  const int mine = route_choose<DT, P, LATE>(a, t, v, b, even, row, open);
+  if (!LATE && open) return false;
+  // the chosen experts' logits: e^x of softmax, e^min(x, 0) / (1 + e^-|x|) of sigmoid, so that none overflows
+  const bool on = mine >= 0;
+  const float x = on ? route_load<DT>(a.logits, t * a.ld + mine) : 0.0f;
+  const float e = a.sigmoid ? (x < 0.0f ? x : 0.0f) : x, q = a.sigmoid ? 1.0f / (1.0f + expf(-__builtin_fabsf(x))) : 1.0f;
+  float w;
+  if (a.renormalize) {
+    const float top = route_fmax(on ? e : -INFINITY), r = on ? expf(e - top) * q : 0.0f;
+    w = a.scale * (r / route_sum(r));
+  } else if (a.sigmoid) {
+    w = a.scale * (expf(e) * q);
+  } else {
+    float top = v[0], z = 0.0f;
+#pragma unroll
+    for (int i = 1; i < P; ++i) top = __builtin_fmaxf(top, v[i]);
+    top = route_fmax(top);
+#pragma unroll
+    for (int i = 0; i < P; ++i) z += v[i] == -INFINITY ? 0.0f : expf(v[i] - top);
+    w = a.scale * (expf(x - top) / route_sum(z));
+  }
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < P; ++i) bad = bad || v[i] != v[i] || (!a.sigmoid && v[i] == INFINITY);
+  if (__ballot(bad)) w = NAN;
+  if (lane < a.k) {
+    a.weight[t * a.k + lane] = on ? w : 0.0f;
+    a.expert[t * a.k + lane] = mine;
+    ent[lane] = (uint16_t)(on ? mine : a.E);
+  }
+  return true;
+}
+// The lane's biases; true if they decide nothing: none, or the same for all.
+template <int P>
+DEV bool route_bias(const RouteArgs& a, float (&b)[P]) {
+  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int i = 0; i < P; ++i) b[i] = a.bias && lane + 64 * i < a.E ? a.bias[lane + 64 * i] : 0.0f;
-  // a bias that is the same for all decides nothing
+  const float b0 = u2f((uint32_t)__builtin_amdgcn_readfirstlane((int)f2u(b[0])));
   bool even = true;
-  if (a.bias) {
-    const float b0 = u2f((uint32_t)__builtin_amdgcn_readfirstlane((int)f2u(b[0])));
 #pragma unroll
-    for (int i = 0; i < P; ++i) even = even && (lane + 64 * i >= a.E || b[i] == b0);
-    even = __ballot(even) == ~0ull && __builtin_fabsf(b0) < INFINITY;
-  }
-  for (int tl = wave; tl < tokens; tl += waves) {
-    const int64_t t = t0 + tl;
-    float v[P];
-#pragma unroll
-    for (int i = 0; i < P; ++i) v[i] = lane + 64 * i < a.E ? route_load<DT>(a.logits, t * a.ld + lane + 64 * i) : -INFINITY;
-    const int mine = route_choose<DT, P>(a, t, v, b, even, row);
-    // the chosen experts' logits: e^x of softmax, e^min(x, 0) / (1 + e^-|x|) of sigmoid, so that none overflows
-    float x = 0.0f;
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const float o = __shfl(v[i], mine & 63);
-      if (mine >> 6 == i) x = o;
-    }
-    const bool on = mine >= 0;
-    const float e = a.sigmoid ? (x < 0.0f ? x : 0.0f) : x, q = a.sigmoid ? 1.0f / (1.0f + expf(-__builtin_fabsf(x))) : 1.0f;
-    float w;
-    if (a.renormalize) {
-      const float top = route_fmax(on ? e : -INFINITY), r = on ? expf(e - top) * q : 0.0f;
-      w = a.scale * (r / route_sum(r));
-    } else if (a.sigmoid) {
-      w = a.scale * (expf(e) * q);
-    } else {
-      float top = v[0], z = 0.0f;
-#pragma unroll
-      for (int i = 1; i < P; ++i) top = __builtin_fmaxf(top, v[i]);
-      top = route_fmax(top);
-#pragma unroll
-      for (int i = 0; i < P; ++i) z += v[i] == -INFINITY ? 0.0f : expf(v[i] - top);
-      w = a.scale * (expf(x - top) / route_sum(z));
-    }
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < P; ++i) bad = bad || v[i] != v[i] || (!a.sigmoid && v[i] == INFINITY);
-    if (__ballot(bad)) w = NAN;
-    if (lane < a.k) {
-      a.weight[t * a.k + lane] = on ? w : 0.0f;
-      a.expert[t * a.k + lane] = mine;
-      ent[tl * a.k + lane] = (uint16_t)(on ? mine : a.E);
-    }
+  for (int i = 0; i < P; ++i) even = even && (lane + 64 * i >= a.E || b[i] == b0);
+  return __ballot(even) == ~0ull && __builtin_fabsf(b0) < INFINITY;
+}
+// A call, so that its registers are not the loop's.
+template <int DT, int P>
+__device__ __attribute__((noinline)) void route_late(const RouteArgs* a, int64_t t, float* row, uint16_t* ent) {
+  float b[P];
+  const bool even = route_bias<P>(*a, b);
+  route_token<DT, P, true>(*a, t, b, even, row, ent);
+}
+
+// A workgroup has a.block tokens, a wave one of them at a time.  Ranks of its choices
+// among those of the same expert go to a.position, the numbers of its choices to
+// a.counts and a.none: k_route_place makes places of them.  One workgroup alone has
+// everything itself.
+template <int P>
+constexpr int ROUTE_THREADS = P <= 4 ? 1024 : 512;  // (registers)
+template <int DT, int P>
+__global__ __launch_bounds__(ROUTE_THREADS<P>, P <= 4 ? 8 : P <= 8 ? 4 : 2) void k_route(RouteArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_index();
+  constexpr int threads = ROUTE_THREADS<P>, waves = threads / 64;
+  // this wave's scores, if there are groups; counts of the experts; this workgroup's choices and their ranks
+  float* const row = (float*)lds + wave * a.pitch;
+  uint32_t* const count = lds + (a.top_groups < a.groups ? waves * a.pitch : 0);
+  uint16_t* const ent = (uint16_t*)(count + a.E + 1);
+  uint16_t* const rank = ent + a.block * a.k;
+  const int64_t t0 = (int64_t)blockIdx.x * a.block;
+  const int tokens = (int)(a.T - t0 < a.block ? a.T - t0 : a.block), n = tokens * a.k;
+  for (int i = tid; i <= a.E; i += threads) count[i] = 0;
+  float b[P];
+  const bool even = route_bias<P>(a, b);
+  uint32_t left = 0;  // of this wave's tokens, at most 8
+  for (int i = 0, tl = wave; tl < tokens; ++i, tl += waves)
+    if (!route_token<DT, P, false>(a, t0 + tl, b, even, row, ent + tl * a.k)) left |= 1u << i;
+  const RouteArgs* const args = (const RouteArgs*)__builtin_amdgcn_kernarg_segment_ptr();  // (the kernel's one argument)
+  for (; left; left &= left - 1) {
+    const int tl = wave + __builtin_ctz(left) * waves;
+    route_late<DT, P>(args, t0 + tl, row, ent + tl * a.k);
   }
   __syncthreads();
-  // ranks among the choices of one expert, 64 choices at a time, in order
-  uint16_t* const rank = ent + a.block * a.k;
-  if (wave == 0) {
-    for (int i0 = 0; i0 < n; i0 += 64) {
-      const bool in = i0 + lane < n;
-      const uint32_t e = in ? ent[i0 + lane] : 0u;
-      uint64_t same = __ballot(in);
-      for (int bit = 0; bit < 11; ++bit) {
-        const bool one = e >> bit & 1;
-        const uint64_t with = __ballot(one);
-        same &= one ? with : ~with;
-      }
-      if (in) {
-        const uint32_t before = count[e];
-        rank[i0 + lane] = (uint16_t)(before + __builtin_popcountll(same & ((1ull << lane) - 1)));
+  // ranks among the choices of one expert, 64 choices a wave, one wave after the other
+  const int bits = 32 - __builtin_clz(a.E), chunks = (n + 63) >> 6;
+  for (int c0 = 0; c0 < chunks; c0 += waves) {
+    const int i = (c0 + wave) * 64 + lane;
+    const bool in = i < n;
+    const uint32_t e = in ? ent[i] : 0u;
+    uint64_t same = __ballot(in);
+    for (int bit = 0; bit < bits; ++bit) {
+      const bool one = e >> bit & 1;
+      const uint64_t with = __ballot(one);
+      same &= one ? with : ~with;
+    }
+    for (int w = 0; w < waves && c0 + w < chunks; ++w) {
+      if (w == wave && in) {
+        const uint32_t before = count[e], to = before + __builtin_popcountll(same & ((1ull << lane) - 1));
+        if (a.blocks > 1) a.position[t0 * a.k + i] = (int32_t)to;
+        else rank[i] = (uint16_t)to;
         __builtin_amdgcn_wave_barrier();
         if (same >> lane == 1) count[e] = before + __builtin_popcountll(same);
       }
-      __builtin_amdgcn_wave_barrier();
+      __syncthreads();
     }
   }
-  __syncthreads();
-  if (a.blocks > 1) {
-    for (int i = tid; i <= a.E; i += blockDim.x) a.counts[(int64_t)blockIdx.x * (a.E + 1) + i] = count[i];
-    for (int i = tid; i < n; i += blockDim.x) a.position[t0 * a.k + i] = rank[i];
+  if (a.blocks > 1) {  // (an expert has at most one choice of a token)
+    for (int i = tid; i < a.pitch; i += threads) a.counts[(int64_t)blockIdx.x * a.pitch + i] = i < a.E ? (uint8_t)count[i] : (uint8_t)0;
+    if (tid == 0) a.none[blockIdx.x] = count[a.E];
     return;
   }
   if (wave == 0) {
@@ -352,21 +468,24 @@ __global__ __launch_bounds__(512) void k_route(RouteArgs a) {
     }
   }
   __syncthreads();
-  for (int i = tid; i < n; i += blockDim.x) a.position[i] = (int32_t)(count[ent[i]] + rank[i]);
+  for (int i = tid; i < n; i += threads) a.position[i] = (int32_t)(count[ent[i]] + rank[i]);
 }
 
-// The choices of the workgroups before each one, per expert: 16 experts a
-// workgroup, 64 threads for each, which take a run of the workgroups, 16 at a time
-// in registers.
+// Many workgroups: the choices of those before each, per expert (and without one).
+// 16 experts a workgroup, 64 threads for each, which take a run of the workgroups,
+// 16 at a time in registers.
 __global__ __launch_bounds__(1024) void k_route_scan(RouteArgs a) {
   __shared__ uint32_t part[16][65];
   const int c = threadIdx.x & 15, seg = threadIdx.x >> 4, e = blockIdx.x * 16 + c, cols = a.E + 1, lane = threadIdx.x & 63;
   const int each = (a.blocks + 63) / 64, b0 = seg * each, b1 = b0 + each < a.blocks ? b0 + each : a.blocks;
-  LM_GLOBAL uint32_t* const at = (LM_GLOBAL uint32_t*)a.counts + e;
   uint32_t x[16], sum = 0;
   auto load = [&](int b) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = e < cols && b + i < b1 ? at[(int64_t)(b + i) * cols] : 0u;
+    for (int i = 0; i < 16; ++i) {
+      const bool in = b + i < b1;
+      x[i] = in && e < a.E ? ((const LM_GLOBAL uint8_t*)a.counts)[(int64_t)(b + i) * a.pitch + e]
+             : in && e == a.E ? ((const LM_GLOBAL uint32_t*)a.none)[b + i] : 0u;
+    }
   };
   for (int b = b0; b < b1; b += 16) {
     load(b);
@@ -380,7 +499,7 @@ __global__ __launch_bounds__(1024) void k_route_scan(RouteArgs a) {
     const int w = threadIdx.x >> 6;
     const uint32_t y = part[w][lane], z = (uint32_t)lin_scan_add((int)y);
     part[w][lane] = z - y;
-    if (lane == 63 && blockIdx.x * 16 + w < cols) ((LM_GLOBAL uint32_t*)a.counts)[(int64_t)a.blocks * cols + blockIdx.x * 16 + w] = z;
+    if (lane == 63 && blockIdx.x * 16 + w < cols) ((LM_GLOBAL uint32_t*)a.starts)[(int64_t)a.blocks * cols + blockIdx.x * 16 + w] = z;
   }
   __syncthreads();
   uint32_t before = part[c][seg];
@@ -389,26 +508,29 @@ __global__ __launch_bounds__(1024) void k_route_scan(RouteArgs a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       if (e < cols && b + i < b1) {
-        at[(int64_t)(b + i) * cols] = before;
+        ((LM_GLOBAL uint32_t*)a.starts)[(int64_t)(b + i) * cols + e] = before;
         before += x[i];
       }
   }
 }
 
-__global__ __launch_bounds__(256) void k_route_place(RouteArgs a, int64_t n) {
-  extern __shared__ uint32_t first[];  // choices of the experts before each
-  const int lane = threadIdx.x & 63, cols = a.E + 1;
-  const uint32_t* total = a.counts + (int64_t)a.blocks * cols;
-  if (threadIdx.x < 64) {
-    uint32_t before = 0;
-    for (int c = 0; c < cols; c += 64) {
-      const int e = c + lane;
-      const uint32_t x = e < cols ? total[e] : 0, sum = (uint32_t)lin_scan_add((int)x);
-      if (e < cols) first[e] = before + sum - x;
-      if (e < a.E && blockIdx.x == 0) a.ends[e] = (int32_t)(before + sum);
-      before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
-    }
+// exclusive sums over the experts, by one wave; their ends
+DEV void route_first(const uint32_t* total, uint32_t* first, int E, int32_t* ends) {
+  const int lane = threadIdx.x & 63;
+  uint32_t before = 0;
+  for (int c = 0; c <= E; c += 64) {
+    const int e = c + lane;
+    const uint32_t x = e < E ? total[e] : 0, sum = (uint32_t)lin_scan_add((int)x);
+    if (e <= E) first[e] = before + sum - x;
+    if (e < E && ends) ends[e] = (int32_t)(before + sum);
+    before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
   }
+}
+
+__global__ __launch_bounds__(256) void k_route_place_far(RouteArgs a, int64_t n) {
+  extern __shared__ uint32_t first[];  // choices of the experts before each
+  const int cols = a.E + 1;
+  if (threadIdx.x < 64) route_first(a.starts + (int64_t)a.blocks * cols, first, a.E, blockIdx.x == 0 ? a.ends : nullptr);
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -416,9 +538,90 @@ __global__ __launch_bounds__(256) void k_route_place(RouteArgs a, int64_t n) {
     if (i < n) {
       const int32_t x = a.expert[i], e = x < 0 ? a.E : x;
       const uint32_t b = div_by(a.entries, (uint32_t)i);
-      a.position[i] = (int32_t)(first[e] + a.counts[(int64_t)b * cols + e] + (uint32_t)a.position[i]);
+      a.position[i] = (int32_t)(first[e] + a.starts[(int64_t)b * cols + e] + (uint32_t)a.position[i]);
     }
   }
+}
+
+// Places of the choices of four workgroups of k_route.  Every workgroup adds up all
+// the counts (a byte each: 128 KB for 16384 tokens and 256 experts, from the L2)
+// instead of waiting for a launch that does it once.  Bound by the latency of its
+// loads, so what does not depend on the sums is asked for first.
+__global__ __launch_bounds__(1024) void k_route_place(RouteArgs a) {
+  __shared__ uint32_t total[1024], first[1028], start[4][1028];
+  __shared__ uint32_t none;
+  const int tid = threadIdx.x, b0 = blockIdx.x * 4, blocks = a.blocks - b0 < 4 ? a.blocks - b0 : 4;
+  const int64_t i0 = (int64_t)b0 * a.block * a.k, all = a.T * a.k - i0;
+  const int n = (int)(all < 4 * a.block * a.k ? all : 4 * a.block * a.k);
+  const LM_GLOBAL uint8_t* const counts = (const LM_GLOBAL uint8_t*)a.counts;
+  const LM_GLOBAL int32_t* const expert = (const LM_GLOBAL int32_t*)a.expert + i0;
+  LM_GLOBAL int32_t* const position = (LM_GLOBAL int32_t*)a.position + i0;
+  int32_t x0 = 0, p0 = 0;
+  if (tid < n) {
+    x0 = expert[tid];
+    p0 = position[tid];
+  }
+  uint32_t own[4], without[4], mine = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    own[i] = tid < a.E && i < blocks ? counts[(int64_t)(b0 + i) * a.pitch + tid] : 0u;
+    without[i] = tid == 0 && i < blocks ? a.none[b0 + i] : 0u;
+  }
+  for (int i = tid; i < b0; i += 1024) mine += a.none[i];
+  total[tid] = start[0][tid] = 0;
+  if (tid == 0) none = 0;
+  __syncthreads();
+  if (mine) atomicAdd(&none, mine);
+  const int words = a.pitch >> 2, shift = words <= 1 ? 0 : 32 - __builtin_clz(words - 1), w = tid & ((1 << shift) - 1), step = 1024 >> shift;
+  if (w < words) {
+    uint32_t t0 = 0, t1 = 0, s0 = 0, s1 = 0;  // of two experts each, in 16 bits: at most ROUTE_NEAR tokens
+    const LM_GLOBAL uint32_t* const at = (const LM_GLOBAL uint32_t*)a.counts + w;
+    for (int r0 = tid >> shift; r0 < a.blocks; r0 += step * 16) {
+      uint32_t x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = r0 + i * step < a.blocks ? at[(int64_t)(r0 + i * step) * words] : 0u;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t even = x[i] & 0x00ff00ffu, odd = x[i] >> 8 & 0x00ff00ffu;
+        const bool in = r0 + i * step < b0;
+        t0 += even;
+        t1 += odd;
+        s0 += in ? even : 0u;
+        s1 += in ? odd : 0u;
+      }
+    }
+    const uint32_t t[4] = {t0 & 0xffffu, t1 & 0xffffu, t0 >> 16, t1 >> 16}, s[4] = {s0 & 0xffffu, s1 & 0xffffu, s0 >> 16, s1 >> 16};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (t[i]) atomicAdd(&total[4 * w + i], t[i]);
+      if (s[i]) atomicAdd(&start[0][4 * w + i], s[i]);
+    }
+  }
+  __syncthreads();
+  if (tid < 64) route_first(total, first, a.E, blockIdx.x == 0 ? a.ends : nullptr);
+  __syncthreads();
+  if (tid < a.E) {
+    uint32_t x = first[tid] + start[0][tid];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      start[i][tid] = x;
+      x += own[i];
+    }
+  }
+  if (tid == 0) {
+    uint32_t x = first[a.E] + none;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      start[i][a.E] = x;
+      x += without[i];
+    }
+  }
+  __syncthreads();
+  auto place = [&](int i, int32_t x, int32_t p) {
+    position[i] = (int32_t)start[div_by(a.entries, (uint32_t)i)][x < 0 ? a.E : x] + p;
+  };
+  if (tid < n) place(tid, x0, p0);
+  for (int i = tid + 1024; i < n; i += 1024) place(i, expert[i], position[i]);
 }
 
 // The gradient to the logits.  g = d loss / d w, for the chosen experts j:
@@ -448,7 +651,7 @@ __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a, const float* dw
     float v[P], s[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) v[i] = lane + 64 * i < a.E ? route_load<DT>(a.logits, t * a.ld + lane + 64 * i) : -INFINITY;
-    route_scores<float, P>(v, false, s);
+    route_scores<float, false, P>(v, false, s);
     float p = 0.0f;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
@@ -610,12 +813,26 @@ static int check_route(const lm_route* r) {
   return LM_OK;
 }
 
-// Tokens of a workgroup: all of them while they are few, so that one launch does.
+// Tokens of a workgroup: all of them while they are few, so that one launch does; one
+// a wave up to 256 workgroups.
 static int route_block(int64_t T) {
   if (T <= 32) return (int)T;
-  int block = 16;
-  while (block < 64 && (T + block - 1) / block > 1024) block *= 2;
-  return block;
+  if (T <= 4096) return 16;
+  return T <= ROUTE_NEAR ? 32 : 64;
+}
+static int64_t route_pitch(int64_t experts) { return (experts + 3) & ~(int64_t)3; }
+
+struct RouteSpace {
+  size_t none, starts, total;
+};
+static RouteSpace route_space(int64_t T, int64_t experts) {
+  const int64_t block = route_block(T), blocks = (T + block - 1) / block;
+  RouteSpace s{};
+  if (blocks <= 1) return s;
+  s.none = align256((size_t)(blocks * route_pitch(experts)));
+  s.starts = s.none + align256((size_t)blocks * 4);
+  s.total = s.starts + (T > ROUTE_NEAR ? align256((size_t)(blocks + 1) * (size_t)(experts + 1) * 4) : 0);
+  return s;
 }
 
 static RouteArgs route_args(const lm_route* r) {
@@ -638,6 +855,7 @@ static RouteArgs route_args(const lm_route* r) {
   a.per_mul = ((1u << 20) + a.per - 1) / a.per;
   a.block = a.T > 0 ? route_block(a.T) : 1;
   a.blocks = (int)((a.T + a.block - 1) / a.block);
+  a.pitch = (int)route_pitch(a.E);
   a.entries = fast_div((uint32_t)(a.block * a.k));
   return a;
 }
@@ -659,8 +877,7 @@ static RouteArgs route_args(const lm_route* r) {
 
 extern "C" size_t lm_route_workspace_size(int64_t T, int32_t experts) {
   if (T <= 0 || T > 0x7fffffff || experts < 1 || experts > LM_LINEAR_MAX_EXPERTS) return 0;
-  const int64_t block = route_block(T), blocks = (T + block - 1) / block;
-  return blocks > 1 ? align256((size_t)(blocks + 1) * (size_t)(experts + 1) * 4) : 0;
+  return route_space(T, experts).total;
 }
 
 extern "C" int lm_route_topk(const lm_route* r, float* weight, int32_t* expert, int32_t* position, int32_t* ends,
@@ -678,21 +895,28 @@ extern "C" int lm_route_topk(const lm_route* r, float* weight, int32_t* expert, 
     if (!workspace || workspace_bytes < need)
       return fail(LM_EWORKSPACE, "workspace too small: %zu < %zu bytes", workspace ? workspace_bytes : 0, need);
     if (((uintptr_t)workspace & 255) != 0) return fail(LM_EINVAL, "workspace must be 256-byte aligned");
-    a.counts = (uint32_t*)workspace;
+    const RouteSpace s = route_space(a.T, a.E);
+    a.counts = (uint8_t*)workspace;
+    a.none = (uint32_t*)((uint8_t*)workspace + s.none);
+    a.starts = (uint32_t*)((uint8_t*)workspace + s.starts);
   }
   hipStream_t st = (hipStream_t)stream;
   TimedLaunch timed("route", st);
-  const int threads = 512;
-  const size_t lds = (size_t)(a.E + 1) * 4 + (size_t)a.block * a.k * 4 + (a.top_groups < a.groups ? (size_t)threads / 64 * a.E * 4 : 0);
+  const int threads = a.E <= 256 ? 1024 : 512;  // ROUTE_THREADS
+  const size_t lds = (a.top_groups < a.groups ? (size_t)threads / 64 * a.pitch * 4 : 0) + (size_t)(a.E + 1) * 4 + (size_t)a.block * a.k * 4;
   ROUTE_BY_TYPE(k_route, dim3((unsigned)(a.blocks > 0 ? a.blocks : 1)), dim3(threads), lds, st, a);
   LAUNCH_CHECK();
-  if (a.blocks > 1) {
-    hipLaunchKernelGGL(k_route_scan, dim3((unsigned)((a.E + 16) / 16)), dim3(1024), 0, st, a);
+  if (a.blocks <= 1) return LM_OK;
+  if (a.T <= ROUTE_NEAR) {
+    hipLaunchKernelGGL(k_route_place, dim3((unsigned)((a.blocks + 3) / 4)), dim3(1024), 0, st, a);
     LAUNCH_CHECK();
-    const int64_t n = a.T * a.k;
-    hipLaunchKernelGGL(k_route_place, dim3((unsigned)((n + 1023) / 1024)), dim3(256), (size_t)(a.E + 1) * 4, st, a, n);
-    LAUNCH_CHECK();
+    return LM_OK;
   }
+  hipLaunchKernelGGL(k_route_scan, dim3((unsigned)((a.E + 16) / 16)), dim3(1024), 0, st, a);
+  LAUNCH_CHECK();
+  const int64_t n = a.T * a.k;
+  hipLaunchKernelGGL(k_route_place_far, dim3((unsigned)((n + 1023) / 1024)), dim3(256), (size_t)(a.E + 1) * 4, st, a, n);
+  LAUNCH_CHECK();
   return LM_OK;
 }
 
