@@ -703,9 +703,12 @@ DEV int rows_end(const RowsArgs& a) {
   const int64_t n = a.T * a.k;
   return end < 0 ? 0 : (end > n ? (int)n : end);
 }
+// NT: past the caches
+template <bool NT>
 DEV void rows_store(uint16_t* p, lm_u32x4 w, int64_t left) {
   if (left >= 8) {
-    *(LM_GLOBAL lm_u32x4_any*)p = w;
+    if constexpr (NT) __builtin_nontemporal_store(w, (LM_GLOBAL lm_u32x4_any*)p);
+    else *(LM_GLOBAL lm_u32x4_any*)p = w;
     asm volatile("s_nop 1" ::"v"(w) : "memory");  // (store_b128_guarded)
   } else {
 #pragma unroll
@@ -714,80 +717,147 @@ DEV void rows_store(uint16_t* p, lm_u32x4 w, int64_t left) {
   }
 }
 
-// A wave has 512 columns of a token.
-__global__ __launch_bounds__(256) void k_rows_out(RowsArgs a, uint32_t chunks) {
-  const int64_t item = (int64_t)blockIdx.x * 4 + wave_index(), t = item / chunks;
-  if (t >= a.T) return;
-  const int64_t c = (item - t * chunks) * 512 + (threadIdx.x & 63) * 8, left = a.N - c;
-  const lm_u32x4 w = lin_chunk((const uint16_t*)a.x + t * a.ld + c, left);
-  const int end = rows_end(a);
-  for (int j = 0; j < a.k; ++j) {
-    const int p = a.position[t * a.k + j];
-    if (p < 0 || p >= a.T * a.k) continue;
-    rows_store((uint16_t*)a.out + p * a.N + c, p < end ? w : lm_u32x4{}, left);
+// 8 values of each of M rows, `left` of which exist; all of them before the first is used.
+//
+// Rows of choices go past the caches, both ways: there are top_k of them for every
+// row of a token, and each is read or written once (8192 x 2048, four choices: rows
+// out 34 -> 26 us, back 33 -> 28, gradients 58 -> 48).  Rows of tokens do not: with
+// both past the caches rows out take 31 us, gradients 53.
+template <bool NT, int M>
+DEV void rows_load(lm_u32x4 (&w)[M], const uint16_t* const (&p)[M], int64_t left) {
+  if (left >= 8) {
+#pragma unroll
+    for (int n = 0; n < M; ++n) w[n] = NT ? __builtin_nontemporal_load((const LM_GLOBAL lm_u32x4_any*)p[n]) : *(const LM_GLOBAL lm_u32x4_any*)p[n];
+  } else {
+#pragma unroll
+    for (int n = 0; n < M; ++n) w[n] = lin_chunk(p[n], left);
   }
 }
 
-template <int DT, bool WEIGHTS>
-__global__ __launch_bounds__(256) void k_rows_back(RowsArgs a, uint32_t chunks) {
-  const int64_t item = (int64_t)blockIdx.x * 4 + wave_index(), t = item / chunks;
-  if (t >= a.T) return;
-  const int64_t c = (item - t * chunks) * 512 + (threadIdx.x & 63) * 8, left = a.N - c;
-  const int end = rows_end(a);
-  float s[8] = {};
-  for (int j0 = 0; j0 < a.k; j0 += 4) {  // four rows on their way at once
-    lm_u32x4 w[4];
-    float by[4];
+// Where a wave works: WPT waves (1, or all 4 of the workgroup) have a token, 512
+// columns each and the next ones after that; blockIdx.y shares the columns out.
+template <int WPT>
+struct RowsAt {
+  int64_t t, c0, step;
+  DEV RowsAt() {
+    t = WPT == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave_index();
+    c0 = ((int64_t)blockIdx.y * WPT + (WPT == 4 ? wave_index() : 0)) * 512 + (threadIdx.x & 63) * 8;
+    step = (int64_t)gridDim.y * WPT * 512;
+  }
+};
+// the places of choices j0 .. j0 + 3 of a token; -1: not one of those below `end`
+DEV void rows_places(const RowsArgs& a, int64_t t, int j0, int end, int (&p)[4]) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int j = j0 + n < a.k ? j0 + n : a.k - 1, p = a.position[t * a.k + j];
-      const bool on = j0 + n < a.k && p >= 0 && p < end;
-      by[n] = !on ? 0.0f : WEIGHTS ? a.weight[t * a.k + j] : 1.0f;
-      w[n] = lm_u32x4{};
-      if (on) w[n] = lin_chunk((const uint16_t*)a.h + p * a.ldh + c, left);
+  for (int n = 0; n < 4; ++n) {
+    p[n] = j0 + n < a.k ? a.position[t * a.k + j0 + n] : -1;
+    if (p[n] >= end) p[n] = -1;
+  }
+}
+
+template <int WPT>
+__global__ __launch_bounds__(256) void k_rows_out(RowsArgs a) {
+  const RowsAt<WPT> at;
+  if (at.t >= a.T) return;
+  const int end = rows_end(a), all = (int)(a.T * a.k);
+  for (int64_t c = at.c0; c < a.N; c += at.step) {
+    lm_u32x4 w[1];
+    const uint16_t* const p[1] = {(const uint16_t*)a.x + at.t * a.ld + c};
+    rows_load<false>(w, p, a.N - c);
+    for (int j = 0; j < a.k; ++j) {
+      const int to = a.position[at.t * a.k + j];
+      if (to < 0 || to >= all) continue;
+      rows_store<true>((uint16_t*)a.out + to * a.N + c, to < end ? w[0] : lm_u32x4{}, a.N - c);
     }
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] = __builtin_fmaf(by[n], val_dt<DT>(i & 1 ? w[n][i >> 1] >> 16 : w[n][i >> 1] & 0xffffu), s[i]);
   }
-  lm_u32x4 w;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = (uint32_t)bits_dt<DT>(s[2 * i]) | (uint32_t)bits_dt<DT>(s[2 * i + 1]) << 16;
-  rows_store((uint16_t*)a.out + t * a.N + c, w, left);
 }
 
-// Gradients of the weighted sums: a workgroup has a token.
-template <int DT>
-__global__ __launch_bounds__(256) void k_rows_back_grad(RowsArgs a) {
-  __shared__ float red[4];
-  const int64_t t = blockIdx.x;
+template <int DT, bool WEIGHTS, int WPT>
+__global__ __launch_bounds__(256) void k_rows_back(RowsArgs a) {
+  const RowsAt<WPT> at;
+  if (at.t >= a.T) return;
   const int end = rows_end(a);
-  for (int j = 0; j < a.k; ++j) {
-    const int p = a.position[t * a.k + j];
-    const bool in = p >= 0 && p < a.T * a.k, on = in && p < end;
-    const float by = a.weight[t * a.k + j];
-    float sum = 0.0f;
-    for (int64_t c = threadIdx.x * 8; in && c < a.N; c += 2048) {
-      lm_u32x4 w = {};
-      if (on) {
-        const lm_u32x4 dy = lin_chunk((const uint16_t*)a.x + t * a.ld + c, a.N - c);
-        const lm_u32x4 h = lin_chunk((const uint16_t*)a.h + p * a.ldh + c, a.N - c);
+  for (int64_t c = at.c0; c < a.N; c += at.step) {
+    float s[8] = {};
+    for (int j0 = 0; j0 < a.k; j0 += 4) {
+      int p[4];
+      rows_places(a, at.t, j0, end, p);
+      lm_u32x4 w[4];
+      const uint16_t* from[4];  // (row 0 instead of none: it is there)
+      float by[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float lo = val_dt<DT>(dy[i] & 0xffffu), hi = val_dt<DT>(dy[i] >> 16);
-          sum = __builtin_fmaf(lo, val_dt<DT>(h[i] & 0xffffu), sum);
-          sum = __builtin_fmaf(hi, val_dt<DT>(h[i] >> 16), sum);
-          w[i] = (uint32_t)bits_dt<DT>(by * lo) | (uint32_t)bits_dt<DT>(by * hi) << 16;
-        }
+      for (int n = 0; n < 4; ++n) {
+        from[n] = (const uint16_t*)a.h + (p[n] < 0 ? 0 : p[n]) * a.ldh + c;
+        by[n] = WEIGHTS && p[n] >= 0 ? a.weight[at.t * a.k + j0 + n] : 1.0f;
       }
-      rows_store((uint16_t*)a.out + p * a.N + c, w, a.N - c);
+      rows_load<true>(w, from, a.N - c);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        if (p[n] < 0) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = __builtin_fmaf(by[n], val_dt<DT>(i & 1 ? w[n][i >> 1] >> 16 : w[n][i >> 1] & 0xffffu), s[i]);
+      }
     }
-    sum = route_sum(sum);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) a.dweight[t * a.k + j] = on ? red[0] + red[1] + red[2] + red[3] : 0.0f;
+    lm_u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)bits_dt<DT>(s[2 * i]) | (uint32_t)bits_dt<DT>(s[2 * i + 1]) << 16;
+    rows_store<false>((uint16_t*)a.out + at.t * a.N + c, w, a.N - c);
+  }
+}
+
+// Gradients of the weighted sums, for four choices of a token at a time.
+template <int DT, int WPT>
+__global__ __launch_bounds__(256) void k_rows_back_grad(RowsArgs a) {
+  __shared__ float red[4][4];
+  const RowsAt<WPT> at;
+  if (at.t >= a.T) return;  // (with WPT 4 all waves or none)
+  const int end = rows_end(a), all = (int)(a.T * a.k), lane = threadIdx.x & 63;
+  for (int j0 = 0; j0 < a.k; j0 += 4) {
+    int p[4], to[4];
+    rows_places(a, at.t, j0, all, to);
+    rows_places(a, at.t, j0, end, p);
+    float by[4], sum[4] = {};
+#pragma unroll
+    for (int n = 0; n < 4; ++n) by[n] = p[n] < 0 ? 0.0f : a.weight[at.t * a.k + j0 + n];
+    for (int64_t c = at.c0; c < a.N; c += at.step) {
+      lm_u32x4 w[4], dy[1];
+      const uint16_t* from[4];
+      const uint16_t* const x[1] = {(const uint16_t*)a.x + at.t * a.ld + c};
+#pragma unroll
+      for (int n = 0; n < 4; ++n) from[n] = (const uint16_t*)a.h + (p[n] < 0 ? 0 : p[n]) * a.ldh + c;
+      rows_load<false>(dy, x, a.N - c);
+      rows_load<true>(w, from, a.N - c);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        lm_u32x4 dh = {};
+        if (p[n] >= 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float lo = val_dt<DT>(dy[0][i] & 0xffffu), hi = val_dt<DT>(dy[0][i] >> 16);
+            sum[n] = __builtin_fmaf(lo, val_dt<DT>(w[n][i] & 0xffffu), sum[n]);
+            sum[n] = __builtin_fmaf(hi, val_dt<DT>(w[n][i] >> 16), sum[n]);
+            dh[i] = (uint32_t)bits_dt<DT>(by[n] * lo) | (uint32_t)bits_dt<DT>(by[n] * hi) << 16;
+          }
+        }
+        if (to[n] >= 0) rows_store<true>((uint16_t*)a.out + to[n] * a.N + c, dh, a.N - c);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) sum[n] = route_sum(sum[n]);
+    if constexpr (WPT == 4) {
+      __syncthreads();  // (the sums before these are read)
+      if (lane == 0) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) red[n][wave_index()] = sum[n];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < 4; ++n) sum[n] = red[n][0] + red[n][1] + red[n][2] + red[n][3];
+    }
+    if (threadIdx.x == 0 || (WPT == 1 && lane == 0)) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        if (j0 + n < a.k) a.dweight[at.t * a.k + j0 + n] = p[n] < 0 ? 0.0f : sum[n];
+    }
   }
 }
 
@@ -954,12 +1024,12 @@ static RowsArgs rows_args(const lm_rows* r) {
   a.k = r->top_k;
   return a;
 }
-static int rows_grid(const RowsArgs& a, uint32_t& chunks, dim3& grid) {
-  chunks = (uint32_t)((a.N + 511) / 512);
-  const int64_t n = (a.T * (int64_t)chunks + 3) / 4;
-  if (n > 0x7fffffff) return fail(LM_EUNSUPPORTED, "rows too large for one launch");
-  grid = dim3((unsigned)n);
-  return LM_OK;
+// Rows of up to 1024 columns are a wave's, longer ones a workgroup's; while there are
+// few tokens the columns are shared out too (not where they are added up).
+static bool rows_short(const RowsArgs& a) { return a.N <= 1024; }
+static dim3 rows_grid(const RowsArgs& a, bool whole) {
+  const int64_t x = rows_short(a) ? (a.T + 3) / 4 : a.T, parts = (a.N + 2047) / 2048;
+  return dim3((unsigned)x, (unsigned)(whole || rows_short(a) || x >= 2048 ? 1 : parts < 64 ? parts : 64));
 }
 
 extern "C" int lm_dispatch_rows(const lm_rows* r, const void* x, int64_t ldx, void* out, void* stream) {
@@ -972,15 +1042,18 @@ extern "C" int lm_dispatch_rows(const lm_rows* r, const void* x, int64_t ldx, vo
   a.x = x;
   a.ld = ldx;
   a.out = out;
-  uint32_t chunks;
-  dim3 grid;
-  if ((rc = rows_grid(a, chunks, grid))) return rc;
   TimedLaunch timed("rows_experts", (hipStream_t)stream);
-  hipLaunchKernelGGL(k_rows_out, grid, dim3(256), 0, (hipStream_t)stream, a, chunks);
+  if (rows_short(a)) hipLaunchKernelGGL(k_rows_out<1>, rows_grid(a, false), dim3(256), 0, (hipStream_t)stream, a);
+  else hipLaunchKernelGGL(k_rows_out<4>, rows_grid(a, false), dim3(256), 0, (hipStream_t)stream, a);
   LAUNCH_CHECK();
   return LM_OK;
 }
 
+template <int DT, bool WEIGHTS>
+static void launch_rows_back(const RowsArgs& a, hipStream_t st) {
+  if (rows_short(a)) hipLaunchKernelGGL((k_rows_back<DT, WEIGHTS, 1>), rows_grid(a, false), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_rows_back<DT, WEIGHTS, 4>), rows_grid(a, false), dim3(256), 0, st, a);
+}
 static int rows_back(const lm_rows* r, const void* h, int64_t ldh, const float* weight, void* out, void* stream) {
   int rc;
   if ((rc = check_rows(r))) return rc;
@@ -992,17 +1065,14 @@ static int rows_back(const lm_rows* r, const void* h, int64_t ldh, const float* 
   a.ldh = ldh;
   a.weight = weight;
   a.out = out;
-  uint32_t chunks;
-  dim3 grid;
-  if ((rc = rows_grid(a, chunks, grid))) return rc;
   hipStream_t st = (hipStream_t)stream;
   TimedLaunch timed("rows_experts", st);
   if (weight) {
-    if (r->dtype == LM_F16) hipLaunchKernelGGL((k_rows_back<F16, true>), grid, dim3(256), 0, st, a, chunks);
-    else hipLaunchKernelGGL((k_rows_back<BF16, true>), grid, dim3(256), 0, st, a, chunks);
+    if (r->dtype == LM_F16) launch_rows_back<F16, true>(a, st);
+    else launch_rows_back<BF16, true>(a, st);
   } else {
-    if (r->dtype == LM_F16) hipLaunchKernelGGL((k_rows_back<F16, false>), grid, dim3(256), 0, st, a, chunks);
-    else hipLaunchKernelGGL((k_rows_back<BF16, false>), grid, dim3(256), 0, st, a, chunks);
+    if (r->dtype == LM_F16) launch_rows_back<F16, false>(a, st);
+    else launch_rows_back<BF16, false>(a, st);
   }
   LAUNCH_CHECK();
   return LM_OK;
@@ -1014,6 +1084,11 @@ extern "C" int lm_dispatch_rows_grad(const lm_rows* r, const void* dy, int64_t l
 extern "C" int lm_combine_rows(const lm_rows* r, const void* h, int64_t ldh, const float* weight, void* out, void* stream) {
   if (r && r->T > 0 && !weight) return fail(LM_EINVAL, "weights must be non-null");
   return rows_back(r, h, ldh, weight, out, stream);
+}
+template <int DT>
+static void launch_rows_back_grad(const RowsArgs& a, hipStream_t st) {
+  if (rows_short(a)) hipLaunchKernelGGL((k_rows_back_grad<DT, 1>), rows_grid(a, true), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_rows_back_grad<DT, 4>), rows_grid(a, true), dim3(256), 0, st, a);
 }
 extern "C" int lm_combine_rows_grad(const lm_rows* r, const void* dy, int64_t lddy, const void* h, int64_t ldh,
                                     const float* weight, void* dh, float* dweight, void* stream) {
@@ -1032,8 +1107,8 @@ extern "C" int lm_combine_rows_grad(const lm_rows* r, const void* dy, int64_t ld
   a.dweight = dweight;
   hipStream_t st = (hipStream_t)stream;
   TimedLaunch timed("rows_experts", st);
-  if (r->dtype == LM_F16) hipLaunchKernelGGL((k_rows_back_grad<F16>), dim3((unsigned)a.T), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_rows_back_grad<BF16>), dim3((unsigned)a.T), dim3(256), 0, st, a);
+  if (r->dtype == LM_F16) launch_rows_back_grad<F16>(a, st);
+  else launch_rows_back_grad<BF16>(a, st);
   LAUNCH_CHECK();
   return LM_OK;
 }
