@@ -47,6 +47,24 @@ DEV __amdgpu_buffer_rsrc_t lin_rsrc(const void* p, int64_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, n, 0x00027000);
 }
 
+// a barrier of the workgroup that waits for no memory by itself
+DEV void lin_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+// wait until at most N vector-memory operations and no LDS operation are left
+template <int N>
+DEV void lin_wait() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+
 // 8 values from p, of which the first `left` exist (any alignment)
 DEV lm_u32x4 lin_chunk(const uint16_t* p, int64_t left) {
   lm_u32x4 v = {};

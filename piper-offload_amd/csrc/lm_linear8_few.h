@@ -19,7 +19,7 @@ DEV lm_u32x4 few8_load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
   return __builtin_bit_cast(lm_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
 }
 // 16 codes from p, of which the first `left` exist (any alignment)
-DEV lm_u32x4 few8_chunk(const uint8_t* p, int left) {
+DEV lm_u32x4 few8_chunk(const uint8_t* p, int64_t left) {
   lm_u32x4 v = {};
   if (left >= 16) {
     v = *(const LM_GLOBAL lm_u32x4_any*)p;
@@ -35,13 +35,65 @@ DEV lm_u32x4 few8_chunk(const uint8_t* p, int left) {
   return v;
 }
 
-template <int DT, bool Q8, int MF, int CF, int NW, int UN>
+// x / r to the nearest whole number, ties to even, as the exact quotient rounds.
+// n, from the inverse, is off by one where the quotient lies next to a border; the
+// remainder x - n r is exact (one fma: x is a multiple of r's last place), and says so.
+DEV float lin8_round(float x, float r, float inv) {
+  const float n = __builtin_rintf(x * inv), e = __builtin_fmaf(-n, r, x), d = 2.0f * __builtin_fabsf(e);
+  const float to = n + (e < 0.0f ? -1.0f : 1.0f);
+  const bool odd = __builtin_rintf(n * 0.5f) * 2.0f != n;
+  return d > r || (d == r && odd) ? to : n;
+}
+
+// The largest magnitude (as its bits) of 8 values, and of a wave
+template <int DT>
+DEV uint32_t lin8_top(lm_u32x4 w, uint32_t top) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t b = f2u(val_dt<DT>(j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu)) & 0x7fffffffu;
+    top = b > top ? b : top;
+  }
+  return top;
+}
+DEV uint32_t lin8_wave_max(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane(lin_scan_max((int)x), 63); }
+// A row, from its largest magnitude: its scale, and codes of its values.  A row of
+// zeros has scale 0; one with an infinity or a NaN has the scale NaN, so its products
+// are NaN instead of finite numbers.
+struct Lin8Row {
+  float scale, up, to, inv;
+  DEV Lin8Row(uint32_t top) {
+    const bool bad = top >= 0x7f800000u;
+    scale = bad ? u2f(0x7fc00000u) : u2f(top) / 127.0f;
+    // (a scale below 2^-100, whose inverse may overflow, is scaled up first: exact)
+    up = scale < 0x1p-100f ? 0x1p100f : 1.0f;
+    to = scale * up;
+    inv = bad || scale == 0.0f ? 0.0f : 1.0f / to;
+  }
+  template <int DT>
+  DEV lm_u32x2 codes(lm_u32x4 w) const {
+    uint32_t q[2] = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v = val_dt<DT>(j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu);
+      const float n = inv == 0.0f ? 0.0f : __builtin_amdgcn_fmed3f(lin8_round(v * up, to, inv), -127.0f, 127.0f);
+      q[j >> 2] |= ((uint32_t)(int)n & 0xffu) << (8 * (j & 3));
+    }
+    return lm_u32x2{q[0], q[1]};
+  }
+};
+
+// OWN: x is not quantised yet.  Its few rows are, into LDS, by every workgroup.
+template <int DT, bool Q8, bool OWN, int MF, int CF, int NW, int UN>
 __global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* codes, int64_t pitch) {
   constexpr bool HALF = DT == F16;
   constexpr int COLS = CF * 16, ROWS = MF * 16, PITCH = COLS + 4;
   constexpr int XL = Q8 ? 2 : 4;            // 16-byte loads of x a unit
   constexpr int AC = MF * CF <= 2 ? 2 : 1;  // accumulators in turn: the MFMAs of a fragment depend on each other
+  static_assert(!OWN || (Q8 && MF == 1), "rows of its own: a few, with 8-bit inputs");
   __shared__ __attribute__((aligned(16))) uint32_t red[NW * ROWS * PITCH];
+  __shared__ uint32_t tops[OWN ? 4 * NW : 1];
+  __shared__ float scales[OWN ? 4 : 1];
+  extern __shared__ __attribute__((aligned(16))) uint8_t mine[];  // OWN: codes of the rows
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, wave = wave_index();
   // (row tiles first, each XCD a contiguous part: as k_lin_few)
   const uint32_t gn = (uint32_t)((a.N + COLS - 1) / COLS), u = (uint32_t)xcd_unit(blockIdx.x, gridDim.x);
@@ -56,9 +108,9 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* 
     const int K = (int)a.K;
     const int64_t ldx = Q8 ? pitch : a.lda * 2;  // bytes
     const int rows = (int)(r1 - r0 < ROWS ? r1 - r0 : ROWS), cols = (int)(a.N - n0 < COLS ? a.N - n0 : COLS);
-    const uint8_t* xp = (Q8 ? codes : (const uint8_t*)a.a) + r0 * ldx;
+    const uint8_t* xp = OWN ? nullptr : (Q8 ? codes : (const uint8_t*)a.a) + r0 * ldx;
     const uint8_t* wp = (const uint8_t*)a.w + (group * a.N + n0) * a.K;
-    const __amdgpu_buffer_rsrc_t rx = lin_rsrc(xp, (rows - 1) * ldx + (Q8 ? pitch : a.K * 2));
+    const __amdgpu_buffer_rsrc_t rx = lin_rsrc(xp, OWN ? 0 : (rows - 1) * ldx + (Q8 ? pitch : a.K * 2));
     const __amdgpu_buffer_rsrc_t rw = lin_rsrc(wp, cols * a.K);
     uint32_t xo[MF], wo[CF];
 #pragma unroll
@@ -72,9 +124,8 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* 
       wo[c] = (uint32_t)(n * a.K) + 16 * g;
     }
     // UN units from u0; TAIL: some of them may pass the end
-    auto body = [&](int u0, auto tail) {
-      constexpr bool TAIL = decltype(tail)::value;
-      lm_u32x4 xv[UN][MF][XL], wv[UN][CF][2];
+    lm_u32x4 wv[UN][CF][2];
+    auto weights = [&](int u0, auto tail) {
 #pragma unroll
       for (int i = 0; i < UN; ++i) {
         const int k0 = (u0 + i) * 128;
@@ -82,14 +133,26 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* 
         for (int c = 0; c < CF; ++c)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if constexpr (TAIL) wv[i][c][h] = few8_chunk(wp + wo[c] + k0 + 64 * h, K - k0 - 64 * h - 16 * g);
+            if constexpr (decltype(tail)::value) wv[i][c][h] = few8_chunk(wp + wo[c] + k0 + 64 * h, K - k0 - 64 * h - 16 * g);
             else wv[i][c][h] = few8_load16(rw, wo[c] + k0 + 64 * h);
           }
+      }
+    };
+    auto body = [&](int u0, auto tail) {
+      constexpr bool TAIL = decltype(tail)::value;
+      lm_u32x4 xv[UN][MF][XL];
+#pragma unroll
+      for (int i = 0; i < UN; ++i) {
+        const int k0 = (u0 + i) * 128;
 #pragma unroll
         for (int m = 0; m < MF; ++m)
 #pragma unroll
           for (int j = 0; j < XL; ++j) {
-            if constexpr (Q8) {
+            if constexpr (OWN) {
+              const int k = k0 + 64 * j + 16 * g;
+              xv[i][m][j] = lm_u32x4{};
+              if (!TAIL || k < K) xv[i][m][j] = *(const lm_u32x4*)(mine + xo[m] + k0 + 64 * j);
+            } else if constexpr (Q8) {
               xv[i][m][j] = few8_load16(rx, TAIL && k0 + 64 * j + 16 * g >= K ? LIN_OUT : xo[m] + k0 + 64 * j);
             } else {
               const int e = k0 + 64 * (j >> 1) + 8 * (j & 1);  // (+ 16 g)
@@ -120,8 +183,53 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* 
     };
     const int units = (K + 127) >> 7, whole = K >> 7;
     int u0 = wave * UN;
-    for (; u0 + UN <= whole; u0 += NW * UN) body(u0, std::false_type{});
-    if (u0 < units) body(u0, std::true_type{});
+    if constexpr (OWN) {
+      // The rows' first pieces, then the first weights (loads come back in order), and
+      // while those are on their way the codes.  Barriers that wait for LDS alone.
+      const uint16_t* x = (const uint16_t*)a.a + r0 * a.lda;
+      const int c0 = tid * 8;
+      lm_u32x4 first[4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+        if (m < rows) first[m] = lin_chunk(x + m * a.lda + c0, K - c0);
+      const bool ahead = u0 + UN <= whole;
+      if (ahead) weights(u0, std::false_type{});
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        if (m >= rows) break;
+        uint32_t top = lin8_top<DT>(first[m], 0);
+        for (int c = c0 + NW * 512; c < K; c += NW * 512) top = lin8_top<DT>(lin_chunk(x + m * a.lda + c, K - c), top);
+        top = lin8_wave_max(top);
+        if (lane == 0) tops[m * NW + wave] = top;
+      }
+      lin_wait<63>();
+      lin_barrier();
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        if (m >= rows) break;
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) top = tops[m * NW + i] > top ? tops[m * NW + i] : top;
+        const Lin8Row r(top);
+        if (tid == 0) scales[m] = r.scale;
+        if (c0 < pitch) *(lm_u32x2*)(mine + m * pitch + c0) = r.codes<DT>(first[m]);
+        for (int c = c0 + NW * 512; c < pitch; c += NW * 512) *(lm_u32x2*)(mine + m * pitch + c) = r.codes<DT>(lin_chunk(x + m * a.lda + c, K - c));
+      }
+      lin_wait<63>();
+      lin_barrier();
+      if (ahead) {
+        body(u0, std::false_type{});
+        u0 += NW * UN;
+      }
+    }
+    for (; u0 + UN <= whole; u0 += NW * UN) {
+      weights(u0, std::false_type{});
+      body(u0, std::false_type{});
+    }
+    if (u0 < units) {
+      weights(u0, std::true_type{});
+      body(u0, std::true_type{});
+    }
 #pragma unroll
     for (int m = 0; m < MF; ++m)
 #pragma unroll
@@ -146,7 +254,7 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* 
 #pragma unroll
         for (int k = 0; k < NW; ++k) sum += red[(k * ROWS + m) * PITCH + c];
         // (in this order no large row overflows on the way)
-        s = (float)(int)sum * lin_scale8(a, group * a.N + n) * a.row_scale[r0 + m];
+        s = (float)(int)sum * lin_scale8(a, group * a.N + n) * (OWN ? scales[OWN ? m : 0] : a.row_scale[r0 + m]);
       } else {
 #pragma unroll
         for (int k = 0; k < NW; ++k) s += u2f(red[(k * ROWS + m) * PITCH + c]);

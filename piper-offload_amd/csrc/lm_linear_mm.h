@@ -59,24 +59,6 @@ typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
 DEV void lin_dma(__amdgpu_buffer_rsrc_t r, lds_u8* base, uint32_t off) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)base, 16, (int)off, 0, 0, 0);
 }
-// a barrier of the workgroup that waits for no memory by itself
-DEV void lin_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("" ::: "memory");
-}
-// wait until at most N vector-memory operations and no LDS operation are left
-template <int N>
-DEV void lin_wait() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("" ::: "memory");
-}
-
 // LDS serves a 16-byte read of a wave 16 lanes at a time, lanes 0-3, 12-15 and
 // 20-27 first, then 4-11, 16-19 and 28-31, and the same in the upper half.  A slot
 // is a quarter of the 64 banks, so four slots (p & 3) share them out and the
