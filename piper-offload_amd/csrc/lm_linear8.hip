@@ -47,12 +47,13 @@ __global__ __launch_bounds__(256) void k_lin8_prep(LinArgs a, uint8_t* codes, fl
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-// Rows of codes that are copied, x's and a weight's, start on whole 64-byte pieces (a stage's
-// loads of a row): 777 x [2001, 2083] TODO
+// Rows of codes that are copied for k_lin_mm, x's and a weight's, start on whole 64-byte
+// pieces, a stage's loads of a row: the product of 777 x [2001, 2083] 14.2 us, on 16 bytes 16.8.
 static int64_t round16(int64_t x) { return (x + 15) & ~(int64_t)15; }
 static int64_t round64(int64_t x) { return (x + 63) & ~(int64_t)63; }
 // Up to this many rows every workgroup of k_lin_few8 quantises them by itself, while its
-// first weights are on their way: TODO
+// first weights are on their way: one row of [1024, 4096] 6.1 us, after a launch of
+// k_lin8_prep 8; four rows of [4096, 4096] 10.9, as much as the two launches, but for the host.
 constexpr int64_t LIN8_OWN_ROWS = 4, LIN8_OWN_BYTES = 32768;
 
 struct Lin8Plan {
@@ -129,16 +130,30 @@ static int launch_few8(const LinArgs& a, const uint8_t* codes, int64_t pitch, hi
   LAUNCH_CHECK();
   return LM_OK;
 }
+// Columns of a workgroup, its waves, units in flight, in graphs over weights from
+// memory.  Few workgroups: 16 columns (one row of [4096, 4096] 6.7 us, with 32 8.6).
+// 8-bit inputs: 32 columns, one unit (one row of [14336, 4096] 14.2 us, four units
+// 15.4; 64 rows of 32 experts [2816, 2048] 30.7, four waves with two 33.5; but one row
+// of [8192, 14336] 28.2, four units 27.4).  16-bit inputs, twice as many bytes of x for
+// a byte of the weight: 64 columns from 9 rows on (16 rows of [14336, 4096] 17.4 us, 32
+// columns 19.4), 32 below (one row 15.4, 64 columns 16.5) and where the contraction is
+// long (16 rows of [8192, 14336] 30.7, 64 columns 47.6); very many workgroups take four
+// waves (64 rows of 32 experts [2816, 2048] 31.2, eight 33.6).
 template <int DT, bool Q8, bool OWN>
 static int run_few8(const LinArgs& a, const uint8_t* codes, int64_t pitch, hipStream_t st) {
-  const int64_t rows = (a.T + a.experts - 1) / a.experts, units = (a.K + 127) / 128;
+  const int64_t rows = (a.T + a.experts - 1) / a.experts;
   const int64_t wgs = lin_tiles<16>(a.T, a.experts, a.experts > 1) * ((a.N + 15) / 16);
   if constexpr (!OWN) {
     if (rows > 32 && wgs > 2048) return launch_few8<DT, Q8, OWN, 4, 4, 8, 1>(a, codes, pitch, st);
   }
   if (wgs <= 256) return launch_few8<DT, Q8, OWN, 1, 1, 8, 4>(a, codes, pitch, st);
-  if (units >= 32) return launch_few8<DT, Q8, OWN, 1, 2, 8, 4>(a, codes, pitch, st);
-  return launch_few8<DT, Q8, OWN, 1, 2, 4, 2>(a, codes, pitch, st);
+  if constexpr (Q8) {
+    return launch_few8<DT, Q8, OWN, 1, 2, 8, 1>(a, codes, pitch, st);
+  } else {
+    if (wgs > 2048) return launch_few8<DT, Q8, OWN, 1, 4, 4, 1>(a, codes, pitch, st);
+    if (a.T > 8 && a.K < 8192) return launch_few8<DT, Q8, OWN, 1, 4, 8, 1>(a, codes, pitch, st);
+    return launch_few8<DT, Q8, OWN, 1, 2, 8, 2>(a, codes, pitch, st);
+  }
 }
 
 static int lin8_setup(LinArgs& a, const Lin8Plan& p, int op, int dtype, void* workspace, size_t workspace_bytes, hipStream_t st) {
