@@ -351,3 +351,85 @@ def test_refusals():
         int8_linear(x, Int8Weight(q, s, (1, 64)), torch.zeros(32, dtype=BF16, device=DEV, requires_grad=True))
     with pytest.raises(ValueError):
         grouped_linear(x, Int8Weight(q, s, (1, 64)), torch.zeros(3, dtype=torch.int32, device=DEV))
+
+
+# up to four rows are quantised by the product's own workgroups while their codes fit; the last but one are too long
+OWN = [(1, 300, 4095), (1, 48, 4104), (2, 4200, 130), (3, 130, 4097), (4, 96, 8192), (4, 70, 8208), (1, 50, 32768), (1, 48, 32784),
+       (4, 4200, 1056), (5, 4200, 300)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("t,n,k", OWN)
+def test_few_rows_with_8_bit_inputs(t, n, k, dtype):
+    g = _gen(t + 3 * n + k)
+    q, s, _ = _weight(g, n, k)
+    x = _normal(g, t, k, dtype=dtype)
+    x[0, k // 2] = 17.0  # (its largest value in the middle)
+    if t > 2:
+        x[1] = 0.0
+    bias = _normal(g, n, std=0.1, dtype=dtype)
+    args = q.to(DEV), s.to(DEV)
+    got = K.int8_matmul(x.to(DEV), *args, bias=bias.to(DEV), activation_dtype=I8)
+    _check(x, q, s, got, True, bias)
+    big = torch.full((t, k + 9), 1e4, dtype=dtype, device=DEV)
+    view = big[:, 3:3 + k].copy_(x.to(DEV))
+    assert (K.int8_matmul(view, *args, bias=bias.to(DEV), activation_dtype=I8) == got).all()
+
+
+# 16-bit inputs: every shape of workgroup (few and many columns, up to and above 8 rows, long rows)
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("t,n,k", [(1, 4097, 200), (8, 4200, 640), (9, 4200, 640), (16, 5000, 129), (40, 4100, 512), (3, 4112, 8200), (20, 4100, 8192)])
+def test_few_rows_with_16_bit_inputs(t, n, k, dtype):
+    g = _gen(t + n + 5 * k)
+    q, s, _ = _weight(g, n, k)
+    x = _normal(g, t, k, dtype=dtype)
+    _check(x, q, s, K.int8_matmul(x.to(DEV), q.to(DEV), s.to(DEV)), False)
+
+
+@pytest.mark.parametrize("quant", [False, True], ids=["x16", "x8"])
+@pytest.mark.parametrize("sizes,t,n,k", [([0, 1, 0, 2, 1], 4, 200, 1408), ([0, 1, 1], 3, 64, 520), ([1, 0, 0, 0], 4, 4100, 144), ([2, 3] * 20, 100, 2050, 136),
+                                         ([40, 50] * 3, 270, 6200, 72)])
+def test_few_rows_of_groups(sizes, t, n, k, quant):
+    g = _gen(t + n + k)
+    q, s, _ = _weight(g, len(sizes), n, k)
+    x, ends = _normal(g, t, k, dtype=BF16), _ends(sizes)
+    x[int(ends[-1]):] = float("nan")  # (rows of no group are not looked at)
+    y = K.grouped_int8_matmul(x.to(DEV), q.to(DEV), s.to(DEV), ends.to(DEV), activation_dtype=I8 if quant else None)
+    begin = 0
+    for i, end in enumerate(ends.tolist()):
+        if end > begin:
+            _check(x[begin:end], q[i], s[i], y[begin:end], quant)
+        begin = end
+    assert (y[begin:] == 0).all()
+
+
+def test_bad_rows_of_few():
+    """An infinity or a NaN makes its own row NaN, also where the rows are quantised by the product's workgroups."""
+    g = _gen(19)
+    q, s, _ = _weight(g, 500, 4300)
+    x = _normal(g, 4, 4300, dtype=BF16)
+    x[1, 4299] = float("inf")
+    x[3, 7] = float("nan")
+    y = K.int8_matmul(x.to(DEV), q.to(DEV), s.to(DEV), activation_dtype=I8)
+    assert torch.isnan(y[[1, 3]]).all()
+    _check(x[[0, 2]], q, s, y[[0, 2]], True)
+
+
+def test_few_rows_in_a_graph_on_another_stream():
+    g = _gen(52)
+    q, s, _ = _weight(g, 700, 1000)
+    q, s = q.to(DEV), s.to(DEV)
+    x = _normal(g, 3, 1000, dtype=BF16).to(DEV)
+    K.int8_matmul(x, q, s, activation_dtype=I8)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = K.int8_matmul(x, q, s, activation_dtype=I8)
+    for _ in range(3):
+        x.copy_(_normal(g, 3, 1000, dtype=BF16))
+        graph.replay()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = K.int8_matmul(x, q, s, activation_dtype=I8)
+        torch.cuda.current_stream().wait_stream(side)
+        assert (y == want).all()

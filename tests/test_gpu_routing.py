@@ -458,3 +458,111 @@ def test_gradients_are_not_lost():
         K.dispatch_rows(torch.zeros(4, 16, dtype=BF16, device=DEV, requires_grad=True), r.position, r.ends)
     with pytest.raises(ValueError, match="detach"):
         route_experts(x, 2, bias=torch.zeros(8, device=DEV, requires_grad=True))
+
+
+def _places_of(expert, e):
+    """Places and ends of given choices, by a stable sort."""
+    key = torch.where(expert < 0, e, expert).reshape(-1).long()
+    place = torch.empty_like(key)
+    place[key.argsort(stable=True)] = torch.arange(key.numel())
+    return place.view(expert.shape), torch.bincount(key, minlength=e + 1)[:e].cumsum(0)
+
+
+@pytest.mark.parametrize("t,e,k", [(4096, 70, 3), (4097, 70, 3), (32768, 12, 2), (32769, 12, 2), (70000, 33, 5), (6000, 1024, 4), (33000, 513, 2)])
+def test_many_tokens(t, e, k):
+    """Around the numbers of tokens where workgroups get larger and places are found another way; closed tokens in between.
+    The logits of a row are whole numbers, so that many are equal: ties go to the lowest index."""
+    g = _gen(t + e)
+    logits = torch.randint(-40, 40, (t, e), generator=g).to(BF16)
+    logits[torch.rand(t, generator=g) < 0.1] = -INF
+    logits[t - 100:] = -INF
+    logits[t // 2, 1:] = -INF
+    r = K.route_topk(logits.to(DEV), k)
+    value, index = logits.float().sort(dim=-1, descending=True, stable=True)
+    expert = torch.where(value[:, :k] > -INF, index[:, :k], -1)
+    assert (r.expert.cpu() == expert).all()
+    place, ends = _places_of(expert, e)
+    assert (r.position.cpu() == place).all() and (r.ends.cpu() == ends).all()
+
+
+@pytest.mark.parametrize("many", [3, 20, 60, 64, 65, 100, 300])
+def test_runs_of_scores_that_agree_in_32_bits(many):
+    """`many` experts whose scores differ by less than a rounding of 2^-24, above the others: some of them are chosen."""
+    g = _gen(many)
+    t, e = 40, 320
+    logits = _normal(g, t, e) - 6.0
+    for i in range(t):
+        logits[i, torch.randperm(e, generator=g)[:many]] = 1.0 + 1e-7 * torch.randint(0, 8, (many,), generator=g).float()
+    bias = 1e-9 * _normal(g, e)
+    for score in ("softmax", "sigmoid"):
+        for k in (1, 8, 64):
+            _check(logits, k, bias, score=score)
+        _check(logits, 8, bias, score=score, groups=8, top_groups=3, group_best=2)
+        _check(logits, 8, torch.full((e,), 0.5), score=score)  # (the same for all)
+
+
+@pytest.mark.parametrize("e,groups", [(12, 3), (128, 64), (128, 2), (96, 1), (640, 5), (1020, 60), (64, 32), (72, 18), (1000, 8)])
+def test_sizes_of_groups(e, groups):
+    g = _gen(e + groups)
+    logits = _normal(g, 60, e, std=1.5)
+    per = e // groups
+    for top in {1, (groups + 1) // 2, groups}:
+        k = min(6, top * per)
+        for best in (1, 2) if per > 1 else (1,):
+            _check(logits, k, _normal(g, e, std=0.1), score="sigmoid", groups=groups, top_groups=top, group_best=best)
+            _check(logits, k, score="softmax", groups=groups, top_groups=top, group_best=best)
+
+
+@pytest.mark.parametrize("cols", [1, 8, 509, 1023, 1024, 1025, 2048, 2055, 4104, 9000])
+def test_rows_there_and_back(cols):
+    """Whole numbers, weights of one: rows and their sums come back exactly, whatever part of a row a wave has."""
+    g = _gen(cols)
+    for t, k in ((1, 1), (3, 5), (41, 4), (2300, 2)):
+        if t * cols > 3e6:
+            continue
+        r = K.route_topk(_normal(g, t, 9).to(DEV), k)
+        x = torch.randint(-8, 9, (t, cols), generator=g).to(BF16).to(DEV)
+        at = (r.position, r.ends)
+        rows = K.dispatch_rows(x, *at)
+        assert (rows[r.position.long().view(-1)] == x.repeat_interleave(k, 0)).all()
+        one = torch.ones_like(r.weight)
+        assert (K.combine_rows(rows, one, *at) == x * k).all() and (K.dispatch_rows_grad(rows, *at) == x * k).all()
+        dh, dw = K.combine_rows_grad(x, rows, one, *at)
+        assert (dh == rows).all()
+        assert (dw == (x.float() ** 2).sum(-1, keepdim=True)).all()
+
+
+def test_backward_through_sums_and_views():
+    """Gradients that come as broadcast or transposed views, captured into a graph as well."""
+    g = _gen(55)
+    logits = _normal(g, 60, 12).to(DEV).requires_grad_()
+    x = _normal(g, 60, 80, dtype=BF16).to(DEV).requires_grad_()
+
+    def grads(dy):
+        r = route_experts(logits, 3, score="sigmoid")
+        y = combine_experts(dispatch_experts(x, r), r)
+        return torch.autograd.grad(y, (logits, x), dy)
+
+    dy = _normal(g, 80, 60, dtype=BF16).to(DEV).t()
+    for a, b in zip(grads(dy), grads(dy.contiguous())):
+        assert (a == b).all()
+    one = torch.ones((), dtype=BF16, device=DEV).expand(60, 80)
+    want = grads(one.contiguous())
+    for a, b in zip(grads(one), want):
+        assert (a == b).all()
+    static = dy.contiguous().clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grads(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = grads(static)
+    for _ in range(3):
+        static.copy_(_normal(g, 60, 80, dtype=BF16))
+        graph.replay()
+        want = grads(static)
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert (a == b).all()
