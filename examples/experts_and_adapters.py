@@ -12,7 +12,7 @@ import argparse
 
 import torch
 
-from piper_offload_amd import MxAdapter, MXWeight, expert_view, grouped_linear, mx_linear
+from piper_offload_amd import MxAdapter, MXWeight, combine_experts, dispatch_experts, expert_view, grouped_linear, mx_linear, route_experts
 from piper_offload_amd import kernels as K
 
 FP4 = torch.float4_e2m1fn_x2
@@ -38,15 +38,11 @@ class Block:
         self.out = pack(rand(hidden, hidden))
 
     def mixture(self, x: torch.Tensor, activation_dtype: torch.dtype | None = None) -> torch.Tensor:
-        weight, expert = (x @ self.router.t()).float().softmax(-1).topk(self.best, -1)
-        order = expert.reshape(-1).argsort(stable=True)  # rows of one expert side by side
-        ends = torch.bincount(expert.reshape(-1), minlength=self.experts).cumsum(0).to(torch.int32)
-        token = order // self.best
-        h = grouped_linear(x[token], self.up, ends, activation_dtype=activation_dtype)
+        routing = route_experts(x @ self.router.t(), self.best, renormalize=False)
+        h = grouped_linear(dispatch_experts(x, routing), self.up, routing.ends, activation_dtype=activation_dtype)
         gate, up = h.chunk(2, -1)
-        h = grouped_linear(torch.nn.functional.silu(gate) * up, self.down, ends, activation_dtype=activation_dtype)
-        h = h.float() * weight.reshape(-1)[order, None]
-        return torch.zeros_like(x, dtype=torch.float32).index_add(0, token, h).to(x.dtype)
+        h = grouped_linear(torch.nn.functional.silu(gate) * up, self.down, routing.ends, activation_dtype=activation_dtype)
+        return combine_experts(h, routing)
 
     def __call__(self, x: torch.Tensor, activation_dtype: torch.dtype | None = None) -> torch.Tensor:
         return mx_linear(self.mixture(x, activation_dtype), self.out, activation_dtype=activation_dtype)

@@ -768,7 +768,7 @@ def _linear_forward(label: str, x: torch.Tensor, weight: L.WeightStruct, bias: t
             raise ValueError(f"{label}: bias must be {x.dtype} [{n}], got {bias.dtype} {tuple(bias.shape)}.")
         _raw(label, bias)
         bias = bias.contiguous()
-    y = x2.new_empty((t, n))
+    y = x2.new_empty(t, n)
     if t:
         px = x2.data_ptr()
         ws_bytes = L.linear_workspace_size(0, t, ldx, 0, n, k, weight.experts, weight.dtype, input_id, not (px | weight.q) & 15)
@@ -780,7 +780,7 @@ def _linear_forward(label: str, x: torch.Tensor, weight: L.WeightStruct, bias: t
 def _linear_input_grad(label: str, dy: torch.Tensor, weight: L.WeightStruct, ends: torch.Tensor | None) -> torch.Tensor:
     n, k = weight.N, weight.K
     dy2, t, ldy = _rows(label, dy, n)
-    dx = dy2.new_empty((t, k))
+    dx = dy2.new_empty(t, k)
     if t:
         py = dy2.data_ptr()
         dtype_id = L.torch_dtype_id(dy.dtype)
@@ -1045,12 +1045,13 @@ def route_topk(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | None = 
     _on_gpu(label, logits, bias)
     _raw(label, logits)
     r, keep = _route(label, logits, top_k, bias, score, groups, top_groups, group_best, renormalize, scale)
-    t, e = logits.shape
-    weight = logits.new_empty((t, top_k), dtype=torch.float32)
-    expert = logits.new_empty((t, top_k), dtype=torch.int32)
-    position = logits.new_empty((t, top_k), dtype=torch.int32)
-    ends = logits.new_empty(e, dtype=torch.int32)
-    _launch(L.lib().lm_route_topk, logits.get_device(), L.route_workspace_size(t, e), logits.device, r, weight.data_ptr(),
+    (t, e), device = logits.shape, logits.device
+    shape, strides = (t, top_k), (top_k, 1)
+    weight = torch.empty_strided(shape, strides, dtype=torch.float32, device=device)
+    expert = torch.empty_strided(shape, strides, dtype=torch.int32, device=device)
+    position = torch.empty_like(expert)
+    ends = torch.empty_strided((e,), (1,), dtype=torch.int32, device=device)
+    _launch(L.lib().lm_route_topk, logits.get_device(), L.route_workspace_size(t, e), device, r, weight.data_ptr(),
             expert.data_ptr(), position.data_ptr(), ends.data_ptr())
     del keep
     return Routing(weight, expert, position, ends)
@@ -1075,25 +1076,25 @@ def route_topk_grad(dweight: torch.Tensor, logits: torch.Tensor, expert: torch.T
     return dlogits
 
 
-def _places(label: str, position: torch.Tensor, ends: torch.Tensor, cols: int, dtype: torch.dtype
-            ) -> tuple[L.RowsStruct, tuple[torch.Tensor, torch.Tensor]]:
-    if position.dtype is not torch.int32 or position.ndim != 2 or position.shape[1] < 1:
-        raise ValueError(f"{label}: position must be int32 [tokens, top_k], got {position.dtype} {tuple(position.shape)}.")
-    if position.numel() >= 1 << 31:
+def _places(label: str, x: torch.Tensor, of_choices: bool, position: torch.Tensor, ends: torch.Tensor
+            ) -> tuple[torch.Tensor, int, L.RowsStruct, tuple[torch.Tensor, torch.Tensor]]:
+    """``x``, rows of tokens or of their choices, with contiguous rows, its stride, and the places described."""
+    places = position.shape
+    if position.dtype is not torch.int32 or len(places) != 2 or places[1] < 1:
+        raise ValueError(f"{label}: position must be int32 [tokens, top_k], got {position.dtype} {tuple(places)}.")
+    tokens, top_k = places
+    if tokens * top_k >= 1 << 31:
         raise ValueError(f"{label} takes fewer than 2^31 choices.")
-    if cols < 1:
+    rows, shape = tokens * top_k if of_choices else tokens, x.shape
+    if len(shape) != 2 or shape[0] != rows:
+        raise ValueError(f"{label}: expected {rows} rows, got shape {tuple(shape)}.")
+    if shape[1] < 1:
         raise ValueError(f"{label} requires non-empty rows.")
+    x, _, ld = _rows(label, x, shape[1])
     ends = _ends(label, ends, ends.shape[0] if ends.ndim == 1 else -1)
     position = position.contiguous()
-    return L.RowsStruct(position.data_ptr(), ends.data_ptr(), position.shape[0], cols, position.shape[1], ends.shape[0],
-                        L.torch_dtype_id(dtype), 0), (position, ends)
-
-
-def _token_rows(label: str, x: torch.Tensor, rows: int) -> tuple[torch.Tensor, int]:
-    if x.ndim != 2 or x.shape[0] != rows:
-        raise ValueError(f"{label}: expected {rows} rows, got shape {tuple(x.shape)}.")
-    x, _, ld = _rows(label, x, x.shape[1])
-    return x, ld
+    return x, ld, L.RowsStruct(position.data_ptr(), ends.data_ptr(), tokens, shape[1], top_k, ends.shape[0],
+                               L.torch_dtype_id(x.dtype), 0), (position, ends)
 
 
 def _choice_weight(label: str, weight: torch.Tensor, position: torch.Tensor) -> torch.Tensor:
@@ -1110,10 +1111,9 @@ def dispatch_rows(x: torch.Tensor, position: torch.Tensor, ends: torch.Tensor) -
     """
     label = "Dispatch"
     _on_gpu(label, x, position, ends)
-    x, ld = _token_rows(label, x, position.shape[0] if position.ndim == 2 else 0)
-    r, keep = _places(label, position, ends, x.shape[1], x.dtype)
-    out = x.new_empty((position.numel(), x.shape[1]))
-    if out.shape[0]:
+    x, ld, r, keep = _places(label, x, False, position, ends)
+    out = x.new_empty(r.T * r.top_k, r.N)
+    if r.T:
         _enqueue(L.lib().lm_dispatch_rows, x.get_device(), x.device, r, x.data_ptr(), ld, out.data_ptr())
     del keep
     return out
@@ -1123,10 +1123,9 @@ def dispatch_rows_grad(dy: torch.Tensor, position: torch.Tensor, ends: torch.Ten
     """The gradient of :func:`dispatch_rows` to ``x``: the sum over a token's choices, in fp32, rounded once."""
     label = "Dispatch gradient"
     _on_gpu(label, dy, position, ends)
-    dy, ld = _token_rows(label, dy, position.numel())
-    r, keep = _places(label, position, ends, dy.shape[1], dy.dtype)
-    dx = dy.new_empty((position.shape[0], dy.shape[1]))
-    if dx.shape[0]:
+    dy, ld, r, keep = _places(label, dy, True, position, ends)
+    dx = dy.new_empty(r.T, r.N)
+    if r.T:
         _enqueue(L.lib().lm_dispatch_rows_grad, dy.get_device(), dy.device, r, dy.data_ptr(), ld, dx.data_ptr())
     del keep
     return dx
@@ -1140,11 +1139,10 @@ def combine_rows(h: torch.Tensor, weight: torch.Tensor, position: torch.Tensor, 
     """
     label = "Combine"
     _on_gpu(label, h, weight, position, ends)
-    h, ld = _token_rows(label, h, position.numel())
+    h, ld, r, keep = _places(label, h, True, position, ends)
     weight = _choice_weight(label, weight, position)
-    r, keep = _places(label, position, ends, h.shape[1], h.dtype)
-    out = h.new_empty((position.shape[0], h.shape[1]))
-    if out.shape[0]:
+    out = h.new_empty(r.T, r.N)
+    if r.T:
         _enqueue(L.lib().lm_combine_rows, h.get_device(), h.device, r, h.data_ptr(), ld, weight.data_ptr(), out.data_ptr())
     del keep
     return out
@@ -1155,15 +1153,14 @@ def combine_rows_grad(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, p
     """The gradients of :func:`combine_rows` to ``h`` (zeros at places of no expert) and to ``weight``."""
     label = "Combine gradient"
     _on_gpu(label, dy, h, weight, position, ends)
-    dy, ldy = _token_rows(label, dy, position.shape[0] if position.ndim == 2 else 0)
-    h, ldh = _token_rows(label, h, position.numel())
-    if dy.dtype is not h.dtype or dy.shape[1] != h.shape[1]:
+    if dy.dtype is not h.dtype or dy.shape[-1:] != h.shape[-1:]:
         raise ValueError(f"{label}: dy {dy.dtype} {tuple(dy.shape)} and h {h.dtype} {tuple(h.shape)} differ.")
+    dy, ldy, _, _ = _places(label, dy, False, position, ends)
+    h, ldh, r, keep = _places(label, h, True, position, ends)
     weight = _choice_weight(label, weight, position)
-    r, keep = _places(label, position, ends, h.shape[1], h.dtype)
-    dh, dweight = h.new_empty(h.shape), weight.new_empty(weight.shape)
-    if position.shape[0]:
-        _enqueue(L.lib().lm_combine_rows_grad, h.get_device(), h.device, r, dy.data_ptr(), ldy, h.data_ptr(), ldh, weight.data_ptr(), dh.data_ptr(),
-              dweight.data_ptr())
+    dh, dweight = h.new_empty(r.T * r.top_k, r.N), torch.empty_like(weight)
+    if r.T:
+        _enqueue(L.lib().lm_combine_rows_grad, h.get_device(), h.device, r, dy.data_ptr(), ldy, h.data_ptr(), ldh, weight.data_ptr(),
+                 dh.data_ptr(), dweight.data_ptr())
     del keep
     return dh, dweight

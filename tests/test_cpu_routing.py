@@ -103,10 +103,11 @@ def test_c_int8_products_refuse(weight, input_dtype):
 def test_c_int8_products_need_their_workspace():
     w = L.WeightStruct(4096, 4096, 64, 128, L.LM_I8, 0, 1, 0)
     handle = L.load_library()
-    need = handle.lm_linear_workspace_size(0, 4, 128, 0, 64, 128, 1, L.LM_I8, L.LM_I8, 1)
-    assert need >= 4 * 128
+    assert handle.lm_linear_workspace_size(0, 4, 128, 0, 64, 128, 1, L.LM_I8, L.LM_I8, 1) == 0  # (quantised by the product itself)
+    need = handle.lm_linear_workspace_size(0, 8, 128, 0, 64, 128, 1, L.LM_I8, L.LM_I8, 1)
+    assert need >= 8 * 128
     for ws, size, want in ((None, 0, L.LM_EWORKSPACE), (4096, need - 1, L.LM_EWORKSPACE), (4100, need, L.LM_EINVAL)):
-        assert handle.lm_linear(4096, 128, ctypes.byref(w), None, None, 4096, 4, L.LM_BF16, L.LM_I8, ws, size, None) == want
+        assert handle.lm_linear(4096, 128, ctypes.byref(w), None, None, 4096, 8, L.LM_BF16, L.LM_I8, ws, size, None) == want
 
 
 def test_cpu_tensors_are_refused():

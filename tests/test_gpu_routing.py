@@ -566,3 +566,59 @@ def test_backward_through_sums_and_views():
         torch.cuda.synchronize()
         for a, b in zip(out, want):
             assert (a == b).all()
+
+
+def test_refusals():
+    logits = torch.zeros(6, 12, device=DEV)
+    zeros = torch.zeros
+    for args, how, text in (((zeros(12, device=DEV), 2), {}, "tokens, experts"), ((logits.double(), 2), {}, "supports"), ((logits, 0), {}, "top_k"),
+                            ((logits, 13), {}, "top_k"), ((logits, 2), dict(score="tanh"), "score"), ((logits, 2), dict(groups=5), "divide"),
+                            ((logits, 2), dict(groups=3, top_groups=4), "top_groups"), ((logits, 5), dict(groups=3, top_groups=1), "top_k"),
+                            ((logits, 2), dict(groups=3, group_best=3), "group_best"), ((logits, 2), dict(groups=12, group_best=2), "group_best"),
+                            ((logits, 2), dict(scale=math.nan), "scale"), ((logits, 2), dict(bias=zeros(11, device=DEV)), "bias"),
+                            ((logits, 2), dict(bias=zeros(12, dtype=BF16, device=DEV)), "bias"), ((logits, 2), dict(bias=zeros(12)), "one GPU"),
+                            ((zeros(2, 1025, device=DEV), 2), {}, "experts"), ((zeros(2, 0, device=DEV), 2), {}, "experts")):
+        with pytest.raises(ValueError, match=text):
+            K.route_topk(*args, **how)
+    r = K.route_topk(logits, 2)
+    for dw, expert, text in ((r.weight[:5], r.expert, "dweight"), (r.weight.double(), r.expert, "dweight"), (r.weight, r.expert.long(), "expert"),
+                             (r.weight, r.expert[:5], "expert"), (r.weight, r.expert.cpu(), "one GPU")):
+        with pytest.raises(ValueError, match=text):
+            K.route_topk_grad(dw, logits, expert)
+    x, h = zeros(6, 16, dtype=BF16, device=DEV), zeros(12, 16, dtype=BF16, device=DEV)
+    at = (r.position, r.ends)
+    bad = (r.position.long(), r.ends), (r.position.view(-1), r.ends), (r.position[:, :0], r.ends), (r.position, r.ends.long()), (r.position, r.ends[:0])
+    for p, e in bad:
+        for call in (lambda: K.dispatch_rows(x, p, e), lambda: K.dispatch_rows_grad(h, p, e), lambda: K.combine_rows(h, r.weight, p, e),
+                     lambda: K.combine_rows_grad(x, h, r.weight, p, e)):
+            with pytest.raises(ValueError):
+                call()
+    for call, text in ((lambda: K.dispatch_rows(h, *at), "6 rows"), (lambda: K.dispatch_rows(x.float(), *at), "supports"),
+                       (lambda: K.dispatch_rows(x[:, :0], *at), "non-empty"), (lambda: K.dispatch_rows_grad(x, *at), "12 rows"),
+                       (lambda: K.combine_rows(x, r.weight, *at), "12 rows"), (lambda: K.combine_rows(h, r.weight.half(), *at), "weight"),
+                       (lambda: K.combine_rows(h, r.weight[:, :1], *at), "weight"), (lambda: K.combine_rows(h.cpu(), r.weight, *at), "GPU"),
+                       (lambda: K.combine_rows_grad(x.half(), h, r.weight, *at), "differ"), (lambda: K.combine_rows_grad(x[:, :8], h, r.weight, *at), "differ"),
+                       (lambda: K.combine_rows_grad(x[0], h, r.weight, *at), "rows")):
+        with pytest.raises(ValueError, match=text):
+            call()
+
+
+def test_places_that_do_not_exist_are_passed_over():
+    """Places outside the rows and ends that pass them: nothing is read or written out of range."""
+    g = _gen(63)
+    x, h, dy = (_normal(g, n, 40, dtype=BF16).to(DEV) for n in (5, 10, 5))
+    w = torch.rand(5, 2, generator=g).to(DEV)
+    position = torch.tensor([[0, 1], [2, 99], [-7, 3], [4, 2**31 - 1], [5, 6]], dtype=torch.int32, device=DEV)
+    for last in (7, 10, 1000, 2**31 - 1):
+        ends = torch.tensor([3, last], dtype=torch.int32, device=DEV)
+        rows = K.dispatch_rows(x, position, ends)
+        assert (rows[0] == x[0]).all() and (rows[4] == x[3]).all() and (rows[6] == x[4]).all()
+        y = K.combine_rows(h, w, position, ends).double()
+        want = w[3, 0].double() * h[4].double()
+        assert ((y[3] - want).abs() <= 2.0**-8 * want.abs() + 1e-30).all()
+        assert (K.dispatch_rows_grad(h, position, ends)[1] == h[2]).all()
+        dh, dw = K.combine_rows_grad(dy, h, w, position, ends)
+        assert (dw[[1, 2, 3], [1, 0, 1]] == 0).all() and torch.isfinite(dw).all()
+    for last in (0, -5):
+        ends = torch.tensor([0, last], dtype=torch.int32, device=DEV)
+        assert (K.combine_rows(h, w, position, ends) == 0).all() and (K.dispatch_rows_grad(h, position, ends) == 0).all()
