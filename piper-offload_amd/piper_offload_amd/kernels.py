@@ -668,8 +668,9 @@ _LAYERS = "mx_linear, int8_linear, grouped_linear, route_experts, dispatch_exper
 # (These calls are as short as 5 us on the GPU: the checks below look at each tensor once.)
 def _raw(label: str, *tensors: torch.Tensor) -> None:
     """Refuse what would lose a gradient: the result has no graph, the layers of :mod:`.linear` give it one."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise NotImplementedError(f"{label} records no gradient; call {_LAYERS}, or run it under torch.no_grad().")
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError(f"{label} records no gradient; call {_LAYERS}, or run it under torch.no_grad().")
 
 
 def _rows(label: str, x: torch.Tensor, cols: int) -> tuple[torch.Tensor, int, int]:
@@ -1063,14 +1064,15 @@ def route_topk_grad(dweight: torch.Tensor, logits: torch.Tensor, expert: torch.T
     label = "Routing gradient"
     _on_gpu(label, dweight, logits, expert)
     _raw(label, dweight, logits)
-    if expert.dtype is not torch.int32 or expert.ndim != 2 or expert.shape[0] != logits.shape[0]:
-        raise ValueError(f"{label}: expert must be int32 [tokens, top_k], got {expert.dtype} {tuple(expert.shape)}.")
-    if dweight.dtype is not torch.float32 or dweight.shape != expert.shape:
-        raise ValueError(f"{label}: dweight must be float32 {tuple(expert.shape)}, got {dweight.dtype} {tuple(dweight.shape)}.")
-    r, keep = _route(label, logits, expert.shape[1], None, score, 1, 1, 1, renormalize, scale)
-    dlogits = logits.new_empty(logits.shape)
+    shape = expert.shape
+    if expert.dtype is not torch.int32 or len(shape) != 2 or shape[0] != logits.shape[0]:
+        raise ValueError(f"{label}: expert must be int32 [tokens, top_k], got {expert.dtype} {tuple(shape)}.")
+    if dweight.dtype is not torch.float32 or dweight.shape != shape:
+        raise ValueError(f"{label}: dweight must be float32 {tuple(shape)}, got {dweight.dtype} {tuple(dweight.shape)}.")
+    r, keep = _route(label, logits, shape[1], None, score, 1, 1, 1, renormalize, scale)
+    dlogits = logits.new_empty(r.T, r.experts)
     dweight, expert = dweight.contiguous(), expert.contiguous()
-    if logits.shape[0]:
+    if r.T:
         _enqueue(L.lib().lm_route_topk_grad, logits.get_device(), logits.device, r, dweight.data_ptr(), expert.data_ptr(), dlogits.data_ptr())
     del keep
     return dlogits
