@@ -102,7 +102,8 @@ static Lin8Plan lin8_plan(int op, int64_t T, int64_t lda, int64_t N, int64_t K, 
     }
   }
   if (!p.few) {
-    p.copy_w = !aligned || K % 16;
+    // (decoded on the way into LDS, rows of codes may lie anywhere; loaded straight into it, not)
+    p.copy_w = quant ? !aligned || K % 16 : K < 16;
     if (p.copy_w) {
       p.ldw = round64(K);
       p.w = take((size_t)E * N * p.ldw);

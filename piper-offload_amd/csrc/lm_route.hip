@@ -883,12 +883,18 @@ static int check_route(const lm_route* r) {
   return LM_OK;
 }
 
+// Waves of a workgroup of k_route (ROUTE_THREADS)
+static int route_waves(int64_t experts) { return experts <= 256 ? 16 : 8; }
 // Tokens of a workgroup: all of them while they are few, so that one launch does; one
-// a wave up to 256 workgroups.
-static int route_block(int64_t T) {
+// a wave up to 4096 tokens, then two (8192 tokens, 64 experts: as fast as one), and more
+// where k_route_place would add up the counts of more than 1024 workgroups.
+static int route_block(int64_t T, int64_t experts) {
   if (T <= 32) return (int)T;
-  if (T <= 4096) return 16;
-  return T <= ROUTE_NEAR ? 32 : 64;
+  const int waves = route_waves(experts);
+  if (T <= 4096) return waves;
+  int block = 2 * waves;
+  while (block < 64 && T > (int64_t)block * 1024) block *= 2;
+  return block;
 }
 static int64_t route_pitch(int64_t experts) { return (experts + 3) & ~(int64_t)3; }
 
@@ -896,7 +902,7 @@ struct RouteSpace {
   size_t none, starts, total;
 };
 static RouteSpace route_space(int64_t T, int64_t experts) {
-  const int64_t block = route_block(T), blocks = (T + block - 1) / block;
+  const int64_t block = route_block(T, experts), blocks = (T + block - 1) / block;
   RouteSpace s{};
   if (blocks <= 1) return s;
   s.none = align256((size_t)(blocks * route_pitch(experts)));
@@ -923,7 +929,7 @@ static RouteArgs route_args(const lm_route* r) {
   a.lanes = 64;
   while (a.lanes * a.groups > 64) a.lanes >>= 1;
   a.per_mul = ((1u << 20) + a.per - 1) / a.per;
-  a.block = a.T > 0 ? route_block(a.T) : 1;
+  a.block = a.T > 0 ? route_block(a.T, a.E) : 1;
   a.blocks = (int)((a.T + a.block - 1) / a.block);
   a.pitch = (int)route_pitch(a.E);
   a.entries = fast_div((uint32_t)(a.block * a.k));
@@ -972,7 +978,7 @@ extern "C" int lm_route_topk(const lm_route* r, float* weight, int32_t* expert, 
   }
   hipStream_t st = (hipStream_t)stream;
   TimedLaunch timed("route", st);
-  const int threads = a.E <= 256 ? 1024 : 512;  // ROUTE_THREADS
+  const int threads = 64 * route_waves(a.E);
   const size_t lds = (a.top_groups < a.groups ? (size_t)threads / 64 * a.pitch * 4 : 0) + (size_t)(a.E + 1) * 4 + (size_t)a.block * a.k * 4;
   ROUTE_BY_TYPE(k_route, dim3((unsigned)(a.blocks > 0 ? a.blocks : 1)), dim3(threads), lds, st, a);
   LAUNCH_CHECK();

@@ -433,3 +433,31 @@ def test_few_rows_in_a_graph_on_another_stream():
             want = K.int8_matmul(x, q, s, activation_dtype=I8)
         torch.cuda.current_stream().wait_stream(side)
         assert (y == want).all()
+
+
+# many rows, weights whose rows start and end anywhere: the last 16 codes of a row in each place of a tile
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("k", [1, 9, 15, 16, 17, 31, 33, 129, 136, 255, 257, 511, 1041])
+def test_rows_of_any_length(k, dtype):
+    g = _gen(k)
+    for t, n in ((70, 100), (300, 4200), (1100, 520)):
+        q, s, w = _weight(g, n, k)
+        store = torch.full((n * k + 37,), 127, dtype=I8, device=DEV)
+        codes = store[5:5 + n * k].view(n, k).copy_(q.to(DEV))
+        x, dy = _normal(g, t, k, dtype=dtype), _normal(g, t, n, dtype=dtype)
+        _check(x, q, s, K.int8_matmul(x.to(DEV), codes, s.to(DEV)), False)
+        _check(x, q, s, K.int8_matmul(x.to(DEV), codes, s.to(DEV), activation_dtype=I8), True)
+        _check_grad(dy, w, K.int8_matmul_input_grad(dy.to(DEV), codes, s.to(DEV)))
+    sizes = [5, 0, 130, 1, 64]
+    q, s, w = _weight(g, len(sizes), 72, k)
+    ends, t = _ends(sizes), 210
+    x, dy = _normal(g, t, k, dtype=dtype), _normal(g, t, 72, dtype=dtype)
+    args = q.to(DEV), s.to(DEV), ends.to(DEV)
+    y, dx = K.grouped_int8_matmul(x.to(DEV), *args), K.grouped_int8_matmul_input_grad(dy.to(DEV), *args)
+    begin = 0
+    for i, end in enumerate(ends.tolist()):
+        if end > begin:
+            _check(x[begin:end], q[i], s[i], y[begin:end], False)
+            _check_grad(dy[begin:end], w[i], dx[begin:end])
+        begin = end
+    assert (y[begin:] == 0).all() and (dx[begin:] == 0).all()
