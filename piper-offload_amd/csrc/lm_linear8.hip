@@ -44,6 +44,29 @@ __global__ __launch_bounds__(256) void k_lin8_prep(LinArgs a, uint8_t* codes, fl
   for (int64_t c = c0 + 4096; c < pitch; c += 2048) *(LM_GLOBAL lm_u32x2*)(to + c) = r.codes<DT>(lin_chunk(x + c, a.K - c));
 }
 
+// Rows of 16 bits copied for k_lin_mm, which reads the last 16 codes of a row that is no
+// whole number of them in one piece: those elements of x that belong to a code of that
+// piece and to none before it, at the piece's end.
+__global__ __launch_bounds__(256) void k_lin8_tail(const uint16_t* src, int64_t lds, int64_t rows, int cols, uint16_t* dst, int ldd) {
+  const int64_t r = (int64_t)blockIdx.x * 4 + wave_index();
+  if (r >= rows) return;
+  const uint16_t* const from = src + r * lds;
+  for (int c = (threadIdx.x & 63) * 8; c < ldd; c += 512) {
+    lm_u32x4 w;
+    if (c < ldd - 16) {
+      w = lin_chunk(from + c, 8);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int i = c + e - (ldd - cols);  // of the last 16
+        const uint32_t x = i >= ldd - 16 ? ((const LM_GLOBAL uint16_t*)from)[i] : 0u;
+        w[e >> 1] = e & 1 ? w[e >> 1] | x << 16 : x;
+      }
+    }
+    store_b128_guarded((LM_GLOBAL lm_u32x4*)(dst + r * ldd + c), w);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -61,6 +84,7 @@ struct Lin8Plan {
   bool few;                  // k_lin_few8, else k_lin_mm
   bool own;                  // k_lin_few8 quantises its rows
   bool copy_x, copy_w;       // rows realigned in the workspace first
+  bool tail;                 // and x's last elements as k_lin8_tail has them
   int64_t pitch, lda, ldw;   // of the codes of x, of 16-bit rows, of the weight (bytes)
   size_t codes, codes_bytes, scales, x, w, part, total;
 };
@@ -95,20 +119,22 @@ static Lin8Plan lin8_plan(int op, int64_t T, int64_t lda, int64_t N, int64_t K, 
     p.codes = take(p.codes_bytes);
     p.scales = take((size_t)T * 4);
   } else {
-    p.copy_x = lda >= (1 << 21) || (!p.few && (!aligned || lda % 8 || inner % 8));
-    if (p.copy_x) {
-      p.lda = round8(inner);
-      p.x = take((size_t)T * p.lda * 2);
-    }
+    p.copy_x = lda >= (1 << 21) || (!p.few && (!aligned || lda % 8 || inner % 8 || (op == LIN_FORWARD && K % 16)));
+    if (p.copy_x) p.lda = round8(inner);
+    if (p.copy_x && p.few) p.x = take((size_t)T * p.lda * 2);
   }
   if (!p.few) {
-    // (decoded on the way into LDS, rows of codes may lie anywhere; loaded straight into it, not)
-    p.copy_w = quant ? !aligned || K % 16 : K < 16;
+    // (decoded on the way into LDS, rows of codes may lie anywhere, if there is one piece,
+    // or tile, of them; loaded straight into it, not)
+    p.copy_w = quant ? !aligned || K % 16 : K < (op == LIN_FORWARD ? 16 : 256) && K % 16;
     if (p.copy_w) {
       p.ldw = round64(K);
       p.w = take((size_t)E * N * p.ldw);
     }
-    p.mm.len = quant ? round16(K) / 2 : round8(inner);
+    p.tail = op == LIN_FORWARD && !quant && !p.copy_w && K % 16;
+    p.mm.len = quant ? round16(K) / 2 : p.tail ? round16(K) : round8(inner);
+    if (p.tail) p.lda = p.mm.len;
+    if (p.copy_x) p.x = take((size_t)T * p.lda * 2);
     p.mm.splits = 1;
     const int64_t J = op == LIN_FORWARD ? N : K;
     lin_tiling(p.mm, op, T, J, p.mm.len, E, !quant, false);
@@ -166,9 +192,10 @@ static int lin8_setup(LinArgs& a, const Lin8Plan& p, int op, int dtype, void* wo
   uint8_t* base = (uint8_t*)workspace;
   TimedLaunch timed("linear_prep", st);
   if (p.copy_x) {
-    const int64_t n = (a.T * (p.lda / 8) + 255) / 256;
+    const int64_t n = p.tail ? (a.T + 3) / 4 : (a.T * (p.lda / 8) + 255) / 256;
     if (n > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
-    hipLaunchKernelGGL(k_lin_align, dim3((unsigned)n), dim3(256), 0, st, (const uint16_t*)a.a, a.lda, a.T, op == LIN_FORWARD ? a.K : a.N,
+    if (p.tail) hipLaunchKernelGGL(k_lin8_tail, dim3((unsigned)n), dim3(256), 0, st, (const uint16_t*)a.a, a.lda, a.T, (int)a.K, (uint16_t*)(base + p.x), (int)p.lda);
+    else hipLaunchKernelGGL(k_lin_align, dim3((unsigned)n), dim3(256), 0, st, (const uint16_t*)a.a, a.lda, a.T, op == LIN_FORWARD ? a.K : a.N,
                        (uint16_t*)(base + p.x), p.lda);
     LAUNCH_CHECK();
     a.a = base + p.x;

@@ -178,13 +178,6 @@ DEV lm_u32x4 mm_frag(const lds_u8* t, uint32_t at, int f) {
   return lm_u32x4{__builtin_bit_cast(lm_u32x2, lo)[0], __builtin_bit_cast(lm_u32x2, lo)[1],
                   __builtin_bit_cast(lm_u32x2, hi)[0], __builtin_bit_cast(lm_u32x2, hi)[1]};
 }
-// 16 bytes without the first n (0 .. 15), zeros after them
-DEV lm_u32x4 mm_drop(lm_u32x4 v, int n) {
-  if (n & 4) v = lm_u32x4{v[1], v[2], v[3], 0};
-  if (n & 8) v = lm_u32x4{v[2], v[3], 0, 0};
-  return lm_u32x4{__builtin_amdgcn_alignbyte(v[1], v[0], n & 3), __builtin_amdgcn_alignbyte(v[2], v[1], n & 3),
-                  __builtin_amdgcn_alignbyte(v[3], v[2], n & 3), __builtin_amdgcn_alignbyte(0, v[3], n & 3)};
-}
 // The compiler would keep this value plus every buffer's address in a register
 // of its own across the loop; like this it adds the buffer's offset in the read.
 DEV uint32_t mm_hide(uint32_t x) {
@@ -235,6 +228,9 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
     jstep = 2 * CS * ldb;
   } else {
     if (!lin_pick<BM, BN>(a, jend, t)) return;
+    // KS8, rows of no whole 16-byte pieces: the last tile ends where they end, so no
+    // piece of 16 codes passes a row's end (the columns that two tiles have are computed alike)
+    if (JK == KS8 && a.ldw == a.K && a.K % 16 != 0 && t.j0 + BN > a.K) t.j0 = a.K - BN;
     len = t.group == a.experts ? 0 : a.len;
     if constexpr (Q4) {
       lda = a.K >> 2;  // two codes a byte, in units of two bytes as the others
@@ -248,9 +244,8 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
     constexpr bool MX = P::MX || Q4;
     const int64_t ldw = MX ? a.K : a.ldw;
     ldb = Q4 ? a.K >> 2 : ldw;
-    const int64_t j0 = JK == KS8 ? 0 : t.j0;  // (KS8: in the lanes' offsets)
-    const int64_t first = OP == LIN_FORWARD ? (t.group * a.N + j0) * ldw : t.group * a.N * ldw + j0;
-    const int64_t count = OP == LIN_FORWARD ? (a.N - j0) * ldw : a.N * ldw - j0;
+    const int64_t first = OP == LIN_FORWARD ? (t.group * a.N + t.j0) * ldw : t.group * a.N * ldw + t.j0;
+    const int64_t count = OP == LIN_FORWARD ? (a.N - t.j0) * ldw : a.N * ldw - t.j0;
     jp = (const uint8_t*)a.w + (MX ? first >> 1 : I8 ? first : first * 2);
     jbytes = MX ? count >> 1 : I8 ? count : count * 2;
     jstep = OP == LIN_FORWARD ? (P::MX ? 16 : I8 ? 0 : 64) : CS * (MX ? ldw >> 1 : I8 ? ldw : ldw * 2);
@@ -354,23 +349,15 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
     const uint32_t in = left32(il, false), jn = left32(jl, false);
     // KS4: this thread decodes 16 codes of contraction row kr.  (Its loads are
     // issued for every stage, inside the weight or not: the waits count them.)
-    // KS8 does the same; KC8: 16 codes of column kr.  INT8 rows may start anywhere and
-    // have any length from 16 on (`tight`; shorter ones are copied to rows with zeros after
-    // them): the 16 codes that would pass the row's end are its last 16, shifted, so no
-    // load leaves the row.
+    // KS8 does the same; KC8: 16 codes of column kr, a row's last 16 from there on: x
+    // holds its elements in that order (k_lin8_tail), zeros where they were had before.
     const int kr = JK == KC8 ? tid >> 1 : tid / (BN / 16), kc = JK == KC8 ? tid & 1 : tid % (BN / 16);
     lm_u32x2 code[JK == KS4 ? 2 : 1];
     lm_u32x4 code8[REG && JK != KS4 ? 2 : 1];
     uint32_t code_s[2];
     const bool cin = JK == KC8 ? t.j0 + kr < a.N : t.j0 + kc * 16 < a.K;
-    const bool tight = a.ldw == a.K;
-    const int k8 = (int)a.K;
-    // codes of this thread's 16 that are past the row's end, 0 .. 15 where any are not
-    auto past = [&](int st) {
-      const int n = (JK == KC8 ? st * CS : (int)t.j0) + kc * 16 + 16 - k8;
-      return tight && n > 0 ? n : 0;
-    };
-    const uint32_t co = !cin ? LIN_OUT : JK == KS4 ? (uint32_t)(kr * (a.K >> 1) + kc * 8) : JK == KS8 ? (uint32_t)(kr * a.ldw + t.j0 + kc * 16 - past(0)) : (uint32_t)(kr * a.ldw + kc * 16);
+    const uint32_t co = !cin ? LIN_OUT : JK == KS4 ? (uint32_t)(kr * (a.K >> 1) + kc * 8) : (uint32_t)(kr * a.ldw + (JK == KC8 ? 0 : kc * 16));
+    const int klast = (int)a.ldw - 16;
     const uint32_t cb = (uint32_t)((t.j0 + kc * 16) >> 5);  // block of the row
     const uint32_t cso = a.swizzled ? (cb >> 2) * 512 + (kr & 31) * 16 + (cb & 3) : (uint32_t)(kr * nb) + cb;
     auto load_codes = [&](int st, int set) {
@@ -381,11 +368,8 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
         jl -= jstep;
         uint32_t o = co;
         if constexpr (JK == KC8) {
-          o += cin ? st * CS : 0;
-          if ((st + 1) * CS > k8) {  // (a row's last stage)
-            const int n = past(st);
-            o = !cin || n >= 16 ? LIN_OUT : o - n;
-          }
+          const int c = st * CS + kc * 16;
+          o += c < klast ? c : klast;
         }
         code8[set] = __builtin_bit_cast(lm_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, (int)o, 0, 0));
       }
@@ -409,9 +393,8 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
         code_s[set] = __builtin_amdgcn_raw_buffer_load_b8(rs, (int)(co < left ? cso : LIN_OUT), 0, 0);
       }
     };
-    auto store_codes = [&](int st, lds_u8* tj, int set) {
+    auto store_codes = [&](lds_u8* tj, int set) {
       if constexpr (JK == KC8 || JK == KS8) {
-        if (tight && (JK == KC8 ? (st + 1) * CS > k8 : t.j0 + BN > a.K)) code8[set] = mm_drop(code8[set], past(st));
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const lm_u32x4 v = lin_decode8i<HALF, JK == KS8>(code8[set][2 * c], code8[set][2 * c + 1], JK == KS8 ? u2f(code_s[set]) : 1.0f);
@@ -536,7 +519,7 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           load_codes(kb + b, 0);
-          store_codes(kb + b, tj[b], 0);
+          store_codes(tj[b], 0);
         }
         load_codes(kb + 2, 0);
       }
@@ -570,7 +553,7 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
           }
           lin_barrier();
           multiply();
-          store_codes(st + b + 2, tj[(b + 2) & 3], b & 1);
+          store_codes(tj[(b + 2) & 3], b & 1);
           if constexpr (PP) lin_barrier();
         }
       };

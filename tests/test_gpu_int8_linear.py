@@ -437,10 +437,10 @@ def test_few_rows_in_a_graph_on_another_stream():
 
 # many rows, weights whose rows start and end anywhere: the last 16 codes of a row in each place of a tile
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
-@pytest.mark.parametrize("k", [1, 9, 15, 16, 17, 31, 33, 129, 136, 255, 257, 511, 1041])
+@pytest.mark.parametrize("k", [1, 9, 15, 16, 17, 31, 33, 129, 136, 255, 257, 264, 511, 1041])
 def test_rows_of_any_length(k, dtype):
     g = _gen(k)
-    for t, n in ((70, 100), (300, 4200), (1100, 520)):
+    for t, n in ((70, 100), (300, 4200), (1100, 520), (30, 33)):
         q, s, w = _weight(g, n, k)
         store = torch.full((n * k + 37,), 127, dtype=I8, device=DEV)
         codes = store[5:5 + n * k].view(n, k).copy_(q.to(DEV))
@@ -461,3 +461,17 @@ def test_rows_of_any_length(k, dtype):
             _check_grad(dy[begin:end], w[i], dx[begin:end])
         begin = end
     assert (y[begin:] == 0).all() and (dx[begin:] == 0).all()
+
+
+def test_the_same_call_gives_the_same_bits():
+    """Columns that two tiles have in common, split sums, rows quantised by every workgroup."""
+    g = _gen(71)
+    for t, n, k in ((300, 260, 1041), (40, 3000, 257), (3, 500, 999), (700, 96, 4099)):
+        q, s, _ = _weight(g, n, k)
+        q, s = q.to(DEV), s.to(DEV)
+        x, dy = _normal(g, t, k, dtype=BF16).to(DEV), _normal(g, t, n, dtype=BF16).to(DEV)
+        first = None
+        for _ in range(5):
+            out = K.int8_matmul(x, q, s), K.int8_matmul(x, q, s, activation_dtype=I8), K.int8_matmul_input_grad(dy, q, s)
+            first = first or out
+            assert all((a == b).all() for a, b in zip(first, out))
