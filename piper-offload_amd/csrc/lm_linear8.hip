@@ -6,6 +6,15 @@
 //   input gradient  dx[t,k] = sum_n dy[t,n] W[n,k] (straight through the rounding of 8-bit inputs)
 //
 // The products of one weight, or of one weight per group of rows.
+//
+// The input gradient rounds s q to 16 bits: s lies along its sum, so the product cannot be
+// multiplied by it afterwards, and to round dy s instead is off by as much.
+//
+// Many rows (k_lin_mm): codes times codes are bound by the power that the matrix unit
+// may take, 4096 rows of [14336, 4096] 232 us (2.07 POP/s at 1.86 GHz, 64% of the cycles
+// busy; the library's product of 8192^3 reaches 2.2).  Decoded to 16 bits, 2048 rows of the
+// same 205 us (1.17 PFLOP/s), input gradient in two parts with their join 222 (the
+// library's bf16 product of 8192^3: 1.33).
 #include "lm_impl.h"
 #include "lm_linear8.h"
 #include "lm_linear8_few.h"
@@ -14,7 +23,8 @@
 // The rows' codes, at a pitch of whole pieces that are filled up with zeros, and their
 // scales: a workgroup a row, whose first 4096 values stay in registers between the two.
 // The workgroups after those copy weights whose rows are not whole 16-byte pieces to
-// rows that are (`aligned`), a wave a row.  Bound by memory.
+// rows that are (`aligned`), a wave a row.  Bound by memory: 4096 rows of 4096 9.8 us
+// (50 MB, 5.1 TB/s).
 template <int DT>
 __global__ __launch_bounds__(256) void k_lin8_prep(LinArgs a, uint8_t* codes, float* scales, int64_t pitch, uint8_t* aligned, int64_t ldw) {
   __shared__ uint32_t red[4];
@@ -78,6 +88,8 @@ static int64_t round64(int64_t x) { return (x + 63) & ~(int64_t)63; }
 // first weights are on their way: one row of [1024, 4096] 6.1 us, after a launch of
 // k_lin8_prep 8; four rows of [4096, 4096] 10.9, as much as the two launches, but for the host.
 constexpr int64_t LIN8_OWN_ROWS = 4, LIN8_OWN_BYTES = 32768;
+
+constexpr int64_t LIN8_GROUPS = 1 << 24;  // workgroups of 256 a launch can have
 
 struct Lin8Plan {
   LinPlan mm;                // tile and splits of k_lin_mm
@@ -152,7 +164,7 @@ template <int DT, bool Q8, bool OWN, int MF, int CF, int NW, int UN>
 static int launch_few8(const LinArgs& a, const uint8_t* codes, int64_t pitch, hipStream_t st) {
   TimedLaunch timed("linear_few", st);
   const int64_t n = lin_tiles<16 * MF>(a.T, a.experts, a.ends != nullptr) * ((a.N + 16 * CF - 1) / (16 * CF));
-  if (n > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+  if (n >= LIN8_GROUPS * 4 / NW) return fail(LM_EUNSUPPORTED, "product too large for one launch");
   hipLaunchKernelGGL((k_lin_few8<DT, Q8, OWN, MF, CF, NW, UN>), dim3((unsigned)n), dim3(NW * 64), OWN ? (size_t)(a.T * pitch) : 0, st, a, codes, pitch);
   LAUNCH_CHECK();
   return LM_OK;
@@ -193,7 +205,7 @@ static int lin8_setup(LinArgs& a, const Lin8Plan& p, int op, int dtype, void* wo
   TimedLaunch timed("linear_prep", st);
   if (p.copy_x) {
     const int64_t n = p.tail ? (a.T + 3) / 4 : (a.T * (p.lda / 8) + 255) / 256;
-    if (n > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+    if (n >= LIN8_GROUPS) return fail(LM_EUNSUPPORTED, "product too large for one launch");
     if (p.tail) hipLaunchKernelGGL(k_lin8_tail, dim3((unsigned)n), dim3(256), 0, st, (const uint16_t*)a.a, a.lda, a.T, (int)a.K, (uint16_t*)(base + p.x), (int)p.lda);
     else hipLaunchKernelGGL(k_lin_align, dim3((unsigned)n), dim3(256), 0, st, (const uint16_t*)a.a, a.lda, a.T, op == LIN_FORWARD ? a.K : a.N,
                        (uint16_t*)(base + p.x), p.lda);
@@ -203,7 +215,7 @@ static int lin8_setup(LinArgs& a, const Lin8Plan& p, int op, int dtype, void* wo
   }
   if (p.codes_bytes > 0 || p.copy_w) {
     const int64_t rows = p.codes_bytes > 0 ? a.T : 0, n = rows + (p.copy_w ? (a.experts * a.N + 3) / 4 : 0);
-    if (n > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+    if (n >= LIN8_GROUPS) return fail(LM_EUNSUPPORTED, "product too large for one launch");
     float* const scales = rows ? (float*)(base + p.scales) : nullptr;
     if (dtype == LM_F16) hipLaunchKernelGGL((k_lin8_prep<F16>), dim3((unsigned)n), dim3(256), 0, st, a, base + p.codes, scales, p.pitch, base + p.w, p.ldw);
     else hipLaunchKernelGGL((k_lin8_prep<BF16>), dim3((unsigned)n), dim3(256), 0, st, a, base + p.codes, scales, p.pitch, base + p.w, p.ldw);

@@ -42,7 +42,7 @@
 // Bound by the matrix unit, on a clock that falls under it, and by the LDS reads
 // beside it: bf16 [8192, 8192] at 8192 rows 1.33 PFLOP/s; MXFP4 [14336, 4096] at
 // 2048 rows 1.13 forward (matrix unit busy 63% of the cycles) and 1.09 for the input
-// gradient with its join, at 4096 rows with 4-bit inputs 3.4 (46%).
+// gradient with its join, at 4096 rows with 4-bit inputs 3.4 (46%).  INT8: lm_linear8.hip.
 #pragma once
 #include <type_traits>
 

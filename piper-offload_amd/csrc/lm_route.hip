@@ -9,6 +9,12 @@
 //
 // An expert with logit (or bias) -inf is closed.  Choices that no expert is left
 // for are -1 with weight 0 and come last.
+//
+// A token is a wave's: lane l has the experts l, l + 64, ... in registers, a maximum
+// over the wave is six DPP steps, and the choice is that maximum taken k times.  Bound
+// by instructions: 16384 tokens, 256 experts in 8 groups, 8 of them chosen 34 us, 660
+// vector and as many scalar instructions a token, the vector unit issuing 70% of the
+// time (its bytes alone: 4 us).  8192 tokens, 64 experts, 4 chosen: 8 us; 8 tokens: 4.
 #include "lm_impl.h"
 #include "lm_route.h"
 
@@ -624,58 +630,58 @@ __global__ __launch_bounds__(1024) void k_route_place(RouteArgs a) {
   for (int i = tid + 1024; i < n; i += 1024) place(i, expert[i], position[i]);
 }
 
-// The gradient to the logits.  g = d loss / d w, for the chosen experts j:
+// The gradient to the logits, a wave a token: 8192 tokens, 64 experts 4.8 us, most of it
+// a launch's ends.  g = d loss / d w, for the chosen experts j:
 //   renormalised   w_j (g_j - sum_i g_i w_i / scale), for sigmoid times 1 - p_j
 //   sigmoid        w_j g_j (1 - p_j)
 //   softmax        w_j g_j - p_e sum_i g_i w_i, the second term for every expert e
 template <int DT, int P>
 __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a, const float* dweight, void* out) {
   const int lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * 4 + wave_index();
-  if (t >= a.T) return;
-  int mine = lane < a.k ? a.expert[t * a.k + lane] : -1;
-  const bool on = mine >= 0 && mine < a.E;
-  const float g = on ? dweight[t * a.k + lane] : 0.0f;
-  const float x = on ? route_load<DT>(a.logits, t * a.ld + mine) : 0.0f;
-  const float e = a.sigmoid ? (x < 0.0f ? x : 0.0f) : x, z = expf(-__builtin_fabsf(x));
-  const float q = a.sigmoid ? 1.0f / (1.0f + z) : 1.0f;
-  const float rest = a.sigmoid ? (x < 0.0f ? 1.0f : z) * q : 1.0f;  // 1 - p of sigmoid
-  float d[P] = {}, mine_d;
-  if (a.renormalize) {
-    const float top = route_fmax(on ? e : -INFINITY), r = on ? expf(e - top) * q : 0.0f, p = r / route_sum(r);
-    const float mean = route_sum(on ? g * p : 0.0f);
-    mine_d = a.scale * p * (g - mean) * rest;
-  } else if (a.sigmoid) {
-    mine_d = a.scale * (expf(e) * q) * g * rest;
-  } else {
-    float v[P], s[P];
+  for (int64_t t = (int64_t)blockIdx.x * 4 + wave_index(); t < a.T; t += (int64_t)gridDim.x * 4) {
+    int mine = lane < a.k ? a.expert[t * a.k + lane] : -1;
+    const bool on = mine >= 0 && mine < a.E;
+    const float g = on ? dweight[t * a.k + lane] : 0.0f;
+    const float x = on ? route_load<DT>(a.logits, t * a.ld + mine) : 0.0f;
+    const float e = a.sigmoid ? (x < 0.0f ? x : 0.0f) : x, z = expf(-__builtin_fabsf(x));
+    const float q = a.sigmoid ? 1.0f / (1.0f + z) : 1.0f;
+    const float rest = a.sigmoid ? (x < 0.0f ? 1.0f : z) * q : 1.0f;  // 1 - p of sigmoid
+    float d[P] = {}, mine_d;
+    if (a.renormalize) {
+      const float top = route_fmax(on ? e : -INFINITY), r = on ? expf(e - top) * q : 0.0f, p = r / route_sum(r);
+      const float mean = route_sum(on ? g * p : 0.0f);
+      mine_d = a.scale * p * (g - mean) * rest;
+    } else if (a.sigmoid) {
+      mine_d = a.scale * (expf(e) * q) * g * rest;
+    } else {
+      float v[P], s[P];
 #pragma unroll
-    for (int i = 0; i < P; ++i) v[i] = lane + 64 * i < a.E ? route_load<DT>(a.logits, t * a.ld + lane + 64 * i) : -INFINITY;
-    route_scores<float, false, P>(v, false, s);
-    float p = 0.0f;
+      for (int i = 0; i < P; ++i) v[i] = lane + 64 * i < a.E ? route_load<DT>(a.logits, t * a.ld + lane + 64 * i) : -INFINITY;
+      route_scores<float, false, P>(v, false, s);
+      float p = 0.0f;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const float o = __shfl(s[i], mine & 63);
+        if (mine >> 6 == i) p = o;
+      }
+      mine_d = a.scale * p * g;
+      const float sum = route_sum(on ? mine_d : 0.0f);
+#pragma unroll
+      for (int i = 0; i < P; ++i) d[i] = v[i] == -INFINITY ? 0.0f : -s[i] * sum;
+    }
+    for (uint64_t left = __ballot(on); left; left &= left - 1) {
+      const int j = __builtin_ctzll(left), to = __builtin_amdgcn_readlane(mine, j);
+      const float add = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(mine_d), j));
+#pragma unroll
+      for (int i = 0; i < P; ++i) d[i] += lane + 64 * i == to ? add : 0.0f;
+    }
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const float o = __shfl(s[i], mine & 63);
-      if (mine >> 6 == i) p = o;
-    }
-    mine_d = a.scale * p * g;
-    const float sum = route_sum(on ? mine_d : 0.0f);
-#pragma unroll
-    for (int i = 0; i < P; ++i) d[i] = v[i] == -INFINITY ? 0.0f : -s[i] * sum;
-  }
-  for (uint64_t left = __ballot(on); left; left &= left - 1) {
-    const int j = __builtin_ctzll(left), to = __builtin_amdgcn_readlane(mine, j);
-    const float add = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(mine_d), j));
-#pragma unroll
-    for (int i = 0; i < P; ++i)
-      if (lane + 64 * i == to) d[i] += add;
-  }
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const int64_t at = t * a.E + lane + 64 * i;
-    if (lane + 64 * i < a.E) {
-      if constexpr (DT == F32) ((float*)out)[at] = d[i];
-      else ((uint16_t*)out)[at] = bits_dt<DT>(d[i]);
+      const int64_t at = t * a.E + lane + 64 * i;
+      if (lane + 64 * i < a.E) {
+        if constexpr (DT == F32) ((float*)out)[at] = d[i];
+        else ((uint16_t*)out)[at] = bits_dt<DT>(d[i]);
+      }
     }
   }
 }
@@ -722,7 +728,8 @@ DEV void rows_store(uint16_t* p, lm_u32x4 w, int64_t left) {
 // Rows of choices go past the caches, both ways: there are top_k of them for every
 // row of a token, and each is read or written once (8192 x 2048, four choices: rows
 // out 34 -> 26 us, back 33 -> 28, gradients 58 -> 48).  Rows of tokens do not: with
-// both past the caches rows out take 31 us, gradients 53.
+// both past the caches rows out take 31 us, gradients 53.  Bound by memory: 6.3 TB/s out,
+// 5.6 back, 5.7 the gradients, where a copy reaches 5.1 to 6.1.
 template <bool NT, int M>
 DEV void rows_load(lm_u32x4 (&w)[M], const uint16_t* const (&p)[M], int64_t left) {
   if (left >= 8) {
@@ -738,9 +745,10 @@ DEV void rows_load(lm_u32x4 (&w)[M], const uint16_t* const (&p)[M], int64_t left
 // columns each and the next ones after that; blockIdx.y shares the columns out.
 template <int WPT>
 struct RowsAt {
-  int64_t t, c0, step;
+  int64_t t, next, c0, step;
   DEV RowsAt() {
     t = WPT == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave_index();
+    next = (int64_t)gridDim.x * (WPT == 4 ? 1 : 4);
     c0 = ((int64_t)blockIdx.y * WPT + (WPT == 4 ? wave_index() : 0)) * 512 + (threadIdx.x & 63) * 8;
     step = (int64_t)gridDim.y * WPT * 512;
   }
@@ -756,114 +764,116 @@ DEV void rows_places(const RowsArgs& a, int64_t t, int j0, int end, int (&p)[4])
 
 template <int WPT>
 __global__ __launch_bounds__(256) void k_rows_out(RowsArgs a) {
-  const RowsAt<WPT> at;
-  if (at.t >= a.T) return;
+  RowsAt<WPT> at;
   const int end = rows_end(a), all = (int)(a.T * a.k);
-  for (int64_t c = at.c0; c < a.N; c += at.step) {
-    lm_u32x4 w[1];
-    const uint16_t* const p[1] = {(const uint16_t*)a.x + at.t * a.ld + c};
-    rows_load<false>(w, p, a.N - c);
-    for (int j = 0; j < a.k; ++j) {
-      const int to = a.position[at.t * a.k + j];
-      if (to < 0 || to >= all) continue;
-      rows_store<true>((uint16_t*)a.out + to * a.N + c, to < end ? w[0] : lm_u32x4{}, a.N - c);
+  for (; at.t < a.T; at.t += at.next)
+    for (int64_t c = at.c0; c < a.N; c += at.step) {
+      lm_u32x4 w[1];
+      const uint16_t* const p[1] = {(const uint16_t*)a.x + at.t * a.ld + c};
+      rows_load<false>(w, p, a.N - c);
+      for (int j = 0; j < a.k; ++j) {
+        const int to = a.position[at.t * a.k + j];
+        if (to < 0 || to >= all) continue;
+        rows_store<true>((uint16_t*)a.out + to * a.N + c, to < end ? w[0] : lm_u32x4{}, a.N - c);
+      }
     }
-  }
 }
 
 template <int DT, bool WEIGHTS, int WPT>
 __global__ __launch_bounds__(256) void k_rows_back(RowsArgs a) {
-  const RowsAt<WPT> at;
-  if (at.t >= a.T) return;
+  RowsAt<WPT> at;
   const int end = rows_end(a);
-  for (int64_t c = at.c0; c < a.N; c += at.step) {
-    float s[8] = {};
-    for (int j0 = 0; j0 < a.k; j0 += 4) {
-      int p[4];
-      rows_places(a, at.t, j0, end, p);
-      lm_u32x4 w[4];
-      const uint16_t* from[4];  // (row 0 instead of none: it is there)
-      float by[4];
+  for (; at.t < a.T; at.t += at.next)
+    for (int64_t c = at.c0; c < a.N; c += at.step) {
+      float s[8] = {};
+      for (int j0 = 0; j0 < a.k; j0 += 4) {
+        int p[4];
+        rows_places(a, at.t, j0, end, p);
+        lm_u32x4 w[4];
+        const uint16_t* from[4];  // (row 0 instead of none: it is there)
+        float by[4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        from[n] = (const uint16_t*)a.h + (p[n] < 0 ? 0 : p[n]) * a.ldh + c;
-        by[n] = WEIGHTS && p[n] >= 0 ? a.weight[at.t * a.k + j0 + n] : 1.0f;
+        for (int n = 0; n < 4; ++n) {
+          from[n] = (const uint16_t*)a.h + (p[n] < 0 ? 0 : p[n]) * a.ldh + c;
+          by[n] = WEIGHTS && p[n] >= 0 ? a.weight[at.t * a.k + j0 + n] : 1.0f;
+        }
+        rows_load<true>(w, from, a.N - c);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          if (p[n] < 0) continue;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) s[i] = __builtin_fmaf(by[n], val_dt<DT>(i & 1 ? w[n][i >> 1] >> 16 : w[n][i >> 1] & 0xffffu), s[i]);
+        }
       }
-      rows_load<true>(w, from, a.N - c);
+      lm_u32x4 w;
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        if (p[n] < 0) continue;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s[i] = __builtin_fmaf(by[n], val_dt<DT>(i & 1 ? w[n][i >> 1] >> 16 : w[n][i >> 1] & 0xffffu), s[i]);
-      }
+      for (int i = 0; i < 4; ++i) w[i] = (uint32_t)bits_dt<DT>(s[2 * i]) | (uint32_t)bits_dt<DT>(s[2 * i + 1]) << 16;
+      rows_store<false>((uint16_t*)a.out + at.t * a.N + c, w, a.N - c);
     }
-    lm_u32x4 w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)bits_dt<DT>(s[2 * i]) | (uint32_t)bits_dt<DT>(s[2 * i + 1]) << 16;
-    rows_store<false>((uint16_t*)a.out + at.t * a.N + c, w, a.N - c);
-  }
 }
 
 // Gradients of the weighted sums, for four choices of a token at a time.
 template <int DT, int WPT>
 __global__ __launch_bounds__(256) void k_rows_back_grad(RowsArgs a) {
   __shared__ float red[4][4];
-  const RowsAt<WPT> at;
-  if (at.t >= a.T) return;  // (with WPT 4 all waves or none)
+  RowsAt<WPT> at;
   const int end = rows_end(a), all = (int)(a.T * a.k), lane = threadIdx.x & 63;
-  for (int j0 = 0; j0 < a.k; j0 += 4) {
-    int p[4], to[4];
-    rows_places(a, at.t, j0, all, to);
-    rows_places(a, at.t, j0, end, p);
-    float by[4], sum[4] = {};
+  for (; at.t < a.T; at.t += at.next)  // (with WPT 4 the same for all waves)
+    for (int j0 = 0; j0 < a.k; j0 += 4) {
+      int p[4], to[4];
+      rows_places(a, at.t, j0, all, to);
+      rows_places(a, at.t, j0, end, p);
+      float by[4], sum[4] = {};
 #pragma unroll
-    for (int n = 0; n < 4; ++n) by[n] = p[n] < 0 ? 0.0f : a.weight[at.t * a.k + j0 + n];
-    for (int64_t c = at.c0; c < a.N; c += at.step) {
-      lm_u32x4 w[4], dy[1];
-      const uint16_t* from[4];
-      const uint16_t* const x[1] = {(const uint16_t*)a.x + at.t * a.ld + c};
+      for (int n = 0; n < 4; ++n) by[n] = p[n] < 0 ? 0.0f : a.weight[at.t * a.k + j0 + n];
+      for (int64_t c = at.c0; c < a.N; c += at.step) {
+        lm_u32x4 w[4], dy[1];
+        const uint16_t* from[4];
+        const uint16_t* const x[1] = {(const uint16_t*)a.x + at.t * a.ld + c};
 #pragma unroll
-      for (int n = 0; n < 4; ++n) from[n] = (const uint16_t*)a.h + (p[n] < 0 ? 0 : p[n]) * a.ldh + c;
-      rows_load<false>(dy, x, a.N - c);
-      rows_load<true>(w, from, a.N - c);
+        for (int n = 0; n < 4; ++n) from[n] = (const uint16_t*)a.h + (p[n] < 0 ? 0 : p[n]) * a.ldh + c;
+        rows_load<false>(dy, x, a.N - c);
+        rows_load<true>(w, from, a.N - c);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        lm_u32x4 dh = {};
-        if (p[n] >= 0) {
+        for (int n = 0; n < 4; ++n) {
+          lm_u32x4 dh = {};
+          if (p[n] >= 0) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float lo = val_dt<DT>(dy[0][i] & 0xffffu), hi = val_dt<DT>(dy[0][i] >> 16);
-            sum[n] = __builtin_fmaf(lo, val_dt<DT>(w[n][i] & 0xffffu), sum[n]);
-            sum[n] = __builtin_fmaf(hi, val_dt<DT>(w[n][i] >> 16), sum[n]);
-            dh[i] = (uint32_t)bits_dt<DT>(by[n] * lo) | (uint32_t)bits_dt<DT>(by[n] * hi) << 16;
+            for (int i = 0; i < 4; ++i) {
+              const float lo = val_dt<DT>(dy[0][i] & 0xffffu), hi = val_dt<DT>(dy[0][i] >> 16);
+              sum[n] = __builtin_fmaf(lo, val_dt<DT>(w[n][i] & 0xffffu), sum[n]);
+              sum[n] = __builtin_fmaf(hi, val_dt<DT>(w[n][i] >> 16), sum[n]);
+              dh[i] = (uint32_t)bits_dt<DT>(by[n] * lo) | (uint32_t)bits_dt<DT>(by[n] * hi) << 16;
+            }
           }
+          if (to[n] >= 0) rows_store<true>((uint16_t*)a.out + to[n] * a.N + c, dh, a.N - c);
         }
-        if (to[n] >= 0) rows_store<true>((uint16_t*)a.out + to[n] * a.N + c, dh, a.N - c);
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) sum[n] = route_sum(sum[n]);
+      if constexpr (WPT == 4) {
+        __syncthreads();  // (the sums before these are read)
+        if (lane == 0) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) red[n][wave_index()] = sum[n];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < 4; ++n) sum[n] = red[n][0] + red[n][1] + red[n][2] + red[n][3];
+      }
+      if (threadIdx.x == 0 || (WPT == 1 && lane == 0)) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          if (j0 + n < a.k) a.dweight[at.t * a.k + j0 + n] = p[n] < 0 ? 0.0f : sum[n];
       }
     }
-#pragma unroll
-    for (int n = 0; n < 4; ++n) sum[n] = route_sum(sum[n]);
-    if constexpr (WPT == 4) {
-      __syncthreads();  // (the sums before these are read)
-      if (lane == 0) {
-#pragma unroll
-        for (int n = 0; n < 4; ++n) red[n][wave_index()] = sum[n];
-      }
-      __syncthreads();
-#pragma unroll
-      for (int n = 0; n < 4; ++n) sum[n] = red[n][0] + red[n][1] + red[n][2] + red[n][3];
-    }
-    if (threadIdx.x == 0 || (WPT == 1 && lane == 0)) {
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-        if (j0 + n < a.k) a.dweight[at.t * a.k + j0 + n] = p[n] < 0 ? 0.0f : sum[n];
-    }
-  }
 }
 
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
+constexpr int64_t ROWS_GRID = 1 << 22;  // workgroups that take a token after the other (a launch has fewer than 2^32 threads)
+
 static int check_route(const lm_route* r) {
   if (!r) return fail(LM_EINVAL, "routing needs its description");
   if (r->dtype != LM_F32 && r->dtype != LM_BF16 && r->dtype != LM_F16) return fail(LM_EUNSUPPORTED, "routing takes fp32, bf16 and fp16 logits");
@@ -877,7 +887,7 @@ static int check_route(const lm_route* r) {
     return fail(LM_EINVAL, "group_best must be 1 or 2 and at most the experts of a group");
   if (r->top_k < 1 || r->top_k > LM_ROUTE_MAX_BEST || r->top_k > r->top_groups * (r->experts / r->groups))
     return fail(LM_EINVAL, "top_k must be 1 to %d and at most the experts of the kept groups", LM_ROUTE_MAX_BEST);
-  if (r->T * r->top_k > 0x7fffffff) return fail(LM_EUNSUPPORTED, "more than 2^31 - 1 choices");
+  if (r->T > (1 << 28) || r->T * r->top_k > 0x7fffffff) return fail(LM_EUNSUPPORTED, "more than 2^28 tokens or 2^31 - 1 choices");
   if (r->T > 0 && !r->logits) return fail(LM_EINVAL, "logits must be non-null");
   if (r->ld < r->experts) return fail(LM_EINVAL, "row stride below the row length");
   return LM_OK;
@@ -952,7 +962,7 @@ static RouteArgs route_args(const lm_route* r) {
   } while (0)
 
 extern "C" size_t lm_route_workspace_size(int64_t T, int32_t experts) {
-  if (T <= 0 || T > 0x7fffffff || experts < 1 || experts > LM_LINEAR_MAX_EXPERTS) return 0;
+  if (T <= 0 || T > (1 << 28) || experts < 1 || experts > LM_LINEAR_MAX_EXPERTS) return 0;
   return route_space(T, experts).total;
 }
 
@@ -1006,7 +1016,7 @@ extern "C" int lm_route_topk_grad(const lm_route* r, const float* dweight, const
   hipStream_t st = (hipStream_t)stream;
   TimedLaunch timed("route", st);
   const int64_t n = (a.T + 3) / 4;
-  ROUTE_BY_TYPE(k_route_grad, dim3((unsigned)n), dim3(256), 0, st, a, dweight, dlogits);
+  ROUTE_BY_TYPE(k_route_grad, dim3((unsigned)(n < ROWS_GRID ? n : ROWS_GRID)), dim3(256), 0, st, a, dweight, dlogits);
   LAUNCH_CHECK();
   return LM_OK;
 }
@@ -1035,7 +1045,7 @@ static RowsArgs rows_args(const lm_rows* r) {
 static bool rows_short(const RowsArgs& a) { return a.N <= 1024; }
 static dim3 rows_grid(const RowsArgs& a, bool whole) {
   const int64_t x = rows_short(a) ? (a.T + 3) / 4 : a.T, parts = (a.N + 2047) / 2048;
-  return dim3((unsigned)x, (unsigned)(whole || rows_short(a) || x >= 2048 ? 1 : parts < 64 ? parts : 64));
+  return dim3((unsigned)(x < ROWS_GRID ? x : ROWS_GRID), (unsigned)(whole || rows_short(a) || x >= 2048 ? 1 : parts < 64 ? parts : 64));
 }
 
 extern "C" int lm_dispatch_rows(const lm_rows* r, const void* x, int64_t ldx, void* out, void* stream) {

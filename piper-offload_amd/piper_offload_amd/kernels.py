@@ -998,8 +998,8 @@ def _route(label: str, logits: torch.Tensor, top_k: int, bias: torch.Tensor | No
         raise ValueError(f"{label}: group_best must be 1 or 2, and at most the experts of a group, got {group_best}.")
     if not 1 <= top_k <= min(_MAX_BEST, top_groups * (experts // groups)):
         raise ValueError(f"{label}: top_k must be 1 to {min(_MAX_BEST, top_groups * (experts // groups))}, got {top_k}.")
-    if tokens * top_k >= 1 << 31:
-        raise ValueError(f"{label} takes fewer than 2^31 choices, got {tokens} tokens of {top_k}.")
+    if tokens > 1 << 28 or tokens * top_k >= 1 << 31:
+        raise ValueError(f"{label} takes up to 2^28 tokens and fewer than 2^31 choices, got {tokens} tokens of {top_k}.")
     if not math.isfinite(scale) or scale == 0:
         raise ValueError(f"{label}: scale must be finite and not zero, got {scale}.")
     if bias is not None:
