@@ -622,3 +622,48 @@ def test_places_that_do_not_exist_are_passed_over():
     for last in (0, -5):
         ends = torch.tensor([0, last], dtype=torch.int32, device=DEV)
         assert (K.combine_rows(h, w, position, ends) == 0).all() and (K.dispatch_rows_grad(h, position, ends) == 0).all()
+
+
+def test_experts_in_int8_from_logits_to_the_sum_and_back():
+    """Routing, rows to experts, products with INT8 weights and 8-bit inputs, weighted sums; gradients of rows and logits.
+
+    Roundings to bfloat16, half a step 2^-8 each: of a product's row and of the sum forward; backward of a row of w dy, a weight, a
+    product's row and the sum (four, of the sum of magnitudes); a weight's gradient sees the rounded product (2^-8 of its
+    magnitudes), a logit's is w_j (g_j - sum_i w_i g_i).  2^-6 of each bound is left for products of roundings and fp32 sums.
+    """
+    from piper_offload_amd import Int8Weight
+
+    g = _gen(131)
+    for t, e, k, n, cols, padded in ((1, 4, 2, 40, 48, 0), (70, 12, 3, 96, 160, 9), (400, 8, 4, 72, 130, 0)):
+        q = torch.randint(-127, 128, (e * n, cols), generator=g, dtype=torch.int8)
+        s = torch.rand(e * n, 1, generator=g) * 1e-3 + 1e-4
+        weight = Int8Weight(q.to(DEV), s.to(DEV), (1, cols))
+        x, logits, dy = _normal(g, t, cols, dtype=BF16), _normal(g, t, e), _normal(g, t, n, dtype=BF16)
+        if padded:
+            logits[t - padded:] = -INF
+        ours = x.to(DEV).requires_grad_(), logits.to(DEV).requires_grad_()
+        r = route_experts(ours[1], k)
+        h = grouped_linear(dispatch_experts(ours[0], r), weight, r.ends, activation_dtype=torch.int8)
+        y = combine_experts(h, r)
+        dx, dl = torch.autograd.grad(y, ours, dy.to(DEV))
+
+        live, expert = t - padded, r.expert.cpu().long()
+        w64 = (q.double() * s.double()).view(e, n, cols)
+        scale = (x.float().abs().amax(-1, keepdim=True) / 127).double()
+        codes = torch.round(x.double() / scale).clamp(-127, 127) * scale
+        of = w64[expert.clamp_min(0)]  # [t, k, n, cols]
+        p = torch.where(expert >= 0, r.weight.detach().double().cpu(), 0.0)
+        hh = (of @ codes[:, None, :, None])[..., 0]
+        want, size = (p[..., None] * hh).sum(1), (p[..., None] * hh).abs().sum(1)
+        more = 1 + 2.0**-6
+        assert ((y.detach().double().cpu() - want).abs() <= more * 2.0**-8 * (size + want.abs()) + 1e-30).all()
+        wdy = p[..., None] * dy.double()[:, None]
+        want, size = (wdy[:, :, None] @ of).sum((1, 2)), (wdy.abs()[:, :, None] @ of.abs()).sum((1, 2))
+        assert ((dx.double().cpu() - want).abs() <= more * 4 * 2.0**-8 * size + 1e-30).all()
+        grad, err = (dy.double()[:, None] * hh).sum(-1), 2.0**-8 * (dy.double()[:, None] * hh).abs().sum(-1)
+        want = p * (grad - (p * grad).sum(-1, keepdim=True))
+        bound = more * p * (err + (p * err).sum(-1, keepdim=True)) + 2.0**-20 * p * (grad.abs() + (p * grad.abs()).sum(-1, keepdim=True))
+        at = expert.clamp_min(0)
+        got = dl.double().cpu()
+        assert ((got.gather(1, at)[:live] - want[:live]).abs() <= bound[:live] + 1e-30).all()
+        assert (got.scatter(1, at, 0.0)[:live] == 0).all() and (got[live:] == 0).all() and (dx[live:] == 0).all() and (y[live:] == 0).all()
