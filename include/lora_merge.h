@@ -288,7 +288,7 @@ int lm_routed_residual(const void* x, const void* y, void* out, int64_t T, int64
  * input_dtype: `dtype`, or LM_E2M1 (MXFP4 weights): x is quantised to MXFP4
  * first, as lm_mx_requant with LM_MX_FLOOR does; a block with an infinity or a
  * NaN makes its row NaN.  Or LM_I8 (INT8 weights, K <= 132104): a row's scale is
- * its largest magnitude / 127 in fp32, its codes are the exact quotients
+ * its largest magnitude times 1 / 127 in fp32, its codes are the exact quotients
  * rounded to nearest (ties to even), their sums with the weight's codes are
  * exact; a row with an infinity or a NaN comes out NaN.  The input gradient
  * passes straight through either rounding.

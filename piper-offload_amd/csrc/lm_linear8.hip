@@ -1,6 +1,6 @@
 // lm_linear8.hip -- products with INT8 weights, W[n,k] = s[n] q[n,k]:
 //
-//   8-bit inputs    r[t] = max_k |x[t,k]| / 127, c[t,k] = x[t,k] / r[t] to the nearest whole number
+//   8-bit inputs    r[t] = max_k |x[t,k]| * 127^-1, c[t,k] = x[t,k] / r[t] to the nearest whole number
 //                   y[t,n] = r[t] s[n] sum_k c[t,k] q[n,k] (+ bias[n]): whole numbers, exact in 32 bits
 //   16-bit inputs   y[t,n] = s[n] sum_k x[t,k] q[n,k] (+ bias[n]): the codes are exact in 16 bits
 //   input gradient  dx[t,k] = sum_n dy[t,n] W[n,k] (straight through the rounding of 8-bit inputs)
@@ -33,7 +33,14 @@ __global__ __launch_bounds__(256) void k_lin8_prep(LinArgs a, uint8_t* codes, fl
     const int64_t r = (t - rows) * 4 + wave_index();
     if (r >= a.experts * a.N) return;
     const uint8_t* const from = (const uint8_t*)a.w + r * a.K;
-    for (int64_t c = (threadIdx.x & 63) * 16; c < ldw; c += 1024) store_b128_guarded((LM_GLOBAL lm_u32x4*)(aligned + r * ldw + c), few8_chunk(from + c, a.K - c));
+    for (int64_t c = (threadIdx.x & 63) * 16; c < ldw; c += 4096) {
+      lm_u32x4 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = few8_chunk(from + c + i * 1024, a.K - c - i * 1024);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i * 1024 < ldw) store_b128_guarded((LM_GLOBAL lm_u32x4*)(aligned + r * ldw + c + i * 1024), w[i]);
+    }
     return;
   }
   const uint16_t* x = (const uint16_t*)a.a + t * a.lda;

@@ -60,14 +60,15 @@ DEV uint32_t lin8_top(lm_u32x4 w, uint32_t top) {
   return top;
 }
 DEV uint32_t lin8_wave_max(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane(lin_scan_max((int)x), 63); }
-// A row, from its largest magnitude: its scale, and codes of its values.  A row of
+// A row, from its largest magnitude: its scale (times 1 / 127, as torch divides by a
+// number on the GPU: a program that quantises by itself gets the same codes), and codes of its values.  A row of
 // zeros has scale 0; one with an infinity or a NaN has the scale NaN, so its products
 // are NaN instead of finite numbers.
 struct Lin8Row {
   float scale, up, to, inv;
   DEV Lin8Row(uint32_t top) {
     const bool bad = top >= 0x7f800000u;
-    scale = bad ? u2f(0x7fc00000u) : u2f(top) / 127.0f;
+    scale = bad ? u2f(0x7fc00000u) : u2f(top) * (1.0f / 127.0f);
     // (a scale below 2^-100, whose inverse may overflow, is scaled up first: exact)
     up = scale < 0x1p-100f ? 0x1p100f : 1.0f;
     to = scale * up;

@@ -705,27 +705,51 @@ __global__ __launch_bounds__(256) void k_lin_join8(LinArgs a, int splits, uint32
   int group = 0;
   int64_t place;
   if (a.ends) lin_row(a, (int)t, group = a.experts, place);
-  const float rs = Q8 && group < a.experts ? a.row_scale[t] : 1.0f;
+  if (j0 >= a.N) return;
+  const bool some = group < a.experts, whole = j0 + 4 <= a.N;
+  float v[4] = {};
+  if (some) {
+    const LM_GLOBAL uint32_t* p = (const LM_GLOBAL uint32_t*)a.part + t * a.N + j0;
+    const int64_t n = a.T * a.N;
+    uint32_t sum[4] = {};
+    auto add = [&](int e, uint32_t x) {
+      if constexpr (Q8) sum[e] += x;
+      else v[e] += u2f(x);
+    };
+    if (whole) {
+      for (int k0 = 0; k0 < splits; k0 += 4) {  // (four parts on their way at once, zeros where there are fewer)
+        lm_u32x4 x[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int64_t j = j0 + e;
-    if (j < a.N) {
-      float v = 0.0f;
-      if (group < a.experts) {
-        const LM_GLOBAL uint32_t* p = (const LM_GLOBAL uint32_t*)a.part + t * a.N + j;
-        if constexpr (Q8) {
-          int sum = 0;
-          for (int k = 0; k < splits; ++k) sum += (int)p[k * a.T * a.N];
-          v = (float)sum;
-        } else {
-          for (int k = 0; k < splits; ++k) v += u2f(p[k * a.T * a.N]);
-        }
-        v *= lin_scale8(a, group * a.N + j);
-        v *= rs;
-        if (a.bias) v += val_dt<DT>(((const LM_GLOBAL uint16_t*)a.bias)[j]);
+        for (int k = 0; k < 4; ++k) x[k] = k0 + k < splits ? *(const LM_GLOBAL lm_u32x4_any*)(p + (k0 + k) * n) : lm_u32x4{};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) add(e, x[k][e]);
       }
-      ((LM_GLOBAL uint16_t*)a.out)[t * a.N + j] = bits_dt<DT>(v);
+    } else {
+      for (int k = 0; k < splits; ++k)
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (j0 + e < a.N) add(e, p[k * n + e]);
     }
+    const float rs = Q8 ? a.row_scale[t] : 1.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t j = j0 + e < a.N ? j0 + e : a.N - 1;
+      if constexpr (Q8) v[e] = (float)(int)sum[e];
+      v[e] *= lin_scale8(a, group * a.N + j);
+      if constexpr (Q8) v[e] *= rs;
+      if (a.bias) v[e] += val_dt<DT>(((const LM_GLOBAL uint16_t*)a.bias)[j]);
+    }
+  }
+  LM_GLOBAL uint16_t* const to = (LM_GLOBAL uint16_t*)a.out + t * a.N + j0;
+  if (whole) {
+    *(LM_GLOBAL lm_u32x2_any*)to = lm_u32x2{(uint32_t)bits_dt<DT>(v[0]) | (uint32_t)bits_dt<DT>(v[1]) << 16,
+                                            (uint32_t)bits_dt<DT>(v[2]) | (uint32_t)bits_dt<DT>(v[3]) << 16};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (j0 + e < a.N) to[e] = bits_dt<DT>(v[e]);
   }
 }
 

@@ -916,7 +916,7 @@ def int8_matmul(x: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, *, bi
 
     ``x`` [..., in] bfloat16 or float16.  The sums run over the codes, which are exact, in fp32; they are multiplied by
     the scale and rounded once to ``x.dtype``.  With ``activation_dtype=torch.int8`` every row of ``x`` is quantised
-    first: its scale is its largest magnitude / 127 in fp32, its codes are the exact quotients rounded to nearest (ties
+    first: its scale is its largest magnitude times 1 / 127 in fp32, its codes are the exact quotients rounded to nearest (ties
     to even), and the sums of products of codes are exact.  A row with an infinity or a NaN then comes out NaN.
     """
     label = "INT8 product"

@@ -40,8 +40,11 @@ def _weight(g, *shape, scale_dtype=torch.float32):
 
 
 def _codes(x):
-    """Codes and scale of every row in 64 bits: the quotients by the fp32 scale, to nearest, ties to even."""
-    s = (x.float().abs().amax(-1, keepdim=True) / 127).double()
+    """Codes and scale of every row in 64 bits: the quotients by the fp32 scale, to nearest, ties to even.
+
+    The scale is the largest magnitude times the number of 32 bits next to 1 / 127, as torch divides by 127 on the GPU (on the
+    CPU it rounds the quotient)."""
+    s = (x.float().abs().amax(-1, keepdim=True) * (torch.ones(()) / 127)).double()
     return torch.round(x.double() / torch.where(s > 0, s, 1.0)).clamp(-127, 127), s
 
 
@@ -475,3 +478,17 @@ def test_the_same_call_gives_the_same_bits():
             out = K.int8_matmul(x, q, s), K.int8_matmul(x, q, s, activation_dtype=I8), K.int8_matmul_input_grad(dy, q, s)
             first = first or out
             assert all((a == b).all() for a, b in zip(first, out))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_codes_are_those_of_a_program_that_quantises_by_itself(dtype):
+    """Read off through a weight of one, against torch on the GPU: no code differs, in launches of few and of many rows."""
+    g = _gen(83)
+    eye = torch.eye(256, dtype=torch.int8, device=DEV)
+    one = torch.ones(256, device=DEV)
+    for t in (2, 4, 60, 4000):
+        x = (_normal(g, t, 256) * torch.exp(_normal(g, t, 1))).to(dtype).to(DEV)
+        s = x.float().abs().amax(-1, keepdim=True) / 127
+        codes = torch.round(x.double() / s.double()).clamp(-127, 127)
+        y = K.int8_matmul(x, eye, one, activation_dtype=I8)
+        assert (y == (codes.float() * s).to(dtype)).all()

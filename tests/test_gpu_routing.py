@@ -649,7 +649,7 @@ def test_experts_in_int8_from_logits_to_the_sum_and_back():
 
         live, expert = t - padded, r.expert.cpu().long()
         w64 = (q.double() * s.double()).view(e, n, cols)
-        scale = (x.float().abs().amax(-1, keepdim=True) / 127).double()
+        scale = (x.float().abs().amax(-1, keepdim=True) * (torch.ones(()) / 127)).double()  # (torch's / 127 on the GPU)
         codes = torch.round(x.double() / scale).clamp(-127, 127) * scale
         of = w64[expert.clamp_min(0)]  # [t, k, n, cols]
         p = torch.where(expert >= 0, r.weight.detach().double().cpu(), 0.0)
