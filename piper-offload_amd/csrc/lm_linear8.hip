@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void k_lin8_prep(LinArgs a, uint8_t* codes, fl
     for (int64_t c = (threadIdx.x & 63) * 16; c < ldw; c += 4096) {
       lm_u32x4 w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = few8_chunk(from + c + i * 1024, a.K - c - i * 1024);
+      for (int i = 0; i < 4; ++i) w[i] = few8_chunk(from, c + i * 1024, a.K);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (c + i * 1024 < ldw) store_b128_guarded((LM_GLOBAL lm_u32x4*)(aligned + r * ldw + c + i * 1024), w[i]);

@@ -22,19 +22,32 @@
 DEV lm_u32x4 few8_load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
   return __builtin_bit_cast(lm_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
 }
-// 16 codes from p, of which the first `left` exist (any alignment)
-DEV lm_u32x4 few8_chunk(const uint8_t* p, int64_t left) {
+// 16 bytes without the first n (1 .. 15), zeros after them
+DEV lm_u32x4 few8_drop(lm_u32x4 v, int n) {
+  if (n & 4) v = lm_u32x4{v[1], v[2], v[3], 0};
+  if (n & 8) v = lm_u32x4{v[2], v[3], 0, 0};
+  return lm_u32x4{__builtin_amdgcn_alignbyte(v[1], v[0], n & 3), __builtin_amdgcn_alignbyte(v[2], v[1], n & 3),
+                  __builtin_amdgcn_alignbyte(v[3], v[2], n & 3), __builtin_amdgcn_alignbyte(0, v[3], n & 3)};
+}
+// Codes k .. k + 15 of a row of K at any address, zeros past its end.  A part of 16 comes
+// from the row's last 16 (one load; byte after byte the ends of rows took longer than
+// all the rest: 117 rows of 8 groups [896, 1021] 16.8 us, [896, 1024] 6.0).
+DEV lm_u32x4 few8_chunk(const uint8_t* row, int64_t k, int64_t K) {
+  const int64_t left = K - k;
   lm_u32x4 v = {};
-  if (left >= 16) {
-    v = *(const LM_GLOBAL lm_u32x4_any*)p;
-  } else if (left > 0) {
-    uint64_t lo = 0, hi = 0;
-    for (int b = 0; b < left; ++b) {
-      const uint64_t c = ((const LM_GLOBAL uint8_t*)p)[b];
-      if (b < 8) lo |= c << (8 * b);
-      else hi |= c << (8 * b - 64);
+  if (left > 0) {
+    if (K >= 16) {
+      v = *(const LM_GLOBAL lm_u32x4_any*)(row + (left < 16 ? K - 16 : k));
+      if (left < 16) v = few8_drop(v, 16 - (int)left);
+    } else {
+      uint64_t lo = 0, hi = 0;
+      for (int b = 0; b < left; ++b) {
+        const uint64_t c = ((const LM_GLOBAL uint8_t*)row)[k + b];
+        if (b < 8) lo |= c << (8 * b);
+        else hi |= c << (8 * b - 64);
+      }
+      v = lm_u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
     }
-    v = lm_u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
   }
   return v;
 }
@@ -158,7 +171,7 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* 
         for (int c = 0; c < CF; ++c)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if constexpr (decltype(tail)::value) wv[i][c][h] = few8_chunk(wp + wo[c] + k0 + 64 * h, K - k0 - 64 * h - 16 * g);
+            if constexpr (decltype(tail)::value) wv[i][c][h] = few8_chunk(wp + (wo[c] - 16 * g), k0 + 64 * h + 16 * g, K);
             else wv[i][c][h] = few8_load16(rw, wo[c] + k0 + 64 * h);
           }
       }
