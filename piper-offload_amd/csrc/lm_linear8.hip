@@ -172,7 +172,11 @@ static int launch_few8(const LinArgs& a, const uint8_t* codes, int64_t pitch, hi
   TimedLaunch timed("linear_few", st);
   const int64_t n = lin_tiles<16 * MF>(a.T, a.experts, a.ends != nullptr) * ((a.N + 16 * CF - 1) / (16 * CF));
   if (n >= LIN8_GROUPS * 4 / NW) return fail(LM_EUNSUPPORTED, "product too large for one launch");
-  hipLaunchKernelGGL((k_lin_few8<DT, Q8, OWN, MF, CF, NW, UN>), dim3((unsigned)n), dim3(NW * 64), OWN ? (size_t)(a.T * pitch) : 0, st, a, codes, pitch);
+  const size_t lds = OWN ? (size_t)(a.T * pitch) : 0;
+  // (16 fragments have no registers left for the words besides)
+  const bool odd = MF == 1 && (((uintptr_t)a.w | (uintptr_t)a.K) & 3 || (!Q8 && ((uintptr_t)a.a | (uintptr_t)(a.lda * 2)) & 3));
+  if (odd) hipLaunchKernelGGL((k_lin_few8<DT, Q8, OWN, MF == 1, MF, CF, NW, UN>), dim3((unsigned)n), dim3(NW * 64), lds, st, a, codes, pitch);
+  else hipLaunchKernelGGL((k_lin_few8<DT, Q8, OWN, false, MF, CF, NW, UN>), dim3((unsigned)n), dim3(NW * 64), lds, st, a, codes, pitch);
   LAUNCH_CHECK();
   return LM_OK;
 }

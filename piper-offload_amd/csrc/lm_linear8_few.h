@@ -22,6 +22,12 @@
 DEV lm_u32x4 few8_load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
   return __builtin_bit_cast(lm_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
 }
+DEV uint32_t few8_load4(__amdgpu_buffer_rsrc_t r, uint32_t off) { return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0); }
+// bytes s .. s + 15 (s < 4) of v and e after it
+DEV lm_u32x4 few8_align(lm_u32x4 v, uint32_t e, uint32_t s) {
+  return lm_u32x4{__builtin_amdgcn_alignbyte(v[1], v[0], s), __builtin_amdgcn_alignbyte(v[2], v[1], s), __builtin_amdgcn_alignbyte(v[3], v[2], s),
+                  __builtin_amdgcn_alignbyte(e, v[3], s)};
+}
 // 16 bytes without the first n (1 .. 15), zeros after them
 DEV lm_u32x4 few8_drop(lm_u32x4 v, int n) {
   if (n & 4) v = lm_u32x4{v[1], v[2], v[3], 0};
@@ -121,7 +127,11 @@ struct Lin8Row {
 };
 
 // OWN: x is not quantised yet.  Its few rows are, into LDS, by every workgroup.
-template <int DT, bool Q8, bool OWN, int MF, int CF, int NW, int UN>
+// ODD: rows of codes, or of x in 16 bits, that do not start on whole words.  16 bytes at
+// such an address take twice as long to load (one row of [14336, 4090] 24.5 us, [14336,
+// 4092] 15.2), so the five words that hold them are loaded instead, and shifted; a piece
+// whose fifth word would pass its row is left to the tail.
+template <int DT, bool Q8, bool OWN, bool ODD, int MF, int CF, int NW, int UN>
 __global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* codes, int64_t pitch) {
   constexpr bool HALF = DT == F16;
   constexpr int COLS = CF * 16, ROWS = MF * 16, PITCH = COLS + 4;
@@ -148,8 +158,10 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* 
     const int rows = (int)(r1 - r0 < ROWS ? r1 - r0 : ROWS), cols = (int)(a.N - n0 < COLS ? a.N - n0 : COLS);
     const uint8_t* xp = OWN ? nullptr : (Q8 ? codes : (const uint8_t*)a.a) + r0 * ldx;
     const uint8_t* wp = (const uint8_t*)a.w + (group * a.N + n0) * a.K;
-    const __amdgpu_buffer_rsrc_t rx = lin_rsrc(xp, OWN ? 0 : (rows - 1) * ldx + (Q8 ? pitch : a.K * 2));
-    const __amdgpu_buffer_rsrc_t rw = lin_rsrc(wp, cols * a.K);
+    constexpr bool ODDX = ODD && !Q8;
+    const uint32_t wm = ODD ? (uint32_t)(uintptr_t)wp & 3u : 0u, xm = ODDX ? (uint32_t)(uintptr_t)xp & 3u : 0u;
+    const __amdgpu_buffer_rsrc_t rx = lin_rsrc(xp - xm, OWN ? 0 : (rows - 1) * ldx + (Q8 ? pitch : a.K * 2) + xm);
+    const __amdgpu_buffer_rsrc_t rw = lin_rsrc(wp - wm, cols * a.K + wm);
     uint32_t xo[MF], wo[CF];
 #pragma unroll
     for (int m = 0; m < MF; ++m) {
@@ -163,6 +175,7 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* 
     }
     // UN units from u0; TAIL: some of them may pass the end
     lm_u32x4 wv[UN][CF][2];
+    uint32_t we[ODD ? UN : 1][ODD ? CF : 1][2];
     auto weights = [&](int u0, auto tail) {
 #pragma unroll
       for (int i = 0; i < UN; ++i) {
@@ -172,13 +185,15 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* 
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if constexpr (decltype(tail)::value) wv[i][c][h] = few8_chunk(wp + (wo[c] - 16 * g), k0 + 64 * h + 16 * g, K);
-            else wv[i][c][h] = few8_load16(rw, wo[c] + k0 + 64 * h);
+            else wv[i][c][h] = few8_load16(rw, (ODD ? (wo[c] + wm) & ~3u : wo[c]) + k0 + 64 * h);
+            if constexpr (ODD && !decltype(tail)::value) we[i][c][h] = few8_load4(rw, ((wo[c] + wm) & ~3u) + k0 + 64 * h + 16);
           }
       }
     };
     auto body = [&](int u0, auto tail) {
       constexpr bool TAIL = decltype(tail)::value;
       lm_u32x4 xv[UN][MF][XL];
+      uint32_t xe[ODDX ? UN : 1][ODDX ? MF : 1][XL];
 #pragma unroll
       for (int i = 0; i < UN; ++i) {
         const int k0 = (u0 + i) * 128;
@@ -195,14 +210,27 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* 
             } else {
               const int e = k0 + 64 * (j >> 1) + 8 * (j & 1);  // (+ 16 g)
               if constexpr (TAIL) xv[i][m][j] = lin_chunk((const uint16_t*)(xp + xo[m]) + e, K - e - 16 * g);
-              else xv[i][m][j] = few8_load16(rx, xo[m] + 2 * e);
+              else xv[i][m][j] = few8_load16(rx, (ODDX ? (xo[m] + xm) & ~3u : xo[m]) + 2 * e);
+              if constexpr (ODDX && !TAIL) xe[i][m][j] = few8_load4(rx, ((xo[m] + xm) & ~3u) + 2 * e + 16);
             }
           }
+      }
+      if constexpr (ODDX && !TAIL) {
+#pragma unroll
+        for (int i = 0; i < UN; ++i)
+#pragma unroll
+          for (int m = 0; m < MF; ++m)
+#pragma unroll
+            for (int j = 0; j < XL; ++j) xv[i][m][j] = few8_align(xv[i][m][j], xe[i][m][j], (xo[m] + xm) & 3u);
       }
 #pragma unroll
       for (int i = 0; i < UN; ++i)
 #pragma unroll
         for (int c = 0; c < CF; ++c) {
+          if constexpr (ODD && !TAIL) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) wv[i][c][h] = few8_align(wv[i][c][h], we[i][c][h], (wo[c] + wm) & 3u);
+          }
           if constexpr (Q8) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -219,7 +247,7 @@ __global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* 
           }
         }
     };
-    const int units = (K + 127) >> 7, whole = K >> 7;
+    const int units = (K + 127) >> 7, whole = (ODD ? K - 4 : K) >> 7;
     int u0 = wave * UN;
     if constexpr (OWN) {
       // The rows' first pieces, then the first weights (loads come back in order), and
