@@ -277,8 +277,8 @@ DEV lm_u32x4 lin_decode8(uint32_t codes, float scale) {
   return v;
 }
 
-// W_Q8: rows and weight are INT8 codes; W_I8: INT8 weight, rows of 16 bits
-enum : int { W_DENSE = 0, W_MX = 1, W_Q4 = 2, W_Q8 = 3, W_I8 = 4 };
+// W_Q8: rows and weight are INT8 codes (W_R8: the weight's rows at any address); W_I8: INT8 weight, rows of 16 bits
+enum : int { W_DENSE = 0, W_MX = 1, W_Q4 = 2, W_Q8 = 3, W_I8 = 4, W_R8 = 5 };
 
 // the scale of row i of an INT8 weight
 DEV float lin_scale8(const LinArgs& a, int64_t i) {

@@ -11,7 +11,7 @@
 // multiplied by it afterwards, and to round dy s instead is off by as much.
 //
 // Many rows (k_lin_mm): codes times codes are bound by the power that the matrix unit
-// may take, 4096 rows of [14336, 4096] 232 us (2.07 POP/s at 1.86 GHz, 64% of the cycles
+// may take, 4096 rows of [14336, 4096] 234 us (2.06 POP/s at 1.86 GHz, 64% of the cycles
 // busy; the library's product of 8192^3 reaches 2.2).  Decoded to 16 bits, 2048 rows of the
 // same 205 us (1.17 PFLOP/s), input gradient in two parts with their join 222 (the
 // library's bf16 product of 8192^3: 1.33).
@@ -22,11 +22,12 @@
 
 // The rows' codes, at a pitch of whole pieces that are filled up with zeros, and their
 // scales: a workgroup a row, whose first 4096 values stay in registers between the two.
+// tail: codes of the last piece of 16 at its end, as k_lin8_tail has values.
 // The workgroups after those copy weights whose rows are not whole 16-byte pieces to
 // rows that are (`aligned`), a wave a row.  Bound by memory: 4096 rows of 4096 9.8 us
 // (50 MB, 5.1 TB/s).
 template <int DT>
-__global__ __launch_bounds__(256) void k_lin8_prep(LinArgs a, uint8_t* codes, float* scales, int64_t pitch, uint8_t* aligned, int64_t ldw) {
+__global__ __launch_bounds__(256) void k_lin8_prep(LinArgs a, uint8_t* codes, float* scales, int64_t pitch, int tail, uint8_t* aligned, int64_t ldw) {
   __shared__ uint32_t red[4];
   const int64_t t = blockIdx.x, rows = scales ? a.T : 0;
   if (t >= rows) {
@@ -56,9 +57,19 @@ __global__ __launch_bounds__(256) void k_lin8_prep(LinArgs a, uint8_t* codes, fl
   const Lin8Row r(top);
   if (threadIdx.x == 0) scales[t] = r.scale;
   LM_GLOBAL uint8_t* const to = (LM_GLOBAL uint8_t*)codes + t * pitch;
-  if (c0 < pitch) *(LM_GLOBAL lm_u32x2*)(to + c0) = r.codes<DT>(w0);
-  if (c0 + 2048 < pitch) *(LM_GLOBAL lm_u32x2*)(to + c0 + 2048) = r.codes<DT>(w1);
-  for (int64_t c = c0 + 4096; c < pitch; c += 2048) *(LM_GLOBAL lm_u32x2*)(to + c) = r.codes<DT>(lin_chunk(x + c, a.K - c));
+  const int64_t last = tail ? a.K & ~(int64_t)15 : pitch;  // codes up to here are in order
+  if (c0 < last) *(LM_GLOBAL lm_u32x2*)(to + c0) = r.codes<DT>(w0);
+  if (c0 + 2048 < last) *(LM_GLOBAL lm_u32x2*)(to + c0 + 2048) = r.codes<DT>(w1);
+  for (int64_t c = c0 + 4096; c < last; c += 2048) *(LM_GLOBAL lm_u32x2*)(to + c) = r.codes<DT>(lin_chunk(x + c, a.K - c));
+  if (last + c0 < pitch) {
+    lm_u32x4 w = {};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int64_t i = a.K - 16 + c0 + e;
+      if (i >= last && i < a.K) w[e >> 1] |= (uint32_t)((const LM_GLOBAL uint16_t*)x)[i] << (16 * (e & 1));
+    }
+    *(LM_GLOBAL lm_u32x2*)(to + last + c0) = r.codes<DT>(w);
+  }
 }
 
 // Rows of 16 bits copied for k_lin_mm, which reads the last 16 codes of a row that is no
@@ -103,7 +114,8 @@ struct Lin8Plan {
   bool few;                  // k_lin_few8, else k_lin_mm
   bool own;                  // k_lin_few8 quantises its rows
   bool copy_x, copy_w;       // rows realigned in the workspace first
-  bool tail;                 // and x's last elements as k_lin8_tail has them
+  bool tail;                 // and x's last elements as k_lin8_tail (8-bit inputs: k_lin8_prep) has them
+  bool raw;                  // 8-bit inputs: codes of the weight at any address
   int64_t pitch, lda, ldw;   // of the codes of x, of 16-bit rows, of the weight (bytes)
   size_t codes, codes_bytes, scales, x, w, part, total;
 };
@@ -143,16 +155,20 @@ static Lin8Plan lin8_plan(int op, int64_t T, int64_t lda, int64_t N, int64_t K, 
     if (p.copy_x && p.few) p.x = take((size_t)T * p.lda * 2);
   }
   if (!p.few) {
-    // (decoded on the way into LDS, rows of codes may lie anywhere, if there is one piece,
-    // or tile, of them; loaded straight into it, not)
-    p.copy_w = quant ? !aligned || K % 16 : K < (op == LIN_FORWARD ? 16 : 256) && K % 16;
+    // Rows of codes may lie anywhere, if there is one piece, or tile, of them, where they go
+    // through registers.  Straight to LDS go whole pieces of 16 bytes alone: weights are
+    // copied to rows of such, or, while they have few rows of x each, go through registers too
+    // (32 groups [6912, 1146] at 1643 rows 111 us, copied 162; 777 rows of [2001, 2083] 30, copied 24).
+    const bool off = !aligned || K % 16;
+    p.raw = quant && off && K >= 16 && T <= 64 * E;
+    p.copy_w = quant ? off && !p.raw : K < (op == LIN_FORWARD ? 16 : 256) && K % 16;
     if (p.copy_w) {
       p.ldw = round64(K);
       p.w = take((size_t)E * N * p.ldw);
     }
-    p.tail = op == LIN_FORWARD && !quant && !p.copy_w && K % 16;
+    p.tail = op == LIN_FORWARD && !p.copy_w && K % 16;
     p.mm.len = quant ? round16(K) / 2 : p.tail ? round16(K) : round8(inner);
-    if (p.tail) p.lda = p.mm.len;
+    if (p.tail && !quant) p.lda = p.mm.len;
     if (p.copy_x) p.x = take((size_t)T * p.lda * 2);
     p.mm.splits = 1;
     const int64_t J = op == LIN_FORWARD ? N : K;
@@ -228,8 +244,8 @@ static int lin8_setup(LinArgs& a, const Lin8Plan& p, int op, int dtype, void* wo
     const int64_t rows = p.codes_bytes > 0 ? a.T : 0, n = rows + (p.copy_w ? (a.experts * a.N + 3) / 4 : 0);
     if (n >= LIN8_GROUPS) return fail(LM_EUNSUPPORTED, "product too large for one launch");
     float* const scales = rows ? (float*)(base + p.scales) : nullptr;
-    if (dtype == LM_F16) hipLaunchKernelGGL((k_lin8_prep<F16>), dim3((unsigned)n), dim3(256), 0, st, a, base + p.codes, scales, p.pitch, base + p.w, p.ldw);
-    else hipLaunchKernelGGL((k_lin8_prep<BF16>), dim3((unsigned)n), dim3(256), 0, st, a, base + p.codes, scales, p.pitch, base + p.w, p.ldw);
+    if (dtype == LM_F16) hipLaunchKernelGGL((k_lin8_prep<F16>), dim3((unsigned)n), dim3(256), 0, st, a, base + p.codes, scales, p.pitch, (int)p.tail, base + p.w, p.ldw);
+    else hipLaunchKernelGGL((k_lin8_prep<BF16>), dim3((unsigned)n), dim3(256), 0, st, a, base + p.codes, scales, p.pitch, (int)p.tail, base + p.w, p.ldw);
     LAUNCH_CHECK();
     a.row_scale = scales;
     if (p.copy_w) a.w = base + p.w;
@@ -255,6 +271,7 @@ int lin8_forward(LinArgs& a, int dtype, bool quant, void* workspace, size_t work
   // (in pairs of codes from here on)
   a.a = codes;
   a.lda = p.pitch / 2;
+  if (p.raw) return run_mm<LIN_FORWARD, W_R8>(a, p.mm, dtype, st);
   a.ldw = p.ldw / 2;
   return run_mm<LIN_FORWARD, W_Q8>(a, p.mm, dtype, st);
 }

@@ -102,11 +102,11 @@ static int launch_mm(const LinArgs& a, const LinPlan& p, hipStream_t st) {
   const dim3 grid((unsigned)n0, OP == LIN_WEIGHT_GRAD ? a.experts : p.splits, OP == LIN_WEIGHT_GRAD ? p.splits : 1);
   hipLaunchKernelGGL((k_lin_mm<DT, OP, W, BM, BN, WM, WN, SHORT>), grid, dim3(WM * WN * 64), 0, st, a);
   LAUNCH_CHECK();
-  if constexpr (OP == LIN_FORWARD && (W == W_Q8 || W == W_I8)) {
+  if constexpr (OP == LIN_FORWARD && (W == W_Q8 || W == W_R8 || W == W_I8)) {
     if (p.splits > 1) {
       const int64_t chunks = (J + 255) / 256, blocks = (a.T * chunks + 3) / 4;
       if (blocks > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
-      hipLaunchKernelGGL((k_lin_join8<DT, W == W_Q8>), dim3((unsigned)blocks), dim3(256), 0, st, a, p.splits, (uint32_t)chunks);
+      hipLaunchKernelGGL((k_lin_join8<DT, W != W_I8>), dim3((unsigned)blocks), dim3(256), 0, st, a, p.splits, (uint32_t)chunks);
       LAUNCH_CHECK();
     }
     return LM_OK;

@@ -23,6 +23,8 @@
 //         and KS16 (times their row's scale, which lies along the sum)
 // Q8: both operands INT8 codes; a slot of 64 bytes has 64 of them, and all but the
 // matrix instruction is as for 16 bits (the arguments count in pairs of codes).
+//   KR8   the weight's codes where rows start anywhere: loads straight to LDS take whole
+//         pieces of 16 bytes only, so these go through registers, and then are KC16
 // Q4: both operands MXFP4 (x quantised beforehand), multiplied as they are by the
 // scaled MFMA, 128 codes a stage, so a slot is 64 bytes here too.  Its scales
 // come packed by k_lin_prep4: per 64 slots and stage 256 bytes, which hold for
@@ -48,7 +50,7 @@
 
 #include "lm_linear.h"
 
-enum : int { KC16, KS16, KC4, KS4, KC8, KS8 };
+enum : int { KC16, KS16, KC4, KS4, KC8, KS8, KR8 };
 
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 typedef __attribute__((address_space(3))) uint32_t lds_u32;
@@ -125,15 +127,15 @@ DEV bool lin_pick(const LinArgs& a, int64_t jend, LinTile& t) {
 
 template <int DT, int OP, int W, int BM, int BN, int WM, int WN>
 struct MmTraits {
-  static constexpr bool Q4 = W == W_Q4, MX = W == W_MX, Q8 = W == W_Q8, I8 = W == W_I8;
+  static constexpr bool Q4 = W == W_Q4, MX = W == W_MX, Q8 = W == W_Q8 || W == W_R8, I8 = W == W_I8;
   static constexpr int NW = WM * WN, NT = NW * 64;
   static constexpr int CS = Q4 ? 128 : 32;  // contraction of a stage
   static constexpr int IK = OP == LIN_WEIGHT_GRAD ? KS16 : KC16;
-  static constexpr int JK = OP == LIN_FORWARD      ? (MX ? KC4 : I8 ? KC8 : KC16)
+  static constexpr int JK = OP == LIN_FORWARD      ? (MX ? KC4 : I8 ? KC8 : W == W_R8 ? KR8 : KC16)
                             : OP == LIN_INPUT_GRAD ? (MX ? KS4 : I8 ? KS8 : KS16)
                                                    : KS16;
-  static constexpr bool REG = JK == KS4 || JK == KC8 || JK == KS8;  // decoded on the way into LDS
-  static constexpr int LK = JK == KS4 || JK == KS8 ? KS16 : JK == KC8 ? KC16 : JK;  // J's tile in LDS
+  static constexpr bool REG = JK == KS4 || JK == KC8 || JK == KS8 || JK == KR8;  // to LDS through registers, decoded but for KR8
+  static constexpr int LK = JK == KS4 || JK == KS8 ? KS16 : JK == KC8 || JK == KR8 ? KC16 : JK;  // J's tile in LDS
   static constexpr int FI = BM / WM / 16, FJ = BN / WN / 16;
   static constexpr int IB = BM * 64, JB = BN * 64;  // bytes of a stage (KC4: of four)
   static constexpr int IL = IB / 1024 / NW;                               // loads per wave
@@ -246,9 +248,10 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
     ldb = Q4 ? a.K >> 2 : ldw;
     const int64_t first = OP == LIN_FORWARD ? (t.group * a.N + t.j0) * ldw : t.group * a.N * ldw + t.j0;
     const int64_t count = OP == LIN_FORWARD ? (a.N - t.j0) * ldw : a.N * ldw - t.j0;
-    jp = (const uint8_t*)a.w + (MX ? first >> 1 : I8 ? first : first * 2);
-    jbytes = MX ? count >> 1 : I8 ? count : count * 2;
-    jstep = OP == LIN_FORWARD ? (P::MX ? 16 : I8 ? 0 : 64) : CS * (MX ? ldw >> 1 : I8 ? ldw : ldw * 2);
+    constexpr bool BYTES = I8 || JK == KR8;
+    jp = (const uint8_t*)a.w + (MX ? first >> 1 : BYTES ? first : first * 2);
+    jbytes = MX ? count >> 1 : BYTES ? count : count * 2;
+    jstep = OP == LIN_FORWARD ? (P::MX ? 16 : BYTES ? 0 : 64) : CS * (MX ? ldw >> 1 : I8 ? ldw : ldw * 2);
   }
   // stages [kb, ke) of nk: this workgroup's part where the contraction is split
   const int nk = (int)((len + CS - 1) / CS);
@@ -351,16 +354,26 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
     // issued for every stage, inside the weight or not: the waits count them.)
     // KS8 does the same; KC8: 16 codes of column kr, a row's last 16 from there on: x
     // holds its elements in that order (k_lin8_tail), zeros where they were had before.
-    const int kr = JK == KC8 ? tid >> 1 : tid / (BN / 16), kc = JK == KC8 ? tid & 1 : tid % (BN / 16);
+    // KR8: twice 16 codes in the same way (k_lin8_prep).
+    constexpr bool ALONG = JK == KC8 || JK == KR8;
+    const int kr = ALONG ? tid >> 1 : tid / (BN / 16), kc = ALONG ? tid & 1 : tid % (BN / 16);
     lm_u32x2 code[JK == KS4 ? 2 : 1];
-    lm_u32x4 code8[REG && JK != KS4 ? 2 : 1];
+    lm_u32x4 code8[JK == KR8 ? 4 : REG && JK != KS4 ? 2 : 1];
     uint32_t code_s[2];
-    const bool cin = JK == KC8 ? t.j0 + kr < a.N : t.j0 + kc * 16 < a.K;
-    const uint32_t co = !cin ? LIN_OUT : JK == KS4 ? (uint32_t)(kr * (a.K >> 1) + kc * 8) : (uint32_t)(kr * a.ldw + (JK == KC8 ? 0 : kc * 16));
+    const bool cin = ALONG ? t.j0 + kr < a.N : t.j0 + kc * 16 < a.K;
+    const uint32_t co = !cin ? LIN_OUT : JK == KS4 ? (uint32_t)(kr * (a.K >> 1) + kc * 8) : (uint32_t)(kr * a.ldw + (ALONG ? 0 : kc * 16));
     const int klast = (int)a.ldw - 16;
     const uint32_t cb = (uint32_t)((t.j0 + kc * 16) >> 5);  // block of the row
     const uint32_t cso = a.swizzled ? (cb >> 2) * 512 + (kr & 31) * 16 + (cb & 3) : (uint32_t)(kr * nb) + cb;
     auto load_codes = [&](int st, int set) {
+      if constexpr (JK == KR8) {
+        const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)jr, 0, left32(jl, st >= ke), 0x00027000);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int c = st * (2 * CS) + kc * 32 + n * 16;
+          code8[2 * set + n] = __builtin_bit_cast(lm_u32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, (int)(co + (c < klast ? c : klast)), 0, 0));
+        }
+      }
       if constexpr (JK == KC8 || JK == KS8) {
         const bool none = st >= ke;
         const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc((void*)jr, 0, left32(jl, none), 0x00027000);
@@ -394,6 +407,10 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
       }
     };
     auto store_codes = [&](lds_u8* tj, int set) {
+      if constexpr (JK == KR8) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) *(lds_u32x4*)(tj + kr * 64 + (((kc * 2 + n) ^ mm_key(kr)) << 4)) = code8[2 * set + n];
+      }
       if constexpr (JK == KC8 || JK == KS8) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {

@@ -492,3 +492,23 @@ def test_codes_are_those_of_a_program_that_quantises_by_itself(dtype):
         codes = torch.round(x.double() / s.double()).clamp(-127, 127)
         y = K.int8_matmul(x, eye, one, activation_dtype=I8)
         assert (y == (codes.float() * s).to(dtype)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("sizes,n,k", [([60, 0, 64, 20, 3, 100, 40, 64], 2050, 1037), ([30] * 40, 700, 1041), ([50, 62] * 6, 1030, 2051),
+                                       ([40] * 3 + [70] * 30, 640, 515), ([33] * 64, 256, 272)])
+def test_groups_of_rows_of_any_length(sizes, n, k, dtype):
+    """8-bit inputs, many groups: weights whose rows are no whole pieces, or start anywhere, are not copied."""
+    g = _gen(n + k)
+    e, t = len(sizes), sum(sizes) + 7
+    q, s, _ = _weight(g, e, n, k)
+    store = torch.full((e * n * k + 19,), 111, dtype=I8, device=DEV)
+    codes = store[3:3 + e * n * k].view(e, n, k).copy_(q.to(DEV))
+    x, ends = _normal(g, t, k, dtype=dtype), _ends(sizes)
+    y = K.grouped_int8_matmul(x.to(DEV), codes, s.to(DEV), ends.to(DEV), activation_dtype=I8)
+    begin = 0
+    for i, end in enumerate(ends.tolist()):
+        if end > begin:
+            _check(x[begin:end], q[i], s[i], y[begin:end], True)
+        begin = end
+    assert (y[begin:] == 0).all()
