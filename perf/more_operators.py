@@ -19,7 +19,6 @@ adds up what the experts return.
 
 from __future__ import annotations
 
-import functools
 import math
 import os
 import random
@@ -346,7 +345,6 @@ def _plain(state):
 # ---------------------------------------------------------------------------
 # the framework's operators
 # ---------------------------------------------------------------------------
-@functools.lru_cache(maxsize=None)
 def _kernels():
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "piper-offload_amd")
     if path not in sys.path:
