@@ -162,8 +162,7 @@ DEV int route_choose64(const float (&v)[P], const float (&b)[P], bool even, int 
 // Two numbers of 32 bits whose order, as numbers of 64, they leave open.  A sigmoid
 // is off by 2^-22 (its exponential's error counts a quarter at most, the sum, the
 // reciprocal and the bias come to it), the scores of a softmax, which add up to 1,
-// by 2^-20 all together; a sum of two scores and two biases by twice that and its
-// own rounding.
+// by 2^-20 all together; with its bias each is rounded once more.
 DEV bool route_close(uint32_t larger, uint32_t smaller) {
   const float x = route_value(larger), d = x - route_value(smaller);
   return !(d > 0x1p-18f * __builtin_fmaxf(1.0f, __builtin_fabsf(x)));
@@ -317,8 +316,14 @@ DEV int route_choose(const RouteArgs& a, int64_t t, const float (&v)[P], const f
       value = __builtin_amdgcn_inverse_ballot_w64(first) ? 0u : value;
     }
     if ((!even || sums) && last != 0) {
-      const uint32_t next = route_max(value);
-      open = next != 0 && route_close(last, next);
+      // A value is off by its addends' errors, whatever they cancel to: at most 2^-20 and a
+      // rounding of 2^-24 of each addend and of the sum, below 2^-19 of their size.  The order
+      // is left open if a kept group may be below one that is not.
+      const float size = sums && two > -INFINITY ? __builtin_fabsf(one) + __builtin_fabsf(two) : __builtin_fabsf(one);
+      const float off = 0x1p-19f * __builtin_fmaxf(1.0f, size);
+      const uint32_t low = route_max(__builtin_amdgcn_inverse_ballot_w64(kept) ? route_key(off - sum) : 0u);  // (minus the least)
+      const uint32_t high = route_max(value != 0 ? route_key(off + sum) : 0u);
+      open = high != 0 && !(-route_value(low) > route_value(high));
     }
 #pragma unroll
     for (int i = 0; i < P; ++i) {

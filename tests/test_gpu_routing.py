@@ -667,3 +667,20 @@ def test_experts_in_int8_from_logits_to_the_sum_and_back():
         got = dl.double().cpu()
         assert ((got.gather(1, at)[:live] - want[:live]).abs() <= bound[:live] + 1e-30).all()
         assert (got.scatter(1, at, 0.0)[:live] == 0).all() and (got[live:] == 0).all() and (dx[live:] == 0).all() and (y[live:] == 0).all()
+
+
+@pytest.mark.parametrize("bound", [100.0, 1e3, 1e4, 1e5])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_values_of_groups_that_cancel(score, bound):
+    """Biases of opposite sign inside every group: its value is of the size of a score, its two addends, rounded to 32 bits,
+    are of the size of the bias."""
+    g = _gen(41)
+    e = 16
+    bias = torch.tensor([bound, -bound]).repeat(e // 2)
+    for t in (20, 6000):
+        logits = _normal(g, t, e, std=0.05)
+        _check(logits, 2, bias, score=score, groups=8, top_groups=4, group_best=2)
+    more = bias.clone()
+    more[4:6] = -1e30  # a group that its bias all but closes
+    more[9] = -INF  # one of a single open expert
+    _check(logits[:500], 2, more, score=score, groups=8, top_groups=4, group_best=2)
