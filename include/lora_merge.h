@@ -328,8 +328,8 @@ int lm_linear_weight_grad(const void* dy, int64_t lddy, const void* x, int64_t l
  *          its group_best (1 or 2) best c, as far as they are open; the
  *          top_groups best runs stay open (ties: the first)
  *   expert the top_k best c, the best first (ties: the lowest index); -1 where
- *          none is left.  c are compared as numbers of 64 bits, without a bias
- *          by their logits.
+ *          none is left.  c are compared as numbers of 64 bits, with a NULL
+ *          bias by their logits.
  *   weight scale * p, renormalize: scale * p / sum of the chosen p; 0 for -1
  * position [T, top_k]: the choices sorted by expert, those of one expert in the
  * order of the tokens, those of none behind all; ends [experts]: the choices of

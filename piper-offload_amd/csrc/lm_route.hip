@@ -252,10 +252,14 @@ DEV void route_two(float& one, float& two) {
 // in 32 bits, and where numbers that decide are close (`open`), in 64: among the chosen
 // and those next to them, or, where groups are close, all of it.  That is what LATE
 // does, and does it apart from the rest: with its registers the kernel runs 5 waves a
-// SIMD instead of 8, and one token in 300 needs it.
+// SIMD instead of 8, and one token in 300 needs it.  (A bias that is the same for all is
+// one too: far logits are the same number beside it, and the lowest index has them.  Its
+// choices are close where logits are equal: 8192 tokens, 64 experts, bf16 logits 19.9 us
+// with a bias of zeros, 16.2 with another, 11.6 without.)
 template <int DT, int P, bool LATE>
-DEV int route_choose(const RouteArgs& a, int64_t t, const float (&v)[P], const float (&b)[P], bool even, float* lds, bool& open) {
+DEV int route_choose(const RouteArgs& a, int64_t t, const float (&v)[P], const float (&b)[P], float* lds, bool& open) {
   const int lane = threadIdx.x & 63;
+  const bool even = !a.bias;  // the logits' order
   const bool in_groups = a.top_groups < a.groups, sums = in_groups && a.group_best == 2;
   float c[P];
   if (!even || sums) {
@@ -352,13 +356,13 @@ DEV int route_choose(const RouteArgs& a, int64_t t, const float (&v)[P], const f
 // One token: its choice, weights, and in ent its choice once more (E: none).  False,
 // and nothing done, where the choice is left to LATE.
 template <int DT, int P, bool LATE>
-DEV bool route_token(const RouteArgs& a, int64_t t, const float (&b)[P], bool even, float* row, uint16_t* ent) {
+DEV bool route_token(const RouteArgs& a, int64_t t, const float (&b)[P], float* row, uint16_t* ent) {
   const int lane = threadIdx.x & 63;
   float v[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) v[i] = lane + 64 * i < a.E ? route_load<DT>(a.logits, t * a.ld + lane + 64 * i) : -INFINITY;
   bool open;
-  const int mine = route_choose<DT, P, LATE>(a, t, v, b, even, row, open);
+  const int mine = route_choose<DT, P, LATE>(a, t, v, b, row, open);
   if (!LATE && open) return false;
   // the chosen experts' logits: e^x of softmax, e^min(x, 0) / (1 + e^-|x|) of sigmoid, so that none overflows
   const bool on = mine >= 0;
@@ -390,24 +394,19 @@ DEV bool route_token(const RouteArgs& a, int64_t t, const float (&b)[P], bool ev
   }
   return true;
 }
-// The lane's biases; true if they decide nothing: none, or the same for all.
+// The lane's biases.
 template <int P>
-DEV bool route_bias(const RouteArgs& a, float (&b)[P]) {
+DEV void route_bias(const RouteArgs& a, float (&b)[P]) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int i = 0; i < P; ++i) b[i] = a.bias && lane + 64 * i < a.E ? a.bias[lane + 64 * i] : 0.0f;
-  const float b0 = u2f((uint32_t)__builtin_amdgcn_readfirstlane((int)f2u(b[0])));
-  bool even = true;
-#pragma unroll
-  for (int i = 0; i < P; ++i) even = even && (lane + 64 * i >= a.E || b[i] == b0);
-  return __ballot(even) == ~0ull && __builtin_fabsf(b0) < INFINITY;
 }
 // A call, so that its registers are not the loop's.
 template <int DT, int P>
 __device__ __attribute__((noinline)) void route_late(const RouteArgs* a, int64_t t, float* row, uint16_t* ent) {
   float b[P];
-  const bool even = route_bias<P>(*a, b);
-  route_token<DT, P, true>(*a, t, b, even, row, ent);
+  route_bias<P>(*a, b);
+  route_token<DT, P, true>(*a, t, b, row, ent);
 }
 
 // A workgroup has a.block tokens, a wave one of them at a time.  Ranks of its choices
@@ -430,10 +429,10 @@ __global__ __launch_bounds__(ROUTE_THREADS<P>, P <= 4 ? 8 : P <= 8 ? 4 : 2) void
   const int tokens = (int)(a.T - t0 < a.block ? a.T - t0 : a.block), n = tokens * a.k;
   for (int i = tid; i <= a.E; i += threads) count[i] = 0;
   float b[P];
-  const bool even = route_bias<P>(a, b);
+  route_bias<P>(a, b);
   uint32_t left = 0;  // of this wave's tokens, at most 8
   for (int i = 0, tl = wave; tl < tokens; ++i, tl += waves)
-    if (!route_token<DT, P, false>(a, t0 + tl, b, even, row, ent + tl * a.k)) left |= 1u << i;
+    if (!route_token<DT, P, false>(a, t0 + tl, b, row, ent + tl * a.k)) left |= 1u << i;
   const RouteArgs* const args = (const RouteArgs*)__builtin_amdgcn_kernarg_segment_ptr();  // (the kernel's one argument)
   for (; left; left &= left - 1) {
     const int tl = wave + __builtin_ctz(left) * waves;

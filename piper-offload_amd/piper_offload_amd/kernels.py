@@ -1038,8 +1038,8 @@ def route_topk(logits: torch.Tensor, top_k: int, *, bias: torch.Tensor | None = 
     ``score`` 'softmax' or 'sigmoid' of the logits.  ``bias`` (float32 [experts]) is added for the choice alone.  With
     ``groups`` the experts form that many runs; the ``top_groups`` runs with the largest sums of their ``group_best``
     best choices stay open.  The weights are ``scale`` times the scores, divided by the sum of the chosen ones if
-    ``renormalize``.  Ties go to the lowest index; scores are compared as numbers of 64 bits (without a bias by their
-    logits).  An expert whose logit (or bias) is -inf is closed: so is every expert of a padding token whose row is
+    ``renormalize``.  Ties go to the lowest index; scores are compared as numbers of 64 bits (by their logits where
+    ``bias`` is None).  An expert whose logit (or bias) is -inf is closed: so is every expert of a padding token whose row is
     -inf.  A row with a NaN (softmax: or +inf) has NaN weights.  float32 throughout.
     """
     label = "Routing"

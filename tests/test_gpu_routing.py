@@ -684,3 +684,23 @@ def test_values_of_groups_that_cancel(score, bound):
     more[4:6] = -1e30  # a group that its bias all but closes
     more[9] = -INF  # one of a single open expert
     _check(logits[:500], 2, more, score=score, groups=8, top_groups=4, group_best=2)
+
+
+def test_a_bias_that_is_the_same_for_all_is_a_bias():
+    """With one the numbers p + bias decide, and those of far logits are equal in 64 bits: the lowest index has them."""
+    rows = {"sigmoid": [[40.0, 50.0, 45.0, -3.0], [50.0, 40.0, 60.0, 41.0], [-60.0, -50.0, -70.0, -55.0], [-2.0, 60.0, 1.0, 70.0]],
+            "softmax": [[-900.0, -800.0, 0.0, -1000.0], [0.0, -900.0, -800.0, -850.0], [-800.0, -790.0, -780.0, 5.0], [1.0, 2.0, -800.0, 900.0]]}
+    for score, logits in rows.items():
+        logits = torch.tensor(logits)
+        for t in (1, 50):
+            for value in (0.0, 0.25):
+                bias = torch.full((4,), value)
+                x = logits.repeat(t, 1)
+                for how in ({}, dict(groups=2, top_groups=1, group_best=1), dict(groups=2, top_groups=1, group_best=2)):
+                    _check(x, 2, bias, score=score, **how)
+                    _check(x, 2, None, score=score, **({} if how.get("group_best") == 1 else how))
+            more = torch.tensor([0.0, 0.0, 0.0, 1e-30])  # (nothing beside a score of 1)
+            _check(logits.repeat(t, 1), 2, more, score=score)
+    many = torch.linspace(40.0, 90.0, 300).flip(0).repeat(3, 1)  # (more equal ones than a wave has lanes)
+    r = _check(many, 5, torch.zeros(300), score="sigmoid")
+    assert r.expert.tolist() == [[0, 1, 2, 3, 4]] * 3
