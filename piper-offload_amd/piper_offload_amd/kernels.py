@@ -906,6 +906,7 @@ def _int8_weight(label: str, qdata: torch.Tensor, scale: torch.Tensor, stacked: 
         raise ValueError(f"{label} requires a non-empty weight.")
     if sshape != shape[:-1] and sshape != (*shape[:-1], 1):
         raise ValueError(f"{label} takes one scale per row of the weight, got scales {tuple(sshape)} for codes {tuple(shape)}.")
+    _raw(label, scale)
     return L.WeightStruct(qdata.data_ptr(), scale.data_ptr(), shape[-2], shape[-1], L.LM_I8, 0, shape[0] if stacked else 1,
                           L.torch_dtype_id(scale.dtype))
 

@@ -10,7 +10,7 @@ After a merge a packed weight is used as it is stored, without a dense copy:
   INT8.
 
 Gradients: to ``x`` for every weight, to the weight where it is dense.  A
-packed weight is frozen, as is a bias.  With quantised inputs the gradient
+packed weight is frozen, its scales too, as is a bias.  With quantised inputs the gradient
 passes straight through the rounding.
 
 The experts of a packed stack lie one below the other in one ``MXWeight`` or
@@ -61,6 +61,12 @@ def _int8(label: str, weight: Int8Weight) -> tuple[torch.Tensor, torch.Tensor]:
     if weight.act_pre_scale is not None:
         raise ValueError(f"{label} does not apply an activation pre-scale; multiply the input by it.")
     return q, weight.scale.reshape(-1, 1)
+
+
+def _frozen(label: str, name: str, t: torch.Tensor | None) -> None:
+    """What belongs to a packed weight has no gradient; refuse to lose one."""
+    if t is not None and t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{label}: the {name} is frozen with its packed weight; detach it.")
 
 
 def _int8_stacked(label: str, weight: Int8Weight, groups: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -168,8 +174,8 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None =
     ``activation_dtype=torch.int8`` quantises every row of ``x`` first.  Differentiable in ``x``.
     """
     q, s = _int8("INT8 linear", weight)
-    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
-        raise ValueError("INT8 linear: the bias is frozen with its packed weight; detach it.")
+    _frozen("INT8 linear", "scale", weight.scale)
+    _frozen("INT8 linear", "bias", bias)
     return _Int8Linear.apply(x, q, s, bias, activation_dtype)
 
 
@@ -183,6 +189,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor, *,
     """
     if isinstance(weight, Int8Weight):
         q, s = _int8_stacked("Grouped linear", weight, ends.shape[0] if ends.ndim == 1 else 0)
+        _frozen("Grouped linear", "scale", weight.scale)
         return _GroupedInt8.apply(x, q, s, ends, activation_dtype)
     if isinstance(weight, MXWeight):
         q, s = _stacked("Grouped linear", weight, ends.shape[0] if ends.ndim == 1 else 0)

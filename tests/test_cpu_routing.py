@@ -9,7 +9,7 @@ import subprocess
 import pytest
 import torch
 
-from piper_offload_amd import Int8Weight, combine_experts, dispatch_experts, expert_view, int8_linear, route_experts
+from piper_offload_amd import Int8Weight, combine_experts, dispatch_experts, expert_view, grouped_linear, int8_linear, route_experts
 from piper_offload_amd import _lib as L
 from piper_offload_amd import kernels as K
 
@@ -148,3 +148,24 @@ def test_routing_arguments_are_checked(over):
     args = dict(logits=torch.zeros(4, 16), top_k=2, bias=None, score="softmax", groups=1, top_groups=1, group_best=1, renormalize=True, scale=1.0) | over
     with pytest.raises(ValueError):
         K._route("Routing", **args)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_of_int8_scales_are_refused(dtype):
+    """A scale is a number that could be trained; the products have no gradient for it and say so."""
+    x, ends = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int32)
+    q, s = torch.zeros(32, 64, dtype=torch.int8), torch.ones(32, 1, dtype=dtype, requires_grad=True)
+    w = Int8Weight(q, s, (1, 64))
+    for rows in (x, x.clone().requires_grad_()):
+        for call in (lambda: int8_linear(rows, w), lambda: grouped_linear(rows, w, ends)):
+            with pytest.raises(ValueError, match="scale is frozen"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+                call()
+    for codes, scale in ((q, s), (q.view(4, 8, 64), s.view(4, 8, 1))):
+        with pytest.raises(NotImplementedError, match="gradient"):
+            K._int8_weight("INT8 product", codes, scale, codes.ndim == 3)
+        with torch.no_grad():
+            assert K._int8_weight("INT8 product", codes, scale, codes.ndim == 3).dtype == L.LM_I8
+        assert K._int8_weight("INT8 product", codes, scale.detach(), codes.ndim == 3).dtype == L.LM_I8
+    expert_view(w, 1, 4)  # (a view is not a product)
