@@ -280,7 +280,10 @@ int lm_routed_residual(const void* x, const void* y, void* out, int64_t T, int64
  * scale a row, codes [experts, N, K] and `scale` fp32 or bf16 [experts, N]
  * (`reserved` says which: LM_F32 or LM_BF16); the product sees the codes
  * exactly and multiplies its sum by the scale, the input gradient sees each
- * weight rounded to `dtype`.  Otherwise a dense weight [experts, N, K] of
+ * weight rounded to bf16, or to fp16's 11 bits: in fp16 an expert's weights count
+ * as 2^f of themselves, its largest finite scale as 128 to 256, and the sum as
+ * 2^-f of itself, so scales may have any size (those below 2^-21 of the largest
+ * lose bits).  Otherwise a dense weight [experts, N, K] of
  * `dtype`.
  * `ends`: device int32[experts]; group e's rows are [ends[e-1], ends[e]).  Rows
  * past ends[experts-1] get zeros, without the bias.  NULL with one expert: all
@@ -294,8 +297,8 @@ int lm_routed_residual(const void* x, const void* y, void* out, int64_t T, int64
  * passes straight through either rounding.
  * Strides are in elements; outputs are contiguous; N, K < 2^21.  Workspace:
  * lm_linear_workspace_size bytes for the call's sizes and strides (ldb: ldx of
- * the weight gradient, else 0; aligned: the pointers of rows and weights are
- * multiples of 16), 256-byte aligned; NULL when that is 0. */
+ * the weight gradient, else 0; input_dtype of the gradients: the rows'; aligned:
+ * the pointers of rows and weights are multiples of 16), 256-byte aligned; NULL when that is 0. */
 enum lm_linear_op { LM_LINEAR_FORWARD = 0, LM_LINEAR_INPUT_GRAD = 1, LM_LINEAR_WEIGHT_GRAD = 2 };
 #define LM_LINEAR_MAX_EXPERTS 1024
 typedef struct lm_weight {

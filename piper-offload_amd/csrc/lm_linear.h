@@ -26,6 +26,7 @@ struct LinArgs {
   // INT8 weights: `scale` has one number a row, fp32 or bf16 (scale16); 8-bit inputs: one fp32 number a row of x
   const float* row_scale;
   int scale16;
+  const int32_t* shift;  // fp16 input gradient of INT8 weights: one a group, its weights count as 2^shift of themselves (k_lin8_shift)
   const void* bias;
   const int32_t* ends;  // [experts] or null: one group of all T rows
   void* out;

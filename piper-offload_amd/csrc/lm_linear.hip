@@ -327,7 +327,7 @@ static int lin_setup(LinArgs& a, const LinPlan& p, int op, void* workspace, size
 extern "C" size_t lm_linear_workspace_size(int32_t op, int64_t T, int64_t lda, int64_t ldb, int64_t N, int64_t K,
                                            int32_t experts, int32_t weight_dtype, int32_t input_dtype, int32_t aligned) {
   if (T <= 0 || N <= 0 || K <= 0 || experts <= 0 || op < LM_LINEAR_FORWARD || op > LM_LINEAR_WEIGHT_GRAD) return 0;
-  if (weight_dtype == LM_I8) return op == LIN_WEIGHT_GRAD ? 0 : lin8_workspace(op, T, lda, N, K, experts, input_dtype == LM_I8, aligned != 0);
+  if (weight_dtype == LM_I8) return op == LIN_WEIGHT_GRAD ? 0 : lin8_workspace(op, T, lda, N, K, experts, input_dtype == LM_I8, aligned != 0, input_dtype != LM_BF16);
   return lin_plan(op, T, lda, ldb, N, K, experts, weight_dtype == LM_E2M1, op == LIN_FORWARD && input_dtype == LM_E2M1, aligned != 0)
       .total;
 }

@@ -6,6 +6,7 @@
 // products of codes, at most 127 * 128 each, add up in 32 bits
 constexpr int LIN8_MAX_SUM = 0x7fffffff / (127 * 128);
 
-size_t lin8_workspace(int op, int64_t T, int64_t lda, int64_t N, int64_t K, int64_t E, bool quant, bool aligned);
+// half: rows of fp16, as far as it matters to the input gradient
+size_t lin8_workspace(int op, int64_t T, int64_t lda, int64_t N, int64_t K, int64_t E, bool quant, bool aligned, bool half);
 int lin8_forward(LinArgs& a, int dtype, bool quant, void* workspace, size_t workspace_bytes, hipStream_t st);
 int lin8_input_grad(LinArgs& a, int dtype, void* workspace, size_t workspace_bytes, hipStream_t st);

@@ -8,7 +8,10 @@
 // The products of one weight, or of one weight per group of rows.
 //
 // The input gradient rounds s q to 16 bits: s lies along its sum, so the product cannot be
-// multiplied by it afterwards, and to round dy s instead is off by as much.
+// multiplied by it afterwards, and to round dy s instead is off by as much.  fp16 has not
+// the range of the scales: there 2^f s q is rounded, f of each weight such that its largest
+// scale counts as 128 to 256 (k_lin8_shift), and the sum is multiplied by 2^-f.  Weights
+// whose scale is above 2^-21 of that one's keep all their bits.
 //
 // Many rows (k_lin_mm): codes times codes are bound by the power that the matrix unit
 // may take, 4096 rows of [14336, 4096] 234 us (2.06 POP/s at 1.86 GHz, 64% of the cycles
@@ -95,6 +98,26 @@ __global__ __launch_bounds__(256) void k_lin8_tail(const uint16_t* src, int64_t 
   }
 }
 
+// The power of two of every weight's scales, from the largest finite one, a workgroup a
+// weight.  A launch, and what it takes: a gradient over [4096, 4096] in fp16 16.8 -> 19.2 us
+// at one row, with 14336 scales and 2048 rows 260 either way.
+__global__ __launch_bounds__(1024) void k_lin8_shift(LinArgs a, int32_t* shift) {
+  __shared__ uint32_t red[16];
+  const int64_t first = blockIdx.x * a.N;
+  uint32_t top = 0;
+  for (int64_t i = threadIdx.x; i < a.N; i += 1024) {
+    const uint32_t b = f2u(lin_scale8(a, first + i)) & 0x7fffffffu;
+    top = b > top && b < 0x7f800000u ? b : top;
+  }
+  top = lin8_wave_max(top);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = red[i] > top ? red[i] : top;
+  shift[blockIdx.x] = top == 0 ? 0 : 8 - __builtin_amdgcn_frexp_expf(u2f(top));
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -117,7 +140,8 @@ struct Lin8Plan {
   bool tail;                 // and x's last elements as k_lin8_tail (8-bit inputs: k_lin8_prep) has them
   bool raw;                  // 8-bit inputs: codes of the weight at any address
   int64_t pitch, lda, ldw;   // of the codes of x, of 16-bit rows, of the weight (bytes)
-  size_t codes, codes_bytes, scales, x, w, part, total;
+  bool half;                 // fp16 input gradient: k_lin8_shift
+  size_t codes, codes_bytes, scales, x, w, part, shift, total;
 };
 
 // As lin_few: a matter of the product's volume.
@@ -128,7 +152,7 @@ static bool lin8_few(int64_t T, int64_t N, int64_t K, int64_t E, bool quant) {
   return rows <= 16 || volume <= 1.1e9 || (quant && T <= 64);
 }
 
-static Lin8Plan lin8_plan(int op, int64_t T, int64_t lda, int64_t N, int64_t K, int64_t E, bool quant, bool aligned) {
+static Lin8Plan lin8_plan(int op, int64_t T, int64_t lda, int64_t N, int64_t K, int64_t E, bool quant, bool aligned, bool half) {
   Lin8Plan p{};
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -175,12 +199,14 @@ static Lin8Plan lin8_plan(int op, int64_t T, int64_t lda, int64_t N, int64_t K, 
     lin_tiling(p.mm, op, T, J, p.mm.len, E, !quant, false);
     if (p.mm.splits > 1) p.part = take((size_t)p.mm.splits * T * J * 4);
   }
+  p.half = op == LIN_INPUT_GRAD && half;
+  if (p.half) p.shift = take((size_t)E * 4);
   p.total = at;
   return p;
 }
 
-size_t lin8_workspace(int op, int64_t T, int64_t lda, int64_t N, int64_t K, int64_t E, bool quant, bool aligned) {
-  return lin8_plan(op, T, lda, N, K, E, quant, aligned).total;
+size_t lin8_workspace(int op, int64_t T, int64_t lda, int64_t N, int64_t K, int64_t E, bool quant, bool aligned, bool half) {
+  return lin8_plan(op, T, lda, N, K, E, quant, aligned, half).total;
 }
 
 template <int DT, bool Q8, bool OWN, int MF, int CF, int NW, int UN>
@@ -250,6 +276,11 @@ static int lin8_setup(LinArgs& a, const Lin8Plan& p, int op, int dtype, void* wo
     a.row_scale = scales;
     if (p.copy_w) a.w = base + p.w;
   }
+  if (p.half) {
+    a.shift = (const int32_t*)(base + p.shift);
+    hipLaunchKernelGGL(k_lin8_shift, dim3((unsigned)a.experts), dim3(1024), 0, st, a, (int32_t*)(base + p.shift));
+    LAUNCH_CHECK();
+  }
   a.ldw = p.ldw;
   a.len = p.mm.len;
   a.part = p.mm.splits > 1 ? (float*)(base + p.part) : nullptr;
@@ -257,7 +288,7 @@ static int lin8_setup(LinArgs& a, const Lin8Plan& p, int op, int dtype, void* wo
 }
 
 int lin8_forward(LinArgs& a, int dtype, bool quant, void* workspace, size_t workspace_bytes, hipStream_t st) {
-  const Lin8Plan p = lin8_plan(LIN_FORWARD, a.T, a.lda, a.N, a.K, a.experts, quant, aligned16(a.a) && aligned16(a.w));
+  const Lin8Plan p = lin8_plan(LIN_FORWARD, a.T, a.lda, a.N, a.K, a.experts, quant, aligned16(a.a) && aligned16(a.w), false);
   int rc;
   if ((rc = lin8_setup(a, p, LIN_FORWARD, dtype, workspace, workspace_bytes, st))) return rc;
   uint8_t* codes = (uint8_t*)workspace + p.codes;
@@ -277,7 +308,7 @@ int lin8_forward(LinArgs& a, int dtype, bool quant, void* workspace, size_t work
 }
 
 int lin8_input_grad(LinArgs& a, int dtype, void* workspace, size_t workspace_bytes, hipStream_t st) {
-  const Lin8Plan p = lin8_plan(LIN_INPUT_GRAD, a.T, a.lda, a.N, a.K, a.experts, false, aligned16(a.a) && aligned16(a.w));
+  const Lin8Plan p = lin8_plan(LIN_INPUT_GRAD, a.T, a.lda, a.N, a.K, a.experts, false, aligned16(a.a) && aligned16(a.w), dtype == LM_F16);
   int rc;
   if ((rc = lin8_setup(a, p, LIN_INPUT_GRAD, dtype, workspace, workspace_bytes, st))) return rc;
   return run_mm<LIN_INPUT_GRAD, W_I8>(a, p.mm, dtype, st);

@@ -20,7 +20,8 @@
 //         their way into LDS and then are KS16
 //   KC8   INT8 codes along the contraction, KS8 across it: decoded on their way into
 //         LDS too, and then KC16 (the codes alone: the scales come with the store)
-//         and KS16 (times their row's scale, which lies along the sum)
+//         and KS16 (times their row's scale, which lies along the sum; in fp16 with a
+//         power of two that brings a weight's scales into its range and comes out of the sums)
 // Q8: both operands INT8 codes; a slot of 64 bytes has 64 of them, and all but the
 // matrix instruction is as for 16 bits (the arguments count in pairs of codes).
 //   KR8   the weight's codes where rows start anywhere: loads straight to LDS take whole
@@ -258,6 +259,8 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
   const int splits = OP == LIN_WEIGHT_GRAD ? gridDim.z : gridDim.y, split = OP == LIN_WEIGHT_GRAD ? blockIdx.z : blockIdx.y;
   const int per = ((nk + splits - 1) / splits + 3) & ~3, kb = split * per, ke = kb + per < nk ? kb + per : nk;
   v4f32 acc[FI][FJ] = {};
+  constexpr bool SHIFT = JK == KS8 && HALF;
+  const int shift = SHIFT && t.group < a.experts ? __builtin_amdgcn_readfirstlane(a.shift[t.group]) : 0;
 
   if (kb < ke) {
     uint32_t io[P::IL], jo[P::JL];
@@ -414,7 +417,8 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
       if constexpr (JK == KC8 || JK == KS8) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const lm_u32x4 v = lin_decode8i<HALF, JK == KS8>(code8[set][2 * c], code8[set][2 * c + 1], JK == KS8 ? u2f(code_s[set]) : 1.0f);
+          const float s = JK != KS8 ? 1.0f : SHIFT ? __builtin_ldexpf(u2f(code_s[set]), shift) : u2f(code_s[set]);
+          const lm_u32x4 v = lin_decode8i<HALF, JK == KS8>(code8[set][2 * c], code8[set][2 * c + 1], s);
           if constexpr (JK == KC8) *(lds_u32x4*)(tj + kr * 64 + (((kc * 2 + c) ^ mm_key(kr)) << 4)) = v;
           else *(lds_u32x4*)(tj + kr * (BN * 2) + (((kc * 2 + c) ^ mm_row_key<BN>(kr)) << 4)) = v;
         }
@@ -587,6 +591,14 @@ __global__ __launch_bounds__(WM* WN * 64, SHORT ? 5 : 2) void k_lin_mm(LinArgs a
     }
   }
 
+  if constexpr (SHIFT) {
+#pragma unroll
+    for (int x = 0; x < FI; ++x)
+#pragma unroll
+      for (int y = 0; y < FJ; ++y)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[x][y][e] = __builtin_ldexpf(acc[x][y][e], -shift);
+  }
   const int64_t rows0 = OP == LIN_WEIGHT_GRAD ? t.group * a.N : 0;  // of the output above this group's
   if (a.part) {  // a part of the sums: k_lin_join adds them up
     float* part = a.part + (split * (OP == LIN_WEIGHT_GRAD ? a.experts * a.N : a.T) + rows0) * jend;

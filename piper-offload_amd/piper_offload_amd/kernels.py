@@ -928,7 +928,8 @@ def int8_matmul(x: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor, *, bi
 def int8_matmul_input_grad(dy: torch.Tensor, qdata: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     """``dy @ W``: the input gradient of :func:`int8_matmul` (straight through a quantised input).
 
-    ``W`` is rounded to ``dy.dtype`` here: its scales lie along the sums.
+    ``W`` is rounded to ``dy.dtype`` here: its scales lie along the sums.  In float16 that is 11 bits whatever the scales'
+    size: the largest counts as 128 to 256 (rows whose scale is below 2^-21 of it lose bits).
     """
     label = "INT8 product gradient"
     _on_gpu(label, dy, qdata, scale)

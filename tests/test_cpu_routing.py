@@ -169,3 +169,14 @@ def test_gradients_of_int8_scales_are_refused(dtype):
             assert K._int8_weight("INT8 product", codes, scale, codes.ndim == 3).dtype == L.LM_I8
         assert K._int8_weight("INT8 product", codes, scale.detach(), codes.ndim == 3).dtype == L.LM_I8
     expert_view(w, 1, 4)  # (a view is not a product)
+
+
+def test_c_int8_gradients_in_fp16_need_their_workspace():
+    """A power of two for each expert's scales; bf16 needs none."""
+    w = L.WeightStruct(4096, 4096, 64, 128, L.LM_I8, 0, 3, 0)
+    handle = L.load_library()
+    assert handle.lm_linear_workspace_size(1, 4, 64, 0, 64, 128, 3, L.LM_I8, L.LM_BF16, 1) == 0
+    need = handle.lm_linear_workspace_size(1, 4, 64, 0, 64, 128, 3, L.LM_I8, L.LM_F16, 1)
+    assert need >= 3 * 4
+    for ws, size, want in ((None, 0, L.LM_EWORKSPACE), (4096, need - 1, L.LM_EWORKSPACE), (4100, need, L.LM_EINVAL)):
+        assert handle.lm_linear_input_grad(4096, 64, ctypes.byref(w), 4096, 4096, 4, L.LM_F16, ws, size, None) == want

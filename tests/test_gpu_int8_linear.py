@@ -512,3 +512,69 @@ def test_groups_of_rows_of_any_length(sizes, n, k, dtype):
             _check(x[begin:end], q[i], s[i], y[begin:end], True)
         begin = end
     assert (y[begin:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("scale_dtype", [torch.float32, BF16], ids=["s32", "s16"])
+@pytest.mark.parametrize("s0,d0", [(1e-9, 2.0**13), (1e-12, 2.0**14), (1e3, 2.0**-12), (2e4, 2.0**-14), (1.0, 1.0)])
+@pytest.mark.parametrize("t,n,k", [(1, 16, 64), (40, 300, 129), (200, 512, 257), (300, 2000, 256)])
+def test_input_grad_with_scales_of_any_size(t, n, k, s0, d0, scale_dtype, dtype):
+    """Weights below and above float16's own range.
+
+    Their largest scale counts as 128 to 256, and no scale here is less than a quarter of it, so the weights (codes of 1 too)
+    are float16's normal numbers and each is off by half a step: 2^-11 of its magnitude.
+    """
+    g = _gen(t + n + k)
+    q = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8)
+    s = ((0.25 + 0.75 * torch.rand(n, 1, generator=g)) * s0).to(scale_dtype)
+    s[n // 2] = s0
+    dy = _normal(g, t, n, std=d0).clamp(-3 * d0, 3 * d0).to(dtype)
+    got = K.int8_matmul_input_grad(dy.to(DEV), q.to(DEV), s.to(DEV))
+    w = q.double() * s.double()
+    half, _ = _half(dtype)
+    _close(got, dy.double() @ w, ((n + 4) * 2.0**-23 + half) * (dy.double().abs() @ w.abs()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_input_grad_of_groups_with_scales_of_any_size(dtype):
+    """Every group's scales of a size of their own; a scale that is not finite makes its own group's rows so."""
+    g = _gen(52)
+    sizes, n, k = [70, 0, 3, 130, 64], 264, 272
+    size = torch.tensor([1e-9, 1.0, 2e3, 1e-4, 1e-6])
+    d0 = torch.tensor([2.0**13, 1.0, 2.0**-12, 1.0, 2.0**6])
+    e, t = len(sizes), sum(sizes) + 5
+    q = torch.randint(-128, 128, (e, n, k), generator=g, dtype=torch.int8)
+    s = (0.25 + 0.75 * torch.rand(e, n, 1, generator=g)) * size[:, None, None]
+    ends = _ends(sizes)
+    of = torch.repeat_interleave(torch.arange(e), torch.tensor(sizes))
+    dy = _normal(g, t, n)
+    dy[:t - 5] *= d0[of][:, None]
+    dy = dy.to(dtype)
+    half, _ = _half(dtype)
+    for bad in (False, True):
+        if bad:
+            s[3, 7] = float("inf")
+            s[4, 100] = float("nan")
+        got = K.grouped_int8_matmul_input_grad(dy.to(DEV), q.to(DEV), s.to(DEV), ends.to(DEV))
+        begin = 0
+        for i, end in enumerate(ends.tolist()):
+            if bad and i >= 3:
+                assert not torch.isfinite(got[begin:end]).any()
+            else:
+                w, rows = q[i].double() * s[i].double(), dy[begin:end].double()
+                _close(got[begin:end], rows @ w, ((n + 4) * 2.0**-23 + half) * (rows.abs() @ w.abs()))
+            begin = end
+        assert (got[begin:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_input_grad_with_scales_of_zero(dtype):
+    g = _gen(53)
+    q = torch.randint(-128, 128, (96, 144), generator=g, dtype=torch.int8)
+    dy = _normal(g, 20, 96, dtype=dtype)
+    s = torch.zeros(96, 1)
+    assert (K.int8_matmul_input_grad(dy.to(DEV), q.to(DEV), s.to(DEV)) == 0).all()
+    s[5] = -3e-9  # (signs count)
+    dy[:, 5] *= 1e4
+    w, rows = q.double() * s.double(), dy.double()
+    _close(K.int8_matmul_input_grad(dy.to(DEV), q.to(DEV), s.to(DEV)), rows @ w, (100 * 2.0**-23 + _half(dtype)[0]) * (rows.abs() @ w.abs()))
