@@ -339,7 +339,7 @@ int lm_linear_weight_grad(const void* dy, int64_t lddy, const void* x, int64_t l
  * the experts up to each, the `ends` of lm_linear.  A row with a NaN (softmax:
  * or a +inf) has NaN weights and experts that exist.
  * The gradient needs the logits, the settings and the experts; it writes
- * [T, experts] of dtype.  `r` is a HOST struct.  T <= 2^28, T top_k < 2^31.
+ * [T, experts] of dtype.  `r` is a HOST struct.  T <= 2^28 - 64, T top_k < 2^31.
  * Workspace: 256-byte aligned, NULL when lm_route_workspace_size is 0. */
 enum lm_route_score { LM_ROUTE_SOFTMAX = 0, LM_ROUTE_SIGMOID = 1 };
 #define LM_ROUTE_MAX_BEST 64

@@ -877,6 +877,7 @@ __global__ __launch_bounds__(256) void k_rows_back_grad(RowsArgs a) {
 // host side
 // ---------------------------------------------------------------------------
 constexpr int64_t ROWS_GRID = 1 << 22;  // workgroups that take a token after the other (a launch has fewer than 2^32 threads)
+constexpr int64_t ROUTE_TOKENS = (1 << 28) - 64;  // (k_route: 64 a workgroup of 1024 threads then)
 
 static int check_route(const lm_route* r) {
   if (!r) return fail(LM_EINVAL, "routing needs its description");
@@ -891,7 +892,7 @@ static int check_route(const lm_route* r) {
     return fail(LM_EINVAL, "group_best must be 1 or 2 and at most the experts of a group");
   if (r->top_k < 1 || r->top_k > LM_ROUTE_MAX_BEST || r->top_k > r->top_groups * (r->experts / r->groups))
     return fail(LM_EINVAL, "top_k must be 1 to %d and at most the experts of the kept groups", LM_ROUTE_MAX_BEST);
-  if (r->T > (1 << 28) || r->T * r->top_k > 0x7fffffff) return fail(LM_EUNSUPPORTED, "more than 2^28 tokens or 2^31 - 1 choices");
+  if (r->T > ROUTE_TOKENS || r->T * r->top_k > 0x7fffffff) return fail(LM_EUNSUPPORTED, "more than 2^28 - 64 tokens or 2^31 - 1 choices");
   if (r->T > 0 && !r->logits) return fail(LM_EINVAL, "logits must be non-null");
   if (r->ld < r->experts) return fail(LM_EINVAL, "row stride below the row length");
   return LM_OK;
@@ -966,7 +967,7 @@ static RouteArgs route_args(const lm_route* r) {
   } while (0)
 
 extern "C" size_t lm_route_workspace_size(int64_t T, int32_t experts) {
-  if (T <= 0 || T > (1 << 28) || experts < 1 || experts > LM_LINEAR_MAX_EXPERTS) return 0;
+  if (T <= 0 || T > ROUTE_TOKENS || experts < 1 || experts > LM_LINEAR_MAX_EXPERTS) return 0;
   return route_space(T, experts).total;
 }
 

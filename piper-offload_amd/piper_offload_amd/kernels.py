@@ -963,6 +963,7 @@ def grouped_int8_matmul_input_grad(dy: torch.Tensor, qdata: torch.Tensor, scale:
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _MAX_BEST = 64
 _MAX_GROUPS = 64
+_MAX_TOKENS = (1 << 28) - 64  # what one launch can hold
 _LOGIT_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
@@ -1000,8 +1001,8 @@ def _route(label: str, logits: torch.Tensor, top_k: int, bias: torch.Tensor | No
         raise ValueError(f"{label}: group_best must be 1 or 2, and at most the experts of a group, got {group_best}.")
     if not 1 <= top_k <= min(_MAX_BEST, top_groups * (experts // groups)):
         raise ValueError(f"{label}: top_k must be 1 to {min(_MAX_BEST, top_groups * (experts // groups))}, got {top_k}.")
-    if tokens > 1 << 28 or tokens * top_k >= 1 << 31:
-        raise ValueError(f"{label} takes up to 2^28 tokens and fewer than 2^31 choices, got {tokens} tokens of {top_k}.")
+    if tokens > _MAX_TOKENS or tokens * top_k >= 1 << 31:
+        raise ValueError(f"{label} takes up to 2^28 - 64 tokens and fewer than 2^31 choices, got {tokens} tokens of {top_k}.")
     if not math.isfinite(scale) or scale == 0:
         raise ValueError(f"{label}: scale must be finite and not zero, got {scale}.")
     if bias is not None:

@@ -180,3 +180,18 @@ def test_c_int8_gradients_in_fp16_need_their_workspace():
     assert need >= 3 * 4
     for ws, size, want in ((None, 0, L.LM_EWORKSPACE), (4096, need - 1, L.LM_EWORKSPACE), (4100, need, L.LM_EINVAL)):
         assert handle.lm_linear_input_grad(4096, 64, ctypes.byref(w), 4096, 4096, 4, L.LM_F16, ws, size, None) == want
+
+
+def test_tokens_that_one_launch_cannot_hold_are_refused():
+    """64 tokens a workgroup of 1024 threads, and fewer than 2^32 threads a launch."""
+    handle, most = L.load_library(), (1 << 28) - 64
+    for t in (most + 1, 1 << 28):
+        r = L.RouteStruct(4096, None, 1, t, 1, L.LM_F32, 0, 1, 1, 1, 1, 1, 1.0, 0)
+        assert handle.lm_route_workspace_size(t, 1) == 0
+        assert handle.lm_route_topk(ctypes.byref(r), 4096, 4096, 4096, 4096, None, 0, None) == L.LM_EUNSUPPORTED
+        assert handle.lm_route_topk_grad(ctypes.byref(r), 4096, 4096, 4096, None) == L.LM_EUNSUPPORTED
+        with pytest.raises(ValueError, match="tokens"):
+            K._route("Routing", torch.zeros(1, 1).expand(t, 1), 1, None, "softmax", 1, 1, 1, True, 1.0)
+    assert handle.lm_route_workspace_size(most, 1) > 0
+    r = L.RouteStruct(4096, None, 1, most, 1, L.LM_F32, 0, 1, 1, 1, 1, 1, 1.0, 0)
+    assert handle.lm_route_topk(ctypes.byref(r), 4096, 4096, 4096, 4096, None, 0, None) == L.LM_EWORKSPACE
