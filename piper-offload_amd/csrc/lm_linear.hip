@@ -236,7 +236,7 @@ static int launch_align(const void* src, int64_t lds, int64_t rows, int64_t cols
   TimedLaunch timed("linear_prep", st);
   const int64_t n = (rows * (ldd / 8) + 255) / 256;
   if (n == 0) return LM_OK;
-  if (n > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+  if (!lin_holds(n, 256)) return fail(LM_EUNSUPPORTED, "product too large for one launch");
   hipLaunchKernelGGL(k_lin_align, dim3((unsigned)n), dim3(256), 0, st, (const uint16_t*)src, lds, rows, cols, (uint16_t*)dst, ldd);
   LAUNCH_CHECK();
   return LM_OK;
@@ -246,7 +246,7 @@ template <int DT, int W, int MF, int CF, int NW, int UN, bool EDGE = false>
 static int launch_few(const LinArgs& a, hipStream_t st) {
   TimedLaunch timed("linear_few", st);
   const int64_t n = lin_tiles<16 * MF>(a.T, a.experts, a.ends != nullptr) * ((a.N + 16 * CF - 1) / (16 * CF));
-  if (n > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+  if (!lin_holds(n, NW * 64)) return fail(LM_EUNSUPPORTED, "product too large for one launch");
   hipLaunchKernelGGL((k_lin_few<DT, W, MF, CF, NW, UN, EDGE>), dim3((unsigned)n), dim3(NW * 64), 0, st, a);
   LAUNCH_CHECK();
   return LM_OK;
@@ -366,7 +366,7 @@ extern "C" int lm_linear(const void* x, int64_t ldx, const lm_weight* w, const v
     TimedLaunch timed("linear_prep", st);
     const int64_t segs = (a.K + 2047) / 2048, rows = (T * segs + 3) / 4;
     const int64_t pieces = p.few ? 0 : (a.experts * ((a.N + 63) / 64) * ((a.K + 511) / 512) + 3) / 4;
-    if (T * segs > 0x7fffffff || rows + pieces > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+    if (T * segs > 0x7fffffff || !lin_holds(rows + pieces, 256)) return fail(LM_EUNSUPPORTED, "product too large for one launch");
     const dim3 grid((unsigned)(rows + pieces));
 #define PREP(DT, PACK) hipLaunchKernelGGL((k_lin_prep4<DT, PACK>), grid, dim3(256), 0, st, a, (uint32_t)rows, (uint32_t)segs, xq, xs, wsc)
     if (p.few) {

@@ -130,8 +130,6 @@ static int64_t round64(int64_t x) { return (x + 63) & ~(int64_t)63; }
 // k_lin8_prep 8; four rows of [4096, 4096] 10.9, as much as the two launches, but for the host.
 constexpr int64_t LIN8_OWN_ROWS = 4, LIN8_OWN_BYTES = 32768;
 
-constexpr int64_t LIN8_GROUPS = 1 << 24;  // workgroups of 256 a launch can have
-
 struct Lin8Plan {
   LinPlan mm;                // tile and splits of k_lin_mm
   bool few;                  // k_lin_few8, else k_lin_mm
@@ -213,7 +211,7 @@ template <int DT, bool Q8, bool OWN, int MF, int CF, int NW, int UN>
 static int launch_few8(const LinArgs& a, const uint8_t* codes, int64_t pitch, hipStream_t st) {
   TimedLaunch timed("linear_few", st);
   const int64_t n = lin_tiles<16 * MF>(a.T, a.experts, a.ends != nullptr) * ((a.N + 16 * CF - 1) / (16 * CF));
-  if (n >= LIN8_GROUPS * 4 / NW) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+  if (!lin_holds(n, NW * 64)) return fail(LM_EUNSUPPORTED, "product too large for one launch");
   const size_t lds = OWN ? (size_t)(a.T * pitch) : 0;
   // (16 fragments have no registers left for the words besides)
   const bool odd = MF == 1 && (((uintptr_t)a.w | (uintptr_t)a.K) & 3 || (!Q8 && ((uintptr_t)a.a | (uintptr_t)(a.lda * 2)) & 3));
@@ -258,7 +256,7 @@ static int lin8_setup(LinArgs& a, const Lin8Plan& p, int op, int dtype, void* wo
   TimedLaunch timed("linear_prep", st);
   if (p.copy_x) {
     const int64_t n = p.tail ? (a.T + 3) / 4 : (a.T * (p.lda / 8) + 255) / 256;
-    if (n >= LIN8_GROUPS) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+    if (!lin_holds(n, 256)) return fail(LM_EUNSUPPORTED, "product too large for one launch");
     if (p.tail) hipLaunchKernelGGL(k_lin8_tail, dim3((unsigned)n), dim3(256), 0, st, (const uint16_t*)a.a, a.lda, a.T, (int)a.K, (uint16_t*)(base + p.x), (int)p.lda);
     else hipLaunchKernelGGL(k_lin_align, dim3((unsigned)n), dim3(256), 0, st, (const uint16_t*)a.a, a.lda, a.T, op == LIN_FORWARD ? a.K : a.N,
                        (uint16_t*)(base + p.x), p.lda);
@@ -268,7 +266,7 @@ static int lin8_setup(LinArgs& a, const Lin8Plan& p, int op, int dtype, void* wo
   }
   if (p.codes_bytes > 0 || p.copy_w) {
     const int64_t rows = p.codes_bytes > 0 ? a.T : 0, n = rows + (p.copy_w ? (a.experts * a.N + 3) / 4 : 0);
-    if (n >= LIN8_GROUPS) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+    if (!lin_holds(n, 256)) return fail(LM_EUNSUPPORTED, "product too large for one launch");
     float* const scales = rows ? (float*)(base + p.scales) : nullptr;
     if (dtype == LM_F16) hipLaunchKernelGGL((k_lin8_prep<F16>), dim3((unsigned)n), dim3(256), 0, st, a, base + p.codes, scales, p.pitch, (int)p.tail, base + p.w, p.ldw);
     else hipLaunchKernelGGL((k_lin8_prep<BF16>), dim3((unsigned)n), dim3(256), 0, st, a, base + p.codes, scales, p.pitch, (int)p.tail, base + p.w, p.ldw);

@@ -5,6 +5,8 @@
 #include "lm_linear_mm.h"
 
 static int64_t round8(int64_t x) { return (x + 7) & ~(int64_t)7; }
+// whether a launch can have so many workgroups: it has fewer than 2^32 threads
+static bool lin_holds(int64_t groups, int threads) { return groups < ((int64_t)1 << 32) / threads; }
 
 struct LinPlan {
   bool few;                       // k_lin_few, else k_lin_mm
@@ -96,7 +98,7 @@ static int launch_mm(const LinArgs& a, const LinPlan& p, hipStream_t st) {
   TimedLaunch timed("linear", st);
   const int64_t J = OP == LIN_FORWARD ? a.N : a.K, gj = (J + BN - 1) / BN;
   const int64_t gi = OP == LIN_WEIGHT_GRAD ? (a.N + BM - 1) / BM : lin_tiles<BM>(a.T, a.experts, a.ends != nullptr);
-  if (gi * gj > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+  if (!lin_holds(gi * gj, WM * WN * 64)) return fail(LM_EUNSUPPORTED, "product too large for one launch");
   // (the rest of whole rounds: at most 128 tiles, four workgroups each)
   const int64_t n0 = BM == 128 && a.rounds ? 512 : gi * gj;
   const dim3 grid((unsigned)n0, OP == LIN_WEIGHT_GRAD ? a.experts : p.splits, OP == LIN_WEIGHT_GRAD ? p.splits : 1);
@@ -105,7 +107,7 @@ static int launch_mm(const LinArgs& a, const LinPlan& p, hipStream_t st) {
   if constexpr (OP == LIN_FORWARD && (W == W_Q8 || W == W_R8 || W == W_I8)) {
     if (p.splits > 1) {
       const int64_t chunks = (J + 255) / 256, blocks = (a.T * chunks + 3) / 4;
-      if (blocks > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+      if (!lin_holds(blocks, 256)) return fail(LM_EUNSUPPORTED, "product too large for one launch");
       hipLaunchKernelGGL((k_lin_join8<DT, W != W_I8>), dim3((unsigned)blocks), dim3(256), 0, st, a, p.splits, (uint32_t)chunks);
       LAUNCH_CHECK();
     }
@@ -113,7 +115,7 @@ static int launch_mm(const LinArgs& a, const LinPlan& p, hipStream_t st) {
   }
   if (p.splits > 1) {
     const int64_t n = (OP == LIN_WEIGHT_GRAD ? a.experts * a.N : a.T) * J, blocks = (n + 1023) / 1024;
-    if (blocks > 0x7fffffff) return fail(LM_EUNSUPPORTED, "product too large for one launch");
+    if (!lin_holds(blocks, 256)) return fail(LM_EUNSUPPORTED, "product too large for one launch");
     hipLaunchKernelGGL((k_lin_join<DT>), dim3((unsigned)blocks), dim3(256), 0, st, a, p.splits, n, J);
     LAUNCH_CHECK();
   }

@@ -103,3 +103,17 @@ def test_expert_view_shares_storage():
         expert_view(MXWeight(q, s, FP4, 32, BF16, True), 4, 4)
     with pytest.raises(ValueError):
         expert_view(MXWeight(q, s, FP4, 32, BF16, True), 0, 5)
+
+
+@pytest.mark.parametrize("dtype,input_dtype", [(L.LM_BF16, L.LM_BF16), (L.LM_I8, L.LM_BF16), (L.LM_I8, L.LM_I8), (L.LM_E2M1, L.LM_BF16),
+                                               (L.LM_E2M1, L.LM_E2M1)])
+def test_products_that_one_launch_cannot_hold_are_refused(dtype, input_dtype):
+    """2^31 - 1 short rows are a number of rows that the header allows, but more tiles than a launch has threads for."""
+    handle, t = L.load_library(), (1 << 31) - 1
+    w = _weight(dtype=dtype, N=32, K=32, reserved=L.LM_F32)
+    args = 4096, 32, ctypes.byref(w), None
+    assert handle.lm_linear(*args, None, 4096, t, L.LM_BF16, input_dtype, 4096, 1 << 60, None) == L.LM_EUNSUPPORTED
+    assert b"launch" in handle.lm_last_error()
+    if input_dtype == L.LM_BF16:
+        assert handle.lm_linear_input_grad(*args, 4096, t, L.LM_BF16, 4096, 1 << 60, None) == L.LM_EUNSUPPORTED
+        assert handle.lm_linear_input_grad(4096, 33, ctypes.byref(w), None, 4096, t, L.LM_BF16, 4096, 1 << 60, None) == L.LM_EUNSUPPORTED
