@@ -963,6 +963,7 @@ def grouped_int8_matmul_input_grad(dy: torch.Tensor, qdata: torch.Tensor, scale:
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _MAX_BEST = 64
 _MAX_GROUPS = 64
+_MIN_SCALE, _MAX_SCALE = 2.0**-149, (2 - 2.0**-23) * 2.0**127  # of float32
 _MAX_TOKENS = (1 << 28) - 64  # what one launch can hold
 _LOGIT_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -1003,8 +1004,8 @@ def _route(label: str, logits: torch.Tensor, top_k: int, bias: torch.Tensor | No
         raise ValueError(f"{label}: top_k must be 1 to {min(_MAX_BEST, top_groups * (experts // groups))}, got {top_k}.")
     if tokens > _MAX_TOKENS or tokens * top_k >= 1 << 31:
         raise ValueError(f"{label} takes up to 2^28 - 64 tokens and fewer than 2^31 choices, got {tokens} tokens of {top_k}.")
-    if not math.isfinite(scale) or scale == 0:
-        raise ValueError(f"{label}: scale must be finite and not zero, got {scale}.")
+    if not _MIN_SCALE <= abs(scale) <= _MAX_SCALE:
+        raise ValueError(f"{label}: scale must be finite and not zero in float32, got {scale}.")
     if bias is not None:
         if bias.dtype is not torch.float32 or tuple(bias.shape) != (experts,):
             raise ValueError(f"{label}: bias must be float32 [{experts}], got {bias.dtype} {tuple(bias.shape)}.")

@@ -195,3 +195,16 @@ def test_tokens_that_one_launch_cannot_hold_are_refused():
     assert handle.lm_route_workspace_size(most, 1) > 0
     r = L.RouteStruct(4096, None, 1, most, 1, L.LM_F32, 0, 1, 1, 1, 1, 1, 1.0, 0)
     assert handle.lm_route_topk(ctypes.byref(r), 4096, 4096, 4096, 4096, None, 0, None) == L.LM_EWORKSPACE
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, 3.5e38, 1e-46, -1e-60, float("nan"), -float("inf"), 0.0])
+def test_scales_that_float32_does_not_have_are_refused(scale):
+    """The kernels take the scale in float32, where these are infinite or zero."""
+    with pytest.raises(ValueError, match="scale"):
+        K._route("Routing", torch.zeros(4, 16), 2, None, "softmax", 1, 1, 1, True, scale)
+
+
+@pytest.mark.parametrize("scale", [2.5, -1, 2.0**-149, torch.finfo(torch.float32).max])
+def test_scales_that_float32_has_are_taken(scale):
+    r, _ = K._route("Routing", torch.zeros(4, 16), 2, None, "softmax", 1, 1, 1, True, scale)
+    assert r.scale == scale
