@@ -8,16 +8,19 @@
 // The products of one weight, or of one weight per group of rows.
 //
 // The input gradient rounds s q to 16 bits: s lies along its sum, so the product cannot be
-// multiplied by it afterwards, and to round dy s instead is off by as much.  fp16 has not
+// multiplied by it afterwards, and to round dy s instead is off by as much.  (So does a
+// program that decodes the weight to 16 bits first; bf16 outputs are off by 2.3e-3 of their norm,
+// 1.7e-3 of it their own rounding.  Both halves of s q would take twice the products.)  fp16 has not
 // the range of the scales: there 2^f s q is rounded, f of each weight such that its largest
 // scale counts as 128 to 256 (k_lin8_shift), and the sum is multiplied by 2^-f.  Weights
 // whose scale is above 2^-21 of that one's keep all their bits.
 //
 // Many rows (k_lin_mm): codes times codes are bound by the power that the matrix unit
-// may take, 4096 rows of [14336, 4096] 234 us (2.06 POP/s at 1.86 GHz, 64% of the cycles
-// busy; the library's product of 8192^3 reaches 2.2).  Decoded to 16 bits, 2048 rows of the
-// same 205 us (1.17 PFLOP/s), input gradient in two parts with their join 222 (the
-// library's bf16 product of 8192^3: 1.33).
+// may take, 4096 rows of [14336, 4096] 244 to 252 us with the rows' codes, 10 of them (2.0
+// POP/s, busy 65% of the cycles; the library's product of 8192^3 reaches 2.2).  Decoded to 16
+// bits, 2048 rows of the same 214 to 224 us (1.07 to 1.12 PFLOP/s), input gradient in two
+// parts with their join 220 to 245 (the library's bf16 product of 8192^3: 1.33).  Calls in
+// graphs on several machines; traced one by one the kernels take up to a tenth longer.
 #include "lm_impl.h"
 #include "lm_linear8.h"
 #include "lm_linear8_few.h"
@@ -27,8 +30,8 @@
 // scales: a workgroup a row, whose first 4096 values stay in registers between the two.
 // tail: codes of the last piece of 16 at its end, as k_lin8_tail has values.
 // The workgroups after those copy weights whose rows are not whole 16-byte pieces to
-// rows that are (`aligned`), a wave a row.  Bound by memory: 4096 rows of 4096 9.8 us
-// (50 MB, 5.1 TB/s).
+// rows that are (`aligned`), a wave a row.  Bound by memory: 4096 rows of 4096 10 us
+// (50 MB, 5 TB/s).
 template <int DT>
 __global__ __launch_bounds__(256) void k_lin8_prep(LinArgs a, uint8_t* codes, float* scales, int64_t pitch, int tail, uint8_t* aligned, int64_t ldw) {
   __shared__ uint32_t red[4];
@@ -142,7 +145,17 @@ struct Lin8Plan {
   size_t codes, codes_bytes, scales, x, w, part, shift, total;
 };
 
-// As lin_few: a matter of the product's volume.
+// As lin_few: a matter of the product's volume.  Measured in graphs, weights from memory,
+// us few / mm.  16-bit inputs: [4096, 4096] at 17 rows 14.3 / 13.8, at 64 rows 14.5 / 17.2, at
+// 96 rows 24.8 / 20.0; [1024, 4096] at 200 rows 14.1 / 15.2, at 300 rows 24.7 / 17.2; [256,
+// 2048] at 700 rows 8.4 / 12.8; [14336, 4096] at 24 rows 27.1 / 26.3; 8 groups [2752, 9304] at
+// 76 rows 77 / 94; 32 groups [2816, 2048] at 512 rows 56 / 55, at 1024 rows 82 / 56.  8-bit:
+// [4096, 4096] at 32 rows 12.9 / 15.5, at 64 rows 17.8 / 17.4, at 96 rows 23.0 / 18.4; [14336,
+// 4096] at 64 rows 26.7 / 32.6; 8 groups [2752, 9304] at 76 rows 56 / 79; 32 groups [2816,
+// 2048] at 1024 rows 85 / 50.  The bounds are those of MXFP4, whose weights have half the
+// bytes, and take the slower kernel for some: 65 rows of [4096, 4096] 24.7 / 19.5, 260 of
+// [1024, 4096] 24.6 / 16.9; 8-bit 64 rows of [4096, 14336] 51.5 / 31.9, 24 of [14336, 4096]
+// 29.3 / 24.2, 64 groups [2048, 1408] at 1024 rows 60 / 45.
 static bool lin8_few(int64_t T, int64_t N, int64_t K, int64_t E, bool quant) {
   const int64_t rows = (T + E - 1) / E;
   const double volume = (double)T * (double)N * (double)K;
@@ -194,6 +207,10 @@ static Lin8Plan lin8_plan(int op, int64_t T, int64_t lda, int64_t N, int64_t K, 
     if (p.copy_x) p.x = take((size_t)T * p.lda * 2);
     p.mm.splits = 1;
     const int64_t J = op == LIN_FORWARD ? N : K;
+    // (codes with the costs of dense products, decoded weights with those of MXFP4.  Tiles and
+    // parts forced in turn over 16 shapes: the choice within 6% of the best for 13; 1590 rows of
+    // [3200, 3184] 83 / 66 us and 390 of [13696, 4344] 126 / 94, both best as 256 x 256 in two
+    // parts, input gradient of 1024 rows of [4096, 4096] 68 / 58 in two parts)
     lin_tiling(p.mm, op, T, J, p.mm.len, E, !quant, false);
     if (p.mm.splits > 1) p.part = take((size_t)p.mm.splits * T * J * 4);
   }
@@ -221,14 +238,14 @@ static int launch_few8(const LinArgs& a, const uint8_t* codes, int64_t pitch, hi
   return LM_OK;
 }
 // Columns of a workgroup, its waves, units in flight, in graphs over weights from
-// memory.  Few workgroups: 16 columns (one row of [4096, 4096] 6.7 us, with 32 8.6).
-// 8-bit inputs: 32 columns, one unit (one row of [14336, 4096] 14.2 us, four units
-// 15.4; 64 rows of 32 experts [2816, 2048] 30.7, four waves with two 33.5; but one row
-// of [8192, 14336] 28.2, four units 27.4).  16-bit inputs, twice as many bytes of x for
-// a byte of the weight: 64 columns from 9 rows on (16 rows of [14336, 4096] 17.4 us, 32
-// columns 19.4), 32 below (one row 15.4, 64 columns 16.5) and where the contraction is
-// long (16 rows of [8192, 14336] 30.7, 64 columns 47.6); very many workgroups take four
-// waves (64 rows of 32 experts [2816, 2048] 31.2, eight 33.6).
+// memory (600 MB of them in turn).  Few workgroups: 16 columns (one row of [4096, 4096] 6.6
+// us, with 32 8.2; 8-bit inputs 7.3 and 8.7).  8-bit inputs: 32 columns, one unit (one row of
+// [14336, 4096] 15.4 us, four units 17.1; 64 rows of 32 experts [2816, 2048] 31.7, four waves
+// with two 33.9; but one row of [8192, 14336] 28.3, 16 columns with four units 26.5).  16-bit
+// inputs, twice as many bytes of x for a byte of the weight: 64 columns from 9 rows on (16
+// rows of [14336, 4096] 18.6 us, 32 columns 20.6), 32 below (one row 16.6, 64 columns 17.6)
+// and where the contraction is long (16 rows of [8192, 14336] 31.2, 64 columns 48.3); very
+// many workgroups take four waves (64 rows of 32 experts [2816, 2048] 32.0, eight 34.1).
 template <int DT, bool Q8, bool OWN>
 static int run_few8(const LinArgs& a, const uint8_t* codes, int64_t pitch, hipStream_t st) {
   const int64_t rows = (a.T + a.experts - 1) / a.experts;

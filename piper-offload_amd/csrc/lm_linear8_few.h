@@ -11,9 +11,10 @@
 // 8, steps (h, 0) and (h, 1), and x is read in the same order: lane group g has
 // elements 64 h + 16 g + 8 c at step (h, c).
 //
-// From memory, with the launch: one row of [14336, 4096] in 16 bits 12.4 us (4.7 TB/s),
-// quantised 14.2; 100 rows of 64 experts [2048, 1408], quantised 29.5 (4.7 TB/s for the
-// experts that have rows); one row of [1024, 4096] 6.1.
+// From memory, with the launch: one row of [14336, 4096] in 16 bits 16.6 us (3.5 TB/s; from
+// the last-level cache in part, three such weights in turn, 12.4), quantised 15.4; 100 rows
+// of 64 experts [2048, 1408], quantised 28.8 (4.8 TB/s for the experts that have rows); one
+// row of [1024, 4096] 6.4.
 #pragma once
 #include <type_traits>
 
@@ -37,7 +38,8 @@ DEV lm_u32x4 few8_drop(lm_u32x4 v, int n) {
 }
 // Codes k .. k + 15 of a row of K at any address, zeros past its end.  A part of 16 comes
 // from the row's last 16 (one load; byte after byte the ends of rows took longer than
-// all the rest: 117 rows of 8 groups [896, 1021] 16.8 us, [896, 1024] 6.0).
+// all the rest: 117 rows of 8 groups [896, 1021] 16.8 us, [896, 1024] 6.0 in the same run; like
+// this, weights from memory, 10.9 and 9.4).
 DEV lm_u32x4 few8_chunk(const uint8_t* row, int64_t k, int64_t K) {
   const int64_t left = K - k;
   lm_u32x4 v = {};
@@ -129,8 +131,9 @@ struct Lin8Row {
 // OWN: x is not quantised yet.  Its few rows are, into LDS, by every workgroup.
 // ODD: rows of codes, or of x in 16 bits, that do not start on whole words.  16 bytes at
 // such an address take twice as long to load (one row of [14336, 4090] 24.5 us, [14336,
-// 4092] 15.2), so the five words that hold them are loaded instead, and shifted; a piece
-// whose fifth word would pass its row is left to the tail.
+// 4092] 15.2 in the same run), so the five words that hold them are loaded instead, and
+// shifted (weights from memory: 20.7 and 19.1); a piece whose fifth word would pass its row
+// is left to the tail.
 template <int DT, bool Q8, bool OWN, bool ODD, int MF, int CF, int NW, int UN>
 __global__ __launch_bounds__(NW * 64) void k_lin_few8(LinArgs a, const uint8_t* codes, int64_t pitch) {
   constexpr bool HALF = DT == F16;

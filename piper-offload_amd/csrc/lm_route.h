@@ -3,8 +3,11 @@
 #include "lm_linear.h"
 
 // Up to this many tokens k_route_place adds up the counts by itself: every workgroup
-// reads those of all (16384 tokens, 256 experts: 7 us, two launches that share the
-// sums 10).  The reading grows with the square of the tokens, so above it they do.
+// reads those of all.  The reading grows with the square of the tokens, so above it two
+// launches share the sums.  Whole calls, itself / shared: 8192 tokens, 64 experts 11.8 /
+// 15.0 us; 16384, 256 experts 28.1 / 30.6; 32768, 64 experts 22.5 / 26.4, 256 experts 48.3 /
+// 48.5.  (It grows with the experts too, which the bound leaves out: 1024 experts 41.7 / 38.2 at
+// 4096 tokens, 174 / 160 at 32768.)
 constexpr int64_t ROUTE_NEAR = 32768;
 
 struct RouteArgs {

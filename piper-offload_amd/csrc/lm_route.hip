@@ -730,10 +730,11 @@ DEV void rows_store(uint16_t* p, lm_u32x4 w, int64_t left) {
 // 8 values of each of M rows, `left` of which exist; all of them before the first is used.
 //
 // Rows of choices go past the caches, both ways: there are top_k of them for every
-// row of a token, and each is read or written once (8192 x 2048, four choices: rows
-// out 34 -> 26 us, back 33 -> 28, gradients 58 -> 48).  Rows of tokens do not: with
-// both past the caches rows out take 31 us, gradients 53.  Bound by memory: 6.3 TB/s out,
-// 5.6 back, 5.7 the gradients, where a copy reaches 5.1 to 6.1.
+// row of a token, and each is read or written once (8192 x 2048, four choices, by
+// themselves: rows out 34 -> 26 us, back 33 -> 28, gradients 58 -> 48).  Rows of tokens do
+// not: with both past the caches rows out take 31 us, gradients 53.  Bound by memory: called
+// in turn with others 26 us out (6.4 TB/s), 29 to 30 back (5.7), 53 to 54 the gradients (5.6),
+// where a copy reaches 5.1 to 6.1.
 template <bool NT, int M>
 DEV void rows_load(lm_u32x4 (&w)[M], const uint16_t* const (&p)[M], int64_t left) {
   if (left >= 8) {
