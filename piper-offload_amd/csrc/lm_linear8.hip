@@ -13,7 +13,7 @@
 // 1.7e-3 of it their own rounding.  Both halves of s q would take twice the products.)  fp16 has not
 // the range of the scales: there 2^f s q is rounded, f of each weight such that its largest
 // scale counts as 128 to 256 (k_lin8_shift), and the sum is multiplied by 2^-f.  Weights
-// whose scale is above 2^-21 of that one's keep all their bits.
+// whose scale is above 2^-21 of that one keep fp16's 11 bits.
 //
 // Many rows (k_lin_mm): codes times codes are bound by the power that the matrix unit
 // may take, 4096 rows of [14336, 4096] 244 to 252 us with the rows' codes, 10 of them (2.0

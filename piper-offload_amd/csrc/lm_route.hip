@@ -12,7 +12,7 @@
 //
 // A token is a wave's: lane l has the experts l, l + 64, ... in registers, a maximum
 // over the wave is six DPP steps, and the choice is that maximum taken k times.  Bound
-// by instructions: 16384 tokens, 256 experts in 8 groups, 8 of them chosen 34 us, 660
+// by instructions: 16384 tokens, 256 experts in 8 groups, 8 of them chosen 34 us, 680
 // vector and as many scalar instructions a token, the vector unit issuing 70% of the
 // time (its bytes alone: 4 us).  8192 tokens, 64 experts, 4 chosen: 8 us; 8 tokens: 4.
 #include "lm_impl.h"

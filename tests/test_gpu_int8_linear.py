@@ -578,3 +578,47 @@ def test_input_grad_with_scales_of_zero(dtype):
     dy[:, 5] *= 1e4
     w, rows = q.double() * s.double(), dy.double()
     _close(K.int8_matmul_input_grad(dy.to(DEV), q.to(DEV), s.to(DEV)), rows @ w, (100 * 2.0**-23 + _half(dtype)[0]) * (rows.abs() @ w.abs()))
+
+
+def test_fp16_gradients_follow_their_scales():
+    """A captured gradient whose scales change between replays, through the layers, on another stream than its tensors'."""
+    g = _gen(54)
+    n, k, t = 200, 272, 90
+    q = torch.randint(-128, 128, (2, n, k), generator=g, dtype=torch.int8)
+    s0 = (0.25 + 0.75 * torch.rand(2, n, 1, generator=g)) * 1e-3
+    ends = torch.tensor([40, t - 3], dtype=torch.int32)
+    dy, x = _normal(g, t, n, dtype=F16), _normal(g, t, k, dtype=F16)
+    q1, s1 = q.view(2 * n, k).to(DEV), s0.view(2 * n, 1).to(DEV)
+    weight, one, at = Int8Weight(q1, s1, (1, k)), Int8Weight(q1[:n], s1[:n], (1, k)), ends.to(DEV)
+    rows, dy1, factor = x.to(DEV).requires_grad_(), dy.to(DEV), torch.ones((), device=DEV)
+
+    def work():
+        y = grouped_linear(rows, weight, at)
+        a, = torch.autograd.grad(y, rows, dy1 * factor.to(F16))
+        b, = torch.autograd.grad(int8_linear(rows, one), rows, dy1 * factor.to(F16))
+        return a, b
+
+    def want(scale, f):
+        w, d = q.double() * scale.double(), (dy * f).double()
+        size = torch.cat((d[:40].abs() @ w[0].abs(), d[40:t - 3].abs() @ w[1].abs(), torch.zeros(3, k)))
+        a = torch.cat((d[:40] @ w[0], d[40:t - 3] @ w[1], torch.zeros(3, k, dtype=torch.double)))
+        return (a, size), (d @ w[0], d.abs() @ w[0].abs())
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = work()
+    torch.cuda.current_stream().wait_stream(side)
+    for down, f in ((1.0, 1.0), (1e-6, 2.0**12), (1e5, 2.0**-10), (1.0, 1.0)):
+        s1.copy_((s0 * down).view(2 * n, 1))
+        factor.fill_(f)
+        graph.replay()
+        got = [o.clone() for o in out]
+        eager = work()
+        for o, e, (a, size) in zip(got, eager, want(s1.cpu().view(2, n, 1), f)):
+            assert (o == e).all()
+            _close(o, a, ((n + 4) * 2.0**-23 + 2.0**-11) * size)
